@@ -12,7 +12,7 @@
  *   - every entry point selects its device itself (the reference calls a backend from one thread per device:
  *     Seq2SeqSharp/Tools/BaseSeq2SeqFramework.cs:912) and is safe to call concurrently for different devices;
  *   - `stream` is a cudaStream_t passed as void*; NULL selects the library's own non-blocking stream of the
- *     device.  Nothing runs on the legacy NULL stream;
+ *     device.  Nothing runs on the legacy NULL stream, unless it is named (cudaStreamLegacy, the handle 1);
  *   - there is no CPU fallback: with no usable sm_100 device every compute entry point fails.
  */
 #ifndef TSB200_H_
@@ -237,6 +237,52 @@ TSB200_API int TSB200_PrefillAttention(int device, int dtype, void* out, const v
  * ReduceDimIndexKernels.cs:96-119).  probs_out may be NULL. */
 TSB200_API int TSB200_SoftmaxArgmax(int device, int32_t* out_ids, float* probs_out, const float* logits, int B, int V,
                                     float temperature, const int32_t* blocked, int n_blocked, void* stream);
+
+/* ------------------------------------------------------------------------------------------------ paged cache
+ * A key / value cache in pages of `page` tokens (a power of two from 8 to 256) for serving: sequences of any lengths share one pool, rows of a
+ * step lie one after the other (starts[b] .. starts[b + 1] are those of sequence b), and each call takes its lengths from device memory, so
+ * that a captured step is replayed with other ones.  Pages belong to one sequence each.  dtype TSB200_F32, TSB200_F16 or TSB200_BF16.  These calls leave the caller's
+ * current device as it was.  (The reference keeps one tensor per sequence batch, MultiHeadAttention.cs:173-193.)
+ *
+ * PagedPlan: before a step, cached [B] tokens are kept of every sequence and fresh [B] are to be added.  The table [B, max_blocks] (rows table_stride
+ * apart) names the held [B] pages of every sequence, the first free_count[0] entries of free_pages [num_pages] the free ones; all four are updated.  Sequences
+ * take what they lack in their order, from the end of the free ones.  One whose pages are not there, whose rows do not fit the `rows` of the call, or
+ * whose tokens do not fit max_blocks pages gets no rows, and no sequence behind it gets what it was refused (pages or rows); pages that
+ * are given back in the call are not taken in it.  A sequence keeps ceil((cached + granted) / page) pages; what it held beyond goes back and its entries
+ * become -1 (fresh = 0: roll back to `cached`; cached = fresh = 0: release).  A negative count leaves its sequence's pages as they are.
+ * Out: lens [B] = cached + granted (may be `cached` itself), starts [B + 1], and for `rows` rows slots = place in the cache (page number * page +
+ * offset) and position in the sequence, both -1 behind the granted ones.  1 <= B <= 8192. */
+TSB200_API int TSB200_PagedPlan(int device, const int32_t* cached, const int32_t* fresh, int B, int page, int32_t* table, int64_t table_stride, int max_blocks,
+                                int32_t* held, int32_t* free_pages, int32_t* free_count, int num_pages, int32_t* lens, int32_t* starts, int32_t* slots,
+                                int32_t* positions, int rows, void* stream);
+/* RMS norm of every query and key head (weights q_norm, k_norm [hd] in dtype; NULL: none), rotation by position, queries to q_out, keys and values to
+ * their places in the cache.  q, q_out [rows, H, hd], k, v [rows, Hkv, hd] with strides in elements (the last one is 1); q_out may be q.
+ * rope_style 0: none, 1: pairs (2i, 2i + 1) of the first rope_dims elements, 2: pairs (i, i + rope_dims / 2) (rope_dims a multiple of 16); angle
+ * position * rope_base^(-2i / rope_dims), in 64 bits.  A row whose slot is not one of the cache (-1) is left out: nothing of it is read or written.
+ * The slots of a call differ.  Place o of page p, head h of cacheK and cacheV: element p * c_page + h * c_head + o * c_tok.  hd: a multiple of 8 up to 256. */
+TSB200_API int TSB200_QKNormRopePaged(int device, int dtype, void* q_out, int64_t o_row, int64_t o_head, const void* q, int64_t q_row, int64_t q_head,
+                                      const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* q_norm,
+                                      const void* k_norm, float eps, const int32_t* positions, const int32_t* slots, int rows, int H, int Hkv, int hd,
+                                      int rope_style, int rope_dims, double rope_base, void* cacheK, void* cacheV, int64_t c_page, int64_t c_head,
+                                      int64_t c_tok, int num_pages, int page, void* stream);
+/* Attention of the new rows over the pages: row i of the n of sequence b is at position lens[b] - n + i and sees the keys up to it (window > 0: the last
+ * `window` of them), out = softmax(scale q k^T) v, query head h reading KV head h / (H / Hkv).  Entries of the table that name no page
+ * hide their keys; a row that sees none becomes zeros; rows of no sequence are left as they were.  What the pages hold behind lens[b] is never used.
+ * max_new: the most new rows of a sequence, as far as the caller knows (it chooses the kernel; more rows are served as well, with a workspace for max_new).
+ * Pointers on a boundary of 16 bytes, strides (elements) multiples of 16 bytes.  workspace >= TSB200_PagedAttentionWorkspaceBytes; calls that may overlap need one each. */
+TSB200_API int64_t TSB200_PagedAttentionWorkspaceBytes(int dtype, int H, int Hkv, int hd, int max_new);
+TSB200_API int TSB200_PagedAttention(int device, int dtype, void* out, int64_t o_row, int64_t o_head, const void* q, int64_t q_row, int64_t q_head,
+                                     const void* cacheK, const void* cacheV, int64_t c_page, int64_t c_head, int64_t c_tok, int num_pages, int page,
+                                     const int32_t* table, int64_t table_stride, int max_blocks, const int32_t* starts, const int32_t* lens, int B, int rows,
+                                     int max_new, int H, int Hkv, int hd, float scale, int window, void* workspace, int64_t workspace_bytes, void* stream);
+/* Check of drafted tokens (speculative decoding).  Row i of sequence b (p, F32, V words, rows p_row apart; rows starts[b] .. starts[b + 1], at most K + 1, or
+ * K + 1 for every sequence where starts is NULL) holds the target's probabilities after i drafts; draft [B, K] the drafted ids (of a sequence with n rows the first
+ * n - 1), q (rows b * K + i, q_row apart) the probabilities they were drawn with, NULL where they were certain; u [B, K + 1] uniform numbers in
+ * [0, 1).  Draft i is accepted while u[i] q_i(x_i) < p_i(x_i); behind the last accepted one a token is drawn with u[K] from max(p_i - q_i, 0), or from p_i where
+ * no draft is left or that is zero everywhere: the smallest id whose cumulative weight exceeds u[K] times the whole.  Ids outside of the vocabulary are refused.
+ * Out: tokens [B, K + 1] (accepted drafts, the drawn token, -1 behind), counts [B] = accepted + 1, 0 for a sequence without rows. */
+TSB200_API int TSB200_VerifyDraft(int device, int32_t* tokens, int32_t* counts, const float* p, int64_t p_row, const float* q, int64_t q_row,
+                                  const int32_t* draft, const int32_t* starts, const float* u, int B, int K, int V, int rows, void* stream);
 
 /* ------------------------------------------------------------------------------------------------ GPT engine
  * The whole token loop of GPT.RunForwardOnSingleDevice / Decoder.GPTDecode / GPTDecoder.Decode

@@ -137,6 +137,11 @@ def lib():
         "TSB200_FlashDecode": (i32, [i32, i32, vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, vp, i64, vp]),
         "TSB200_PrefillAttention": (i32, [i32, i32, vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp]),
         "TSB200_SoftmaxArgmax": (i32, [i32, vp, vp, vp, i32, i32, f32, vp, i32, vp]),
+        "TSB200_PagedPlan": (i32, [i32, vp, vp, i32, i32, vp, i64, i32, vp, vp, vp, i32, vp, vp, vp, vp, i32, vp]),
+        "TSB200_QKNormRopePaged": (i32, [i32, i32] + [vp, i64, i64] * 4 + [vp, vp, f32, vp, vp] + [i32] * 6 + [C.c_double, vp, vp, i64, i64, i64, i32, i32, vp]),
+        "TSB200_PagedAttentionWorkspaceBytes": (i64, [i32] * 5),
+        "TSB200_PagedAttention": (i32, [i32, i32] + [vp, i64, i64] * 2 + [vp, vp, i64, i64, i64, i32, i32, vp, i64, i32, vp, vp] + [i32] * 6 + [f32, i32, vp, i64, vp]),
+        "TSB200_VerifyDraft": (i32, [i32, vp, vp, vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, i32, vp]),
         "TSB200_GptCreate": (i32, [C.POINTER(GptConfig), C.POINTER(vp)]),
         "TSB200_GptCreateLayered": (i32, [C.POINTER(LayeredConfigC), C.POINTER(LayerDescC), C.POINTER(vp)]),
         "TSB200_GptDestroy": (i32, [vp]),

@@ -55,6 +55,20 @@ struct DeviceState {
 };
 // Makes `device` current, lazily creates its state.  Fails when the device is absent or not sm_100.
 int use_device(int device, DeviceState** st);
+// a stand-alone call leaves the caller's current device as it was
+struct KeepDevice {
+  int was = -1;
+  KeepDevice() {
+    if (cudaGetDevice(&was) != cudaSuccess) {
+      cudaGetLastError();
+      was = -1;
+    }
+  }
+  ~KeepDevice() {
+    int now = -1;
+    if (was >= 0 && cudaGetDevice(&now) == cudaSuccess && now != was) cudaSetDevice(was);
+  }
+};
 inline cudaStream_t pick_stream(DeviceState* st, void* stream) { return stream ? (cudaStream_t)stream : st->stream; }
 void count_launch(int device, long long n = 1);
 int check_launch(const char* what);

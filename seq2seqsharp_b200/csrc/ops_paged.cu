@@ -1,0 +1,657 @@
+// A key / value cache in pages: the plan that hands pages out and maps rows to places, the norm / rotation / append of new rows, and the attention over
+// the pages (kernel for every type and head size; attn_paged_mma.cu and attn_paged_tc.cu for 16-bit types and head sizes 64 and 128).
+#include <cfloat>
+#include <cmath>
+
+#include "paged.cuh"
+
+namespace tsb {
+
+// ------------------------------------------------------------------------------------------------------------------------ plan
+// want = ceil((cached + fresh) / page);  need = max(0, want - held), taken from the top of the stack of free pages in the order of the sequences;
+// held - want pages of a sequence that wants fewer go back, so that taking and giving back leaves the stack as it was;
+// starts = exclusive sum of the granted rows;  slot(row) = table[pos / page] * page + pos % page.
+// What bounds it: latency (two block scans, a few hundred KB at most).  Sums of rows and pages over sequences are 64-bit: their bounds are the caller's.
+struct PlanArgs {
+  const int *cached, *fresh;
+  int B, page_shift, max_blocks, num_pages, rows;
+  int* table;
+  int64_t table_stride;
+  int *held, *free_pages, *free_count, *lens, *starts, *slots, *positions;
+};
+constexpr int kPlanThreads = 1024, kPlanMaxB = 8192;
+
+__device__ __forceinline__ long long plan_scan(long long v, long long* warps, long long& all) {   // exclusive, kPlanThreads
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  long long x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) warps[w] = x;
+  __syncthreads();
+  long long y = warps[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long z = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) y += z;
+  }
+  all = __shfl_sync(0xffffffffu, y, 31);
+  const long long before = __shfl_sync(0xffffffffu, y, w > 0 ? w - 1 : 0);
+  return (w > 0 ? before : 0) + x - v;
+}
+// the last i of [0, n) with first[i] <= v (first ascending, first[0] <= v)
+__device__ __forceinline__ int plan_find(const int* first, int n, int v) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int m = (lo + hi) >> 1;
+    if (first[m] <= v) lo = m;
+    else hi = m;
+  }
+  return lo;
+}
+
+// One cluster.  Every CTA makes the scans for itself; the pages to move and the rows are shared out over all threads.
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs a, int ctas) {
+  extern __shared__ int plan_sm[];
+  __shared__ long long warps[32];
+  __shared__ int granted;
+  const int B = a.B, tid = threadIdx.x, page = 1 << a.page_shift;
+  // of every sequence: pages held before, cached tokens, pages kept; number of its first new row, first page taken, first page given back
+  int *have_s = plan_sm, *old_s = have_s + B, *keep_s = old_s + B, *row_s = keep_s + B, *take_s = row_s + B, *give_s = take_s + B;
+  const int avail = min(max(*a.free_count, 0), a.num_pages);
+  if (tid == 0) granted = 0;
+  long long rows = 0, asked = 0, moved = 0;   // over the sequences so far; moved: pages taken in the upper, given back in the lower half
+  for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int old = 0, fresh = 0, have = 0;
+    if (b < B) {
+      old = a.cached[b];
+      fresh = a.fresh[b];
+      have = min(max(a.held[b], 0), a.max_blocks);
+    }
+    const bool fits = b < B && old >= 0 && fresh >= 0 && (long long)old + fresh <= ((long long)a.max_blocks << a.page_shift);
+    int now = fits ? fresh : 0;
+    const int kept = fits ? (int)(((long long)old + page - 1) >> a.page_shift) : have;
+    const int want = fits ? (int)(((long long)old + now + page - 1) >> a.page_shift) : have;
+    int need = now > 0 ? max(0, want - have) : 0;
+    long long all;
+    const long long need_before = asked + plan_scan(need, warps, all);
+    asked += all;
+    if (need > 0 && need_before + need > avail) now = 0;
+    const long long rows_before = rows + plan_scan(now, warps, all);
+    rows += all;
+    if (rows_before + now > a.rows) now = 0;   // nor is any row behind granted: the sums only grow
+    if (now == 0) need = 0;
+    const int keep = now > 0 ? want : min(have, kept);
+    const long long move = ((long long)need << 32) | (unsigned)max(0, have - keep);
+    const long long move_before = moved + plan_scan(move, warps, all);
+    moved += all;
+    if (b < B) {
+      have_s[b] = have;
+      old_s[b] = old;
+      keep_s[b] = keep;
+      row_s[b] = (int)min(rows_before, (long long)a.rows);
+      take_s[b] = (int)(move_before >> 32);
+      give_s[b] = (int)(move_before & 0xffffffffLL);
+      if (now > 0) atomicMax(&granted, (int)(rows_before + now));
+    }
+  }
+  __syncthreads();
+  const int total = granted, taken = (int)(moved >> 32), given = (int)(moved & 0xffffffffLL);
+  for (int b = tid; b < B; b += kPlanThreads) row_s[b] = min(row_s[b], total);
+  const int first = (int)blockIdx.x * kPlanThreads + tid, step = ctas * kPlanThreads;
+  for (int m = first; m < taken; m += step) {
+    const int b = plan_find(take_s, B, m);
+    a.table[b * a.table_stride + have_s[b] + (m - take_s[b])] = a.free_pages[avail - 1 - m];
+  }
+  cluster_sync();   // all that other CTAs read of the state has been read, and the pages taken are in the table
+  const int height = avail - taken + given;
+  for (int m = first; m < given; m += step) {
+    const int b = plan_find(give_s, B, m), at = height - 1 - m;
+    int* entry = a.table + b * a.table_stride + keep_s[b] + (m - give_s[b]);
+    if (at >= 0 && at < a.num_pages) a.free_pages[at] = *entry;
+    *entry = -1;
+  }
+  for (int b = first; b <= B; b += step) {
+    a.starts[b] = b < B ? row_s[b] : total;
+    if (b == B) continue;
+    const int now = (b + 1 < B ? row_s[b + 1] : total) - row_s[b];
+    a.held[b] = keep_s[b];
+    a.lens[b] = old_s[b] + now;
+  }
+  if (first == 0) *a.free_count = min(height, a.num_pages);
+  for (int r = first; r < a.rows; r += step) {
+    int pos = -1, slot = -1;
+    if (r < total) {
+      const int b = plan_find(row_s, B, r);
+      pos = old_s[b] + (r - row_s[b]);
+      const int entry = a.table[b * a.table_stride + (pos >> a.page_shift)];
+      if (entry >= 0 && entry < a.num_pages) slot = entry * page + (pos & (page - 1));
+    }
+    a.slots[r] = slot;
+    a.positions[r] = pos;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------ norm, rotation, append
+//   y = x / sqrt(mean(x^2) + eps) * w;   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin),   angle = position * base^(-2 i / rot)
+// for every query and key head of a row; queries go to `out`, keys and values to the row's place in the cache.  Norm and rotation in fp32, rounded once;
+// angles in 64 bits (fp32 loses the angle of position 10^5 from the third digit on) as half turns, which are brought to [-1, 1] before they are rounded.
+// L = 2^k lanes hold a head, eight elements each (elements of a 16-bit head: 16 bytes per lane).  The cos / sin of a row are made once per CTA.
+struct RopePagedArgs {
+  void* out;
+  const void *q, *k, *v, *q_norm, *k_norm;
+  int64_t o_row, o_head, q_row, q_head, k_row, k_head, v_row, v_head;
+  float eps;
+  const int *positions, *slots;
+  int rows, H, Hkv, hd, rot, style;   // style 0: no rotation, 1: pairs (2i, 2i + 1), 2: pairs (i, i + rot / 2)
+  double first, ratio;                // half turns per position of pair 0; of pair i: first * ratio^i
+  void *K, *V;
+  int64_t c_page, c_head, c_tok;
+  int num_pages, page_shift;
+  int rows_here;                      // rows per CTA
+};
+constexpr int kRopeThreads = 256, kRopeMaxHd = 256;
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void rope_load8(const T* p, float* f) {
+  if constexpr (!WIDE) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = to_f<T>(p[e]);
+  } else if constexpr (sizeof(T) == 4) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t r[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 t = Pair16<T>::get(r[e]);
+      f[2 * e] = t.x;
+      f[2 * e + 1] = t.y;
+    }
+  }
+}
+template <typename T, bool WIDE>
+__device__ __forceinline__ void rope_store8(T* p, const float* f) {
+  if constexpr (!WIDE) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = from_f<T>(f[e]);
+  } else if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(Pair16<T>::put(f[0], f[1]), Pair16<T>::put(f[2], f[3]), Pair16<T>::put(f[4], f[5]), Pair16<T>::put(f[6], f[7]));
+  }
+}
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_paged_kernel(const __grid_constant__ RopePagedArgs a) {
+  __shared__ float wq[kRopeMaxHd], wk[kRopeMaxHd];
+  __shared__ float2 turn[kRopeThreads];
+  const int tid = threadIdx.x, half = a.rot / 2;
+  for (int e = tid; e < a.hd; e += kRopeThreads) {
+    wq[e] = a.q_norm ? to_f<T>(reinterpret_cast<const T*>(a.q_norm)[e]) : 1.0f;
+    wk[e] = a.k_norm ? to_f<T>(reinterpret_cast<const T*>(a.k_norm)[e]) : 1.0f;
+  }
+  int L = 1;
+  while (L * 8 < a.hd) L <<= 1;
+  const int li = tid & (L - 1), lane = tid & 31, per = kRopeThreads / L, heads = a.H + 2 * a.Hkv;
+  const bool on = li * 8 < a.hd;
+  const int64_t places = (int64_t)a.num_pages << a.page_shift;
+  const int row_first = (int)blockIdx.x * a.rows_here, row_end = min(a.rows, row_first + a.rows_here);
+  // a pass: as many rows as the CTA has threads for their angles
+  const int rows_pass = a.style && half > 0 ? max(1, kRopeThreads / half) : 1;
+  for (int row0 = row_first; row0 < row_end; row0 += rows_pass) {
+    const int n = min(rows_pass, row_end - row0);
+    __syncthreads();
+    if (a.style && tid < n * half) {
+      const int i = tid % half;
+      double x = (double)a.positions[row0 + tid / half] * (a.first * pow(a.ratio, (double)i));
+      x -= 2.0 * rint(0.5 * x);
+      float s, c;
+      sincospif((float)x, &s, &c);
+      turn[tid] = make_float2(c, s);
+    }
+    __syncthreads();
+    for (int it = (int)blockIdx.y * per + tid / L; __any_sync(0xffffffffu, it < n * heads); it += per * (int)gridDim.y) {
+      const bool live = it < n * heads && on;
+      const int r = min(it / heads, n - 1), head = it % heads, row = row0 + r;
+      const int slot = a.slots[row];
+      const bool there = live && slot >= 0 && slot < places;
+      const bool is_q = head < a.H, is_v = head >= a.H + a.Hkv;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+      if (there) {
+        const T* src = is_q ? reinterpret_cast<const T*>(a.q) + row * a.q_row + head * a.q_head
+                            : (is_v ? reinterpret_cast<const T*>(a.v) + row * a.v_row + (head - a.H - a.Hkv) * a.v_head
+                                    : reinterpret_cast<const T*>(a.k) + row * a.k_row + (head - a.H) * a.k_head);
+        rope_load8<T, WIDE>(src + li * 8, x);
+      }
+      const bool normed = !is_v && (is_q ? a.q_norm : a.k_norm) != nullptr;
+      float ss = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+      for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (normed && on) {
+        const float f = 1.0f / sqrtf(ss / (float)a.hd + a.eps);
+        const float* w = is_q ? wq : wk;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * f * w[li * 8 + e];
+      }
+      if (a.style == 1) {
+        if (!is_v)
+#pragma unroll
+          for (int e = 0; e < 8; e += 2)
+            if (li * 8 + e < a.rot) {
+              const float2 t = turn[r * half + (li * 8 + e) / 2];
+              const float y0 = x[e] * t.x - x[e + 1] * t.y, y1 = x[e + 1] * t.x + x[e] * t.y;
+              x[e] = y0;
+              x[e + 1] = y1;
+            }
+      } else if (a.style == 2) {
+        // the partner of element e < rot / 2 is e + rot / 2: whole lanes apart
+        const int away = half / 8, low = li < away;
+        const int from = (lane & ~(L - 1)) + (li * 8 < a.rot ? (low ? li + away : li - away) : li);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = __shfl_sync(0xffffffffu, x[e], from);
+          if (!is_v && li * 8 < a.rot) {
+            const float2 t = turn[r * half + (low ? li : li - away) * 8 + e];
+            x[e] = low ? x[e] * t.x - y * t.y : x[e] * t.x + y * t.y;
+          }
+        }
+      }
+      if (there) {
+        T* dst;
+        if (is_q) {
+          dst = reinterpret_cast<T*>(a.out) + row * a.o_row + head * a.o_head;
+        } else {
+          const int64_t at = (int64_t)(slot >> a.page_shift) * a.c_page + (int64_t)(slot & ((1 << a.page_shift) - 1)) * a.c_tok + (is_v ? head - a.H - a.Hkv : head - a.H) * a.c_head;
+          dst = reinterpret_cast<T*>(is_v ? a.V : a.K) + at;
+        }
+        rope_store8<T, WIDE>(dst + li * 8, x);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------ attention, every type
+// Four warps of RW rows; a tile of 32 keys and values is brought to shared memory by cp.async while the one before is used (places
+// that hold no visible key are filled with zeros, whatever the cache has there).  Scores: a lane per key; values: a lane per hd / 32 elements.
+// fp32 throughout: the products run on the FMA pipe, which is what bounds chunks; single tokens are bound by bytes.
+constexpr int kFmaThreads = 128, kFmaKeys = 32;
+__device__ __forceinline__ void paged_cp16(void* dst, const void* src, bool there) {   // zeros where there is nothing
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+template <typename T>
+constexpr int fma_row_bytes(int NH) { return NH * 32 * (int)sizeof(T) + 16; }   // odd in units of 16 bytes: lanes of neighbouring keys meet no bank twice
+template <typename T>
+constexpr int fma_smem(int NH, int RW) { return 4 * kFmaKeys * fma_row_bytes<T>(NH) + 4 * RW * NH * 32 * 4; }
+
+template <typename T, int NH, int RW>
+__global__ void __launch_bounds__(kFmaThreads) paged_fma_kernel(const __grid_constant__ PagedArgs a) {
+  constexpr int RT = 4 * RW, KT = kFmaKeys, D = NH * 32, RB = fma_row_bytes<T>(NH), EV = 16 / (int)sizeof(T);
+  extern __shared__ __align__(16) unsigned char fma_sm[];
+  __shared__ PagedPlanShared plan;
+  float* qs = reinterpret_cast<float*>(fma_sm + 4 * KT * RB);   // [RT][D]
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  pdl_trigger();
+  long long all;
+  int runs;
+  if (!paged_locate<kFmaThreads, RT, KT>(a, blockIdx.x, gridDim.x, plan, all, runs)) return;
+  const int pieces = a.hd / EV, mask = (1 << a.page_shift) - 1;
+  PagedRun run;
+  run.begin(a, plan, RT);
+  for (; run.next(a, plan, RT, KT); run.step(a)) {
+    const PagedSeq& s = run.seq;
+    const int p0 = run.t * RT, pairs = s.n * a.G;
+    const int cap = min(s.len, a.max_blocks << a.page_shift);
+    const int* table = a.table + run.b * a.table_stride;
+    auto fetch = [&](int kt) {
+      unsigned char* ks = fma_sm + (kt & 1) * 2 * KT * RB;
+      for (int i = tid; i < KT * (D / EV); i += kFmaThreads) {
+        const int k = i / (D / EV), e = i % (D / EV), j = kt * KT + k;
+        bool there = j < cap && e < pieces;
+        const int page = there ? table[j >> a.page_shift] : 0;
+        there = there && page >= 0 && page < a.num_pages;
+        const int64_t at = there ? page * a.c_page + run.h * a.c_head + (j & mask) * a.c_tok + e * EV : 0;
+        paged_cp16(ks + k * RB + e * 16, reinterpret_cast<const T*>(a.K) + at, there);
+        paged_cp16(ks + (KT + k) * RB + e * 16, reinterpret_cast<const T*>(a.V) + at, there);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    __syncthreads();   // the item before has been read
+    fetch(run.k0);
+    for (int i = tid; i < RT * D; i += kFmaThreads) {
+      const int r = i / D, e = i % D, p = p0 + r;
+      float v = 0.0f;
+      if (p < pairs && e < a.hd) v = to_f<T>(reinterpret_cast<const T*>(a.q)[(int64_t)(s.row0 + p / a.G) * a.q_row + (run.h * a.G + p % a.G) * a.q_head + e]) * a.c;
+      qs[i] = v;
+    }
+    float m[RW], l[RW], acc[RW][NH];
+    int lo[RW], hi[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.0f;
+      const int p = p0 + w * RW + r, pos = s.len - s.n + p / a.G;
+      hi[r] = p < pairs ? min(pos + 1, cap) : 0;
+      lo[r] = a.window > 0 ? pos - a.window + 1 : 0;
+#pragma unroll
+      for (int e = 0; e < NH; ++e) acc[r][e] = 0.0f;
+    }
+    for (int kt = run.k0; kt < run.k1; ++kt) {
+      if (kt + 1 < run.k1) fetch(kt + 1);
+      else asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncthreads();
+      const unsigned char* ks = fma_sm + (kt & 1) * 2 * KT * RB;
+      const int j = kt * KT + lane;
+      bool seen = j < cap;
+      if (seen) {
+        const int page = table[j >> a.page_shift];
+        seen = page >= 0 && page < a.num_pages;
+      }
+      float sc[RW];
+#pragma unroll
+      for (int r = 0; r < RW; ++r) sc[r] = 0.0f;
+#pragma unroll 4
+      for (int e = 0; e < D / EV; ++e) {
+        float kf[EV];
+        if constexpr (sizeof(T) == 4) {
+          const float4 k4 = *reinterpret_cast<const float4*>(ks + lane * RB + e * 16);
+          kf[0] = k4.x; kf[1] = k4.y; kf[2] = k4.z; kf[3] = k4.w;
+        } else {
+          rope_load8<T, true>(reinterpret_cast<const T*>(ks + lane * RB + e * 16), kf);
+        }
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+#pragma unroll
+          for (int g = 0; g < EV; g += 4) {
+            const float4 q4 = *reinterpret_cast<const float4*>(qs + (w * RW + r) * D + e * EV + g);
+            sc[r] += q4.x * kf[g] + q4.y * kf[g + 1] + q4.z * kf[g + 2] + q4.w * kf[g + 3];
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        if (!(seen && j < hi[r] && j >= lo[r])) sc[r] = -INFINITY;
+        const float up = fmaxf(m[r], warp_max(sc[r]));
+        const float from = fmaxf(up, -FLT_MAX);   // no key seen yet: every weight is exp2(-inf)
+        const float f = exp2f(m[r] - from);
+        sc[r] = exp2f(sc[r] - from);
+        m[r] = up;
+        l[r] = l[r] * f + sc[r];   // this lane's keys
+#pragma unroll
+        for (int e = 0; e < NH; ++e) acc[r][e] *= f;
+      }
+#pragma unroll 4
+      for (int k = 0; k < KT; ++k) {
+        float vf[NH];
+        const T* v = reinterpret_cast<const T*>(ks + (KT + k) * RB) + lane * NH;
+#pragma unroll
+        for (int e = 0; e < NH; ++e) vf[e] = to_f<T>(v[e]);
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+          const float p = __shfl_sync(0xffffffffu, sc[r], k);
+#pragma unroll
+          for (int e = 0; e < NH; ++e) acc[r][e] += p * vf[e];
+        }
+      }
+      __syncthreads();
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    const bool whole = run.first && run.last;
+    float* rec = a.part + (2 * (int64_t)blockIdx.x + (run.first ? 1 : 0)) * paged_record_floats(RT, a.hd);
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      const float sum = warp_sum(l[r]);
+      const int row = w * RW + r, p = p0 + row;
+      if (p >= pairs) continue;
+      if (whole) {
+        T* o = reinterpret_cast<T*>(a.out) + (int64_t)(s.row0 + p / a.G) * a.o_row + (run.h * a.G + p % a.G) * a.o_head;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int e = 0; e < NH; ++e)
+          if (lane * NH + e < a.hd) o[lane * NH + e] = from_f<T>(acc[r][e] * inv);
+      } else {
+        if (lane == 0) {
+          rec[2 * row] = m[r];
+          rec[2 * row + 1] = sum;
+        }
+#pragma unroll
+        for (int e = 0; e < NH; ++e)
+          if (lane * NH + e < a.hd) rec[2 * RT + row * a.hd + lane * NH + e] = acc[r][e];
+      }
+    }
+  }
+}
+
+// Joins the records of the items that runs end in.  CTA c looks at the end of run c - 1: where it is the first that falls inside an item, the records
+// of that item are those of run c - 1 (its last) and of the runs behind, up to the one that has the item's end (their first).
+template <typename T, int RT, int KT>
+__global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ PagedArgs a, int ctas) {
+  __shared__ PagedPlanShared plan;
+  const int c = (int)blockIdx.x + 1, tid = threadIdx.x;
+  long long all;
+  int runs;
+  // all that this needs was there before the attention began
+  const bool any = paged_locate<128, RT, KT>(a, c - 1, ctas, plan, all, runs) && c < runs;
+  const PagedLoc prev = plan.loc[0], l = plan.loc[1];
+  pdl_wait();
+  if (!any || l.off == 0 || l.off == l.units) return;
+  if (prev.s == l.s && prev.off > 0) return;   // an end in front falls inside the same item
+  int n = 2;   // records
+  const long long tol = all / runs / 8, end = l.s + l.units;
+  while (c + n - 1 < runs && end - all * (c + n - 1) / runs > tol) ++n;
+  const PagedSeq s = paged_seq(a, l.b);
+  const int64_t rf = paged_record_floats(RT, a.hd);
+  const int pairs = min(RT, s.n * a.G - l.t * RT);
+  auto record = [&](int i) { return a.part + (i == 0 ? 2 * (int64_t)(c - 1) + 1 : 2 * (int64_t)(c - 1 + i)) * rf; };
+  for (int i = (int)blockIdx.y * 128 + tid; i < pairs * a.hd; i += 128 * (int)gridDim.y) {
+    const int row = i / a.hd, e = i % a.hd, p = l.t * RT + row;
+    float m = -INFINITY;
+    for (int k = 0; k < n; ++k) m = fmaxf(m, record(k)[2 * row]);
+    float sum = 0.0f, acc = 0.0f;
+    for (int k = 0; k < n; ++k) {
+      const float* r = record(k);
+      const float f = r[2 * row] == -INFINITY ? 0.0f : exp2f(r[2 * row] - m);
+      sum += r[2 * row + 1] * f;
+      acc += r[2 * RT + row * a.hd + e] * f;
+    }
+    reinterpret_cast<T*>(a.out)[(int64_t)(s.row0 + p / a.G) * a.o_row + (l.h * a.G + p % a.G) * a.o_head + e] = from_f<T>(sum == 0.0f ? 0.0f : acc / sum);
+  }
+}
+
+int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int KT, int ctas, cudaStream_t s) {
+  if (ctas < 2) return 1;
+  const dim3 grid(ctas - 1, RT >= 64 ? 4 : 1);
+  PdlScope chained(true);
+#define TSB_COMBINE(T, R, K) \
+  if (RT == R && KT == K) TSB_CUDA(launch_k(paged_combine_kernel<T, R, K>, grid, dim3(128), 0, s, a, ctas))
+#define TSB_COMBINES(T)      \
+  do {                       \
+    TSB_COMBINE(T, 4, 32);   \
+    TSB_COMBINE(T, 16, 32);  \
+  } while (0)
+  if (dtype == TSB200_F32) TSB_COMBINES(float);
+  else if (dtype == TSB200_F16) TSB_COMBINES(__half);
+  else TSB_COMBINES(__nv_bfloat16);
+#undef TSB_COMBINES
+#undef TSB_COMBINE
+  count_launch(device);
+  return check_launch("paged_combine");
+}
+
+// rows of a tile and CTAs of the kernel that serves a call: what its records take
+struct PagedChoice {
+  int RT, KT, ctas;
+};
+static PagedChoice paged_choose(int sm_count, int dtype, int64_t pairs, int hd) {
+  (void)dtype;
+  PagedChoice c;
+  c.KT = kFmaKeys;
+  c.RT = pairs <= 4 ? 4 : 16;
+  c.ctas = sm_count * (hd <= 128 ? 3 : 1);
+  return c;
+}
+constexpr int kSmCountMost = 160;   // of a compute capability 10.x device: workspace sizes must not need one
+static int64_t paged_ws_bytes(int dtype, int64_t pairs, int hd) {
+  const PagedChoice c = paged_choose(kSmCountMost, dtype, pairs, hd);
+  return 2LL * c.ctas * paged_record_floats(c.RT, hd) * 4;
+}
+
+template <typename T, int NH>
+static int launch_paged_fma_n(int device, DeviceState* st, const PagedArgs& a, const PagedChoice& c, cudaStream_t s) {
+  if (c.RT == 4) {
+    TSB_CUDA(cudaFuncSetAttribute(paged_fma_kernel<T, NH, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, fma_smem<T>(NH, 1)));
+    paged_fma_kernel<T, NH, 1><<<c.ctas, kFmaThreads, fma_smem<T>(NH, 1), s>>>(a);
+  } else {
+    TSB_CUDA(cudaFuncSetAttribute(paged_fma_kernel<T, NH, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, fma_smem<T>(NH, 4)));
+    paged_fma_kernel<T, NH, 4><<<c.ctas, kFmaThreads, fma_smem<T>(NH, 4), s>>>(a);
+  }
+  count_launch(device);
+  return check_launch("paged_fma");
+}
+template <typename T>
+static int launch_paged_fma(int device, DeviceState* st, const PagedArgs& a, const PagedChoice& c, cudaStream_t s) {
+  if (a.hd <= 32) return launch_paged_fma_n<T, 1>(device, st, a, c, s);
+  if (a.hd <= 64) return launch_paged_fma_n<T, 2>(device, st, a, c, s);
+  if (a.hd <= 128) return launch_paged_fma_n<T, 4>(device, st, a, c, s);
+  return launch_paged_fma_n<T, 8>(device, st, a, c, s);
+}
+
+static bool page_size_ok(int page, int* shift) {
+  for (int i = 3; i <= 8; ++i)
+    if (page == 1 << i) {
+      *shift = i;
+      return true;
+    }
+  return false;
+}
+
+}  // namespace tsb
+
+using namespace tsb;
+
+extern "C" {
+
+int TSB200_PagedPlan(int device, const int32_t* cached, const int32_t* fresh, int B, int page, int32_t* table, int64_t table_stride, int max_blocks, int32_t* held,
+                     int32_t* free_pages, int32_t* free_count, int num_pages, int32_t* lens, int32_t* starts, int32_t* slots, int32_t* positions, int rows,
+                     void* stream) {
+  PlanArgs a{};
+  TSB_CHECK(cached && fresh && table && held && free_pages && free_count && lens && starts && (rows == 0 || (slots && positions)), "paged_plan: null pointer");
+  TSB_CHECK(B >= 1 && B <= kPlanMaxB, "paged_plan: %d sequences, 1 to %d are served", B, kPlanMaxB);
+  TSB_CHECK(page_size_ok(page, &a.page_shift), "paged_plan: pages of %d tokens, a power of two from 8 to 256 is wanted", page);
+  TSB_CHECK(max_blocks >= 1 && table_stride >= max_blocks && (int64_t)B * max_blocks <= 0x7fffffff && (int64_t)max_blocks * page <= 0x7fffffff,
+            "paged_plan: a table of %d rows of %d pages (stride %lld)", B, max_blocks, (long long)table_stride);
+  TSB_CHECK(num_pages >= 0 && (int64_t)num_pages * page <= 0x7fffffff, "paged_plan: %d pages of %d tokens", num_pages, page);
+  TSB_CHECK(rows >= 0, "paged_plan: %d rows", rows);
+  KeepDevice keep;
+  DeviceState* st;
+  TSB_TRY(use_device(device, &st));
+  a.cached = cached; a.fresh = fresh; a.B = B; a.max_blocks = max_blocks; a.num_pages = num_pages; a.rows = rows; a.table = table; a.table_stride = table_stride;
+  a.held = held; a.free_pages = free_pages; a.free_count = free_count; a.lens = lens; a.starts = starts; a.slots = slots; a.positions = positions;
+  const int smem = 6 * B * (int)sizeof(int), ctas = 1;
+  if (smem > 40 * 1024) TSB_CUDA(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 6 * kPlanMaxB * (int)sizeof(int)));
+  paged_plan_kernel<<<ctas, kPlanThreads, smem, pick_stream(st, stream)>>>(a, ctas);
+  count_launch(device);
+  return check_launch("paged_plan");
+}
+
+int TSB200_QKNormRopePaged(int device, int dtype, void* q_out, int64_t o_row, int64_t o_head, const void* q, int64_t q_row, int64_t q_head, const void* k,
+                           int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* q_norm, const void* k_norm, float eps,
+                           const int32_t* positions, const int32_t* slots, int rows, int H, int Hkv, int hd, int rope_style, int rope_dims, double rope_base,
+                           void* cacheK, void* cacheV, int64_t c_page, int64_t c_head, int64_t c_tok, int num_pages, int page, void* stream) {
+  RopePagedArgs a{};
+  TSB_CHECK(rows >= 0 && H >= 1 && Hkv >= 1 && (int64_t)H + 2LL * Hkv <= 65536, "qk_norm_rope_paged: %d rows of %d and %d heads", rows, H, Hkv);
+  TSB_CHECK(dtype == TSB200_F32 || dtype == TSB200_F16 || dtype == TSB200_BF16, "qk_norm_rope_paged: unsupported dtype %d", dtype);
+  TSB_CHECK(hd >= 8 && hd % 8 == 0 && hd <= kRopeMaxHd, "qk_norm_rope_paged: head size %d, a multiple of 8 up to %d is wanted", hd, kRopeMaxHd);
+  TSB_CHECK(rope_style >= 0 && rope_style <= 2, "qk_norm_rope_paged: rotation style %d", rope_style);
+  TSB_CHECK(rope_style == 0 || (rope_dims >= 2 && rope_dims <= hd && rope_dims % (rope_style == 2 ? 16 : 2) == 0),
+            "qk_norm_rope_paged: %d rotated elements of %d (pairs: an even number, halves: a multiple of 16)", rope_dims, hd);
+  TSB_CHECK(rope_style == 0 || (rope_base > 0 && std::isfinite(rope_base)), "qk_norm_rope_paged: rotation base %g", rope_base);
+  TSB_CHECK(page_size_ok(page, &a.page_shift), "qk_norm_rope_paged: pages of %d tokens, a power of two from 8 to 256 is wanted", page);
+  TSB_CHECK(num_pages >= 0 && (int64_t)num_pages * page <= 0x7fffffff, "qk_norm_rope_paged: %d pages of %d tokens", num_pages, page);
+  if (rows == 0) return 1;
+  TSB_CHECK(q_out && q && k && v && slots && (positions || rope_style == 0) && cacheK && cacheV, "qk_norm_rope_paged: null pointer");
+  KeepDevice keep;
+  DeviceState* st;
+  TSB_TRY(use_device(device, &st));
+  a.out = q_out; a.q = q; a.k = k; a.v = v; a.q_norm = q_norm; a.k_norm = k_norm;
+  a.o_row = o_row; a.o_head = o_head; a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
+  a.eps = eps; a.positions = positions; a.slots = slots; a.rows = rows; a.H = H; a.Hkv = Hkv; a.hd = hd; a.rot = rope_style ? rope_dims : 0; a.style = rope_style;
+  a.first = 1.0 / 3.14159265358979323846;
+  a.ratio = rope_style ? std::pow(rope_base, -2.0 / rope_dims) : 1.0;
+  a.K = cacheK; a.V = cacheV; a.c_page = c_page; a.c_head = c_head; a.c_tok = c_tok; a.num_pages = num_pages;
+  const int V = 16 / (int)dtype_size(dtype);
+  const bool wide = ((o_row | o_head | q_row | q_head | k_row | k_head | v_row | v_head | c_page | c_head | c_tok) % V) == 0 &&
+                    (((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cacheK | (uintptr_t)cacheV) % 16) == 0;
+  a.rows_here = 1;
+  const dim3 grid((rows + a.rows_here - 1) / a.rows_here);
+  cudaStream_t s = pick_stream(st, stream);
+#define TSB_ROPE_PAGED(T)                                                                 \
+  do {                                                                                    \
+    if (wide) qk_norm_rope_paged_kernel<T, true><<<grid, kRopeThreads, 0, s>>>(a);        \
+    else qk_norm_rope_paged_kernel<T, false><<<grid, kRopeThreads, 0, s>>>(a);            \
+  } while (0)
+  if (dtype == TSB200_F32) TSB_ROPE_PAGED(float);
+  else if (dtype == TSB200_F16) TSB_ROPE_PAGED(__half);
+  else TSB_ROPE_PAGED(__nv_bfloat16);
+#undef TSB_ROPE_PAGED
+  count_launch(device);
+  return check_launch("qk_norm_rope_paged");
+}
+
+int64_t TSB200_PagedAttentionWorkspaceBytes(int dtype, int H, int Hkv, int hd, int max_new) {
+  if (H < 1 || Hkv < 1 || H % Hkv || hd < 8 || hd > 256 || max_new < 1) return 0;
+  return paged_ws_bytes(dtype, (int64_t)max_new * (H / Hkv), hd);
+}
+
+int TSB200_PagedAttention(int device, int dtype, void* out, int64_t o_row, int64_t o_head, const void* q, int64_t q_row, int64_t q_head, const void* cacheK,
+                          const void* cacheV, int64_t c_page, int64_t c_head, int64_t c_tok, int num_pages, int page, const int32_t* table, int64_t table_stride,
+                          int max_blocks, const int32_t* starts, const int32_t* lens, int B, int rows, int max_new, int H, int Hkv, int hd, float scale, int window,
+                          void* workspace, int64_t workspace_bytes, void* stream) {
+  PagedArgs a{};
+  TSB_CHECK(dtype == TSB200_F32 || dtype == TSB200_F16 || dtype == TSB200_BF16, "paged_attention: unsupported dtype %d", dtype);
+  TSB_CHECK(B >= 0 && rows >= 0 && max_new >= 1, "paged_attention: %d sequences, %d rows, at most %d new", B, rows, max_new);
+  TSB_CHECK(H >= 1 && Hkv >= 1 && H % Hkv == 0, "paged_attention: %d query heads over %d key / value heads", H, Hkv);
+  TSB_CHECK(hd >= 8 && hd % 8 == 0 && hd <= 256, "paged_attention: head size %d, a multiple of 8 up to 256 is wanted", hd);
+  TSB_CHECK(page_size_ok(page, &a.page_shift), "paged_attention: pages of %d tokens, a power of two from 8 to 256 is wanted", page);
+  TSB_CHECK(max_blocks >= 1 && table_stride >= max_blocks && (int64_t)max_blocks * page <= 0x7fffff00, "paged_attention: %d pages per sequence (stride %lld)", max_blocks,
+            (long long)table_stride);
+  TSB_CHECK(num_pages >= 0 && (int64_t)num_pages * page <= 0x7fffffff, "paged_attention: %d pages of %d tokens", num_pages, page);
+  TSB_CHECK((int64_t)rows * H <= 0x7fff0000, "paged_attention: %d rows of %d heads", rows, H);
+  TSB_CHECK(window >= 0, "paged_attention: window %d", window);
+  if (B == 0 || rows == 0) return 1;
+  TSB_CHECK(out && q && cacheK && cacheV && table && starts && lens, "paged_attention: null pointer");
+  const int V = 16 / (int)dtype_size(dtype);
+  TSB_CHECK(((o_row | o_head | q_row | q_head | c_page | c_head | c_tok) % V) == 0 && (((uintptr_t)out | (uintptr_t)q | (uintptr_t)cacheK | (uintptr_t)cacheV) % 16) == 0,
+            "paged_attention: pointers and strides must be multiples of 16 bytes");
+  KeepDevice keep;
+  DeviceState* st;
+  TSB_TRY(use_device(device, &st));
+  const int64_t pairs = (int64_t)max_new * (H / Hkv), need = paged_ws_bytes(dtype, pairs, hd);
+  TSB_CHECK(workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0, "paged_attention: a workspace of %lld bytes on a boundary of 16 is needed (%lld given)",
+            (long long)need, (long long)(workspace ? workspace_bytes : 0));
+  a.out = out; a.q = q; a.K = cacheK; a.V = cacheV; a.o_row = o_row; a.o_head = o_head; a.q_row = q_row; a.q_head = q_head;
+  a.c_page = c_page; a.c_head = c_head; a.c_tok = c_tok; a.table = table; a.table_stride = table_stride; a.max_blocks = max_blocks; a.num_pages = num_pages;
+  a.starts = starts; a.lens = lens; a.B = B; a.rows = rows; a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.hd = hd;
+  a.c = scale * 1.44269504088896340736f;
+  a.window = window; a.part = reinterpret_cast<float*>(workspace);
+  a.min_units = 4;
+  cudaStream_t s = pick_stream(st, stream);
+  const PagedChoice c = paged_choose(st->sm_count, dtype, pairs, hd);
+  TSB_CHECK(st->sm_count <= kSmCountMost, "paged_attention: %d SMs", st->sm_count);
+  if (dtype == TSB200_F32) TSB_TRY(launch_paged_fma<float>(device, st, a, c, s));
+  else if (dtype == TSB200_F16) TSB_TRY(launch_paged_fma<__half>(device, st, a, c, s));
+  else TSB_TRY(launch_paged_fma<__nv_bfloat16>(device, st, a, c, s));
+  return launch_paged_combine(device, dtype, a, c.RT, c.KT, c.ctas, s);
+}
+
+}  // extern "C"
