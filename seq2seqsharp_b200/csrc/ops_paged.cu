@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
 
 int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int KT, int ctas, cudaStream_t s) {
   if (ctas < 2) return 1;
-  const dim3 grid(ctas - 1, RT >= 64 ? 4 : 1);
+  const dim3 grid(ctas - 1, RT >= 64 ? 8 : 1);
   PdlScope chained(true);
 #define TSB_COMBINE(T, R, K) \
   if (RT == R && KT == K) TSB_CUDA(launch_k(paged_combine_kernel<T, R, K>, grid, dim3(128), 0, s, a, ctas))
@@ -478,6 +478,7 @@ int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int 
   do {                       \
     TSB_COMBINE(T, 4, 32);   \
     TSB_COMBINE(T, 16, 32);  \
+    TSB_COMBINE(T, 256, 128); \
   } while (0)
   if (dtype == TSB200_F32) TSB_COMBINES(float);
   else if (dtype == TSB200_F16) TSB_COMBINES(__half);
@@ -488,13 +489,21 @@ int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int 
   return check_launch("paged_combine");
 }
 
-// rows of a tile and CTAs of the kernel that serves a call: what its records take
+// The kernel that serves a call, its rows of a tile and its CTAs
 struct PagedChoice {
+  enum { FMA, TC } kind;
   int RT, KT, ctas;
 };
-static PagedChoice paged_choose(int sm_count, int dtype, int64_t pairs, int hd) {
-  (void)dtype;
+static PagedChoice paged_choose(int sm_count, int dtype, int64_t pairs, int hd, bool positive) {
   PagedChoice c;
+  if (is_16bit(dtype) && (hd == 64 || hd == 128) && positive) {
+    c.kind = PagedChoice::TC;
+    c.RT = 256;
+    c.KT = 128;
+    c.ctas = sm_count;
+    return c;
+  }
+  c.kind = PagedChoice::FMA;
   c.KT = kFmaKeys;
   c.RT = pairs <= 4 ? 4 : 16;
   c.ctas = sm_count * (hd <= 128 ? 3 : 1);
@@ -502,8 +511,13 @@ static PagedChoice paged_choose(int sm_count, int dtype, int64_t pairs, int hd) 
 }
 constexpr int kSmCountMost = 160;   // of a compute capability 10.x device: workspace sizes must not need one
 static int64_t paged_ws_bytes(int dtype, int64_t pairs, int hd) {
-  const PagedChoice c = paged_choose(kSmCountMost, dtype, pairs, hd);
-  return 2LL * c.ctas * paged_record_floats(c.RT, hd) * 4;
+  int64_t most = 0;
+  for (int positive = 0; positive < 2; ++positive) {
+    const PagedChoice c = paged_choose(kSmCountMost, dtype, pairs, hd, positive);
+    const int64_t n = 2LL * c.ctas * paged_record_floats(c.RT, hd) * 4;
+    if (n > most) most = n;
+  }
+  return most;
 }
 
 template <typename T, int NH>
@@ -646,8 +660,10 @@ int TSB200_PagedAttention(int device, int dtype, void* out, int64_t o_row, int64
   a.window = window; a.part = reinterpret_cast<float*>(workspace);
   a.min_units = 4;
   cudaStream_t s = pick_stream(st, stream);
-  const PagedChoice c = paged_choose(st->sm_count, dtype, pairs, hd);
+  // the kernels on tensor cores look for the largest score before it is scaled
+  const PagedChoice c = paged_choose(st->sm_count, dtype, pairs, hd, scale > 0);
   TSB_CHECK(st->sm_count <= kSmCountMost, "paged_attention: %d SMs", st->sm_count);
+  if (c.kind == PagedChoice::TC) return launch_paged_tc(device, st, dtype, a, s);
   if (dtype == TSB200_F32) TSB_TRY(launch_paged_fma<float>(device, st, a, c, s));
   else if (dtype == TSB200_F16) TSB_TRY(launch_paged_fma<__half>(device, st, a, c, s));
   else TSB_TRY(launch_paged_fma<__nv_bfloat16>(device, st, a, c, s));
