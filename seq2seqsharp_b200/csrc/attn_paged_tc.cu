@@ -5,10 +5,11 @@
 // operand; the products of one tile run behind the exponentials of the other (PV0(j) QK0(j+1) PV1(j) QK1(j+1)), and those of the next item's first keys
 // behind the output of this one's last.
 //
-// Rows come by cp.async, 16 bytes a lane, into the 128-byte swizzle that the products read: eight keys lie in one page whatever its size, so a warp looks up one
-// entry per eight rows; places behind the sequence's end or without a page become zeros (a weight of 0 times what the cache holds there would be
-// NaN where that is), any strides do, and a page may end anywhere in a tile.  The copies are generic-proxy writes: they report to the stage's mbarrier when they
-// have landed, and the issuing thread orders them before its products with a proxy fence.
+// Whole tiles of keys and values come by TMA tensor copies, a box per page (128-byte swizzle, any strides that are multiples of 16 bytes); an entry that names no
+// page is a coordinate outside of the map, which arrives as zeros.  The last tile of a sequence and the queries come by cp.async, 16 bytes a lane, into
+// the same swizzle, with zeros behind the end (a weight of 0 times what the cache holds there would be NaN where that is).  Those are generic-proxy writes: they
+// report to the stage's mbarrier when they have landed, and the issuing thread orders them before its products with a proxy fence.
+// (cp.async for every tile: 2.4 instead of 1.8 ms for two chunks of 2048 over 32768; its latency and issue do not fit the time of one tile.)
 #include "attn_tmem.cuh"
 #include "paged.cuh"
 
@@ -27,6 +28,13 @@ __device__ __forceinline__ void pt_cp16(uint32_t dst, const void* src, bool ther
 // one arrival of this thread when its copies so far have landed
 __device__ __forceinline__ void pt_arrive_copies(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(s_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void pt_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map),
+      "r"(s_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
 }
 
 // key tiles of the run that the two row tiles of an item need
@@ -48,7 +56,8 @@ __device__ __forceinline__ PtCounts pt_counts(const PagedArgs& a, const PagedRun
 
 // BX: 64-column boxes of a row (head size 64 BX); NS: key and value tiles in flight
 template <typename H, int BX, int NS>
-__global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_constant__ PagedArgs a) {
+__global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
+                                                                 const __grid_constant__ PagedArgs a) {
   constexpr int HD = BX * 64, CPR = HD / 8;   // 16-byte pieces of a row
   extern __shared__ __align__(1024) unsigned char pt_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)pt_raw + 1023) & ~(uintptr_t)1023);
@@ -58,6 +67,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
   uint64_t *q_full = v_empty + NS, *q_empty = q_full + 1, *s_full = q_empty + 1, *p_full = s_full + 2, *o_full = p_full + 2, *o_empty = o_full + 2, *drain = o_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   __shared__ PagedPlanShared plan;
+  __shared__ PagedRun wrun[12];   // of every warp: where it is (registers are the softmax's)
+  __shared__ unsigned gone_of[8]; // bit i: keys 8 i .. of the key tile have no page
   __shared__ int s_err;
 
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
@@ -67,7 +78,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
 
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      tc_mbar_init(&k_full[i], kPtCopiers);
+      tc_mbar_init(&k_full[i], kPtCopiers + 1);
       tc_mbar_init(&k_empty[i], 1);
       tc_mbar_init(&v_full[i], kPtCopiers);
       tc_mbar_init(&v_empty[i], 1);
@@ -95,8 +106,23 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
   const uint32_t tmem = *tmem_slot;
   pdl_trigger();
   volatile int* err = &s_err;
-  PagedRun run;
-  run.begin(a, plan, kPtTile);
+  PagedRun& run = wrun[w];
+  bool begun = false;
+  auto next_item = [&]() {   // by a whole warp
+    bool more = false;
+    __syncwarp();
+    if (lane == 0) {
+      PagedRun r = run;
+      if (begun) r.step(a);
+      else r.begin(a, plan, kPtTile);
+      more = r.next(a, plan, kPtTile, kPtKeys);
+      run = r;
+    }
+    begun = true;
+    more = __shfl_sync(0xffffffffu, more, 0);
+    __syncwarp();
+    return more;
+  };
 
   if (w >= 8) {
     pa_fewer_registers<kPtOtherRegs>();
@@ -107,29 +133,52 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
       constexpr int RP = 32 / CPR;                            // rows of a pass
       const int page_mask = (1 << a.page_shift) - 1;
       const uint32_t lane_box = (uint32_t)(lc >> 3) * kPtBox;
+      uint32_t place[8 / RP];                                 // of this lane's piece of the rows lr + RP i of eight
+#pragma unroll
+      for (int i = 0; i < 8 / RP; ++i) place[i] = lane_box + (lr + i * RP) * 128 + (((lc & 7) ^ (lr + i * RP)) << 4);
+      const int box_blocks = min(kPtKeys, 1 << a.page_shift) / 8;   // eights of keys in a box of the maps
       uint32_t kc = 0, qc = 0;
+      int ks = 0, vs = 0;                                     // tiles asked for so far
       bool ok = true;
-      for (; ok && run.next(a, plan, kPtTile, kPtKeys); run.step(a)) {
+      while (ok && next_item()) {
         const PtCounts n = pt_counts(a, run);
         if (n.most == 0) continue;
-        const PagedSeq& s = run.seq;
+        const PagedSeq s = run.seq;
         const int cap = min(s.len, a.max_blocks << a.page_shift);
         const int* table = a.table + run.b * a.table_stride;
         const int64_t head = run.h * a.c_head + lc * 8;
         // one tile of keys (or values): lane i < 16 knows the page of keys 8 i ..
-        auto load = [&](const void* src, uint32_t dst, int tile, int entry) {
-#pragma unroll 2
-          for (int blk = cw; blk < kPtKeys / 8; blk += 3) {
-            const int page = __shfl_sync(0xffffffffu, entry, blk);
-            const int key = tile * kPtKeys + blk * 8 + lr;
-            const H* p = reinterpret_cast<const H*>(src) + (page >= 0 ? page * a.c_page + head + (key & page_mask) * a.c_tok : 0);
-            const uint32_t d = dst + lane_box + blk * 1024;
+        auto load = [&](const CUtensorMap* map, const void* src, uint32_t dst, uint64_t* full, int tile, int entry) {
+          if ((tile + 1) * kPtKeys <= cap) {
+            // whole pages; one that there is not lies outside of the map and arrives as zeros
+            if (cw == 0) {
+              if (lane == 0) tc_mbar_expect_tx(full, BX * kPtBox);
+              __syncwarp();
+              const int page = __shfl_sync(0xffffffffu, entry, lane * box_blocks & 15);
+              if (lane * box_blocks < 16)
+#pragma unroll
+                for (int i = 0; i < BX; ++i)
+                  pt_load_4d(dst + i * kPtBox + lane * box_blocks * 1024, map, 64 * i, tile * kPtKeys & page_mask, run.h, page >= 0 ? page : a.num_pages, full);
+              if (lane > 0) pa_arrive(full);
+            } else {
+              pa_arrive(full);
+            }
+            return;
+          }
+          // the sequence's end: what lies behind it becomes zeros
+          const H* base = reinterpret_cast<const H*>(src) + head;
+          const int key0 = tile * kPtKeys + cw * 8 + lr;
+#pragma unroll 1
+          for (int b = cw; b < kPtKeys / 8; b += 3) {
+            const int page = __shfl_sync(0xffffffffu, entry, b), key = key0 + (b - cw) * 8;
+            const H* p = base + (page >= 0 ? page * a.c_page + (key & page_mask) * a.c_tok : 0);
 #pragma unroll
             for (int i = 0; i < 8 / RP; ++i) {
-              const int r = lr + i * RP;
-              pt_cp16(d + r * 128 + (((lc & 7) ^ r) << 4), page >= 0 && key + i * RP < cap ? p + (int64_t)(i * RP) * a.c_tok : reinterpret_cast<const H*>(src), page >= 0 && key + i * RP < cap);
+              const bool there = page >= 0 && key + i * RP < cap;
+              pt_cp16(dst + place[i] + b * 1024, there ? p + (int64_t)(i * RP) * a.c_tok : reinterpret_cast<const H*>(src), there);
             }
           }
+          pt_arrive_copies(full);
         };
         auto entry_of = [&](int tile) {
           const int key = tile * kPtKeys + (lane & 15) * 8;
@@ -139,11 +188,17 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
         auto load_k = [&](int j, int entry) {
           const uint32_t c = kc + j, st = c % NS;
           if (c >= NS && !tc_wait_or(s_u32(&k_empty[st]), (c / NS - 1) & 1, err, a.wait_limit)) return false;
-          load(a.K, sK + st * BX * kPtBox, run.k0 + j, entry);
-          pt_arrive_copies(&k_full[st]);
+          load(&mapK, a.K, sK + st * BX * kPtBox, &k_full[st], run.k0 + j, entry);
+          ks = c + 1;
+          const unsigned gone = __ballot_sync(0xffffffffu, entry < 0) & 0xffffu;
+          if (cw == 0 && lane == 0) {   // read behind the tile's scores; a tile NS + 1 in front has been weighed when this one's copies begin
+            gone_of[c & 7] = gone;
+            pa_arrive(&k_full[st]);
+          }
           return true;
         };
-        int entry = entry_of(run.k0), ahead = entry;
+        // entries are looked up two tiles ahead
+        int entry = entry_of(run.k0), next = entry_of(run.k0 + 1), ahead = next;
         ok = load_k(0, entry);
         if (ok && qc > 0) ok = tc_wait_or(s_u32(q_empty), (qc - 1) & 1, err, a.wait_limit);
         if (!ok) break;
@@ -158,19 +213,23 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
         }
         pt_arrive_copies(q_full);
         for (int j = 0; j < n.most; ++j) {
-          if (j + 1 < n.most) {
-            ahead = entry_of(run.k0 + j + 1);
-            if (!(ok = load_k(j + 1, ahead))) break;
-          }
+          ahead = entry_of(run.k0 + j + 2);
+          if (j + 1 < n.most && !(ok = load_k(j + 1, next))) break;
           const uint32_t c = kc + j, st = c % NS;
           if (c >= NS && !(ok = tc_wait_or(s_u32(&v_empty[st]), (c / NS - 1) & 1, err, a.wait_limit))) break;
-          load(a.V, sV + st * BX * kPtBox, run.k0 + j, entry);
-          pt_arrive_copies(&v_full[st]);
-          entry = ahead;
+          load(&mapV, a.V, sV + st * BX * kPtBox, &v_full[st], run.k0 + j, entry);
+          vs = c + 1;
+          entry = next;
+          next = ahead;
         }
         kc += n.most;
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");   // nothing is written to this shared memory any more, whichever wait has run out
+      // nothing is written to this shared memory any more, whichever wait has run out (tc_land)
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (cw == 0) {
+        tc_land(s_u32(k_full), NS, ks);
+        tc_land(s_u32(v_full), NS, vs);
+      }
     } else if (lane == 0) {
       // ---------------- products.  Instruction descriptors: fp32 accumulator, A K-major, 128 rows; K: N = 128 K-major; V: N = HD MN-major
       const uint32_t fmt = (1u << 4) | (Pair16<H>::kUmmaFormat << 7) | (Pair16<H>::kUmmaFormat << 10) | ((uint32_t)(kPtRows >> 4) << 24);
@@ -191,6 +250,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         return in;
       };
+      PagedRun run;
+      run.begin(a, plan, kPtTile);
       for (; ok && run.next(a, plan, kPtTile, kPtKeys); run.step(a)) {
         const PtCounts n = pt_counts(a, run);
         if (n.most == 0) continue;
@@ -232,37 +293,30 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
   } else {
     // ---------------- softmax: thread = row of tile t
     pa_more_registers<kPtSoftmaxRegs>();
-    const int t = w >> 2, row = tid & 127, page_shift = a.page_shift;
+    const int t = w >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((w & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + t * kPtKeys, tO = tmem + lanes + 2 * kPtKeys + t * HD;
     const float c = a.c;
-    uint32_t sc = 0, oc = 0;
+    uint32_t sc = 0, oc = 0, kc = 0;
     bool ok = true;
-    for (; ok && run.next(a, plan, kPtTile, kPtKeys); run.step(a)) {
-      const PagedSeq& s = run.seq;
-      const int p0 = run.t * kPtTile + t * kPtRows, pairs = s.n * a.G, p = p0 + row;
-      if (p0 >= pairs) continue;
+    while (ok && next_item()) {
       const PtCounts counts = pt_counts(a, run);
-      const int n = t ? counts.n[1] : counts.n[0];
-      const int cap = min(s.len, a.max_blocks << page_shift), base = s.len - s.n;
-      const bool live = p < pairs;
-      const int pos = base + p / a.G, head = run.h * a.G + p % a.G;
+      const int n = t ? counts.n[1] : counts.n[0], k0_item = run.k0;
+      const uint32_t c0 = kc;
+      kc += counts.most;
       // keys [lo, lim) are visible (a row without a query: zeros, never stored); of the warp: the smallest lim, the largest lo
-      const int lim = live ? min(pos + 1, cap) : 0x7fffffff, lo = live && a.window > 0 ? pos - a.window + 1 : 0;
-      const int wp = p0 + (row & ~31);
-      const int warp_lim = min(base + wp / a.G + 1, cap);
-      const int warp_lo = a.window > 0 ? base + min(wp + 31, pairs - 1) / a.G - a.window + 1 : 0;
-      const int* table = a.table + run.b * a.table_stride;
-      auto hidden = [&](int tile) {   // bit i: keys 8 i .. of the tile have no page
-        const int key = tile * kPtKeys + (lane & 15) * 8;
-        const int page = key < cap ? table[key >> page_shift] : 0;
-        return page < 0 || page >= a.num_pages;
-      };
-      bool none = n > 0 && hidden(run.k0);
+      int lim, lo, warp_lim, warp_lo;
+      {
+        const int p0 = run.t * kPtTile + t * kPtRows, pairs = run.seq.n * a.G, p = p0 + row;
+        if (p0 >= pairs) continue;
+        const int cap = min(run.seq.len, a.max_blocks << a.page_shift), base = run.seq.len - run.seq.n, pos = base + p / a.G, wp = p0 + (row & ~31);
+        lim = p < pairs ? min(pos + 1, cap) : 0x7fffffff;
+        lo = p < pairs && a.window > 0 ? pos - a.window + 1 : 0;
+        warp_lim = min(base + wp / a.G + 1, cap);
+        warp_lo = a.window > 0 ? base + min(wp + 31, pairs - 1) / a.G - a.window + 1 : 0;
+      }
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; j < n; ++j) {
-        const unsigned gone = __ballot_sync(0xffffffffu, none) & 0xffffu;
-        if (j + 1 < n) none = hidden(run.k0 + j + 1);
         ok = __all_sync(0xffffffffu, pa_wait(&s_full[t], sc & 1, err, a.wait_limit));
         if (!ok) break;
         ++sc;
@@ -272,7 +326,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
         for (int q = 0; q < 4; ++q) pa_ld32(tS + q * 32, x[q]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) pa_ld_wait(x[q]);
-        const int k0 = (run.k0 + j) * kPtKeys;
+        const unsigned gone = gone_of[(c0 + j) & 7];
+        const int k0 = (k0_item + j) * kPtKeys;
         if (k0 + kPtKeys > warp_lim || k0 < warp_lo) {
           const int from = lo - k0, to = lim - k0;
 #pragma unroll
@@ -341,7 +396,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
         ++oc;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
-      const bool whole = run.first && run.last;
+      const PagedSeq s = run.seq;
+      const int p = run.t * kPtTile + t * kPtRows + row, head = run.h * a.G + p % a.G;
+      const bool live = p < s.n * a.G, whole = run.first && run.last;
       float* rec = a.part + (2 * (int64_t)blockIdx.x + (run.first ? 1 : 0)) * paged_record_floats(kPtTile, HD);
       const int r = t * kPtRows + row;
       if (!whole && live) *reinterpret_cast<float2*>(rec + 2 * r) = make_float2(m == -INFINITY ? m : m * c, l);   // the combine's maxima are in units of exp2
@@ -392,6 +449,26 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
   if (tid == 0 && s_err && a.error) *a.error = 1;
 }
 
+// a box: 64 columns of up to 128 tokens of a page
+static int pt_map(CUtensorMap* map, int dtype, const void* base, const PagedArgs& a) {
+  EncodeTiledFn enc = get_encode();
+  TSB_CHECK(enc, "paged_attention: the driver has no cuTensorMapEncodeTiled");
+  const cuuint64_t page = (cuuint64_t)1 << a.page_shift;
+  const cuuint64_t dims[4] = {(cuuint64_t)a.hd, page, (cuuint64_t)a.Hkv, (cuuint64_t)a.num_pages};
+  // the stride of a single head or page means nothing
+  const cuuint64_t strides[3] = {(cuuint64_t)a.c_tok * 2, (cuuint64_t)(a.Hkv > 1 ? a.c_head : a.hd) * 2, (cuuint64_t)(a.num_pages > 1 ? a.c_page : a.hd) * 2};
+  const cuuint32_t box[4] = {64, page < kPtKeys ? (cuuint32_t)page : kPtKeys, 1, 1}, el[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, dtype == TSB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, el,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TSB_CHECK(r == CUDA_SUCCESS, "paged_attention: cuTensorMapEncodeTiled failed with %d", (int)r);
+  return 1;
+}
+// strides that a tensor map takes
+bool paged_tc_strides(const PagedArgs& a) {
+  const int64_t most = (int64_t)1 << 39;   // bytes below 2^40
+  return a.num_pages > 0 && a.c_tok > 0 && a.c_tok < most && (a.Hkv == 1 || (a.c_head > 0 && a.c_head < most)) && (a.num_pages == 1 || (a.c_page > 0 && a.c_page < most));
+}
+
 template <typename H, int BX, int NS>
 static int pt_launch(int device, DeviceState* st, const PagedArgs& a, cudaStream_t s) {
   constexpr int smem = pt_smem(BX, NS);
@@ -401,7 +478,11 @@ static int pt_launch(int device, DeviceState* st, const PagedArgs& a, cudaStream
     TSB_CUDA(cudaFuncSetAttribute(paged_tc_kernel<H, BX, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     done[device] = true;
   }
-  paged_tc_kernel<H, BX, NS><<<st->sm_count, kPtThreads, smem, s>>>(a);
+  CUtensorMap mk, mv;
+  constexpr int dtype = Pair16<H>::kBf16 ? TSB200_BF16 : TSB200_F16;
+  TSB_TRY(pt_map(&mk, dtype, a.K, a));
+  TSB_TRY(pt_map(&mv, dtype, a.V, a));
+  paged_tc_kernel<H, BX, NS><<<st->sm_count, kPtThreads, smem, s>>>(mk, mv, a);
   count_launch(device);
   return check_launch("paged_tc");
 }
@@ -410,6 +491,8 @@ int launch_paged_tc(int device, DeviceState* st, int dtype, PagedArgs a, cudaStr
   a.wait_limit = tc_wait_limit();
   a.error = tc_error_word(device);
   a.min_units = 4;
+  a.snap = 4;
+  a.start = 3;
   st->waits = true;
   if (dtype == TSB200_F16) {
     if (a.hd == 64) TSB_TRY((pt_launch<__half, 1, 4>(device, st, a, s)));
@@ -418,7 +501,7 @@ int launch_paged_tc(int device, DeviceState* st, int dtype, PagedArgs a, cudaStr
     if (a.hd == 64) TSB_TRY((pt_launch<__nv_bfloat16, 1, 4>(device, st, a, s)));
     else TSB_TRY((pt_launch<__nv_bfloat16, 2, 2>(device, st, a, s)));
   }
-  return launch_paged_combine(device, dtype, a, kPtTile, kPtKeys, st->sm_count, s);
+  return launch_paged_combine(device, dtype, a, kPtTile, st->sm_count, s);
 }
 
 }  // namespace tsb

@@ -432,59 +432,54 @@ __global__ void __launch_bounds__(kFmaThreads) paged_fma_kernel(const __grid_con
   }
 }
 
-// Joins the records of the items that runs end in.  CTA c looks at the end of run c - 1: where it is the first that falls inside an item, the records
-// of that item are those of run c - 1 (its last) and of the runs behind, up to the one that has the item's end (their first).
-template <typename T, int RT, int KT>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ PagedArgs a, int ctas) {
-  __shared__ PagedPlanShared plan;
-  const int c = (int)blockIdx.x + 1, tid = threadIdx.x;
-  long long all;
-  int runs;
-  // all that this needs was there before the attention began
-  const bool any = paged_locate<128, RT, KT>(a, c - 1, ctas, plan, all, runs) && c < runs;
-  const PagedLoc prev = plan.loc[0], l = plan.loc[1];
+// Joins the records of the items that runs end in, four elements of a row per thread.  What bounds it: latency of two dependent reads, then the records.
+constexpr int kJoinThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) paged_combine_kernel(const __grid_constant__ PagedArgs a, int RT) {
+  const int c = (int)blockIdx.x + 1;
   pdl_wait();
-  if (!any || l.off == 0 || l.off == l.units) return;
-  if (prev.s == l.s && prev.off > 0) return;   // an end in front falls inside the same item
-  int n = 2;   // records
-  const long long tol = all / runs / 8, end = l.s + l.units;
-  while (c + n - 1 < runs && end - all * (c + n - 1) / runs > tol) ++n;
-  const PagedSeq s = paged_seq(a, l.b);
+  const int4 j = __ldcg(&a.joins[2 * c]);
+  if (j.x == 0) return;
+  const int h = __ldcg(&a.joins[2 * c + 1]).x, n = j.x, quads = a.hd / 4;
+  const int i = (int)blockIdx.y * kJoinThreads + (int)threadIdx.x, row = i / quads, e = (i - row * quads) * 4;
+  if (row >= j.w) return;
   const int64_t rf = paged_record_floats(RT, a.hd);
-  const int pairs = min(RT, s.n * a.G - l.t * RT);
-  auto record = [&](int i) { return a.part + (i == 0 ? 2 * (int64_t)(c - 1) + 1 : 2 * (int64_t)(c - 1 + i)) * rf; };
-  for (int i = (int)blockIdx.y * 128 + tid; i < pairs * a.hd; i += 128 * (int)gridDim.y) {
-    const int row = i / a.hd, e = i % a.hd, p = l.t * RT + row;
-    float m = -INFINITY;
-    for (int k = 0; k < n; ++k) m = fmaxf(m, record(k)[2 * row]);
-    float sum = 0.0f, acc = 0.0f;
-    for (int k = 0; k < n; ++k) {
-      const float* r = record(k);
-      const float f = r[2 * row] == -INFINITY ? 0.0f : exp2f(r[2 * row] - m);
-      sum += r[2 * row + 1] * f;
-      acc += r[2 * RT + row * a.hd + e] * f;
-    }
-    reinterpret_cast<T*>(a.out)[(int64_t)(s.row0 + p / a.G) * a.o_row + (l.h * a.G + p % a.G) * a.o_head + e] = from_f<T>(sum == 0.0f ? 0.0f : acc / sum);
-  }
+  const float* first = a.part + (2 * (int64_t)(c - 1) + 1) * rf;   // of run c - 1: its last; of the runs behind: their first
+  const float* other = a.part + 2 * (int64_t)c * rf;
+  float m = __ldcg(first + 2 * row);
+#pragma unroll 4
+  for (int k = 0; k < n - 1; ++k) m = fmaxf(m, __ldcg(other + 2 * k * rf + 2 * row));
+  const float from = fmaxf(m, -FLT_MAX);
+  float sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto add = [&](const float* r) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(r + 2 * row));
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(r + 2 * RT + (int64_t)row * a.hd + e));
+    const float f = exp2f(ml.x - from);
+    sum += ml.y * f;
+    acc[0] += x.x * f;
+    acc[1] += x.y * f;
+    acc[2] += x.z * f;
+    acc[3] += x.w * f;
+  };
+  add(first);
+#pragma unroll 4
+  for (int k = 0; k < n - 1; ++k) add(other + 2 * k * rf);
+  const int p = j.z + row;
+  T* out = reinterpret_cast<T*>(a.out) + (int64_t)(j.y + p / a.G) * a.o_row + (int64_t)(h * a.G + p % a.G) * a.o_head + e;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) acc[k] *= inv;
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  else *reinterpret_cast<uint2*>(out) = make_uint2(Pair16<T>::put(acc[0], acc[1]), Pair16<T>::put(acc[2], acc[3]));
 }
 
-int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int KT, int ctas, cudaStream_t s) {
+int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int ctas, cudaStream_t s) {
   if (ctas < 2) return 1;
-  const dim3 grid(ctas - 1, RT >= 64 ? 8 : 1);
+  const dim3 grid(ctas - 1, (RT * a.hd / 4 + kJoinThreads - 1) / kJoinThreads);
   PdlScope chained(true);
-#define TSB_COMBINE(T, R, K) \
-  if (RT == R && KT == K) TSB_CUDA(launch_k(paged_combine_kernel<T, R, K>, grid, dim3(128), 0, s, a, ctas))
-#define TSB_COMBINES(T)      \
-  do {                       \
-    TSB_COMBINE(T, 4, 32);   \
-    TSB_COMBINE(T, 16, 32);  \
-    TSB_COMBINE(T, 256, 128); \
-  } while (0)
-  if (dtype == TSB200_F32) TSB_COMBINES(float);
-  else if (dtype == TSB200_F16) TSB_COMBINES(__half);
-  else TSB_COMBINES(__nv_bfloat16);
-#undef TSB_COMBINES
-#undef TSB_COMBINE
+  if (dtype == TSB200_F32) TSB_CUDA(launch_k(paged_combine_kernel<float>, grid, dim3(kJoinThreads), 0, s, a, RT));
+  else if (dtype == TSB200_F16) TSB_CUDA(launch_k(paged_combine_kernel<__half>, grid, dim3(kJoinThreads), 0, s, a, RT));
+  else TSB_CUDA(launch_k(paged_combine_kernel<__nv_bfloat16>, grid, dim3(kJoinThreads), 0, s, a, RT));
   count_launch(device);
   return check_launch("paged_combine");
 }
@@ -514,7 +509,7 @@ static int64_t paged_ws_bytes(int dtype, int64_t pairs, int hd) {
   int64_t most = 0;
   for (int positive = 0; positive < 2; ++positive) {
     const PagedChoice c = paged_choose(kSmCountMost, dtype, pairs, hd, positive);
-    const int64_t n = 2LL * c.ctas * paged_record_floats(c.RT, hd) * 4;
+    const int64_t n = 2LL * c.ctas * (paged_record_floats(c.RT, hd) * 4 + (int64_t)sizeof(int4));
     if (n > most) most = n;
   }
   return most;
@@ -657,17 +652,20 @@ int TSB200_PagedAttention(int device, int dtype, void* out, int64_t o_row, int64
   a.c_page = c_page; a.c_head = c_head; a.c_tok = c_tok; a.table = table; a.table_stride = table_stride; a.max_blocks = max_blocks; a.num_pages = num_pages;
   a.starts = starts; a.lens = lens; a.B = B; a.rows = rows; a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.hd = hd;
   a.c = scale * 1.44269504088896340736f;
-  a.window = window; a.part = reinterpret_cast<float*>(workspace);
-  a.min_units = 4;
-  cudaStream_t s = pick_stream(st, stream);
+  a.window = window; cudaStream_t s = pick_stream(st, stream);
   // the kernels on tensor cores look for the largest score before it is scaled
-  const PagedChoice c = paged_choose(st->sm_count, dtype, pairs, hd, scale > 0);
+  const PagedChoice c = paged_choose(st->sm_count, dtype, pairs, hd, scale > 0 && paged_tc_strides(a));
   TSB_CHECK(st->sm_count <= kSmCountMost, "paged_attention: %d SMs", st->sm_count);
+  a.joins = reinterpret_cast<int4*>(workspace);
+  a.part = reinterpret_cast<float*>(a.joins + 2 * c.ctas);
+  a.min_units = 4;
+  a.snap = 1;
+  a.start = 1;
   if (c.kind == PagedChoice::TC) return launch_paged_tc(device, st, dtype, a, s);
   if (dtype == TSB200_F32) TSB_TRY(launch_paged_fma<float>(device, st, a, c, s));
   else if (dtype == TSB200_F16) TSB_TRY(launch_paged_fma<__half>(device, st, a, c, s));
   else TSB_TRY(launch_paged_fma<__nv_bfloat16>(device, st, a, c, s));
-  return launch_paged_combine(device, dtype, a, c.RT, c.KT, c.ctas, s);
+  return launch_paged_combine(device, dtype, a, c.RT, c.ctas, s);
 }
 
 }  // extern "C"

@@ -4,11 +4,12 @@
 // so row i of n sees the keys j <= lens[b] - n + i, and with a window only j > that position - window.  Key j lies in page table[b][j / page]
 // at place j % page.  Entries that name no page hide their keys, and a row that sees no key is written as zeros.
 //
-// Work: an item is (sequence, tile of RT of its n * G (query, head) pairs, KV head), a unit a tile of KT of the item's keys.  What is known on the
+// Work: an item is (sequence, tile of RT of its n * G (query, head) pairs, KV head), a unit a tile of KT of the item's keys, or the time of one: an item
+// begins with `start` units for what it costs beside its keys.  What is known on the
 // host are bounds only (a captured call is replayed with other lengths), so each CTA reads the lengths, numbers all units and takes an equal run of
 // them: one sequence of any length, or sequences of very different lengths, keep every SM busy.  A run may begin or end inside an item; such a
 // CTA leaves its maximum, sum and accumulator in the workspace and paged_combine_kernel joins them in the order of the runs (the same
-// order whatever CTA ends first).  Ends within an eighth of a run of an item's end are moved there, since a record costs about a unit to write and to read.
+// order whatever CTA ends first).  Ends within a 32nd of a run of an item's end, or within `snap` units, are moved there: a record has to be written and read.
 #pragma once
 #include "kernels.cuh"
 
@@ -27,7 +28,9 @@ struct PagedArgs {
   float c;                         // scale * log2(e)
   int window;                      // 0: none
   float* part;                     // records: paged_record_floats() each, two per CTA
-  int min_units;                   // no run is shorter
+  int4* joins;                     // two per CTA: the item that the run's beginning is the first to fall into (PagedJoin)
+  int min_units, snap;             // no run is shorter; ends this near to an item's are moved there (at least `start`)
+  int start;                       // units that an item costs beside those of its keys
   unsigned wait_limit;
   int* error;
 };
@@ -59,11 +62,16 @@ __device__ __forceinline__ PagedTile paged_tile(const PagedArgs& a, const PagedS
   r.units = max(1, (hi + KT - 1) / KT - r.k0);   // a tile without keys is still written
   return r;
 }
-// where a run begins or ends: unit `off` (0 .. units) of an item whose first unit is number `s` of all
+// where a run begins or ends: key tile `off` (0 .. units) of an item whose first unit is number `s` of all
 struct PagedLoc {
   int b, t, h, off, units;
   long long s;
 };
+// (records, first row of the sequence, first pair of the item, its pairs), (KV head, -, -, -)
+struct PagedJoin {
+  int records, row0, p0, pairs, h, pad[3];
+};
+static_assert(sizeof(PagedJoin) == 2 * sizeof(int4), "a join is written as two pieces");
 struct PagedPlanShared {
   long long warp[32], base[2];
   PagedLoc loc[2];
@@ -91,13 +99,59 @@ __device__ __forceinline__ long long paged_block_scan(long long v, PagedPlanShar
   all = total;
   return before + x - v;
 }
+// Units of this lane's sequence (b, or none).  Few tiles are added up by the lane, many (a chunk) by the warp.
+constexpr int kPagedFewTiles = 4;
 __device__ __forceinline__ long long paged_seq_units(const PagedArgs& a, int b, int RT, int KT) {
-  if (b >= a.B) return 0;
-  const PagedSeq s = paged_seq(a, b);
-  const int tiles = (s.n * a.G + RT - 1) / RT;
-  long long u = 0;
-  for (int t = 0; t < tiles; ++t) u += paged_tile(a, s, t, RT, KT).units;
-  return u * a.Hkv;
+  PagedSeq s{0, 0, 0};
+  if (b < a.B) s = paged_seq(a, b);
+  const int tiles = (s.n * a.G + RT - 1) / RT, lane = threadIdx.x & 31;
+  int u = 0;
+  if (tiles <= kPagedFewTiles)
+    for (int t = 0; t < tiles; ++t) u += paged_tile(a, s, t, RT, KT).units + a.start;
+  long long mine = u;
+  for (unsigned many = __ballot_sync(0xffffffffu, tiles > kPagedFewTiles); many; many &= many - 1) {
+    const int src = __ffs(many) - 1, nt = __shfl_sync(0xffffffffu, tiles, src);
+    const PagedSeq q{0, __shfl_sync(0xffffffffu, s.n, src), __shfl_sync(0xffffffffu, s.len, src)};
+    long long x = 0;
+    for (int t = lane; t < nt; t += 32) x += paged_tile(a, q, t, RT, KT).units + a.start;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (lane == src) mine = x;
+  }
+  return mine * a.Hkv;
+}
+// Unit x of all, where sequence b's first is s: tile, head and place in the item.  By a whole warp, for its lane `src`'s sequence.
+__device__ __forceinline__ PagedLoc paged_find(const PagedArgs& a, int b, long long s, long long x, long long tol, int RT, int KT) {
+  const int lane = threadIdx.x & 31;
+  const PagedSeq q = paged_seq(a, b);
+  for (int t0 = 0;; t0 += 32) {
+    const bool there = (long long)(t0 + lane) * RT < (long long)q.n * a.G;
+    const int u = there ? paged_tile(a, q, t0 + lane, RT, KT).units + a.start : 0;   // of one head
+    long long end = (long long)u * a.Hkv;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += y;
+    }
+    const unsigned in = __ballot_sync(0xffffffffu, there && x < s + end);
+    if (in == 0 && __any_sync(0xffffffffu, there)) {
+      s += __shfl_sync(0xffffffffu, end, 31);
+      continue;
+    }
+    const int src = in ? __ffs(in) - 1 : 0;
+    PagedLoc l;
+    l.b = b;
+    l.t = t0 + src;
+    const int cost = __shfl_sync(0xffffffffu, u, src);
+    const long long at = s + __shfl_sync(0xffffffffu, end, src) - (long long)cost * a.Hkv;
+    l.h = (int)((x - at) / max(cost, 1));
+    l.s = at + (long long)l.h * cost;
+    l.units = cost - a.start;
+    const int in_item = (int)(x - l.s), rest = cost - in_item;
+    if (in_item <= a.start || (in_item <= tol && in_item <= rest)) l.off = 0;
+    else l.off = rest <= tol ? l.units : in_item - a.start;
+    return l;
+  }
 }
 // Run `c` of the plan: sh.loc[0] and sh.loc[1] where it begins and ends.  Returns whether there is such a run.  `all` / `runs`: units and runs of
 // the whole call.  All threads of the CTA.
@@ -105,13 +159,15 @@ template <int NT, int RT, int KT>
 __device__ __forceinline__ bool paged_locate(const PagedArgs& a, int c, int ctas, PagedPlanShared& sh, long long& all, int& runs) {
   const int tid = threadIdx.x;
   long long mine = paged_seq_units(a, tid, RT, KT), total = mine;
-  for (int b = tid + NT; b < a.B; b += NT) total += paged_seq_units(a, b, RT, KT);
+  for (int b0 = NT; b0 < a.B; b0 += NT) total += paged_seq_units(a, b0 + tid, RT, KT);
   paged_block_scan<NT>(total, sh, all);
-  if (all == 0) return false;
   const long long most = all / a.min_units;
   runs = (int)(most < 1 ? 1 : (most < ctas ? most : ctas));
-  if (c >= runs) return false;
-  const long long tol = all / runs / 8;
+  if (all == 0 || c >= runs) {
+    if (tid == 0) a.joins[2 * c] = make_int4(0, 0, 0, 0);
+    return false;
+  }
+  const long long tol = max(all / runs / 32, (long long)a.snap);
   const long long x[2] = {all * c / runs, all * (c + 1) / runs};
   if (tid == 0) sh.loc[1] = PagedLoc{a.B, 0, 0, 0, 0, all};
   long long base = 0;
@@ -121,26 +177,34 @@ __device__ __forceinline__ bool paged_locate(const PagedArgs& a, int c, int ctas
     long long here;
     const long long s = base + paged_block_scan<NT>(mine, sh, here);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (mine > 0 && x[i] >= s && x[i] < s + mine) {
-        const PagedSeq q = paged_seq(a, b);
-        long long at = s;
-        for (int t = 0;; ++t) {
-          const int u = paged_tile(a, q, t, RT, KT).units;
-          if (x[i] < at + (long long)u * a.Hkv) {
-            const int h = (int)((x[i] - at) / u);
-            PagedLoc l{b, t, h, (int)(x[i] - at - (long long)h * u), u, at + (long long)h * u};
-            if (l.off <= tol) l.off = 0;
-            else if (u - l.off <= tol) l.off = u;
-            sh.loc[i] = l;
-            break;
-          }
-          at += (long long)u * a.Hkv;
-        }
+    for (int i = 0; i < 2; ++i) {
+      const unsigned hit = __ballot_sync(0xffffffffu, mine > 0 && x[i] >= s && x[i] < s + mine);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        const PagedLoc l = paged_find(a, __shfl_sync(0xffffffffu, b, src), __shfl_sync(0xffffffffu, s, src), x[i], tol, RT, KT);
+        if ((tid & 31) == 0) sh.loc[i] = l;
       }
+    }
     base += here;
   }
   __syncthreads();
+  if (tid == 0) {
+    // the records of an item that runs end in: those of the run in front of the first such end (its last) and of the runs behind, up to the one
+    // that has the item's end (their first)
+    const PagedLoc l = sh.loc[0];
+    PagedJoin j{};
+    if (l.off > 0 && l.off < l.units && all * (c - 1) / runs - l.s <= max(tol, (long long)a.start)) {
+      const PagedSeq q = paged_seq(a, l.b);
+      j.records = 2;
+      while (c + j.records - 1 < runs && l.s + a.start + l.units - all * (c + j.records - 1) / runs > tol) ++j.records;
+      j.row0 = q.row0;
+      j.p0 = l.t * RT;
+      j.pairs = min(RT, q.n * a.G - l.t * RT);
+      j.h = l.h;
+    }
+    a.joins[2 * c] = make_int4(j.records, j.row0, j.p0, j.pairs);
+    a.joins[2 * c + 1] = make_int4(j.h, 0, 0, 0);
+  }
   return true;
 }
 // Items of a run, one after the other.  done() when there is none left; [k0, k1) the key tiles of the item that are this run's.
@@ -188,9 +252,10 @@ struct PagedRun {
   }
 };
 
-int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int KT, int ctas, cudaStream_t s);
+int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int ctas, cudaStream_t s);
 // kernels for 16-bit types and head sizes 64 and 128: rows of few pairs per sequence on mma.sync, chunks on tcgen05
 int launch_paged_mma(int device, DeviceState* st, int dtype, PagedArgs a, int pairs, cudaStream_t s);
+bool paged_tc_strides(const PagedArgs& a);
 int launch_paged_tc(int device, DeviceState* st, int dtype, PagedArgs a, cudaStream_t s);
 
 }  // namespace tsb
