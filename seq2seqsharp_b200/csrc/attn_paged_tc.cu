@@ -15,7 +15,7 @@
 
 namespace tsb {
 
-constexpr int kPtThreads = 384, kPtRows = 128, kPtKeys = 128, kPtTile = 2 * kPtRows, kPtBox = kPtKeys * 128, kPtCopiers = 96;
+constexpr int kPtThreads = 384, kPtRows = 128, kPtKeys = 128, kPtTile = 2 * kPtRows, kPtBox = kPtKeys * 128, kPtCopiers = 96, kPtAhead = 4;
 // registers per thread: 384 x 168 at launch
 constexpr int kPtSoftmaxRegs = 208, kPtOtherRegs = 88;
 static_assert(256 * kPtSoftmaxRegs + 128 * kPtOtherRegs <= kPtThreads * 168, "the warpgroups' registers come out of the launch's");
@@ -36,6 +36,15 @@ __device__ __forceinline__ void pt_load_4d(uint32_t dst, const CUtensorMap* map,
       "r"(s_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
+__device__ __forceinline__ void pt_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map),
+      "r"(s_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void pt_prefetch_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
 
 // key tiles of the run that the two row tiles of an item need
 struct PtCounts {
@@ -47,7 +56,7 @@ __device__ __forceinline__ PtCounts pt_counts(const PagedArgs& a, const PagedRun
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int p0 = r.t * kPtTile + t * kPtRows, p1 = min(pairs, p0 + kPtRows) - 1;
-    const int hi = min(r.seq.len - r.seq.n + p1 / a.G + 1, cap);
+    const int hi = min(r.seq.len - r.seq.n + a.by_G(p1) + 1, cap);
     c.n[t] = p0 < pairs ? max(0, min((hi + kPtKeys - 1) / kPtKeys, r.k1) - r.k0) : 0;
   }
   c.most = max(c.n[0], c.n[1]);
@@ -57,7 +66,7 @@ __device__ __forceinline__ PtCounts pt_counts(const PagedArgs& a, const PagedRun
 // BX: 64-column boxes of a row (head size 64 BX); NS: key and value tiles in flight
 template <typename H, int BX, int NS>
 __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
-                                                                 const __grid_constant__ PagedArgs a) {
+                                                                 const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ PagedArgs a, int q_boxes) {
   constexpr int HD = BX * 64, CPR = HD / 8;   // 16-byte pieces of a row
   extern __shared__ __align__(1024) unsigned char pt_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)pt_raw + 1023) & ~(uintptr_t)1023);
@@ -204,15 +213,45 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
         if (!ok) break;
         ++qc;
         const int p0 = run.t * kPtTile, pairs = s.n * a.G;
+        if (q_boxes) {
+          // whole queries to a tile: boxes of G heads (rows behind the sequence's are another's, and are not stored)
+          if (cw == 0) {
+            const int tiles = n.n[1] > 0 ? 2 : 1;
+            if (lane == 0) tc_mbar_expect_tx(q_full, tiles * BX * kPtBox);
+            __syncwarp();
+            if (lane < tiles * BX) pt_load_3d(sQ + lane * kPtBox, &mapQ, lane % BX * 64, run.h * a.G, s.row0 + a.by_G(p0 + lane / BX * kPtRows), q_full);
+            if (lane > 0) pa_arrive(q_full);
+          } else {
+            pa_arrive(q_full);
+          }
+        } else {
         for (int r0 = cw * RP; r0 < (n.n[1] > 0 ? kPtTile : kPtRows); r0 += 3 * RP) {
           const int r = r0 + lr, p = p0 + r;
           const bool there = p < pairs;
           const H* src = reinterpret_cast<const H*>(a.q);
-          if (there) src += (int64_t)(s.row0 + p / a.G) * a.q_row + (int64_t)(run.h * a.G + p % a.G) * a.q_head + lc * 8;
+          if (there) src += (int64_t)(s.row0 + a.by_G(p)) * a.q_row + (int64_t)(run.h * a.G + (p - a.by_G(p) * a.G)) * a.q_head + lc * 8;
           if (r < kPtTile) pt_cp16(sQ + (r >> 7) * BX * kPtBox + lane_box + (r & 127) * 128 + (((lc & 7) ^ (r & 7)) << 4), src, there);
         }
         pt_arrive_copies(q_full);
+        }
+        // tiles on their way to L2: shared memory holds two or four, less than what memory takes to answer
+        auto warm = [&](int tile, int entry) {
+          const int page = __shfl_sync(0xffffffffu, entry, lane * box_blocks & 15);
+          if (lane * box_blocks < 16 && page >= 0)
+#pragma unroll
+            for (int i = 0; i < BX; ++i) {
+              pt_prefetch_4d(&mapK, 64 * i, tile * kPtKeys & page_mask, run.h, page);
+              pt_prefetch_4d(&mapV, 64 * i, tile * kPtKeys & page_mask, run.h, page);
+            }
+        };
+        int far = entry_of(run.k0 + kPtAhead);
+        if (cw == 1)
+          for (int i = 1; i < min(kPtAhead, n.most); ++i) warm(run.k0 + i, entry_of(run.k0 + i));
         for (int j = 0; j < n.most; ++j) {
+          if (cw == 1 && j + kPtAhead < n.most) {
+            warm(run.k0 + j + kPtAhead, far);
+            far = entry_of(run.k0 + j + kPtAhead + 1);
+          }
           ahead = entry_of(run.k0 + j + 2);
           if (j + 1 < n.most && !(ok = load_k(j + 1, next))) break;
           const uint32_t c = kc + j, st = c % NS;
@@ -309,11 +348,11 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
       {
         const int p0 = run.t * kPtTile + t * kPtRows, pairs = run.seq.n * a.G, p = p0 + row;
         if (p0 >= pairs) continue;
-        const int cap = min(run.seq.len, a.max_blocks << a.page_shift), base = run.seq.len - run.seq.n, pos = base + p / a.G, wp = p0 + (row & ~31);
+        const int cap = min(run.seq.len, a.max_blocks << a.page_shift), base = run.seq.len - run.seq.n, pos = base + a.by_G(p), wp = p0 + (row & ~31);
         lim = p < pairs ? min(pos + 1, cap) : 0x7fffffff;
         lo = p < pairs && a.window > 0 ? pos - a.window + 1 : 0;
-        warp_lim = min(base + wp / a.G + 1, cap);
-        warp_lo = a.window > 0 ? base + min(wp + 31, pairs - 1) / a.G - a.window + 1 : 0;
+        warp_lim = min(base + a.by_G(wp) + 1, cap);
+        warp_lo = a.window > 0 ? base + a.by_G(min(wp + 31, pairs - 1)) - a.window + 1 : 0;
       }
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; j < n; ++j) {
@@ -397,13 +436,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
       const PagedSeq s = run.seq;
-      const int p = run.t * kPtTile + t * kPtRows + row, head = run.h * a.G + p % a.G;
+      const int p = run.t * kPtTile + t * kPtRows + row, head = run.h * a.G + (p - a.by_G(p) * a.G);
       const bool live = p < s.n * a.G, whole = run.first && run.last;
       float* rec = a.part + (2 * (int64_t)blockIdx.x + (run.first ? 1 : 0)) * paged_record_floats(kPtTile, HD);
       const int r = t * kPtRows + row;
       if (!whole && live) *reinterpret_cast<float2*>(rec + 2 * r) = make_float2(m == -INFINITY ? m : m * c, l);   // the combine's maxima are in units of exp2
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      H* out = reinterpret_cast<H*>(a.out) + (int64_t)(s.row0 + p / a.G) * a.o_row + (int64_t)head * a.o_head;
+      H* out = reinterpret_cast<H*>(a.out) + (int64_t)(s.row0 + a.by_G(p)) * a.o_row + (int64_t)head * a.o_head;
 #pragma unroll 1
       for (int q = 0; q < HD / 32; ++q) {
         uint32_t o[32];
@@ -449,23 +488,34 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
   if (tid == 0 && s_err && a.error) *a.error = 1;
 }
 
-// a box: 64 columns of up to 128 tokens of a page
-static int pt_map(CUtensorMap* map, int dtype, const void* base, const PagedArgs& a) {
+// a box: 64 columns of up to `keys` tokens of a page
+int paged_map(CUtensorMap* map, int dtype, const void* base, const PagedArgs& a, int keys) {
   EncodeTiledFn enc = get_encode();
   TSB_CHECK(enc, "paged_attention: the driver has no cuTensorMapEncodeTiled");
   const cuuint64_t page = (cuuint64_t)1 << a.page_shift;
   const cuuint64_t dims[4] = {(cuuint64_t)a.hd, page, (cuuint64_t)a.Hkv, (cuuint64_t)a.num_pages};
   // the stride of a single head or page means nothing
   const cuuint64_t strides[3] = {(cuuint64_t)a.c_tok * 2, (cuuint64_t)(a.Hkv > 1 ? a.c_head : a.hd) * 2, (cuuint64_t)(a.num_pages > 1 ? a.c_page : a.hd) * 2};
-  const cuuint32_t box[4] = {64, page < kPtKeys ? (cuuint32_t)page : kPtKeys, 1, 1}, el[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, page < (cuuint64_t)keys ? (cuuint32_t)page : (cuuint32_t)keys, 1, 1}, el[4] = {1, 1, 1, 1};
   const CUresult r = enc(map, dtype == TSB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, el,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TSB_CHECK(r == CUDA_SUCCESS, "paged_attention: cuTensorMapEncodeTiled failed with %d", (int)r);
+  return 1;
+}
+constexpr int64_t paged_stride_most = (int64_t)1 << 39;   // elements: bytes below 2^40
+static int pt_map_q(CUtensorMap* map, int dtype, const PagedArgs& a) {
+  EncodeTiledFn enc = get_encode();
+  const cuuint64_t dims[3] = {(cuuint64_t)a.hd, (cuuint64_t)a.H, (cuuint64_t)a.rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)(a.H > 1 ? a.q_head : a.hd) * 2, (cuuint64_t)a.q_row * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)a.G, (cuuint32_t)(kPtRows / a.G)}, el[3] = {1, 1, 1};
+  const CUresult r = enc(map, dtype == TSB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(a.q), dims, strides, box, el,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TSB_CHECK(r == CUDA_SUCCESS, "paged_attention: cuTensorMapEncodeTiled failed with %d", (int)r);
   return 1;
 }
 // strides that a tensor map takes
 bool paged_tc_strides(const PagedArgs& a) {
-  const int64_t most = (int64_t)1 << 39;   // bytes below 2^40
+  const int64_t most = paged_stride_most;
   return a.num_pages > 0 && a.c_tok > 0 && a.c_tok < most && (a.Hkv == 1 || (a.c_head > 0 && a.c_head < most)) && (a.num_pages == 1 || (a.c_page > 0 && a.c_page < most));
 }
 
@@ -478,11 +528,14 @@ static int pt_launch(int device, DeviceState* st, const PagedArgs& a, cudaStream
     TSB_CUDA(cudaFuncSetAttribute(paged_tc_kernel<H, BX, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     done[device] = true;
   }
-  CUtensorMap mk, mv;
+  CUtensorMap mk, mv, mq;
   constexpr int dtype = Pair16<H>::kBf16 ? TSB200_BF16 : TSB200_F16;
-  TSB_TRY(pt_map(&mk, dtype, a.K, a));
-  TSB_TRY(pt_map(&mv, dtype, a.V, a));
-  paged_tc_kernel<H, BX, NS><<<st->sm_count, kPtThreads, smem, s>>>(mk, mv, a);
+  TSB_TRY(paged_map(&mk, dtype, a.K, a, kPtKeys));
+  TSB_TRY(paged_map(&mv, dtype, a.V, a, kPtKeys));
+  const int q_boxes = kPtRows % a.G == 0 && a.q_row > 0 && a.q_row < paged_stride_most && (a.H == 1 || (a.q_head > 0 && a.q_head < paged_stride_most));
+  if (q_boxes) TSB_TRY(pt_map_q(&mq, dtype, a));
+  else mq = mk;
+  paged_tc_kernel<H, BX, NS><<<st->sm_count, kPtThreads, smem, s>>>(mk, mv, mq, a, q_boxes);
   count_launch(device);
   return check_launch("paged_tc");
 }

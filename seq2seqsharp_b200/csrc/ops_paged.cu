@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kFmaThreads) paged_fma_kernel(const __grid_con
     for (int i = tid; i < RT * D; i += kFmaThreads) {
       const int r = i / D, e = i % D, p = p0 + r;
       float v = 0.0f;
-      if (p < pairs && e < a.hd) v = to_f<T>(reinterpret_cast<const T*>(a.q)[(int64_t)(s.row0 + p / a.G) * a.q_row + (run.h * a.G + p % a.G) * a.q_head + e]) * a.c;
+      if (p < pairs && e < a.hd) v = to_f<T>(reinterpret_cast<const T*>(a.q)[(int64_t)(s.row0 + a.by_G(p)) * a.q_row + (run.h * a.G + (p - a.by_G(p) * a.G)) * a.q_head + e]) * a.c;
       qs[i] = v;
     }
     float m[RW], l[RW], acc[RW][NH];
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kFmaThreads) paged_fma_kernel(const __grid_con
     for (int r = 0; r < RW; ++r) {
       m[r] = -INFINITY;
       l[r] = 0.0f;
-      const int p = p0 + w * RW + r, pos = s.len - s.n + p / a.G;
+      const int p = p0 + w * RW + r, pos = s.len - s.n + a.by_G(p);
       hi[r] = p < pairs ? min(pos + 1, cap) : 0;
       lo[r] = a.window > 0 ? pos - a.window + 1 : 0;
 #pragma unroll
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kFmaThreads) paged_fma_kernel(const __grid_con
       const int row = w * RW + r, p = p0 + row;
       if (p >= pairs) continue;
       if (whole) {
-        T* o = reinterpret_cast<T*>(a.out) + (int64_t)(s.row0 + p / a.G) * a.o_row + (run.h * a.G + p % a.G) * a.o_head;
+        T* o = reinterpret_cast<T*>(a.out) + (int64_t)(s.row0 + a.by_G(p)) * a.o_row + (run.h * a.G + (p - a.by_G(p) * a.G)) * a.o_head;
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
         for (int e = 0; e < NH; ++e)
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_combine_kernel(const __gri
 #pragma unroll 4
   for (int k = 0; k < n - 1; ++k) add(other + 2 * k * rf);
   const int p = j.z + row;
-  T* out = reinterpret_cast<T*>(a.out) + (int64_t)(j.y + p / a.G) * a.o_row + (int64_t)(h * a.G + p % a.G) * a.o_head + e;
+  T* out = reinterpret_cast<T*>(a.out) + (int64_t)(j.y + a.by_G(p)) * a.o_row + (int64_t)(h * a.G + (p - a.by_G(p) * a.G)) * a.o_head + e;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
   for (int k = 0; k < 4; ++k) acc[k] *= inv;
@@ -486,12 +486,19 @@ int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int 
 
 // The kernel that serves a call, its rows of a tile and its CTAs
 struct PagedChoice {
-  enum { FMA, TC } kind;
+  enum { FMA, MMA, TC } kind;
   int RT, KT, ctas;
 };
 static PagedChoice paged_choose(int sm_count, int dtype, int64_t pairs, int hd, bool positive) {
   PagedChoice c;
   if (is_16bit(dtype) && (hd == 64 || hd == 128) && positive) {
+    if (pairs <= 64) {
+      c.kind = PagedChoice::MMA;
+      c.RT = pairs <= 16 ? 16 : pairs <= 32 ? 32 : 64;
+      c.KT = 64;
+      c.ctas = 2 * sm_count;
+      return c;
+    }
     c.kind = PagedChoice::TC;
     c.RT = 256;
     c.KT = 128;
@@ -651,6 +658,7 @@ int TSB200_PagedAttention(int device, int dtype, void* out, int64_t o_row, int64
   a.out = out; a.q = q; a.K = cacheK; a.V = cacheV; a.o_row = o_row; a.o_head = o_head; a.q_row = q_row; a.q_head = q_head;
   a.c_page = c_page; a.c_head = c_head; a.c_tok = c_tok; a.table = table; a.table_stride = table_stride; a.max_blocks = max_blocks; a.num_pages = num_pages;
   a.starts = starts; a.lens = lens; a.B = B; a.rows = rows; a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.hd = hd;
+  a.by_G.set((uint32_t)a.G);
   a.c = scale * 1.44269504088896340736f;
   a.window = window; cudaStream_t s = pick_stream(st, stream);
   // the kernels on tensor cores look for the largest score before it is scaled
@@ -661,6 +669,7 @@ int TSB200_PagedAttention(int device, int dtype, void* out, int64_t o_row, int64
   a.min_units = 4;
   a.snap = 1;
   a.start = 1;
+  if (c.kind == PagedChoice::MMA) return launch_paged_mma(device, st, dtype, a, c.RT, s);
   if (c.kind == PagedChoice::TC) return launch_paged_tc(device, st, dtype, a, s);
   if (dtype == TSB200_F32) TSB_TRY(launch_paged_fma<float>(device, st, a, c, s));
   else if (dtype == TSB200_F16) TSB_TRY(launch_paged_fma<__half>(device, st, a, c, s));

@@ -11,10 +11,22 @@
 // CTA leaves its maximum, sum and accumulator in the workspace and paged_combine_kernel joins them in the order of the runs (the same
 // order whatever CTA ends first).  Ends within a 32nd of a run of an item's end, or within `snap` units, are moved there: a record has to be written and read.
 #pragma once
+#include <cuda.h>
+
 #include "kernels.cuh"
 
 namespace tsb {
 
+// division of numbers below 2^31 by one that the host knows
+struct PagedDiv {
+  uint32_t mul, shift;
+  void set(uint32_t d) {
+    shift = 0;
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi(mul, (uint32_t)n) + (uint32_t)n) >> shift); }
+};
 struct PagedArgs {
   void* out;                       // [rows, H, hd], strides o_row, o_head
   const void* q;                   // [rows, H, hd], strides q_row, q_head
@@ -25,6 +37,7 @@ struct PagedArgs {
   int max_blocks, num_pages, page_shift;
   const int *starts, *lens;
   int B, rows, H, Hkv, G, hd;
+  PagedDiv by_G;
   float c;                         // scale * log2(e)
   int window;                      // 0: none
   float* part;                     // records: paged_record_floats() each, two per CTA
@@ -54,7 +67,7 @@ struct PagedTile {
 };
 __device__ __forceinline__ PagedTile paged_tile(const PagedArgs& a, const PagedSeq& s, int t, int RT, int KT) {
   const int p1 = min(s.n * a.G, (t + 1) * RT) - 1;
-  const int first = s.len - s.n + t * RT / a.G, last = s.len - s.n + p1 / a.G;   // positions of the tile
+  const int first = s.len - s.n + a.by_G(t * RT), last = s.len - s.n + a.by_G(p1);   // positions of the tile
   const int hi = min(last + 1, a.max_blocks << a.page_shift);
   const int lo = a.window > 0 && a.window <= first ? first - a.window + 1 : 0;
   PagedTile r;
@@ -144,7 +157,7 @@ __device__ __forceinline__ PagedLoc paged_find(const PagedArgs& a, int b, long l
     l.t = t0 + src;
     const int cost = __shfl_sync(0xffffffffu, u, src);
     const long long at = s + __shfl_sync(0xffffffffu, end, src) - (long long)cost * a.Hkv;
-    l.h = (int)((x - at) / max(cost, 1));
+    l.h = (int)((double)(x - at) / (double)max(cost, 1));   // exact below 2^53, and a tenth of the instructions of a 64-bit division
     l.s = at + (long long)l.h * cost;
     l.units = cost - a.start;
     const int in_item = (int)(x - l.s), rest = cost - in_item;
@@ -153,29 +166,35 @@ __device__ __forceinline__ PagedLoc paged_find(const PagedArgs& a, int b, long l
     return l;
   }
 }
+// where run c begins: c / runs of all units
+__device__ __forceinline__ long long paged_begin(long long all, int c, int runs) { return (long long)((double)all * (double)c / (double)runs); }
 // Run `c` of the plan: sh.loc[0] and sh.loc[1] where it begins and ends.  Returns whether there is such a run.  `all` / `runs`: units and runs of
 // the whole call.  All threads of the CTA.
 template <int NT, int RT, int KT>
 __device__ __forceinline__ bool paged_locate(const PagedArgs& a, int c, int ctas, PagedPlanShared& sh, long long& all, int& runs) {
   const int tid = threadIdx.x;
-  long long mine = paged_seq_units(a, tid, RT, KT), total = mine;
-  for (int b0 = NT; b0 < a.B; b0 += NT) total += paged_seq_units(a, b0 + tid, RT, KT);
-  paged_block_scan<NT>(total, sh, all);
-  const long long most = all / a.min_units;
-  runs = (int)(most < 1 ? 1 : (most < ctas ? most : ctas));
+  long long mine = paged_seq_units(a, tid, RT, KT), before;
+  if (a.B <= NT) {
+    before = paged_block_scan<NT>(mine, sh, all);
+  } else {
+    long long total = mine;
+    for (int b0 = NT; b0 < a.B; b0 += NT) total += paged_seq_units(a, b0 + tid, RT, KT);
+    paged_block_scan<NT>(total, sh, all);
+  }
+  runs = all >= (long long)a.min_units * ctas ? ctas : max(1, (int)all / a.min_units);
   if (all == 0 || c >= runs) {
     if (tid == 0) a.joins[2 * c] = make_int4(0, 0, 0, 0);
     return false;
   }
-  const long long tol = max(all / runs / 32, (long long)a.snap);
-  const long long x[2] = {all * c / runs, all * (c + 1) / runs};
+  const long long tol = max(paged_begin(all, 1, runs) >> 5, (long long)a.snap);
+  const long long x[2] = {paged_begin(all, c, runs), paged_begin(all, c + 1, runs)};
   if (tid == 0) sh.loc[1] = PagedLoc{a.B, 0, 0, 0, 0, all};
   long long base = 0;
   for (int b0 = 0; b0 < a.B && base <= x[1]; b0 += NT) {
     const int b = b0 + tid;
     if (b0 > 0) mine = paged_seq_units(a, b, RT, KT);
-    long long here;
-    const long long s = base + paged_block_scan<NT>(mine, sh, here);
+    long long here = all;
+    const long long s = a.B <= NT ? before : base + paged_block_scan<NT>(mine, sh, here);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const unsigned hit = __ballot_sync(0xffffffffu, mine > 0 && x[i] >= s && x[i] < s + mine);
@@ -193,10 +212,10 @@ __device__ __forceinline__ bool paged_locate(const PagedArgs& a, int c, int ctas
     // that has the item's end (their first)
     const PagedLoc l = sh.loc[0];
     PagedJoin j{};
-    if (l.off > 0 && l.off < l.units && all * (c - 1) / runs - l.s <= max(tol, (long long)a.start)) {
+    if (l.off > 0 && l.off < l.units && paged_begin(all, c - 1, runs) - l.s <= max(tol, (long long)a.start)) {
       const PagedSeq q = paged_seq(a, l.b);
       j.records = 2;
-      while (c + j.records - 1 < runs && l.s + a.start + l.units - all * (c + j.records - 1) / runs > tol) ++j.records;
+      while (c + j.records - 1 < runs && l.s + a.start + l.units - paged_begin(all, c + j.records - 1, runs) > tol) ++j.records;
       j.row0 = q.row0;
       j.p0 = l.t * RT;
       j.pairs = min(RT, q.n * a.G - l.t * RT);
@@ -254,7 +273,8 @@ struct PagedRun {
 
 int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int ctas, cudaStream_t s);
 // kernels for 16-bit types and head sizes 64 and 128: rows of few pairs per sequence on mma.sync, chunks on tcgen05
-int launch_paged_mma(int device, DeviceState* st, int dtype, PagedArgs a, int pairs, cudaStream_t s);
+int paged_map(CUtensorMap* map, int dtype, const void* base, const PagedArgs& a, int keys);
+int launch_paged_mma(int device, DeviceState* st, int dtype, PagedArgs a, int RT, cudaStream_t s);
 bool paged_tc_strides(const PagedArgs& a);
 int launch_paged_tc(int device, DeviceState* st, int dtype, PagedArgs a, cudaStream_t s);
 
