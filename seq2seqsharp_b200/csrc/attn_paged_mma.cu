@@ -41,7 +41,8 @@ __device__ __forceinline__ float pm_ex2(float x) {
 template <typename H, int BX, int WR>
 __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                                                                         const __grid_constant__ PagedArgs a) {
-  constexpr int HD = BX * 64, NS = pm_stages(BX), RT = 16 * WR, KG = kPmWarps / WR, KS = HD / 16, NB = HD / 8, SLICES = kPmKeys / KG / 16;
+  constexpr int HD = BX * 64, NS = pm_stages(BX), RT = 16 * WR, KG = kPmWarps / WR, KS = HD / 16, NB = HD / 8;
+  constexpr int SK = KG == 4 ? 16 : 32, STEPS = kPmKeys / KG / SK, SN = SK / 8;   // keys a warp weighs at a time
   extern __shared__ __align__(1024) unsigned char pm_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)pm_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t ring = s_u32(smem);
@@ -121,6 +122,9 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
       const int posA = s.len - s.n + iA, posB = s.len - s.n + iB;
       const int hiA = liveA ? min(posA + 1, cap) : 0, hiB = liveB ? min(posB + 1, cap) : 0;
       const int loA = a.window > 0 ? posA - a.window + 1 : 0, loB = a.window > 0 ? posB - a.window + 1 : 0;
+      // of the warp's rows: keys that all of them see
+      const int first = run.t * RT + rg * 16, last = min(first + 15, pairs - 1);
+      const int see_to = min(s.len - s.n + a.by_G(first) + 1, cap), see_from = a.window > 0 ? s.len - s.n + a.by_G(max(last, 0)) - a.window + 1 : 0;
       uint32_t qa[KS][4];
       {
         const H* qA = reinterpret_cast<const H*>(a.q) + (liveA ? (int64_t)(s.row0 + iA) * a.q_row + hA * a.q_head : 0) + 2 * t4;
@@ -155,43 +159,49 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
           __syncwarp();
         }
 #pragma unroll 1
-        for (int sl = 0; sl < SLICES; ++sl) {
-          const int t0 = kg * (kPmKeys / KG) + sl * 16, key0 = kt * kPmKeys + t0;
-          float sc[2][4];
+        for (int sl = 0; sl < STEPS; ++sl) {
+          const int t0 = kg * (kPmKeys / KG) + sl * SK, key0 = kt * kPmKeys + t0;
+          float sc[SN][4];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
+          for (int n = 0; n < SN; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sc[n][e] = 0.0f;
-            const int r = t0 + n * 8 + (lane & 7);
 #pragma unroll
-            for (int k = 0; k < KS / 2; ++k) {
+          for (int k = 0; k < KS / 2; ++k)
+#pragma unroll
+            for (int n = 0; n < SN; ++n) {
               uint32_t b[4];
-              const int ch = k * 4 + (lane >> 3);
+              const int ch = k * 4 + (lane >> 3), r = t0 + n * 8 + (lane & 7);
               pm_ldmatrix(kb + (ch >> 3) * kPmBox + r * 128 + (((ch & 7) ^ (r & 7)) << 4), b);
               mma_16816<H>(sc[n], qa[2 * k][0], qa[2 * k][1], qa[2 * k][2], qa[2 * k][3], b[0], b[1]);
               mma_16816<H>(sc[n], qa[2 * k + 1][0], qa[2 * k + 1][1], qa[2 * k + 1][2], qa[2 * k + 1][3], b[2], b[3]);
             }
-          }
-          float xA = -INFINITY, xB = -INFINITY;
+          if (gone != 0 || key0 + SK > see_to || key0 < see_from) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const bool none = gone >> ((t0 >> 3) + n) & 1;
+            for (int n = 0; n < SN; ++n) {
+              const bool none = gone >> ((t0 >> 3) + n) & 1;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int j = key0 + n * 8 + 2 * t4 + e;
-              sc[n][e] = j < hiA && j >= loA && !none ? sc[n][e] * a.c : -INFINITY;
-              sc[n][2 + e] = j < hiB && j >= loB && !none ? sc[n][2 + e] * a.c : -INFINITY;
-              xA = fmaxf(xA, sc[n][e]);
-              xB = fmaxf(xB, sc[n][2 + e]);
+              for (int e = 0; e < 2; ++e) {
+                const int j = key0 + n * 8 + 2 * t4 + e;
+                if (!(j < hiA && j >= loA && !none)) sc[n][e] = -INFINITY;
+                if (!(j < hiB && j >= loB && !none)) sc[n][2 + e] = -INFINITY;
+              }
             }
+          }
+          float xA = fmaxf(sc[0][0], sc[0][1]), xB = fmaxf(sc[0][2], sc[0][3]);
+#pragma unroll
+          for (int n = 1; n < SN; ++n) {
+            xA = fmaxf(xA, fmaxf(sc[n][0], sc[n][1]));
+            xB = fmaxf(xB, fmaxf(sc[n][2], sc[n][3]));
           }
           xA = fmaxf(xA, __shfl_xor_sync(0xffffffffu, xA, 1));
           xB = fmaxf(xB, __shfl_xor_sync(0xffffffffu, xB, 1));
           xA = fmaxf(xA, __shfl_xor_sync(0xffffffffu, xA, 2));
           xB = fmaxf(xB, __shfl_xor_sync(0xffffffffu, xB, 2));
           if (__any_sync(0xffffffffu, xA > mA || xB > mB)) {
+            // maxima of scores as they are, and from there exp2(c (score - maximum)); no key seen yet: every weight is exp2(-inf)
             const float uA = fmaxf(mA, xA), uB = fmaxf(mB, xB);
-            const float fA = pm_ex2(mA - fmaxf(uA, -FLT_MAX)), fB = pm_ex2(mB - fmaxf(uB, -FLT_MAX));
+            const float fA = uA == -INFINITY ? 1.0f : pm_ex2((mA - uA) * a.c), fB = uB == -INFINITY ? 1.0f : pm_ex2((mB - uB) * a.c);
             mA = uA;
             mB = uB;
             lA *= fA;
@@ -204,31 +214,36 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
               o[n][3] *= fB;
             }
           }
-          const float nA = fmaxf(mA, -FLT_MAX), nB = fmaxf(mB, -FLT_MAX);   // no key seen yet: every weight is exp2(-inf)
-          uint32_t p[4];
+          const float nA = mA == -INFINITY ? 0.0f : -mA * a.c, nB = mB == -INFINITY ? 0.0f : -mB * a.c;
+          uint32_t p[SN][2];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            p[2 * n] = Pair16<H>::put(pm_ex2(sc[n][0] - nA), pm_ex2(sc[n][1] - nA));
-            p[2 * n + 1] = Pair16<H>::put(pm_ex2(sc[n][2] - nB), pm_ex2(sc[n][3] - nB));
+          for (int n = 0; n < SN; ++n) {
+            p[n][0] = Pair16<H>::put(pm_ex2(fmaf(sc[n][0], a.c, nA)), pm_ex2(fmaf(sc[n][1], a.c, nA)));
+            p[n][1] = Pair16<H>::put(pm_ex2(fmaf(sc[n][2], a.c, nB)), pm_ex2(fmaf(sc[n][3], a.c, nB)));
             // the weights as they are rounded for the product: what rounding does to the numerator it does to the denominator
-            const float2 a2 = Pair16<H>::get(p[2 * n]), b2 = Pair16<H>::get(p[2 * n + 1]);
+            const float2 a2 = Pair16<H>::get(p[n][0]), b2 = Pair16<H>::get(p[n][1]);
             lA += a2.x + a2.y;
             lB += b2.x + b2.y;
           }
-          const int vr = t0 + (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
-          for (int n = 0; n < NB / 2; ++n) {
-            uint32_t b[4];
-            const int ch = n * 2 + (lane >> 4);
-            pm_ldmatrix_trans(vb + (ch >> 3) * kPmBox + vr * 128 + (((ch & 7) ^ (vr & 7)) << 4), b);
-            mma_16816<H>(o[2 * n], p[0], p[1], p[2], p[3], b[0], b[1]);
-            mma_16816<H>(o[2 * n + 1], p[0], p[1], p[2], p[3], b[2], b[3]);
+          for (int i = 0; i < SN / 2; ++i) {
+            const int vr = t0 + i * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+            for (int n = 0; n < NB / 2; ++n) {
+              uint32_t b[4];
+              const int ch = n * 2 + (lane >> 4);
+              pm_ldmatrix_trans(vb + (ch >> 3) * kPmBox + vr * 128 + (((ch & 7) ^ (vr & 7)) << 4), b);
+              mma_16816<H>(o[2 * n], p[2 * i][0], p[2 * i][1], p[2 * i + 1][0], p[2 * i + 1][1], b[0], b[1]);
+              mma_16816<H>(o[2 * n + 1], p[2 * i][0], p[2 * i][1], p[2 * i + 1][0], p[2 * i + 1][1], b[2], b[3]);
+            }
           }
         }
         if (ragged) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the zeros above, before the next copy to this place
         __syncwarp();
         if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s_u32(&empty[st])) : "memory");
       }
+      if (mA != -INFINITY) mA *= a.c;   // in units of exp2 from here on
+      if (mB != -INFINITY) mB *= a.c;
       lA += __shfl_xor_sync(0xffffffffu, lA, 1);
       lB += __shfl_xor_sync(0xffffffffu, lB, 1);
       lA += __shfl_xor_sync(0xffffffffu, lA, 2);

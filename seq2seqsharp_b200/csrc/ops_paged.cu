@@ -190,78 +190,102 @@ __device__ __forceinline__ void rope_store8(T* p, const float* f) {
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_paged_kernel(const __grid_constant__ RopePagedArgs a) {
-  __shared__ float wq[kRopeMaxHd], wk[kRopeMaxHd];
-  __shared__ float2 turn[kRopeThreads];
-  const int tid = threadIdx.x, half = a.rot / 2;
+  __shared__ __align__(16) float wq[kRopeMaxHd], wk[kRopeMaxHd];
+  __shared__ __align__(16) float2 turn[kRopeThreads];
+  __shared__ int place[kRopeThreads];
+  const int tid = threadIdx.x, half = a.rot / 2, lane = tid & 31;
+  const bool turns = a.style != 0;
+  // a pass: as many rows as the CTA has threads for their angles
+  const int rows_pass = turns ? kRopeThreads / half : a.rows_here;
+  const int ar = turns ? tid / half : 0, ai = turns ? tid - ar * half : 0;
+  const double rate = turns ? a.first * pow(a.ratio, (double)ai) : 0.0;   // half turns per position
   for (int e = tid; e < a.hd; e += kRopeThreads) {
     wq[e] = a.q_norm ? to_f<T>(reinterpret_cast<const T*>(a.q_norm)[e]) : 1.0f;
     wk[e] = a.k_norm ? to_f<T>(reinterpret_cast<const T*>(a.k_norm)[e]) : 1.0f;
   }
   int L = 1;
   while (L * 8 < a.hd) L <<= 1;
-  const int li = tid & (L - 1), lane = tid & 31, per = kRopeThreads / L, heads = a.H + 2 * a.Hkv;
+  const int li = tid & (L - 1), per = kRopeThreads / L, heads = a.H + 2 * a.Hkv;
   const bool on = li * 8 < a.hd;
-  const int64_t places = (int64_t)a.num_pages << a.page_shift;
+  // style 2: the partner of element e < rot / 2 is e + rot / 2, whole lanes away
+  const int away = half / 8, low = li < away;
+  const int from = (lane & ~(L - 1)) + (li * 8 < a.rot ? (low ? li + away : li - away) : li);
+  const int places = a.num_pages << a.page_shift;
   const int row_first = (int)blockIdx.x * a.rows_here, row_end = min(a.rows, row_first + a.rows_here);
-  // a pass: as many rows as the CTA has threads for their angles
-  const int rows_pass = a.style && half > 0 ? max(1, kRopeThreads / half) : 1;
   for (int row0 = row_first; row0 < row_end; row0 += rows_pass) {
     const int n = min(rows_pass, row_end - row0);
-    __syncthreads();
-    if (a.style && tid < n * half) {
-      const int i = tid % half;
-      double x = (double)a.positions[row0 + tid / half] * (a.first * pow(a.ratio, (double)i));
+    __syncthreads();   // the pass before is done with both
+    if (turns && ar < n) {
+      double x = (double)a.positions[row0 + ar] * rate;
       x -= 2.0 * rint(0.5 * x);
       float s, c;
       sincospif((float)x, &s, &c);
       turn[tid] = make_float2(c, s);
     }
+    if (tid < n) {
+      const int slot = a.slots[row0 + tid];
+      place[tid] = slot >= 0 && slot < places ? slot : -1;
+    }
     __syncthreads();
-    for (int it = (int)blockIdx.y * per + tid / L; __any_sync(0xffffffffu, it < n * heads); it += per * (int)gridDim.y) {
-      const bool live = it < n * heads && on;
-      const int r = min(it / heads, n - 1), head = it % heads, row = row0 + r;
-      const int slot = a.slots[row];
-      const bool there = live && slot >= 0 && slot < places;
-      const bool is_q = head < a.H, is_v = head >= a.H + a.Hkv;
+    // (row, head) pairs go round the groups of L lanes; the next one is on its way while one is turned
+    int head = (int)blockIdx.y * per + tid / L, r = 0;
+    const int stride = per * (int)gridDim.y;
+    auto settle = [&]() {
+      while (head >= heads) {
+        head -= heads;
+        ++r;
+      }
+    };
+    auto source = [&]() {
+      const int64_t row = row0 + r;
+      return (head < a.H ? reinterpret_cast<const T*>(a.q) + row * a.q_row + head * a.q_head
+                         : (head >= a.H + a.Hkv ? reinterpret_cast<const T*>(a.v) + row * a.v_row + (head - a.H - a.Hkv) * a.v_head
+                                                : reinterpret_cast<const T*>(a.k) + row * a.k_row + (head - a.H) * a.k_head)) + li * 8;
+    };
+    float ahead[8];
+    auto fetch = [&]() {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ahead[e] = 0.0f;
+      if (r < n && on && place[r] >= 0) rope_load8<T, WIDE>(source(), ahead);
+    };
+    settle();
+    fetch();
+    while (__any_sync(0xffffffffu, r < n)) {
       float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-      if (there) {
-        const T* src = is_q ? reinterpret_cast<const T*>(a.q) + row * a.q_row + head * a.q_head
-                            : (is_v ? reinterpret_cast<const T*>(a.v) + row * a.v_row + (head - a.H - a.Hkv) * a.v_head
-                                    : reinterpret_cast<const T*>(a.k) + row * a.k_row + (head - a.H) * a.k_head);
-        rope_load8<T, WIDE>(src + li * 8, x);
-      }
-      const bool normed = !is_v && (is_q ? a.q_norm : a.k_norm) != nullptr;
+      for (int e = 0; e < 8; ++e) x[e] = ahead[e];
+      const int hd_now = head, r_now = r, row = row0 + r, slot = r < n ? place[r] : -1;
+      const bool there = on && slot >= 0, is_q = hd_now < a.H, is_v = hd_now >= a.H + a.Hkv;
+      head += stride;
+      settle();
+      fetch();
       float ss = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
       for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (normed && on) {
+      if (!is_v && on && (is_q ? a.q_norm : a.k_norm) != nullptr) {
         const float f = 1.0f / sqrtf(ss / (float)a.hd + a.eps);
-        const float* w = is_q ? wq : wk;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * f * w[li * 8 + e];
+        const float4* w = reinterpret_cast<const float4*>((is_q ? wq : wk) + li * 8);
+        const float4 w0 = w[0], w1 = w[1];
+        x[0] *= f * w0.x; x[1] *= f * w0.y; x[2] *= f * w0.z; x[3] *= f * w0.w;
+        x[4] *= f * w1.x; x[5] *= f * w1.y; x[6] *= f * w1.z; x[7] *= f * w1.w;
       }
       if (a.style == 1) {
         if (!is_v)
 #pragma unroll
           for (int e = 0; e < 8; e += 2)
-            if (li * 8 + e < a.rot) {
-              const float2 t = turn[r * half + (li * 8 + e) / 2];
+            if (li * 8 + e < a.rot && r_now < n) {
+              const float2 t = turn[r_now * half + (li * 8 + e) / 2];
               const float y0 = x[e] * t.x - x[e + 1] * t.y, y1 = x[e + 1] * t.x + x[e] * t.y;
               x[e] = y0;
               x[e + 1] = y1;
             }
       } else if (a.style == 2) {
-        // the partner of element e < rot / 2 is e + rot / 2: whole lanes apart
-        const int away = half / 8, low = li < away;
-        const int from = (lane & ~(L - 1)) + (li * 8 < a.rot ? (low ? li + away : li - away) : li);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float y = __shfl_sync(0xffffffffu, x[e], from);
-          if (!is_v && li * 8 < a.rot) {
-            const float2 t = turn[r * half + (low ? li : li - away) * 8 + e];
+          if (!is_v && li * 8 < a.rot && r_now < n) {
+            const float2 t = turn[r_now * half + (low ? li : li - away) * 8 + e];
             x[e] = low ? x[e] * t.x - y * t.y : x[e] * t.x + y * t.y;
           }
         }
@@ -269,9 +293,9 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_paged_kernel(const 
       if (there) {
         T* dst;
         if (is_q) {
-          dst = reinterpret_cast<T*>(a.out) + row * a.o_row + head * a.o_head;
+          dst = reinterpret_cast<T*>(a.out) + row * a.o_row + hd_now * a.o_head;
         } else {
-          const int64_t at = (int64_t)(slot >> a.page_shift) * a.c_page + (int64_t)(slot & ((1 << a.page_shift) - 1)) * a.c_tok + (is_v ? head - a.H - a.Hkv : head - a.H) * a.c_head;
+          const int64_t at = (int64_t)(slot >> a.page_shift) * a.c_page + (int64_t)(slot & ((1 << a.page_shift) - 1)) * a.c_tok + (is_v ? hd_now - a.H - a.Hkv : hd_now - a.H) * a.c_head;
           dst = reinterpret_cast<T*>(is_v ? a.V : a.K) + at;
         }
         rope_store8<T, WIDE>(dst + li * 8, x);
@@ -432,54 +456,99 @@ __global__ void __launch_bounds__(kFmaThreads) paged_fma_kernel(const __grid_con
   }
 }
 
-// Joins the records of the items that runs end in, four elements of a row per thread.  What bounds it: latency of two dependent reads, then the records.
+// Joins the records of the items that runs end in, four elements of a row per thread.  What bounds it: latency of dependent reads, then the records.
+// W warps share the records of 32 x 4 elements: an item of few rows may have a record of every run (one token of 16384, 8 KV heads: 37 each; W = 1 took 16 us,
+// W = 8 takes 6), one of many rows has few.
 constexpr int kJoinThreads = 256;
-template <typename T>
+template <typename T, int W>
 __global__ void __launch_bounds__(kJoinThreads) paged_combine_kernel(const __grid_constant__ PagedArgs a, int RT) {
-  const int c = (int)blockIdx.x + 1;
+  constexpr int Q = kJoinThreads / W;   // quads of a CTA
+  __shared__ float shared_acc[W > 1 ? W : 1][W > 1 ? Q : 1][4];
+  __shared__ float2 shared_ml[W > 1 ? W : 1][W > 1 ? Q : 1];
+  const int c = (int)blockIdx.x + 1, share = W > 1 ? (int)threadIdx.x / Q : 0, at = (int)threadIdx.x % Q;
   pdl_wait();
   const int4 j = __ldcg(&a.joins[2 * c]);
-  if (j.x == 0) return;
   const int h = __ldcg(&a.joins[2 * c + 1]).x, n = j.x, quads = a.hd / 4;
-  const int i = (int)blockIdx.y * kJoinThreads + (int)threadIdx.x, row = i / quads, e = (i - row * quads) * 4;
-  if (row >= j.w) return;
+  if (n == 0) return;
   const int64_t rf = paged_record_floats(RT, a.hd);
-  const float* first = a.part + (2 * (int64_t)(c - 1) + 1) * rf;   // of run c - 1: its last; of the runs behind: their first
-  const float* other = a.part + 2 * (int64_t)c * rf;
-  float m = __ldcg(first + 2 * row);
-#pragma unroll 4
-  for (int k = 0; k < n - 1; ++k) m = fmaxf(m, __ldcg(other + 2 * k * rf + 2 * row));
-  const float from = fmaxf(m, -FLT_MAX);
-  float sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  auto add = [&](const float* r) {
-    const float2 ml = __ldcg(reinterpret_cast<const float2*>(r + 2 * row));
-    const float4 x = __ldcg(reinterpret_cast<const float4*>(r + 2 * RT + (int64_t)row * a.hd + e));
-    const float f = exp2f(ml.x - from);
-    sum += ml.y * f;
-    acc[0] += x.x * f;
-    acc[1] += x.y * f;
-    acc[2] += x.z * f;
-    acc[3] += x.w * f;
-  };
-  add(first);
-#pragma unroll 4
-  for (int k = 0; k < n - 1; ++k) add(other + 2 * k * rf);
-  const int p = j.z + row;
-  T* out = reinterpret_cast<T*>(a.out) + (int64_t)(j.y + a.by_G(p)) * a.o_row + (int64_t)(h * a.G + (p - a.by_G(p) * a.G)) * a.o_head + e;
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  // of run c - 1: its last; of the runs behind: their first
+  auto record = [&](int k) { return a.part + (k == 0 ? 2 * (int64_t)(c - 1) + 1 : 2 * (int64_t)(c - 1 + k)) * rf; };
+  for (int i0 = (int)blockIdx.y * Q; i0 < j.w * quads; i0 += Q * (int)gridDim.y) {
+    const int i = i0 + at, row = i / quads, e = (i - row * quads) * 4;
+    const bool live = row < j.w;
+    float m = -INFINITY, sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (live)
+      for (int k0 = share; k0 < n; k0 += 4 * W) {
+        // four records on their way at a time, both parts of them
+        float2 ml[4];
+        float4 x[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) acc[k] *= inv;
-  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-  else *reinterpret_cast<uint2*>(out) = make_uint2(Pair16<T>::put(acc[0], acc[1]), Pair16<T>::put(acc[2], acc[3]));
+        for (int u = 0; u < 4; ++u) {
+          const float* r = record(min(k0 + u * W, n - 1));
+          ml[u] = __ldcg(reinterpret_cast<const float2*>(r + 2 * row));
+          x[u] = __ldcg(reinterpret_cast<const float4*>(r + 2 * RT + (int64_t)row * a.hd + e));
+          if (k0 + u * W >= n) ml[u] = make_float2(-INFINITY, 0.0f), x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        const float up = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), m), from = fmaxf(up, -FLT_MAX), f0 = exp2f(m - from);
+        m = up;
+        sum *= f0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[q] *= f0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float f = exp2f(ml[u].x - from);
+          sum += ml[u].y * f;
+          acc[0] += x[u].x * f;
+          acc[1] += x[u].y * f;
+          acc[2] += x[u].z * f;
+          acc[3] += x[u].w * f;
+        }
+      }
+    if constexpr (W > 1) {
+      __syncthreads();   // the elements before have been read
+      if (share > 0) {
+        *reinterpret_cast<float4*>(shared_acc[share][at]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        shared_ml[share][at] = make_float2(m, sum);
+      }
+      __syncthreads();
+      if (share > 0) continue;
+      const int most = min(n, W);
+      float up = m;
+      for (int k = 1; k < most; ++k) up = fmaxf(up, shared_ml[k][at].x);
+      const float from = fmaxf(up, -FLT_MAX), f0 = exp2f(m - from);
+      sum *= f0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[q] *= f0;
+      for (int k = 1; k < most; ++k) {
+        const float f = exp2f(shared_ml[k][at].x - from);
+        sum += shared_ml[k][at].y * f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[q] += shared_acc[k][at][q] * f;
+      }
+    }
+    if (!live) continue;
+    const int p = j.z + row, query = a.by_G(p);
+    T* out = reinterpret_cast<T*>(a.out) + (int64_t)(j.y + query) * a.o_row + (int64_t)(h * a.G + p - query * a.G) * a.o_head + e;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] *= inv;
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(out) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    else *reinterpret_cast<uint2*>(out) = make_uint2(Pair16<T>::put(acc[0], acc[1]), Pair16<T>::put(acc[2], acc[3]));
+  }
 }
 
+template <typename T>
+static cudaError_t launch_join(const PagedArgs& a, int RT, int ctas, cudaStream_t s) {
+  const int W = RT <= 64 ? 8 : 1, parts = (RT * a.hd / 4 * W + kJoinThreads - 1) / kJoinThreads;
+  const dim3 grid(ctas - 1, parts < 16 ? parts : 16);   // most runs end between items: few CTAs each, which go round
+  return launch_k(W == 8 ? paged_combine_kernel<T, 8> : paged_combine_kernel<T, 1>, grid, dim3(kJoinThreads), 0, s, a, RT);
+}
 int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int ctas, cudaStream_t s) {
   if (ctas < 2) return 1;
-  const dim3 grid(ctas - 1, (RT * a.hd / 4 + kJoinThreads - 1) / kJoinThreads);
   PdlScope chained(true);
-  if (dtype == TSB200_F32) TSB_CUDA(launch_k(paged_combine_kernel<float>, grid, dim3(kJoinThreads), 0, s, a, RT));
-  else if (dtype == TSB200_F16) TSB_CUDA(launch_k(paged_combine_kernel<__half>, grid, dim3(kJoinThreads), 0, s, a, RT));
-  else TSB_CUDA(launch_k(paged_combine_kernel<__nv_bfloat16>, grid, dim3(kJoinThreads), 0, s, a, RT));
+  if (dtype == TSB200_F32) TSB_CUDA(launch_join<float>(a, RT, ctas, s));
+  else if (dtype == TSB200_F16) TSB_CUDA(launch_join<__half>(a, RT, ctas, s));
+  else TSB_CUDA(launch_join<__nv_bfloat16>(a, RT, ctas, s));
   count_launch(device);
   return check_launch("paged_combine");
 }
@@ -573,9 +642,21 @@ int TSB200_PagedPlan(int device, const int32_t* cached, const int32_t* fresh, in
   TSB_TRY(use_device(device, &st));
   a.cached = cached; a.fresh = fresh; a.B = B; a.max_blocks = max_blocks; a.num_pages = num_pages; a.rows = rows; a.table = table; a.table_stride = table_stride;
   a.held = held; a.free_pages = free_pages; a.free_count = free_count; a.lens = lens; a.starts = starts; a.slots = slots; a.positions = positions;
-  const int smem = 6 * B * (int)sizeof(int), ctas = 1;
+  // a cluster for many rows
+  const int smem = 6 * B * (int)sizeof(int), ctas = rows > 2048 ? 8 : 1;
   if (smem > 40 * 1024) TSB_CUDA(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 6 * kPlanMaxB * (int)sizeof(int)));
-  paged_plan_kernel<<<ctas, kPlanThreads, smem, pick_stream(st, stream)>>>(a, ctas);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = pick_stream(st, stream);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  TSB_CUDA(cudaLaunchKernelEx(&cfg, paged_plan_kernel, a, ctas));
   count_launch(device);
   return check_launch("paged_plan");
 }
@@ -608,8 +689,18 @@ int TSB200_QKNormRopePaged(int device, int dtype, void* q_out, int64_t o_row, in
   const int V = 16 / (int)dtype_size(dtype);
   const bool wide = ((o_row | o_head | q_row | q_head | k_row | k_head | v_row | v_head | c_page | c_head | c_tok) % V) == 0 &&
                     (((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cacheK | (uintptr_t)cacheV) % 16) == 0;
-  a.rows_here = 1;
-  const dim3 grid((rows + a.rows_here - 1) / a.rows_here);
+  // Few rows: a CTA each, or several, so that every head has its lanes at once; many: eight CTAs of an SM share them, at least a pass of angles each
+  const int L = hd <= 8 ? 1 : hd <= 16 ? 2 : hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32, heads = H + 2 * Hkv, parts = (heads * L + kRopeThreads - 1) / kRopeThreads;
+  const int ctas = 8 * st->sm_count;
+  dim3 grid;
+  if (rows <= ctas / 2) {
+    a.rows_here = 1;
+    grid = dim3(rows, (int64_t)rows * parts <= ctas ? parts : 1);
+  } else {
+    a.rows_here = (rows + ctas - 1) / ctas;
+    if (a.rows_here > kRopeThreads) a.rows_here = kRopeThreads;
+    grid = dim3((rows + a.rows_here - 1) / a.rows_here);
+  }
   cudaStream_t s = pick_stream(st, stream);
 #define TSB_ROPE_PAGED(T)                                                                 \
   do {                                                                                    \

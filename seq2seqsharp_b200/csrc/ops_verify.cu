@@ -5,6 +5,10 @@
 // the last accepted draft from p_i: the smallest t with w_0 + .. + w_t > u (w_0 + .. + w_{V-1}).  So the tokens are distributed as the target's own.
 // Products, differences and sums are 64-bit: u q and p - q are then exact, and a sum's rounding is far below the distance of two fp32 weights, so that
 // the order in which a vocabulary is added up does not decide which token is drawn.
+//
+// A cluster per sequence.  Its warps share the vocabulary in equal runs and push what theirs weigh to every CTA; after one cluster barrier the one warp whose run the
+// draw falls into looks for the token in it.  Rows that no draw needs are not read.  What bounds it: four dependent reads of memory and the launch for few sequences
+// (one of 32000 words: 44 us with one CTA and a run of the vocabulary per thread -> ...), bytes for many.
 #include "kernels.cuh"
 
 namespace tsb {
@@ -20,87 +24,152 @@ struct VerifyArgs {
   const float* u;         // [B, K + 1]: u[K] draws the last token
   int K, V, rows;
 };
-constexpr int kVerifyThreads = 512;
+constexpr int kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32, kVerifyMaxCtas = 8;
 
-__global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __grid_constant__ VerifyArgs a) {
-  __shared__ double sums[kVerifyThreads / 32];
-  __shared__ int found, last;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+__device__ __forceinline__ void push_double(double* local, uint32_t cta, double v) {
+  uint32_t ra;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(cta));
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(ra), "d"(v) : "memory");
+}
+__device__ __forceinline__ double warp_scan(double v, int lane) {   // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+
+__global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __grid_constant__ VerifyArgs a, int ctas) {
+  __shared__ double sums[2][kVerifyMaxCtas * kVerifyWarps];   // of every warp's run: of max(p - q, 0), and of p
+  const int b = (int)blockIdx.x / ctas, rank = (int)blockIdx.x % ctas, tid = threadIdx.x, lane = tid & 31, w = rank * kVerifyWarps + (tid >> 5);
   const int row0 = a.starts ? a.starts[b] : b * (a.K + 1);
   int n = a.starts ? a.starts[b + 1] - row0 : a.K + 1;
   if (row0 < 0 || n < 0 || n > a.rows - row0) n = 0;
   n = min(n, a.K + 1);
   int* out = a.tokens + (int64_t)b * (a.K + 1);
-  if (n == 0) {
-    for (int i = tid; i <= a.K; i += kVerifyThreads) out[i] = -1;
-    if (tid == 0) a.counts[b] = 0;
+  if (n == 0) {   // of all of the cluster's CTAs
+    if (rank == 0) {
+      for (int i = tid; i <= a.K; i += kVerifyThreads) out[i] = -1;
+      if (tid == 0) a.counts[b] = 0;
+    }
     return;
   }
+  cluster_arrive_relaxed();   // the other CTAs exist before anything is pushed to them
   const int* x = a.draft + (int64_t)b * a.K;
   const float* u = a.u + (int64_t)b * (a.K + 1);
-  // every thread tests the drafts for itself: a handful of loads
+  // every warp tests the drafts, a lane each
   int taken = 0;
-  for (; taken < n - 1; ++taken) {
-    const int t = x[taken];
-    if (t < 0 || t >= a.V) break;
-    const double q = a.q ? (double)a.q[((int64_t)b * a.K + taken) * a.q_row + t] : 1.0;
-    if (!((double)u[taken] * q < (double)a.p[(row0 + taken) * a.p_row + t])) break;
-  }
-  const float* p = a.p + (row0 + taken) * a.p_row;
-  const bool refused = taken < n - 1;
-  const float* q = refused && a.q ? a.q + ((int64_t)b * a.K + taken) * a.q_row : nullptr;
-  const int certain = refused && !a.q ? x[taken] : -1;
-  // a thread's run of the vocabulary
-  const int per = (a.V + kVerifyThreads - 1) / kVerifyThreads, v0 = min(a.V, tid * per), v1 = min(a.V, v0 + per);
-  auto weight = [&](int t, bool rest) {
-    double x = (double)p[t];
-    if (rest) x -= q ? (double)q[t] : (t == certain ? 1.0 : 0.0);
-    return x > 0.0 ? x : 0.0;
-  };
-  for (int round = refused ? 0 : 1; round < 2; ++round) {   // where nothing is left of p - q: p itself
-    const bool rest = round == 0;
-    double mine = 0.0;
-    for (int t = v0; t < v1; ++t) mine += weight(t, rest);
-    double s = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
-    }
-    __syncthreads();
-    if (lane == 31) sums[w] = s;
-    if (tid == 0) {
-      found = a.V;
-      last = -1;
-    }
-    __syncthreads();
-    double before = 0.0, all = 0.0;
-    for (int i = 0; i < kVerifyThreads / 32; ++i) {
-      if (i < w) before += sums[i];
-      all += sums[i];
-    }
-    if (!(all > 0.0)) continue;
-    const double r = (double)u[a.K] * all;
-    double at = before + s - mine;
-    int some = -1;
-    for (int t = v0; t < v1; ++t) {
-      const double x = weight(t, rest);
-      at += x;
-      if (x > 0.0) some = t;
-      if (x > 0.0 && at > r) {
-        atomicMin(&found, t);
-        break;
+  for (; taken < n - 1; taken += 32) {
+    const int i = taken + lane;
+    bool ok = false;
+    if (i < n - 1) {
+      const int t = x[i];
+      if (t >= 0 && t < a.V) {
+        const double q = a.q ? (double)a.q[((int64_t)b * a.K + i) * a.q_row + t] : 1.0;
+        ok = (double)u[i] * q < (double)a.p[(int64_t)(row0 + i) * a.p_row + t];
       }
     }
-    if (some >= 0) atomicMax(&last, some);
-    __syncthreads();
-    if (tid == 0 && found == a.V) found = last;   // a sum that rounded below u times the whole
-    __syncthreads();
-    break;
+    const unsigned bad = __ballot_sync(0xffffffffu, !ok);
+    if (bad) {
+      taken += __ffs(bad) - 1;
+      break;
+    }
   }
-  __syncthreads();
-  for (int i = tid; i <= a.K; i += kVerifyThreads) out[i] = i < taken ? x[i] : (i == taken && found < a.V ? found : -1);
-  if (tid == 0) a.counts[b] = taken + 1;
+  taken = min(taken, n - 1);
+  const bool refused = taken < n - 1;
+  const float* p = a.p + (int64_t)(row0 + taken) * a.p_row;
+  const float* q = refused && a.q ? a.q + ((int64_t)b * a.K + taken) * a.q_row : nullptr;
+  const int certain = refused && !a.q ? x[taken] : -1;
+  auto weigh = [&](int t, double& rest, double& all) {
+    const float pt = p[t], qt = q ? q[t] : 0.0f;
+    all = pt > 0.0f ? (double)pt : 0.0;
+    const double r = (double)pt - (q ? (double)qt : (t == certain ? 1.0 : 0.0));
+    rest = r > 0.0 ? r : 0.0;
+  };
+  // this warp's run of the vocabulary, 32 words at a time
+  const int warps = ctas * kVerifyWarps, per = ((a.V + warps - 1) / warps + 31) & ~31, v0 = min((int64_t)a.V, (int64_t)w * per), v1 = min((int64_t)a.V, (int64_t)v0 + per);
+  {
+    double rest = 0.0, all = 0.0;
+#pragma unroll 8
+    for (int t = v0 + lane; t < v1; t += 32) {
+      double r, s;
+      weigh(t, r, s);
+      rest += r;
+      all += s;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      rest += __shfl_xor_sync(0xffffffffu, rest, o);
+      all += __shfl_xor_sync(0xffffffffu, all, o);
+    }
+    cluster_wait();
+    if (lane < ctas) {
+      push_double(&sums[0][w], lane, rest);
+      push_double(&sums[1][w], lane, all);
+    }
+  }
+  cluster_sync();
+  // where nothing is left of p - q: p itself.  A lane has the runs of four neighbouring warps
+  double run[4], before = 0.0, whole = 0.0;
+  bool rest = refused;
+  for (;; rest = false) {
+    double mine = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      run[k] = lane * 4 + k < warps ? sums[rest ? 0 : 1][lane * 4 + k] : 0.0;
+      mine += run[k];
+    }
+    const double to = warp_scan(mine, lane);
+    before = to - mine;
+    whole = __shfl_sync(0xffffffffu, to, 31);
+    if (!rest || whole > 0.0) break;
+  }
+  if (rank == 0) {
+    for (int i = tid; i <= a.K; i += kVerifyThreads)
+      if (i != taken) out[i] = i < taken ? x[i] : -1;
+    if (tid == 0) {
+      a.counts[b] = taken + 1;
+      if (!(whole > 0.0)) out[taken] = -1;
+    }
+  }
+  if (!(whole > 0.0)) return;
+  // the run that the draw falls into; where the sum rounded below u times the whole: the last one that weighs anything
+  const double r = (double)u[a.K] * whole;
+  int hit = 1 << 30, last = -1;
+  double start = 0.0, at = before;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (run[k] > 0.0) {
+      last = lane * 4 + k;
+      if (hit == 1 << 30 && at + run[k] > r) hit = lane * 4 + k, start = at;
+    }
+    at += run[k];
+  }
+  const unsigned any = __ballot_sync(0xffffffffu, hit < 1 << 30);
+  if (any) {
+    const int src = __ffs(any) - 1;
+    hit = __shfl_sync(0xffffffffu, hit, src);
+    start = __shfl_sync(0xffffffffu, start, src);
+  } else {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+    hit = last;
+    start = r;   // its last word
+  }
+  if (hit != w) return;
+  int token = -1, some = -1;
+  for (int t0 = v0; t0 < v1 && token < 0; t0 += 32) {
+    const int t = t0 + lane;
+    double wr = 0.0, wa = 0.0;
+    if (t < v1) weigh(t, wr, wa);
+    const double mine = rest ? wr : wa, to = start + warp_scan(mine, lane);
+    const unsigned over = __ballot_sync(0xffffffffu, any && mine > 0.0 && to > r), weighs = __ballot_sync(0xffffffffu, mine > 0.0);
+    if (weighs) some = t0 + 31 - __clz(weighs);
+    if (over) token = t0 + __ffs(over) - 1;
+    start = __shfl_sync(0xffffffffu, to, 31);
+  }
+  if (lane == 0) out[taken] = token >= 0 ? token : some;
 }
 
 }  // namespace tsb
@@ -113,13 +182,27 @@ int TSB200_VerifyDraft(int device, int32_t* tokens, int32_t* counts, const float
                        const int32_t* starts, const float* u, int B, int K, int V, int rows, void* stream) {
   TSB_CHECK(B >= 0 && K >= 0 && V >= 1 && rows >= 0, "verify_draft: %d sequences, %d drafts, %d words, %d rows", B, K, V, rows);
   TSB_CHECK(starts || (int64_t)B * (K + 1) <= rows, "verify_draft: %d rows, %d sequences of %d drafts need more", rows, B, K);
+  TSB_CHECK((int64_t)B * kVerifyMaxCtas <= 0x7fffffff && V <= 0x40000000, "verify_draft: %d sequences of %d words", B, V);
   if (B == 0) return 1;
   TSB_CHECK(tokens && counts && (p || rows == 0) && (draft || K == 0) && u, "verify_draft: null pointer");
   KeepDevice keep;
   DeviceState* st;
   TSB_TRY(use_device(device, &st));
   VerifyArgs a{tokens, counts, p, q, p_row, q_row, draft, starts, u, K, V, rows};
-  verify_draft_kernel<<<B, kVerifyThreads, 0, pick_stream(st, stream)>>>(a);
+  // as many CTAs to a sequence as are there at once (four on an SM), and at least 512 words to each
+  int ctas = kVerifyMaxCtas;
+  while (ctas > 1 && ((int64_t)B * ctas > 4 * st->sm_count || V < 512 * ctas)) ctas /= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(B * ctas);
+  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.stream = pick_stream(st, stream);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  TSB_CUDA(cudaLaunchKernelEx(&cfg, verify_draft_kernel, a, ctas));
   count_launch(device);
   return check_launch("verify_draft");
 }

@@ -59,54 +59,62 @@ def _target(result, like, sizes=None, dtype=None):
 
 
 _MODEL_DT = {torch.float32: N.F32, torch.float16: N.F16, torch.bfloat16: N.BF16}
+_I32, _F32 = torch.int32, torch.float32
 
 
+# The calls on the paged cache take five microseconds and less on the device, so their checks look at each tensor once, and say what is wrong only when something is.
 def _queue(device):
     """The stream that torch's work on `device` goes to.  Its default stream has the handle 0, which selects the library's own; named as
     cudaStreamLegacy (1) the call takes its place among torch's work there without a wait of the host."""
     return torch._C._cuda_getCurrentRawStream(device) or 1
 
 
-def _placed(op, first, **tensors):
-    """Index of the device that all `tensors` (name=(tensor, dtype)) and `first` lie on."""
-    if not first.is_cuda:
+def _device(op, t):
+    dev = t.get_device()
+    if dev < 0:
         raise N.TSB200Error("%s: the B200 backend only accepts device tensors (no CPU fallback)" % op)
-    dev = first.device
-    for name, (t, dtype) in tensors.items():
-        if t is None:
-            continue
-        if t.dtype != dtype:
-            raise N.TSB200Error("%s: %s is %s, %s is wanted" % (op, name, t.dtype, dtype))
-        if t.device != dev:
-            raise N.TSB200Error("%s: %s is on %s, not on %s" % (op, name, t.device, dev))
-    return dev.index
+    return dev
 
 
-def _plain(op, **tensors):
-    """Contiguous tensors of the given shapes (name=(tensor, shape))."""
-    for name, (t, shape) in tensors.items():
-        if t is not None and (tuple(t.shape) != shape or not t.is_contiguous()):
-            raise N.TSB200Error("%s: %s is %s, contiguous %s is wanted" % (op, name, tuple(t.shape), shape))
+def _wrong(op, dev, dtype, **tensors):
+    """Raises for the first of `tensors` that is not of `dtype` on device `dev`."""
+    for name, t in tensors.items():
+        if t is not None and (t.dtype is not dtype or t.get_device() != dev):
+            raise N.TSB200Error("%s: %s is %s on %s, %s on cuda:%d is wanted" % (op, name, t.dtype, t.device, dtype, dev))
 
 
-def _steps(t):
-    """Strides of all dimensions but the last; those of a single entry mean nothing and are 0."""
-    return [st if n > 1 else 0 for n, st in zip(t.shape[:-1], t.stride())]
+def _plain(op, dev, dtype, name, t, *shape):
+    """Address of a contiguous tensor of this shape."""
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        raise N.TSB200Error("%s: %s is %s of %s on %s, contiguous %s of %s on cuda:%d is wanted" % (op, name, t.dtype, tuple(t.shape), t.device, dtype, shape, dev))
+    return t.data_ptr()
 
 
-def _heads(op, name, t, heads, hd):
-    """Row and head stride of a [rows, heads, hd] tensor."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd or t.stride(2) != 1:
-        raise N.TSB200Error("%s: %s is %s with strides %s, [rows, %d, %d] with elements side by side is wanted" % (op, name, tuple(t.shape), t.stride(), heads, hd))
-    return _steps(t)
+def _heads(op, dev, dtype, name, t, rows, heads, hd):
+    """Address, row and head stride of a [rows, heads, hd] tensor.  The stride of a single entry means nothing and is 0."""
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != (rows, heads, hd) or t.stride(2) != 1:
+        raise N.TSB200Error("%s: %s is %s of %s with strides %s on %s, %s of %s with elements side by side on cuda:%d is wanted" % (
+            op, name, t.dtype, tuple(t.shape), t.stride(), t.device, dtype, (rows, heads, hd), dev))
+    return t.data_ptr(), t.stride(0) if rows > 1 else 0, t.stride(1) if heads > 1 else 0
 
 
-def _cache(op, cacheK, cacheV):
-    """(pages, KV heads, page, head size) and the strides of a paged cache."""
-    if cacheK.dim() != 4 or cacheK.shape != cacheV.shape or _steps(cacheK) != _steps(cacheV) or cacheK.stride(3) != 1 or cacheV.stride(3) != 1:
+def _cache(op, dev, dtype, K, V):
+    """Shape of a paged cache, its addresses and its page, head and token strides."""
+    _wrong(op, dev, dtype, cacheK=K, cacheV=V)
+    shape, steps = K.shape, K.stride()
+    if len(shape) != 4 or V.shape != shape or steps[3] != 1 or (V.stride() != steps and any(n > 1 and x != y for n, x, y in zip(shape, steps, V.stride()))):
         raise N.TSB200Error("%s: keys %s with strides %s and values %s with strides %s, the same [pages, heads, page, head size] with elements side by side is wanted"
-                            % (op, tuple(cacheK.shape), cacheK.stride(), tuple(cacheV.shape), cacheV.stride()))
-    return cacheK.shape, _steps(cacheK)
+                            % (op, tuple(shape), steps, tuple(V.shape), V.stride()))
+    return shape, (K.data_ptr(), V.data_ptr(), steps[0] if shape[0] > 1 else 0, steps[1] if shape[1] > 1 else 0, steps[2])
+
+
+def _table(op, dev, t, B):
+    """Address, row stride and width of a page table."""
+    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != 2 or t.size(0) != B or t.stride(1) != 1:
+        raise N.TSB200Error("%s: table is %s of %s with strides %s on %s, int32 of [%d, pages of a sequence] with entries side by side on cuda:%d is wanted" % (
+            op, t.dtype, tuple(t.shape), t.stride(), t.device, B, dev))
+    width = t.size(1)
+    return t.data_ptr(), t.stride(0) if B > 1 else width, width
 
 
 class Ops:
@@ -292,84 +300,74 @@ class Ops:
     def PagedPlan(cached, fresh, table, held, freePages, freeCount, pageSize, rows):
         """Pages and places for `fresh` [B] new tokens behind `cached` [B] kept ones.  table [B, max_blocks], held [B], freePages [pages] and freeCount [1]
         (all int32) are updated.  Returns lens [B], starts [B + 1], and slots and positions of `rows` rows (-1 behind the granted ones)."""
-        i32 = torch.int32
-        dev = _placed("PagedPlan", cached, cached=(cached, i32), fresh=(fresh, i32), table=(table, i32), held=(held, i32), freePages=(freePages, i32), freeCount=(freeCount, i32))
-        B = cached.shape[0] if cached.dim() == 1 else -1
-        _plain("PagedPlan", cached=(cached, (B,)), fresh=(fresh, (B,)), held=(held, (B,)), freePages=(freePages, (freePages.numel(),)), freeCount=(freeCount, (1,)))
-        if table.dim() != 2 or table.shape[0] != B or table.stride(1) != 1:
-            raise N.TSB200Error("PagedPlan: table is %s, [%d, pages of a sequence] with entries side by side is wanted" % (tuple(table.shape), B))
+        op, dev, B, pages = "PagedPlan", _device("PagedPlan", cached), cached.numel(), freePages.numel()
         if rows < 0:
             raise N.TSB200Error("PagedPlan: %d rows" % rows)
-        lens, starts, slots, positions = torch.empty(2 * B + 1 + 2 * rows, dtype=i32, device=cached.device).split((B, B + 1, rows, rows))
-        N.call("TSB200_PagedPlan", dev, cached.data_ptr(), fresh.data_ptr(), B, pageSize, table.data_ptr(), table.stride(0), table.shape[1], held.data_ptr(),
-               freePages.data_ptr(), freeCount.data_ptr(), freePages.numel(), lens.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), rows, _queue(dev))
-        return lens, starts, slots, positions
+        args = (_plain(op, dev, _I32, "cached", cached, B), _plain(op, dev, _I32, "fresh", fresh, B), B, pageSize, *_table(op, dev, table, B), _plain(op, dev, _I32, "held", held, B),
+                _plain(op, dev, _I32, "freePages", freePages, pages), _plain(op, dev, _I32, "freeCount", freeCount, 1), pages)
+        out = torch.empty(2 * B + 1 + 2 * rows, dtype=_I32, device=cached.device)
+        at = out.data_ptr()
+        N.check(N.lib().TSB200_PagedPlan(dev, *args, at, at + 4 * B, at + 8 * B + 4, at + 8 * B + 4 + 4 * rows, rows, _queue(dev)), "TSB200_PagedPlan")
+        return out.split_with_sizes((B, B + 1, rows, rows))
 
     @staticmethod
     def QKNormRopePaged(result, q, k, v, qNorm, kNorm, eps, positions, slots, cacheK, cacheV, ropeStyle=1, ropeDims=None, base=500000.0):
         """q [rows, H, hd] normed per head (qNorm [hd] or None) and rotated into `result` (None: a new tensor; q itself is allowed); k, v [rows, Hkv, hd] (k
         normed and rotated) to their slots of cacheK, cacheV [pages, Hkv, page, hd].  Rows of slot -1 are left out.  ropeStyle 0 none, 1 pairs (2i, 2i + 1), 2 pairs
         (i, i + ropeDims / 2).  Strides are free but for the elements of a head."""
-        dt, hd = q.dtype, q.shape[-1]
-        if dt not in _MODEL_DT:
-            raise N.TSB200Error("QKNormRopePaged: unsupported dtype %s" % dt)
-        dev = _placed("QKNormRopePaged", q, result=(result, dt), k=(k, dt), v=(v, dt), qNorm=(qNorm, dt), kNorm=(kNorm, dt), positions=(positions, torch.int32),
-                      slots=(slots, torch.int32), cacheK=(cacheK, dt), cacheV=(cacheV, dt))
-        (pages, Hkv, page, c_hd), c_str = _cache("QKNormRopePaged", cacheK, cacheV)
-        rows, H = q.shape[0], q.shape[1] if q.dim() == 3 else 0
-        strides = [_heads("QKNormRopePaged", "q", q, H, c_hd)]
-        r = torch.empty((rows, H, hd), dtype=dt, device=q.device) if result is None else result
-        for name, t, heads in (("k", k, Hkv), ("v", v, Hkv), ("result", r, H)):
-            strides.append(_heads("QKNormRopePaged", name, t, heads, c_hd))
-            if t.shape[0] != rows:
-                raise N.TSB200Error("QKNormRopePaged: %s has %d rows, q %d" % (name, t.shape[0], rows))
-        _plain("QKNormRopePaged", qNorm=(qNorm, (hd,)), kNorm=(kNorm, (hd,)), positions=(positions, (rows,)), slots=(slots, (rows,)))
-        N.call("TSB200_QKNormRopePaged", dev, _MODEL_DT[dt], r.data_ptr(), *strides[3], q.data_ptr(), *strides[0], k.data_ptr(), *strides[1],
-               v.data_ptr(), *strides[2], None if qNorm is None else qNorm.data_ptr(), None if kNorm is None else kNorm.data_ptr(), eps,
-               positions.data_ptr(), slots.data_ptr(), rows, H, Hkv, hd, ropeStyle, hd if ropeDims is None else ropeDims, base, cacheK.data_ptr(), cacheV.data_ptr(),
-               *c_str, pages, page, _queue(dev))
-        return r
+        op, dev, dt = "QKNormRopePaged", _device("QKNormRopePaged", q), q.dtype
+        code = _MODEL_DT.get(dt)
+        if code is None or q.dim() != 3:
+            raise N.TSB200Error("QKNormRopePaged: unsupported q, %s of %s" % (dt, tuple(q.shape)))
+        rows, H, hd = q.shape
+        (pages, Hkv, page, c_hd), c = _cache(op, dev, dt, cacheK, cacheV)
+        q3, k3, v3 = _heads(op, dev, dt, "q", q, rows, H, c_hd), _heads(op, dev, dt, "k", k, rows, Hkv, hd), _heads(op, dev, dt, "v", v, rows, Hkv, hd)
+        qn = None if qNorm is None else _plain(op, dev, dt, "qNorm", qNorm, hd)
+        kn = None if kNorm is None else _plain(op, dev, dt, "kNorm", kNorm, hd)
+        at = _plain(op, dev, _I32, "positions", positions, rows), _plain(op, dev, _I32, "slots", slots, rows)
+        if result is None:
+            result = torch.empty((rows, H, hd), dtype=dt, device=q.device)
+        N.check(N.lib().TSB200_QKNormRopePaged(dev, code, *_heads(op, dev, dt, "result", result, rows, H, hd), *q3, *k3, *v3, qn, kn, eps, *at, rows, H, Hkv, hd, ropeStyle,
+                                               hd if ropeDims is None else ropeDims, base, *c, pages, page, _queue(dev)), "TSB200_QKNormRopePaged")
+        return result
 
     @staticmethod
     def PagedAttention(result, q, cacheK, cacheV, table, starts, lens, maxNew, scale=None, window=0):
         """Attention of packed new rows q [rows, H, hd] over cacheK, cacheV [pages, Hkv, page, hd]: rows starts[b] .. starts[b + 1] are the last tokens of the lens[b]
         of sequence b, whose pages are table[b]; each sees the keys up to its own (window > 0: the last `window` of them).  maxNew: the most rows of a
         sequence.  scale None: 1 / sqrt(hd).  Rows of no sequence keep what `result` held."""
-        dt, i32 = q.dtype, torch.int32
-        if dt not in _MODEL_DT:
-            raise N.TSB200Error("PagedAttention: unsupported dtype %s" % dt)
-        dev = _placed("PagedAttention", q, result=(result, dt), cacheK=(cacheK, dt), cacheV=(cacheV, dt), table=(table, i32), starts=(starts, i32), lens=(lens, i32))
-        (pages, Hkv, page, hd), c_str = _cache("PagedAttention", cacheK, cacheV)
-        rows, H = q.shape[0], q.shape[1] if q.dim() == 3 else 0
-        q_str = _heads("PagedAttention", "q", q, H, hd)
-        r = torch.empty((rows, H, hd), dtype=dt, device=q.device) if result is None else result
-        r_str = _heads("PagedAttention", "result", r, H, hd)
-        if r.shape[0] != rows:
-            raise N.TSB200Error("PagedAttention: result has %d rows, q %d" % (r.shape[0], rows))
-        B = table.shape[0]
-        if table.dim() != 2 or table.stride(1) != 1:
-            raise N.TSB200Error("PagedAttention: table is %s, [sequences, pages of a sequence] with entries side by side is wanted" % (tuple(table.shape),))
-        _plain("PagedAttention", starts=(starts, (B + 1,)), lens=(lens, (B,)))
-        ws_bytes = N.lib().TSB200_PagedAttentionWorkspaceBytes(_MODEL_DT[dt], H, Hkv, hd, maxNew)
+        op, dev, dt = "PagedAttention", _device("PagedAttention", q), q.dtype
+        code = _MODEL_DT.get(dt)
+        if code is None or q.dim() != 3:
+            raise N.TSB200Error("PagedAttention: unsupported q, %s of %s" % (dt, tuple(q.shape)))
+        rows, H, hd = q.shape
+        (pages, Hkv, page, c_hd), c = _cache(op, dev, dt, cacheK, cacheV)
+        q3, B = _heads(op, dev, dt, "q", q, rows, H, c_hd), lens.numel()
+        args = (*c, pages, page, *_table(op, dev, table, B), _plain(op, dev, _I32, "starts", starts, B + 1), _plain(op, dev, _I32, "lens", lens, B), B, rows, maxNew, H, Hkv, hd,
+                hd ** -0.5 if scale is None else scale, window)
+        if result is None:
+            result = torch.empty((rows, H, hd), dtype=dt, device=q.device)
+        L = N.lib()
+        ws_bytes = L.TSB200_PagedAttentionWorkspaceBytes(code, H, Hkv, hd, maxNew)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-        N.call("TSB200_PagedAttention", dev, _MODEL_DT[dt], r.data_ptr(), *r_str, q.data_ptr(), *q_str, cacheK.data_ptr(), cacheV.data_ptr(), *c_str, pages, page, table.data_ptr(), table.stride(0), table.shape[1], starts.data_ptr(), lens.data_ptr(), B, rows, maxNew, H, Hkv, hd,
-               hd ** -0.5 if scale is None else scale, window, ws.data_ptr(), ws_bytes, _queue(dev))
-        return r
+        N.check(L.TSB200_PagedAttention(dev, code, *_heads(op, dev, dt, "result", result, rows, H, hd), *q3, *args, ws.data_ptr(), ws_bytes, _queue(dev)), "TSB200_PagedAttention")
+        return result
 
     @staticmethod
     def VerifyDraft(targetProbs, draftProbs, draftTokens, u, starts=None):
         """targetProbs [rows, V], draftProbs [B * K, V] (None: the drafts were certain), draftTokens [B, K], u [B, K + 1] uniform numbers; rows starts[b] ..
         starts[b + 1] (None: K + 1 each) of sequence b.  Returns tokens [B, K + 1] (accepted drafts, one drawn token, -1 behind) and counts [B]."""
-        f32, i32 = torch.float32, torch.int32
-        dev = _placed("VerifyDraft", targetProbs, targetProbs=(targetProbs, f32), draftProbs=(draftProbs, f32), draftTokens=(draftTokens, i32), u=(u, f32), starts=(starts, i32))
+        op, dev = "VerifyDraft", _device("VerifyDraft", targetProbs)
         if targetProbs.dim() != 2 or draftTokens.dim() != 2:
             raise N.TSB200Error("VerifyDraft: targetProbs [rows, words] and draftTokens [sequences, drafts] are wanted")
         (rows, V), (B, K) = targetProbs.shape, draftTokens.shape
-        _plain("VerifyDraft", draftTokens=(draftTokens, (B, K)), u=(u, (B, K + 1)), starts=(starts, (B + 1,)))
+        _wrong(op, dev, _F32, targetProbs=targetProbs, draftProbs=draftProbs)
         for name, t, n in (("targetProbs", targetProbs, rows), ("draftProbs", draftProbs, B * K)):
-            if t is not None and (tuple(t.shape) != (n, V) or (V > 1 and t.stride(1) != 1)):
+            if t is not None and (t.shape != (n, V) or (V > 1 and t.stride(1) != 1)):
                 raise N.TSB200Error("VerifyDraft: %s is %s, [%d, %d] with words side by side is wanted" % (name, tuple(t.shape), n, V))
-        tokens, counts = torch.empty((B, K + 1), dtype=i32, device=u.device), torch.empty(B, dtype=i32, device=u.device)
-        N.call("TSB200_VerifyDraft", dev, tokens.data_ptr(), counts.data_ptr(), targetProbs.data_ptr(), targetProbs.stride(0), None if draftProbs is None else draftProbs.data_ptr(),
-               0 if draftProbs is None else draftProbs.stride(0), draftTokens.data_ptr(), None if starts is None else starts.data_ptr(), u.data_ptr(), B, K, V, rows, _queue(dev))
-        return tokens, counts
+        args = (targetProbs.data_ptr(), targetProbs.stride(0), None if draftProbs is None else draftProbs.data_ptr(), 0 if draftProbs is None else draftProbs.stride(0),
+                _plain(op, dev, _I32, "draftTokens", draftTokens, B, K), None if starts is None else _plain(op, dev, _I32, "starts", starts, B + 1),
+                _plain(op, dev, _F32, "u", u, B, K + 1), B, K, V, rows)
+        out = torch.empty(B * (K + 2), dtype=_I32, device=u.device)
+        N.check(N.lib().TSB200_VerifyDraft(dev, out.data_ptr(), out.data_ptr() + 4 * B * (K + 1), *args, _queue(dev)), "TSB200_VerifyDraft")
+        return out[:B * (K + 1)].view(B, K + 1), out[B * (K + 1):]
