@@ -144,164 +144,194 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs a, in
 struct RopePagedArgs {
   void* out;
   const void *q, *k, *v, *q_norm, *k_norm;
-  int64_t o_row, o_head, q_row, q_head, k_row, k_head, v_row, v_head;
+  int o_row, o_head, q_row, q_head, k_row, k_head, v_row, v_head;   // 32 bits: one multiplication for an address
   float eps;
   const int *positions, *slots;
   int rows, H, Hkv, hd, rot, style;   // style 0: no rotation, 1: pairs (2i, 2i + 1), 2: pairs (i, i + rot / 2)
   double first, ratio;                // half turns per position of pair 0; of pair i: first * ratio^i
   void *K, *V;
-  int64_t c_page, c_head, c_tok;
+  int c_page, c_head, c_tok;
   int num_pages, page_shift;
   int rows_here;                      // rows per CTA
 };
-constexpr int kRopeThreads = 256, kRopeMaxHd = 256;
+constexpr int kRopeThreads = 256, kRopeMaxHd = 256, kRopeTurns = 1024;
 
+// eight elements as they lie in memory, four at p0 and four at p1: WIDE by 8 or 16 bytes, else one by one
 template <typename T, bool WIDE>
-__device__ __forceinline__ void rope_load8(const T* p, float* f) {
-  if constexpr (!WIDE) {
+struct Eight {
+  static constexpr int N = WIDE ? (sizeof(T) == 4 ? 8 : 4) : 8;   // registers
+  uint32_t r[N];
+  template <bool WHOLE>   // p1 = p0 + 4
+  __device__ __forceinline__ void load(const T* p0, const T* p1) {
+    if constexpr (!WIDE) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = to_f<T>(p[e]);
-  } else if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t r[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 t = Pair16<T>::get(r[e]);
-      f[2 * e] = t.x;
-      f[2 * e + 1] = t.y;
+      for (int e = 0; e < 4; ++e) r[e] = __float_as_uint(to_f<T>(p0[e])), r[4 + e] = __float_as_uint(to_f<T>(p1[e]));
+    } else if constexpr (N == 8) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p0), y = *reinterpret_cast<const uint4*>(p1);
+      r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w;
+      r[4] = y.x; r[5] = y.y; r[6] = y.z; r[7] = y.w;
+    } else if constexpr (WHOLE) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p0);
+      r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(p0), y = *reinterpret_cast<const uint2*>(p1);
+      r[0] = x.x; r[1] = x.y; r[2] = y.x; r[3] = y.y;
     }
   }
-}
-template <typename T, bool WIDE>
-__device__ __forceinline__ void rope_store8(T* p, const float* f) {
-  if constexpr (!WIDE) {
+  __device__ __forceinline__ void get(float* f) const {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) p[e] = from_f<T>(f[e]);
-  } else if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-  } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(Pair16<T>::put(f[0], f[1]), Pair16<T>::put(f[2], f[3]), Pair16<T>::put(f[4], f[5]), Pair16<T>::put(f[6], f[7]));
+    for (int i = 0; i < N; ++i) {
+      if constexpr (N == 8) {
+        f[i] = __uint_as_float(r[i]);
+      } else {
+        const float2 t = Pair16<T>::get(r[i]);
+        f[2 * i] = t.x;
+        f[2 * i + 1] = t.y;
+      }
+    }
   }
-}
+  template <bool WHOLE>
+  static __device__ __forceinline__ void store(T* p0, T* p1, const float* f) {
+    if constexpr (!WIDE) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) p0[e] = from_f<T>(f[e]), p1[e] = from_f<T>(f[4 + e]);
+    } else if constexpr (N == 8) {
+      *reinterpret_cast<float4*>(p0) = make_float4(f[0], f[1], f[2], f[3]);
+      *reinterpret_cast<float4*>(p1) = make_float4(f[4], f[5], f[6], f[7]);
+    } else if constexpr (WHOLE) {
+      *reinterpret_cast<uint4*>(p0) = make_uint4(Pair16<T>::put(f[0], f[1]), Pair16<T>::put(f[2], f[3]), Pair16<T>::put(f[4], f[5]), Pair16<T>::put(f[6], f[7]));
+    } else {
+      *reinterpret_cast<uint2*>(p0) = make_uint2(Pair16<T>::put(f[0], f[1]), Pair16<T>::put(f[2], f[3]));
+      *reinterpret_cast<uint2*>(p1) = make_uint2(Pair16<T>::put(f[4], f[5]), Pair16<T>::put(f[6], f[7]));
+    }
+  }
+};
 
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_paged_kernel(const __grid_constant__ RopePagedArgs a) {
+// STYLE as in RopePagedArgs; LT: lanes of a head, 0: as many as its size needs
+template <typename T, bool WIDE, int STYLE, int LT>
+__global__ void __launch_bounds__(kRopeThreads, WIDE && sizeof(T) == 2 ? 6 : 4) qk_norm_rope_paged_kernel(const __grid_constant__ RopePagedArgs a) {
+  constexpr bool WHOLE = STYLE != 2;
   __shared__ __align__(16) float wq[kRopeMaxHd], wk[kRopeMaxHd];
-  __shared__ __align__(16) float2 turn[kRopeThreads];
-  __shared__ int place[kRopeThreads];
-  const int tid = threadIdx.x, half = a.rot / 2, lane = tid & 31;
-  const bool turns = a.style != 0;
-  // a pass: as many rows as the CTA has threads for their angles
-  const int rows_pass = turns ? kRopeThreads / half : a.rows_here;
-  const int ar = turns ? tid / half : 0, ai = turns ? tid - ar * half : 0;
-  const double rate = turns ? a.first * pow(a.ratio, (double)ai) : 0.0;   // half turns per position
+  __shared__ __align__(16) float2 turn[kRopeTurns];
+  __shared__ int place[kRopeTurns];
+  const int tid = threadIdx.x, half = a.rot / 2;
+  // angles of a row, filled up to whole fours of pairs with turns by nothing; a pass: as many rows as there is room for
+  const int slots = STYLE ? (half + 3) / 4 * 4 : 0, rows_pass = STYLE ? kRopeTurns / slots : kRopeTurns;
+  // a thread makes the angles of one pair, of every (256 / slots)-th row
+  const int turn_rows = STYLE ? kRopeThreads / slots : 1, ar = STYLE ? tid / slots : 0, ai = STYLE ? tid - ar * slots : 0;
+  const double rate = STYLE && ai < half ? a.first * pow(a.ratio, (double)ai) : 0.0;   // half turns per position
   for (int e = tid; e < a.hd; e += kRopeThreads) {
     wq[e] = a.q_norm ? to_f<T>(reinterpret_cast<const T*>(a.q_norm)[e]) : 1.0f;
     wk[e] = a.k_norm ? to_f<T>(reinterpret_cast<const T*>(a.k_norm)[e]) : 1.0f;
   }
-  int L = 1;
-  while (L * 8 < a.hd) L <<= 1;
+  int L = LT ? LT : 1;
+  if (LT == 0)
+    while (L * 8 < a.hd) L <<= 1;
   const int li = tid & (L - 1), per = kRopeThreads / L, heads = a.H + 2 * a.Hkv;
-  const bool on = li * 8 < a.hd;
-  // style 2: the partner of element e < rot / 2 is e + rot / 2, whole lanes away
-  const int away = half / 8, low = li < away;
-  const int from = (lane & ~(L - 1)) + (li * 8 < a.rot ? (low ? li + away : li - away) : li);
+  const bool on = li * 8 < a.hd, turned = STYLE && li * 8 < a.rot, norms = a.q_norm || a.k_norm;
+  const float inv_hd = 1.0f / (float)a.hd;
+  // a lane has four elements and the four that they turn with (pairs (i, i + rot / 2)), or eight neighbours
+  const int e0 = STYLE == 2 && turned ? li * 4 : li * 8, e1 = STYLE == 2 && turned ? half + li * 4 : e0 + 4;
   const int places = a.num_pages << a.page_shift;
   const int row_first = (int)blockIdx.x * a.rows_here, row_end = min(a.rows, row_first + a.rows_here);
   for (int row0 = row_first; row0 < row_end; row0 += rows_pass) {
     const int n = min(rows_pass, row_end - row0);
     __syncthreads();   // the pass before is done with both
-    if (turns && ar < n) {
-      double x = (double)a.positions[row0 + ar] * rate;
-      x -= 2.0 * rint(0.5 * x);
-      float s, c;
-      sincospif((float)x, &s, &c);
-      turn[tid] = make_float2(c, s);
-    }
-    if (tid < n) {
-      const int slot = a.slots[row0 + tid];
-      place[tid] = slot >= 0 && slot < places ? slot : -1;
+    if (STYLE && ar < turn_rows)
+      for (int r = ar; r < n; r += turn_rows) {
+        double x = (double)a.positions[row0 + r] * rate;
+        x -= 2.0 * rint(0.5 * x);
+        float s, c;
+        sincospif((float)x, &s, &c);
+        turn[r * slots + ai] = make_float2(c, s);
+      }
+    for (int r = tid; r < n; r += kRopeThreads) {
+      const int slot = a.slots[row0 + r];
+      place[r] = slot >= 0 && slot < places ? slot : -1;
     }
     __syncthreads();
     // (row, head) pairs go round the groups of L lanes; the next one is on its way while one is turned
+    const int stride = per * (int)gridDim.y, passes = (n * heads + stride - 1) / stride;
     int head = (int)blockIdx.y * per + tid / L, r = 0;
-    const int stride = per * (int)gridDim.y;
-    auto settle = [&]() {
+    Eight<T, WIDE> ahead;
+    int slot = -1;
+    auto fetch = [&]() {
       while (head >= heads) {
         head -= heads;
         ++r;
       }
-    };
-    auto source = [&]() {
+      slot = r < n && on ? place[r] : -1;
+      if (slot < 0) return;
       const int64_t row = row0 + r;
-      return (head < a.H ? reinterpret_cast<const T*>(a.q) + row * a.q_row + head * a.q_head
-                         : (head >= a.H + a.Hkv ? reinterpret_cast<const T*>(a.v) + row * a.v_row + (head - a.H - a.Hkv) * a.v_head
-                                                : reinterpret_cast<const T*>(a.k) + row * a.k_row + (head - a.H) * a.k_head)) + li * 8;
+      const T* p = head < a.H ? reinterpret_cast<const T*>(a.q) + row * a.q_row + (int64_t)head * a.q_head
+                              : (head < a.H + a.Hkv ? reinterpret_cast<const T*>(a.k) + row * a.k_row + (int64_t)(head - a.H) * a.k_head
+                                                    : reinterpret_cast<const T*>(a.v) + row * a.v_row + (int64_t)(head - a.H - a.Hkv) * a.v_head);
+      ahead.template load<WHOLE>(p + e0, p + e1);
     };
-    float ahead[8];
-    auto fetch = [&]() {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ahead[e] = 0.0f;
-      if (r < n && on && place[r] >= 0) rope_load8<T, WIDE>(source(), ahead);
-    };
-    settle();
+    for (int i = 0; i < Eight<T, WIDE>::N; ++i) ahead.r[i] = 0u;
     fetch();
-    while (__any_sync(0xffffffffu, r < n)) {
+#pragma unroll 1
+    for (int pass = 0; pass < passes; ++pass) {
       float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = ahead[e];
-      const int hd_now = head, r_now = r, row = row0 + r, slot = r < n ? place[r] : -1;
-      const bool there = on && slot >= 0, is_q = hd_now < a.H, is_v = hd_now >= a.H + a.Hkv;
+      ahead.get(x);
+      const int head_now = head, r_now = r, slot_now = slot;
+      const bool is_q = head_now < a.H, is_v = head_now >= a.H + a.Hkv;
       head += stride;
-      settle();
       fetch();
-      float ss = 0.0f;
+      if (norms) {
+        float ss = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-      for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (!is_v && on && (is_q ? a.q_norm : a.k_norm) != nullptr) {
-        const float f = 1.0f / sqrtf(ss / (float)a.hd + a.eps);
-        const float4* w = reinterpret_cast<const float4*>((is_q ? wq : wk) + li * 8);
-        const float4 w0 = w[0], w1 = w[1];
-        x[0] *= f * w0.x; x[1] *= f * w0.y; x[2] *= f * w0.z; x[3] *= f * w0.w;
-        x[4] *= f * w1.x; x[5] *= f * w1.y; x[6] *= f * w1.z; x[7] *= f * w1.w;
+        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+        if constexpr (LT > 0) {
+#pragma unroll
+          for (int o = LT / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        } else {
+          for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        }
+        if (on && !is_v && (is_q ? a.q_norm : a.k_norm)) {
+          const float f = rsqrtf(ss * inv_hd + a.eps);   // off by two units in the last place, which the rounding to 16 bits and the sum of squares exceed
+          const float* w = is_q ? wq : wk;
+          const float4 w0 = *reinterpret_cast<const float4*>(w + e0), w1 = *reinterpret_cast<const float4*>(w + e1);
+          x[0] *= f * w0.x; x[1] *= f * w0.y; x[2] *= f * w0.z; x[3] *= f * w0.w;
+          x[4] *= f * w1.x; x[5] *= f * w1.y; x[6] *= f * w1.z; x[7] *= f * w1.w;
+        }
       }
-      if (a.style == 1) {
-        if (!is_v)
+      if (slot_now >= 0) {
+        if (STYLE && turned && !is_v) {
+          const float4* t = reinterpret_cast<const float4*>(turn + r_now * slots + li * 4);
+          const float4 t0 = t[0], t1 = t[1];
+          const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y, t0.w, t1.y, t1.w};
 #pragma unroll
-          for (int e = 0; e < 8; e += 2)
-            if (li * 8 + e < a.rot && r_now < n) {
-              const float2 t = turn[r_now * half + (li * 8 + e) / 2];
-              const float y0 = x[e] * t.x - x[e + 1] * t.y, y1 = x[e + 1] * t.x + x[e] * t.y;
-              x[e] = y0;
-              x[e + 1] = y1;
-            }
-      } else if (a.style == 2) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = __shfl_sync(0xffffffffu, x[e], from);
-          if (!is_v && li * 8 < a.rot && r_now < n) {
-            const float2 t = turn[r_now * half + (low ? li : li - away) * 8 + e];
-            x[e] = low ? x[e] * t.x - y * t.y : x[e] * t.x + y * t.y;
+          for (int i = 0; i < 4; ++i) {
+            float &u = x[STYLE == 2 ? i : 2 * i], &v = x[STYLE == 2 ? 4 + i : 2 * i + 1];
+            const float y0 = u * c[i] - v * s[i], y1 = v * c[i] + u * s[i];
+            u = y0;
+            v = y1;
           }
         }
-      }
-      if (there) {
         T* dst;
-        if (is_q) {
-          dst = reinterpret_cast<T*>(a.out) + row * a.o_row + hd_now * a.o_head;
-        } else {
-          const int64_t at = (int64_t)(slot >> a.page_shift) * a.c_page + (int64_t)(slot & ((1 << a.page_shift) - 1)) * a.c_tok + (is_v ? hd_now - a.H - a.Hkv : hd_now - a.H) * a.c_head;
-          dst = reinterpret_cast<T*>(is_v ? a.V : a.K) + at;
-        }
-        rope_store8<T, WIDE>(dst + li * 8, x);
+        if (is_q) dst = reinterpret_cast<T*>(a.out) + (int64_t)(row0 + r_now) * a.o_row + (int64_t)head_now * a.o_head;
+        else
+          dst = reinterpret_cast<T*>(is_v ? a.V : a.K) + (int64_t)(slot_now >> a.page_shift) * a.c_page + (int64_t)(slot_now & ((1 << a.page_shift) - 1)) * a.c_tok +
+                (int64_t)(head_now - (is_v ? a.H + a.Hkv : a.H)) * a.c_head;
+        Eight<T, WIDE>::template store<WHOLE>(dst + e0, dst + e1, x);
       }
     }
   }
+}
+
+template <typename T, bool WIDE, int STYLE>
+static void launch_rope_paged_l(const RopePagedArgs& a, dim3 grid, cudaStream_t s) {
+  if (WIDE && a.hd > 32 && a.hd <= 64) qk_norm_rope_paged_kernel<T, WIDE, STYLE, WIDE ? 8 : 0><<<grid, kRopeThreads, 0, s>>>(a);
+  else if (WIDE && a.hd > 64 && a.hd <= 128) qk_norm_rope_paged_kernel<T, WIDE, STYLE, WIDE ? 16 : 0><<<grid, kRopeThreads, 0, s>>>(a);
+  else qk_norm_rope_paged_kernel<T, WIDE, STYLE, 0><<<grid, kRopeThreads, 0, s>>>(a);
+}
+template <typename T, bool WIDE>
+static void launch_rope_paged(const RopePagedArgs& a, dim3 grid, cudaStream_t s) {
+  if (a.style == 0) launch_rope_paged_l<T, WIDE, 0>(a, grid, s);
+  else if (a.style == 1) launch_rope_paged_l<T, WIDE, 1>(a, grid, s);
+  else launch_rope_paged_l<T, WIDE, 2>(a, grid, s);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------ attention, every type
@@ -391,7 +421,9 @@ __global__ void __launch_bounds__(kFmaThreads) paged_fma_kernel(const __grid_con
           const float4 k4 = *reinterpret_cast<const float4*>(ks + lane * RB + e * 16);
           kf[0] = k4.x; kf[1] = k4.y; kf[2] = k4.z; kf[3] = k4.w;
         } else {
-          rope_load8<T, true>(reinterpret_cast<const T*>(ks + lane * RB + e * 16), kf);
+          Eight<T, true> k8;
+          k8.template load<true>(reinterpret_cast<const T*>(ks + lane * RB + e * 16), nullptr);
+          k8.get(kf);
         }
 #pragma unroll
         for (int r = 0; r < RW; ++r) {
@@ -680,32 +712,33 @@ int TSB200_QKNormRopePaged(int device, int dtype, void* q_out, int64_t o_row, in
   KeepDevice keep;
   DeviceState* st;
   TSB_TRY(use_device(device, &st));
+  for (const int64_t stride : {o_row, o_head, q_row, q_head, k_row, k_head, v_row, v_head, c_page, c_head, c_tok})
+    TSB_CHECK(stride >= 0 && stride <= 0x7fffffff, "qk_norm_rope_paged: a stride of %lld elements", (long long)stride);
   a.out = q_out; a.q = q; a.k = k; a.v = v; a.q_norm = q_norm; a.k_norm = k_norm;
-  a.o_row = o_row; a.o_head = o_head; a.q_row = q_row; a.q_head = q_head; a.k_row = k_row; a.k_head = k_head; a.v_row = v_row; a.v_head = v_head;
+  a.o_row = (int)o_row; a.o_head = (int)o_head; a.q_row = (int)q_row; a.q_head = (int)q_head; a.k_row = (int)k_row; a.k_head = (int)k_head; a.v_row = (int)v_row; a.v_head = (int)v_head;
   a.eps = eps; a.positions = positions; a.slots = slots; a.rows = rows; a.H = H; a.Hkv = Hkv; a.hd = hd; a.rot = rope_style ? rope_dims : 0; a.style = rope_style;
   a.first = 1.0 / 3.14159265358979323846;
   a.ratio = rope_style ? std::pow(rope_base, -2.0 / rope_dims) : 1.0;
-  a.K = cacheK; a.V = cacheV; a.c_page = c_page; a.c_head = c_head; a.c_tok = c_tok; a.num_pages = num_pages;
+  a.K = cacheK; a.V = cacheV; a.c_page = (int)c_page; a.c_head = (int)c_head; a.c_tok = (int)c_tok; a.num_pages = num_pages;
   const int V = 16 / (int)dtype_size(dtype);
   const bool wide = ((o_row | o_head | q_row | q_head | k_row | k_head | v_row | v_head | c_page | c_head | c_tok) % V) == 0 &&
                     (((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cacheK | (uintptr_t)cacheV) % 16) == 0;
-  // Few rows: a CTA each, or several, so that every head has its lanes at once; many: eight CTAs of an SM share them, at least a pass of angles each
+  // Few rows: a CTA each, or several, so that every head has its lanes at once; many: six CTAs of an SM share them, at least a pass of angles each
   const int L = hd <= 8 ? 1 : hd <= 16 ? 2 : hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32, heads = H + 2 * Hkv, parts = (heads * L + kRopeThreads - 1) / kRopeThreads;
-  const int ctas = 8 * st->sm_count;
+  const int ctas = 6 * st->sm_count;
   dim3 grid;
   if (rows <= ctas / 2) {
     a.rows_here = 1;
     grid = dim3(rows, (int64_t)rows * parts <= ctas ? parts : 1);
   } else {
     a.rows_here = (rows + ctas - 1) / ctas;
-    if (a.rows_here > kRopeThreads) a.rows_here = kRopeThreads;
     grid = dim3((rows + a.rows_here - 1) / a.rows_here);
   }
   cudaStream_t s = pick_stream(st, stream);
 #define TSB_ROPE_PAGED(T)                                                                 \
   do {                                                                                    \
-    if (wide) qk_norm_rope_paged_kernel<T, true><<<grid, kRopeThreads, 0, s>>>(a);        \
-    else qk_norm_rope_paged_kernel<T, false><<<grid, kRopeThreads, 0, s>>>(a);            \
+    if (wide) launch_rope_paged<T, true>(a, grid, s);                                     \
+    else launch_rope_paged<T, false>(a, grid, s);                                         \
   } while (0)
   if (dtype == TSB200_F32) TSB_ROPE_PAGED(float);
   else if (dtype == TSB200_F16) TSB_ROPE_PAGED(__half);
