@@ -46,6 +46,10 @@ __device__ __forceinline__ void pt_prefetch_4d(const CUtensorMap* map, int c0, i
   asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
 }
 
+// A row's output is rescaled when its maximum is this much (in powers of two) above the one in use: weights are then up to 2^8, which neither type loses
+// anything by, and one of a warp's 32 rows has a new maximum in nearly every tile of the first hundred
+constexpr float kPtLag = 8.0f;
+
 // key tiles of the run that the two row tiles of an item need
 struct PtCounts {
   int n[2], most;
@@ -269,62 +273,63 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
         tc_land(s_u32(k_full), NS, ks);
         tc_land(s_u32(v_full), NS, vs);
       }
-    } else if (lane == 0) {
-      // ---------------- products.  Instruction descriptors: fp32 accumulator, A K-major, 128 rows; K: N = 128 K-major; V: N = HD MN-major
+    } else {
+      // ---------------- products, issued by whole warps: 32 of them to a unit leave no time for a single lane's descriptors (2.35 -> ... us a unit).
+      // Instruction descriptors: fp32 accumulator, A K-major, 128 rows; K: N = 128 K-major; V: N = HD MN-major
       const uint32_t fmt = (1u << 4) | (Pair16<H>::kUmmaFormat << 7) | (Pair16<H>::kUmmaFormat << 10) | ((uint32_t)(kPtRows >> 4) << 24);
       const uint32_t id_qk = fmt | ((uint32_t)(kPtKeys >> 3) << 17), id_pv = fmt | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
+      const uint32_t hi = desc_hi(1024);
       uint32_t kc = 0, qc = 0, pc[2] = {0, 0}, oc[2] = {0, 0};
       bool ok = true;
-      auto qk = [&](int t, uint32_t st) {
-        const uint32_t q = sQ + t * BX * kPtBox, k = sK + st * BX * kPtBox;
-#pragma unroll
-        for (int i = 0; i < BX * 4; ++i) {
-          const uint32_t off = (i >> 2) * kPtBox + (i & 3) * 32;
-          umma_f16(tmem + t * kPtKeys, make_desc(q + off, 16, 1024), make_desc(k + off, 16, 1024), id_qk, i > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[t]);
-      };
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return tc_wait_or(s_u32(bar), parity & 1, err, a.wait_limit); };
       auto landed = [&](uint64_t* bar, uint32_t parity) {
-        const bool in = pa_wait(bar, parity, err, a.wait_limit);
+        const bool in = wait(bar, parity);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         return in;
       };
-      PagedRun run;
-      run.begin(a, plan, kPtTile);
-      for (; ok && run.next(a, plan, kPtTile, kPtKeys); run.step(a)) {
+      auto qk = [&](int t, uint32_t st) {
+        const uint32_t q = desc_lo(sQ + t * BX * kPtBox, 16), k = desc_lo(sK + st * BX * kPtBox, 16);
+#pragma unroll
+        for (int i = 0; i < BX * 4; ++i) {
+          const uint32_t off = ((i >> 2) * kPtBox + (i & 3) * 32) >> 4;
+          umma_el(tmem + t * kPtKeys, q + off, hi, k + off, hi, id_qk, i > 0 ? 1u : 0u);
+        }
+        umma_commit_el(s_u32(&s_full[t]));
+      };
+      while (ok && next_item()) {
         const PtCounts n = pt_counts(a, run);
         if (n.most == 0) continue;
-        ok = landed(q_full, qc & 1) && landed(&k_full[kc % NS], (kc / NS) & 1);
+        ok = landed(q_full, qc) && landed(&k_full[kc % NS], kc / NS);
         ++qc;
         if (!ok) break;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
           if (n.n[t] > 0) qk(t, kc % NS);
-        umma_commit(&k_empty[kc % NS]);
-        if (n.most == 1) umma_commit(q_empty);
+        umma_commit_el(s_u32(&k_empty[kc % NS]));
+        if (n.most == 1) umma_commit_el(s_u32(q_empty));
         for (int j = 0; j < n.most && ok; ++j) {
           const bool more = j + 1 < n.most;
           const uint32_t c = kc + j, st = c % NS, next = (c + 1) % NS;
-          ok = landed(&v_full[st], (c / NS) & 1);
-          if (ok && more) ok = landed(&k_full[next], ((c + 1) / NS) & 1);
+          ok = landed(&v_full[st], c / NS);
+          if (ok && more) ok = landed(&k_full[next], (c + 1) / NS);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (!ok || j >= n.n[t]) continue;
-            ok = pa_wait(&p_full[t], pc[t]++ & 1, err, a.wait_limit);
-            if (ok && j == 0 && oc[t]++ > 0) ok = pa_wait(&o_empty[t], oc[t] & 1, err, a.wait_limit);   // the output of the item before has been read
+            ok = wait(&p_full[t], pc[t]++);
+            if (ok && j == 0 && oc[t]++ > 0) ok = wait(&o_empty[t], oc[t]);   // the output of the item before has been read
             if (!ok) continue;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             // V stage = [box][128 keys][128 B]: 8-key groups 1024 B apart (SBO), boxes kPtBox apart (LBO); 16 keys = 2048 B
-            const uint32_t v = sV + st * BX * kPtBox;
+            const uint32_t v = desc_lo(sV + st * BX * kPtBox, kPtBox);
 #pragma unroll
             for (int i = 0; i < kPtKeys / 16; ++i)
-              pa_umma_ts(tmem + 2 * kPtKeys + t * HD, tmem + t * kPtKeys + i * 8, make_desc(v + i * 2048, kPtBox, 1024), id_pv, (j > 0 || i > 0) ? 1u : 0u);
+              pa_umma_ts_el(tmem + 2 * kPtKeys + t * HD, tmem + t * kPtKeys + i * 8, v + i * (2048 >> 4), hi, id_pv, (j > 0 || i > 0) ? 1u : 0u);
             if (j + 1 < n.n[t]) qk(t, next);
-            else umma_commit(&o_full[t]);
+            else umma_commit_el(s_u32(&o_full[t]));
           }
-          umma_commit(&v_empty[st]);
-          if (more) umma_commit(&k_empty[next]);
-          if (j + 2 == n.most) umma_commit(q_empty);
+          umma_commit_el(s_u32(&v_empty[st]));
+          if (more) umma_commit_el(s_u32(&k_empty[next]));
+          if (j + 2 == n.most) umma_commit_el(s_u32(q_empty));
         }
         kc += n.most;
       }
@@ -386,13 +391,15 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
         for (int q = 0; q < 4; ++q) mx[q] = __uint_as_float(x[q][0]);
 #pragma unroll
-        for (int i = 1; i < 32; ++i)
+        for (int i = 1; i < 31; i += 2)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], __uint_as_float(x[q][i]));
+          for (int q = 0; q < 4; ++q) mx[q] = fmaxf(fmaxf(mx[q], __uint_as_float(x[q][i])), __uint_as_float(x[q][i + 1]));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], __uint_as_float(x[q][31]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         if (j == 0) {
           m = top;
-        } else if (__any_sync(0xffffffffu, top > m)) {
+        } else if (__any_sync(0xffffffffu, (top - m) * c > kPtLag || m == -INFINITY)) {
           const float up = fmaxf(m, top);
           const float f = up == -INFINITY ? 1.0f : pa_ex2((m - up) * c);
           m = up;
@@ -408,7 +415,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
           }
         }
         const float mc = m == -INFINITY ? 0.0f : -m * c;   // no key seen yet: every weight is exp2(-inf)
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t y[32];
@@ -419,11 +426,11 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
             v.x = pa_ex2(v.x);
             v.y = pa_ex2(v.y);
             y[i] = Pair16<H>::put(v.x, v.y);
-            pa_add_pair<H>(sum[i & 3], y[i]);   // the weights as they are rounded for the product: what rounding does to the numerator it does to the denominator
+            sum[i & 1] = pa_add2(sum[i & 1], v);
           }
           pa_st32(tS + h * 32, y);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         pa_st_wait();
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         pa_arrive(&p_full[t]);
@@ -477,10 +484,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (w == 9) {
-    if (lane == 0) {   // products in flight end before TMEM is given back, whichever wait has run out
-      umma_commit(drain);
-      tc_mbar_wait(drain, 0);
-    }
+    umma_commit_el(s_u32(drain));   // products in flight end before TMEM is given back, whichever wait has run out
+    tc_wait_short(s_u32(drain), 0);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
