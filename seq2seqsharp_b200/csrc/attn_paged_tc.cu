@@ -20,7 +20,8 @@ constexpr int kPtThreads = 384, kPtRows = 128, kPtKeys = 128, kPtTile = 2 * kPtR
 constexpr int kPtSoftmaxRegs = 208, kPtOtherRegs = 88;
 static_assert(256 * kPtSoftmaxRegs + 128 * kPtOtherRegs <= kPtThreads * 168, "the warpgroups' registers come out of the launch's");
 
-constexpr int pt_smem(int BX, int NS) { return (2 + 2 * NS) * BX * kPtBox + 1024 + 256; }
+constexpr int kPtStage = 32 * 64;   // bytes of a softmax warp to turn rows of outputs into lines
+constexpr int pt_smem(int BX, int NS) { return (2 + 2 * NS) * BX * kPtBox + 8 * kPtStage + 1024; }
 
 __device__ __forceinline__ void pt_cp16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -75,10 +76,9 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
   extern __shared__ __align__(1024) unsigned char pt_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)pt_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sQ = s_u32(smem), sK = sQ + 2 * BX * kPtBox, sV = sK + NS * BX * kPtBox;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (2 + 2 * NS) * BX * kPtBox);
-  uint64_t *k_full = bars, *k_empty = k_full + NS, *v_full = k_empty + NS, *v_empty = v_full + NS;
-  uint64_t *q_full = v_empty + NS, *q_empty = q_full + 1, *s_full = q_empty + 1, *p_full = s_full + 2, *o_full = p_full + 2, *o_empty = o_full + 2, *drain = o_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  unsigned char* stage = smem + (2 + 2 * NS) * BX * kPtBox;
+  __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], q_full[1], q_empty[1], s_full[2], p_full[4], o_full[2], o_empty[2], drain[1];
+  __shared__ uint32_t tmem_slot[1];
   __shared__ PagedPlanShared plan;
   __shared__ PagedRun wrun[12];   // of every warp: where it is (registers are the softmax's)
   __shared__ unsigned gone_of[8]; // bit i: keys 8 i .. of the key tile have no page
@@ -100,7 +100,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
     tc_mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       tc_mbar_init(&s_full[i], 1);
-      tc_mbar_init(&p_full[i], kPtRows);
+      tc_mbar_init(&p_full[2 * i], kPtRows);       // of the tile's first 64 keys, and of its others
+      tc_mbar_init(&p_full[2 * i + 1], kPtRows);
       tc_mbar_init(&o_full[i], 1);
       tc_mbar_init(&o_empty[i], kPtRows);
     }
@@ -315,15 +316,20 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (!ok || j >= n.n[t]) continue;
-            ok = wait(&p_full[t], pc[t]++);
-            if (ok && j == 0 && oc[t]++ > 0) ok = wait(&o_empty[t], oc[t]);   // the output of the item before has been read
-            if (!ok) continue;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             // V stage = [box][128 keys][128 B]: 8-key groups 1024 B apart (SBO), boxes kPtBox apart (LBO); 16 keys = 2048 B
             const uint32_t v = desc_lo(sV + st * BX * kPtBox, kPtBox);
 #pragma unroll
-            for (int i = 0; i < kPtKeys / 16; ++i)
-              pa_umma_ts_el(tmem + 2 * kPtKeys + t * HD, tmem + t * kPtKeys + i * 8, v + i * (2048 >> 4), hi, id_pv, (j > 0 || i > 0) ? 1u : 0u);
+            for (int h = 0; h < 2; ++h) {
+              ok = ok && wait(&p_full[2 * t + h], pc[t]);
+              if (ok && h == 0 && j == 0 && oc[t]++ > 0) ok = wait(&o_empty[t], oc[t]);   // the output of the item before has been read
+              if (!ok) break;
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+              for (int i = 4 * h; i < 4 * h + 4; ++i)
+                pa_umma_ts_el(tmem + 2 * kPtKeys + t * HD, tmem + t * kPtKeys + i * 8, v + i * (2048 >> 4), hi, id_pv, (j > 0 || i > 0) ? 1u : 0u);
+            }
+            ++pc[t];
+            if (!ok) continue;
             if (j + 1 < n.n[t]) qk(t, next);
             else umma_commit_el(s_u32(&o_full[t]));
           }
@@ -429,11 +435,11 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
             sum[i & 1] = pa_add2(sum[i & 1], v);
           }
           pa_st32(tS + h * 32, y);
+          pa_st_wait();
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          pa_arrive(&p_full[2 * t + h]);
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        pa_st_wait();
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        pa_arrive(&p_full[t]);
       }
       if (!ok) break;
       if (n > 0) {
@@ -443,13 +449,27 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
       const PagedSeq s = run.seq;
-      const int p = run.t * kPtTile + t * kPtRows + row, head = run.h * a.G + (p - a.by_G(p) * a.G);
-      const bool live = p < s.n * a.G, whole = run.first && run.last;
-      float* rec = a.part + (2 * (int64_t)blockIdx.x + (run.first ? 1 : 0)) * paged_record_floats(kPtTile, HD);
-      const int r = t * kPtRows + row;
-      if (!whole && live) *reinterpret_cast<float2*>(rec + 2 * r) = make_float2(m == -INFINITY ? m : m * c, l);   // the combine's maxima are in units of exp2
+      const int p0 = run.t * kPtTile + t * kPtRows + (row & ~31), pairs = s.n * a.G, p = p0 + lane;   // of the warp, of the lane
+      const bool whole = run.first && run.last;
+      const int64_t rf = paged_record_floats(kPtTile, HD);
+      float* rec = a.part + (2 * (int64_t)blockIdx.x + (run.first ? 1 : 0)) * rf;
+      if (!whole && p < pairs) *reinterpret_cast<float2*>(rec + 2 * (t * kPtRows + row)) = make_float2(m == -INFINITY ? m : m * c, l);   // the combine's maxima are in units of exp2
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      H* out = reinterpret_cast<H*>(a.out) + (int64_t)(s.row0 + a.by_G(p)) * a.o_row + (int64_t)head * a.o_head;
+      // 64 bytes of 32 rows at a time, through shared memory: the rows of lanes lie far from each other, and a store of 32 lines takes as long as four of eight
+      unsigned char* mine = stage + w * kPtStage;
+      const int line = lane >> 2, ch = lane & 3;   // of eight rows, and the piece of 16 bytes
+      auto turn = [&](const uint32_t* v, auto put) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(mine + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = k * 8 + line;
+          const uint4 u = *reinterpret_cast<const uint4*>(mine + r * 64 + ((ch ^ (r >> 1 & 3)) << 4));
+          if (p0 + r < pairs) put(r, u);
+        }
+      };
 #pragma unroll 1
       for (int q = 0; q < HD / 32; ++q) {
         uint32_t o[32];
@@ -460,19 +480,21 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-        if (!live) continue;
         if (whole) {
+          uint32_t y[16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = Pair16<H>::put(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-            reinterpret_cast<uint4*>(out + q * 32)[i] = make_uint4(y[0], y[1], y[2], y[3]);
-          }
+          for (int i = 0; i < 16; ++i) y[i] = Pair16<H>::put(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+          turn(y, [&](int r, uint4 u) {
+            const int pr = p0 + r, query = a.by_G(pr);
+            H* out = reinterpret_cast<H*>(a.out) + (int64_t)(s.row0 + query) * a.o_row + (int64_t)(run.h * a.G + pr - query * a.G) * a.o_head + q * 32;
+            reinterpret_cast<uint4*>(out)[ch] = u;
+          });
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            reinterpret_cast<uint4*>(rec + 2 * kPtTile + (int64_t)r * HD + q * 32)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int half = 0; half < 2; ++half)
+            turn(o + 16 * half, [&](int r, uint4 u) {
+              reinterpret_cast<uint4*>(rec + 2 * kPtTile + (int64_t)(t * kPtRows + (row & ~31) + r) * HD + q * 32 + half * 16)[ch] = u;
+            });
         }
       }
       if (n > 0) {
@@ -527,7 +549,7 @@ bool paged_tc_strides(const PagedArgs& a) {
 template <typename H, int BX, int NS>
 static int pt_launch(int device, DeviceState* st, const PagedArgs& a, cudaStream_t s) {
   constexpr int smem = pt_smem(BX, NS);
-  static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+  static_assert(smem <= 225 * 1024, "shared memory of a CTA, beside 2 KB of fixed size");
   static bool done[kMaxDevices] = {};
   if (!done[device]) {
     TSB_CUDA(cudaFuncSetAttribute(paged_tc_kernel<H, BX, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));

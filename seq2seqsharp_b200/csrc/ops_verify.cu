@@ -159,15 +159,24 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __gr
   }
   if (hit != w) return;
   int token = -1, some = -1;
-  for (int t0 = v0; t0 < v1 && token < 0; t0 += 32) {
-    const int t = t0 + lane;
-    double wr = 0.0, wa = 0.0;
-    if (t < v1) weigh(t, wr, wa);
-    const double mine = rest ? wr : wa, to = start + warp_scan(mine, lane);
-    const unsigned over = __ballot_sync(0xffffffffu, any && mine > 0.0 && to > r), weighs = __ballot_sync(0xffffffffu, mine > 0.0);
-    if (weighs) some = t0 + 31 - __clz(weighs);
-    if (over) token = t0 + __ffs(over) - 1;
-    start = __shfl_sync(0xffffffffu, to, 31);
+  constexpr int N = 8;   // steps of 32 words on their way at a time
+  for (int t0 = v0; t0 < v1 && token < 0; t0 += 32 * N) {
+    double mine[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int t = t0 + 32 * k + lane;
+      double wr = 0.0, wa = 0.0;
+      if (t < v1) weigh(t, wr, wa);
+      mine[k] = rest ? wr : wa;
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const double to = start + warp_scan(mine[k], lane);
+      const unsigned over = __ballot_sync(0xffffffffu, any && mine[k] > 0.0 && to > r), weighs = __ballot_sync(0xffffffffu, mine[k] > 0.0);
+      if (token < 0 && weighs) some = t0 + 32 * k + 31 - __clz(weighs);
+      if (token < 0 && over) token = t0 + 32 * k + __ffs(over) - 1;
+      start = __shfl_sync(0xffffffffu, to, 31);
+    }
   }
   if (lane == 0) out[taken] = token >= 0 ? token : some;
 }
@@ -189,9 +198,9 @@ int TSB200_VerifyDraft(int device, int32_t* tokens, int32_t* counts, const float
   DeviceState* st;
   TSB_TRY(use_device(device, &st));
   VerifyArgs a{tokens, counts, p, q, p_row, q_row, draft, starts, u, K, V, rows};
-  // as many CTAs to a sequence as are there at once (four on an SM), and at least 512 words to each
+  // as many CTAs to a sequence as are there at once (two on an SM), and at least 512 words to each
   int ctas = kVerifyMaxCtas;
-  while (ctas > 1 && ((int64_t)B * ctas > 4 * st->sm_count || V < 512 * ctas)) ctas /= 2;
+  while (ctas > 1 && ((int64_t)B * ctas > 2 * st->sm_count || V < 512 * ctas)) ctas /= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(B * ctas);
   cfg.blockDim = dim3(kVerifyThreads);

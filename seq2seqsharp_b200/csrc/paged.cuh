@@ -137,6 +137,19 @@ __device__ __forceinline__ long long paged_seq_units(const PagedArgs& a, int b, 
 __device__ __forceinline__ PagedLoc paged_find(const PagedArgs& a, int b, long long s, long long x, long long tol, int RT, int KT) {
   const int lane = threadIdx.x & 31;
   const PagedSeq q = paged_seq(a, b);
+  auto place = [&](int t, int cost, long long at) {
+    PagedLoc l;
+    l.b = b;
+    l.t = t;
+    l.h = (int)((double)(x - at) / (double)max(cost, 1));   // exact below 2^53, and a tenth of the instructions of a 64-bit division
+    l.s = at + (long long)l.h * cost;
+    l.units = cost - a.start;
+    const int in_item = (int)(x - l.s), rest = cost - in_item;
+    if (in_item <= a.start || (in_item <= tol && in_item <= rest)) l.off = 0;
+    else l.off = rest <= tol ? l.units : in_item - a.start;
+    return l;
+  };
+  if (q.n * a.G <= RT) return place(0, paged_tile(a, q, 0, RT, KT).units + a.start, s);   // a single tile: tokens, drafts
   for (int t0 = 0;; t0 += 32) {
     const bool there = (long long)(t0 + lane) * RT < (long long)q.n * a.G;
     const int u = there ? paged_tile(a, q, t0 + lane, RT, KT).units + a.start : 0;   // of one head
@@ -152,18 +165,8 @@ __device__ __forceinline__ PagedLoc paged_find(const PagedArgs& a, int b, long l
       continue;
     }
     const int src = in ? __ffs(in) - 1 : 0;
-    PagedLoc l;
-    l.b = b;
-    l.t = t0 + src;
     const int cost = __shfl_sync(0xffffffffu, u, src);
-    const long long at = s + __shfl_sync(0xffffffffu, end, src) - (long long)cost * a.Hkv;
-    l.h = (int)((double)(x - at) / (double)max(cost, 1));   // exact below 2^53, and a tenth of the instructions of a 64-bit division
-    l.s = at + (long long)l.h * cost;
-    l.units = cost - a.start;
-    const int in_item = (int)(x - l.s), rest = cost - in_item;
-    if (in_item <= a.start || (in_item <= tol && in_item <= rest)) l.off = 0;
-    else l.off = rest <= tol ? l.units : in_item - a.start;
-    return l;
+    return place(t0 + src, cost, s + __shfl_sync(0xffffffffu, end, src) - (long long)cost * a.Hkv);
   }
 }
 // where run c begins: c / runs of all units
@@ -172,9 +175,20 @@ __device__ __forceinline__ long long paged_begin(long long all, int c, int runs)
 // the whole call.  All threads of the CTA.
 template <int NT, int RT, int KT>
 __device__ __forceinline__ bool paged_locate(const PagedArgs& a, int c, int ctas, PagedPlanShared& sh, long long& all, int& runs) {
-  const int tid = threadIdx.x;
-  long long mine = paged_seq_units(a, tid, RT, KT), before;
-  if (a.B <= NT) {
+  const int tid = threadIdx.x, w = tid >> 5;
+  // few sequences: every warp adds them up for itself, the first two look for an end each
+  const bool few = a.B <= 32;
+  long long mine = paged_seq_units(a, few ? tid & 31 : tid, RT, KT), before = 0;
+  if (few) {
+    long long to = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, to, o);
+      if ((tid & 31) >= o) to += y;
+    }
+    before = to - mine;
+    all = __shfl_sync(0xffffffffu, to, 31);
+  } else if (a.B <= NT) {
     before = paged_block_scan<NT>(mine, sh, all);
   } else {
     long long total = mine;
@@ -188,9 +202,22 @@ __device__ __forceinline__ bool paged_locate(const PagedArgs& a, int c, int ctas
   }
   const long long tol = max(paged_begin(all, 1, runs) >> 5, (long long)a.snap);
   const long long x[2] = {paged_begin(all, c, runs), paged_begin(all, c + 1, runs)};
-  if (tid == 0) sh.loc[1] = PagedLoc{a.B, 0, 0, 0, 0, all};
+  if (few) {
+    if (w < 2) {
+      const long long y = x[w];
+      const unsigned hit = __ballot_sync(0xffffffffu, mine > 0 && y >= before && y < before + mine);
+      PagedLoc l{a.B, 0, 0, 0, 0, all};
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        l = paged_find(a, src, __shfl_sync(0xffffffffu, before, src), y, tol, RT, KT);
+      }
+      if ((tid & 31) == 0) sh.loc[w] = l;
+    }
+  } else if (tid == 0) {
+    sh.loc[1] = PagedLoc{a.B, 0, 0, 0, 0, all};
+  }
   long long base = 0;
-  for (int b0 = 0; b0 < a.B && base <= x[1]; b0 += NT) {
+  for (int b0 = few ? a.B : 0; b0 < a.B && base <= x[1]; b0 += NT) {
     const int b = b0 + tid;
     if (b0 > 0) mine = paged_seq_units(a, b, RT, KT);
     long long here = all;
