@@ -488,6 +488,162 @@ __global__ void __launch_bounds__(kFmaThreads) paged_fma_kernel(const __grid_con
   }
 }
 
+// fp32 chunks: 64 rows and 64 keys at a time, a thread has 4 x 4 scores and 4 x D / 16 outputs (four elements of a row from shared memory feed 16 products).  What
+// bounds it: the FMA pipe and shared memory, about even.  (With 16 rows and a lane per key, shared memory alone: 2 x 512 rows over 3000, 32 / 8 heads of 128, 1890 us.)
+constexpr int kTileThreads = 256, kTileRows = 64, kTileKeys = 64;
+template <int D>
+constexpr int tile_smem() { return (kTileRows * (D + 4) + 2 * kTileKeys * (D + 4) + 2 * kTileKeys * D + kTileRows * (kTileKeys + 4)) * 4; }
+
+template <int D>
+__global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) paged_f32_kernel(const __grid_constant__ PagedArgs a) {
+  constexpr int RT = kTileRows, KT = kTileKeys, C = D / 64, PS = KT + 4;
+  extern __shared__ __align__(16) float tile_sm[];
+  __shared__ PagedPlanShared plan;
+  __shared__ int there_s[2][KT / 8];   // whether eight keys have a page
+  float *qs = tile_sm, *ks = qs + RT * (D + 4), *vs = ks + 2 * KT * (D + 4), *ps = vs + 2 * KT * D;
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  pdl_trigger();
+  long long all;
+  int runs;
+  if (!paged_locate<kTileThreads, RT, KT>(a, blockIdx.x, gridDim.x, plan, all, runs)) return;
+  const int pieces = a.hd / 4, mask = (1 << a.page_shift) - 1;
+  PagedRun run;
+  run.begin(a, plan, RT);
+  for (; run.next(a, plan, RT, KT); run.step(a)) {
+    const PagedSeq& s = run.seq;
+    const int p0 = run.t * RT, pairs = s.n * a.G, cap = min(s.len, a.max_blocks << a.page_shift);
+    const int* table = a.table + run.b * a.table_stride;
+    auto fetch = [&](int kt) {
+      float *k = ks + (kt & 1) * KT * (D + 4), *v = vs + (kt & 1) * KT * D;
+      const int e = tid % (D / 4);
+#pragma unroll
+      for (int r = tid / (D / 4); r < KT; r += kTileThreads / (D / 4)) {
+        const int j = kt * KT + r, page = j < cap ? table[j >> a.page_shift] : -1;
+        const bool there = page >= 0 && page < a.num_pages;
+        if (e == 0 && (r & 7) == 0) there_s[kt & 1][r >> 3] = there;
+        const bool get = there && e < pieces;
+        const int64_t at = get ? page * a.c_page + run.h * a.c_head + (j & mask) * a.c_tok + e * 4 : 0;
+        paged_cp16(k + r * (D + 4) + e * 4, reinterpret_cast<const float*>(a.K) + at, get);
+        paged_cp16(v + r * D + e * 4, reinterpret_cast<const float*>(a.V) + at, get);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    __syncthreads();   // the item before has been read
+    fetch(run.k0);
+    for (int i = tid; i < RT * (D / 4); i += kTileThreads) {
+      const int r = i / (D / 4), e = i % (D / 4), p = p0 + r, query = a.by_G(p);
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (p < pairs && e < pieces) x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + (int64_t)(s.row0 + query) * a.q_row + (run.h * a.G + p - query * a.G) * a.q_head + e * 4);
+      *reinterpret_cast<float4*>(qs + r * (D + 4) + e * 4) = make_float4(x.x * a.c, x.y * a.c, x.z * a.c, x.w * a.c);
+    }
+    float m[4], l[4], acc[4][C][4];
+    int lo[4], hi[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + ty * 4 + i, pos = s.len - s.n + a.by_G(p);
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+      hi[i] = p < pairs ? min(pos + 1, cap) : 0;
+      lo[i] = a.window > 0 ? pos - a.window + 1 : 0;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][c][e] = 0.0f;
+    }
+    for (int kt = run.k0; kt < run.k1; ++kt) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncthreads();   // this tile has landed, the one before has been used
+      if (kt + 1 < run.k1) fetch(kt + 1);
+      const float *k = ks + (kt & 1) * KT * (D + 4), *v = vs + (kt & 1) * KT * D;
+      float x[4][4];   // rows 4 ty + i, keys tx + 16 j
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
+#pragma unroll 4
+      for (int e = 0; e < D; e += 4) {
+        float4 q4[4], k4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q4[i] = *reinterpret_cast<const float4*>(qs + (ty * 4 + i) * (D + 4) + e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k4[j] = *reinterpret_cast<const float4*>(k + (tx + 16 * j) * (D + 4) + e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[i][j] += q4[i].x * k4[j].x + q4[i].y * k4[j].y + q4[i].z * k4[j].z + q4[i].w * k4[j].w;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = tx + 16 * j, at = kt * KT + key;
+          if (!(at < hi[i] && at >= lo[i] && there_s[kt & 1][key >> 3])) x[i][j] = -INFINITY;
+          top = fmaxf(top, x[i][j]);
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float up = fmaxf(m[i], top), from = fmaxf(up, -FLT_MAX);   // no key seen yet: every weight is exp2(-inf)
+        const float f = exp2f(m[i] - from);
+        m[i] = up;
+        l[i] *= f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[i][j] = exp2f(x[i][j] - from);
+          l[i] += x[i][j];
+          ps[(ty * 4 + i) * PS + tx + 16 * j] = x[i][j];
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][c][e] *= f;
+      }
+      __syncwarp();   // a row's weights are made and used by the same half of a warp
+#pragma unroll 2
+      for (int key = 0; key < KT; key += 4) {
+        float4 p4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p4[i] = *reinterpret_cast<const float4*>(ps + (ty * 4 + i) * PS + key);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const float4 v4 = *reinterpret_cast<const float4*>(v + (key + u) * D + c * 64 + tx * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = u == 0 ? p4[i].x : u == 1 ? p4[i].y : u == 2 ? p4[i].z : p4[i].w;
+              acc[i][c][0] += p * v4.x;
+              acc[i][c][1] += p * v4.y;
+              acc[i][c][2] += p * v4.z;
+              acc[i][c][3] += p * v4.w;
+            }
+          }
+      }
+      __syncwarp();
+    }
+    const bool whole = run.first && run.last;
+    float* rec = a.part + (2 * (int64_t)blockIdx.x + (run.first ? 1 : 0)) * paged_record_floats(RT, a.hd);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float sum = l[i];
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const int row = ty * 4 + i, p = p0 + row;
+      if (p >= pairs) continue;
+      const int query = a.by_G(p);
+      float* out = reinterpret_cast<float*>(a.out) + (int64_t)(s.row0 + query) * a.o_row + (int64_t)(run.h * a.G + p - query * a.G) * a.o_head;
+      const float inv = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+      if (!whole && tx == 0) *reinterpret_cast<float2*>(rec + 2 * row) = make_float2(m[i], sum);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int e = c * 64 + tx * 4;
+        if (e >= a.hd) continue;
+        *reinterpret_cast<float4*>((whole ? out : rec + 2 * RT + row * a.hd) + e) = make_float4(acc[i][c][0] * inv, acc[i][c][1] * inv, acc[i][c][2] * inv, acc[i][c][3] * inv);
+      }
+    }
+  }
+}
+
 // Joins the records of the items that runs end in, four elements of a row per thread.  What bounds it: latency of dependent reads, then the records.
 // W warps share the records of 32 x 4 elements: an item of few rows may have a record of every run (one token of 16384, 8 KV heads: 37 each; W = 1 took 16 us,
 // W = 8 takes 6), one of many rows has few.
@@ -571,9 +727,9 @@ __global__ void __launch_bounds__(kJoinThreads) paged_combine_kernel(const __gri
 
 template <typename T>
 static cudaError_t launch_join(const PagedArgs& a, int RT, int ctas, cudaStream_t s) {
-  const int W = RT <= 64 ? 8 : 1, parts = (RT * a.hd / 4 * W + kJoinThreads - 1) / kJoinThreads;
+  const int W = RT <= 32 ? 8 : RT <= 64 ? 2 : 1, parts = (RT * a.hd / 4 * W + kJoinThreads - 1) / kJoinThreads;
   const dim3 grid(ctas - 1, parts < 16 ? parts : 16);   // most runs end between items: few CTAs each, which go round
-  return launch_k(W == 8 ? paged_combine_kernel<T, 8> : paged_combine_kernel<T, 1>, grid, dim3(kJoinThreads), 0, s, a, RT);
+  return launch_k(W == 8 ? paged_combine_kernel<T, 8> : W == 2 ? paged_combine_kernel<T, 2> : paged_combine_kernel<T, 1>, grid, dim3(kJoinThreads), 0, s, a, RT);
 }
 int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int ctas, cudaStream_t s) {
   if (ctas < 2) return 1;
@@ -587,7 +743,7 @@ int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int 
 
 // The kernel that serves a call, its rows of a tile and its CTAs
 struct PagedChoice {
-  enum { FMA, MMA, TC } kind;
+  enum { FMA, TILE, MMA, TC } kind;
   int RT, KT, ctas;
 };
 static PagedChoice paged_choose(int sm_count, int dtype, int64_t pairs, int hd, bool positive) {
@@ -604,6 +760,13 @@ static PagedChoice paged_choose(int sm_count, int dtype, int64_t pairs, int hd, 
     c.RT = 256;
     c.KT = 128;
     c.ctas = sm_count;
+    return c;
+  }
+  if (dtype == TSB200_F32 && hd <= 128 && pairs > 16) {
+    c.kind = PagedChoice::TILE;
+    c.RT = kTileRows;
+    c.KT = kTileKeys;
+    c.ctas = sm_count * (hd <= 64 ? 2 : 1);
     return c;
   }
   c.kind = PagedChoice::FMA;
@@ -634,6 +797,13 @@ static int launch_paged_fma_n(int device, DeviceState* st, const PagedArgs& a, c
   }
   count_launch(device);
   return check_launch("paged_fma");
+}
+template <int D>
+static int launch_paged_tile(int device, const PagedArgs& a, const PagedChoice& c, cudaStream_t s) {
+  TSB_CUDA(cudaFuncSetAttribute(paged_f32_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem<D>()));
+  paged_f32_kernel<D><<<c.ctas, kTileThreads, tile_smem<D>(), s>>>(a);
+  count_launch(device);
+  return check_launch("paged_f32");
 }
 template <typename T>
 static int launch_paged_fma(int device, DeviceState* st, const PagedArgs& a, const PagedChoice& c, cudaStream_t s) {
@@ -790,12 +960,15 @@ int TSB200_PagedAttention(int device, int dtype, void* out, int64_t o_row, int64
   TSB_CHECK(st->sm_count <= kSmCountMost, "paged_attention: %d SMs", st->sm_count);
   a.joins = reinterpret_cast<int4*>(workspace);
   a.part = reinterpret_cast<float*>(a.joins + 2 * c.ctas);
-  a.min_units = 4;
-  a.snap = 1;
+  a.min_units = c.kind == PagedChoice::TILE ? 1 : 4;   // a unit of the fp32 tiles takes as long as eight of a lane per key
+  a.snap = c.kind == PagedChoice::TILE ? 0 : 1;
   a.start = 1;
   if (c.kind == PagedChoice::MMA) return launch_paged_mma(device, st, dtype, a, c.RT, s);
   if (c.kind == PagedChoice::TC) return launch_paged_tc(device, st, dtype, a, s);
-  if (dtype == TSB200_F32) TSB_TRY(launch_paged_fma<float>(device, st, a, c, s));
+  if (c.kind == PagedChoice::TILE) {
+    if (hd <= 64) TSB_TRY(launch_paged_tile<64>(device, a, c, s));
+    else TSB_TRY(launch_paged_tile<128>(device, a, c, s));
+  } else if (dtype == TSB200_F32) TSB_TRY(launch_paged_fma<float>(device, st, a, c, s));
   else if (dtype == TSB200_F16) TSB_TRY(launch_paged_fma<__half>(device, st, a, c, s));
   else TSB_TRY(launch_paged_fma<__nv_bfloat16>(device, st, a, c, s));
   return launch_paged_combine(device, dtype, a, c.RT, c.ctas, s);
