@@ -5,17 +5,17 @@
 // operand; the products of one tile run behind the exponentials of the other (PV0(j) QK0(j+1) PV1(j) QK1(j+1)), and those of the next item's first keys
 // behind the output of this one's last.
 //
-// Whole tiles of keys and values come by TMA tensor copies, a box per page (128-byte swizzle, any strides that are multiples of 16 bytes); an entry that names no
-// page is a coordinate outside of the map, which arrives as zeros.  The last tile of a sequence and the queries come by cp.async, 16 bytes a lane, into
-// the same swizzle, with zeros behind the end (a weight of 0 times what the cache holds there would be NaN where that is).  Those are generic-proxy writes: they
-// report to the stage's mbarrier when they have landed, and the issuing thread orders them before its products with a proxy fence.
-// (cp.async for every tile: 2.4 instead of 1.8 ms for two chunks of 2048 over 32768; its latency and issue do not fit the time of one tile.)
+// Keys and values come by TMA tensor copies, a box per page (128-byte swizzle, any strides that are multiples of 16 bytes); an entry that names no page is a coordinate
+// outside of the map, which arrives as zeros, and the values behind a sequence's end are overwritten with zeros before their product.  Queries come by TMA where
+// whole ones fill a tile (1, 2, 4 .. heads to a KV head), else by cp.async into the same swizzle: generic-proxy writes, which the issuing warp orders before
+// its products with a proxy fence.  (cp.async for keys and values too: 2.4 instead of 1.8 ms for two chunks of 2048 over 32768; its latency and issue do
+// not fit the time of a unit.)
 #include "attn_tmem.cuh"
 #include "paged.cuh"
 
 namespace tsb {
 
-constexpr int kPtThreads = 384, kPtRows = 128, kPtKeys = 128, kPtTile = 2 * kPtRows, kPtBox = kPtKeys * 128, kPtCopiers = 96, kPtAhead = 4;
+constexpr int kPtThreads = 384, kPtRows = 128, kPtKeys = 128, kPtTile = 2 * kPtRows, kPtBox = kPtKeys * 128, kPtCopiers = 96;
 // registers per thread: 384 x 168 at launch
 constexpr int kPtSoftmaxRegs = 208, kPtOtherRegs = 88;
 static_assert(256 * kPtSoftmaxRegs + 128 * kPtOtherRegs <= kPtThreads * 168, "the warpgroups' registers come out of the launch's");
@@ -43,9 +43,6 @@ __device__ __forceinline__ void pt_load_3d(uint32_t dst, const CUtensorMap* map,
       "r"(s_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-__device__ __forceinline__ void pt_prefetch_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3) {
-  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
-}
 
 // A row's output is rescaled when its maximum is this much (in powers of two) above the one in use: weights are then up to 2^8, which neither type loses
 // anything by, and one of a warp's 32 rows has a new maximum in nearly every tile of the first hundred
@@ -72,7 +69,7 @@ __device__ __forceinline__ PtCounts pt_counts(const PagedArgs& a, const PagedRun
 template <typename H, int BX, int NS>
 __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                                                                  const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ PagedArgs a, int q_boxes) {
-  constexpr int HD = BX * 64, CPR = HD / 8;   // 16-byte pieces of a row
+  constexpr int HD = BX * 64, CPR = HD / 8;   // CPR: 16-byte pieces of a row
   extern __shared__ __align__(1024) unsigned char pt_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)pt_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sQ = s_u32(smem), sK = sQ + 2 * BX * kPtBox, sV = sK + NS * BX * kPtBox;
@@ -91,12 +88,12 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
 
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      tc_mbar_init(&k_full[i], kPtCopiers + 1);
+      tc_mbar_init(&k_full[i], 1);
       tc_mbar_init(&k_empty[i], 1);
-      tc_mbar_init(&v_full[i], kPtCopiers);
+      tc_mbar_init(&v_full[i], 1);
       tc_mbar_init(&v_empty[i], 1);
     }
-    tc_mbar_init(q_full, kPtCopiers);
+    tc_mbar_init(q_full, q_boxes ? 1 : kPtCopiers);
     tc_mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       tc_mbar_init(&s_full[i], 1);
@@ -141,127 +138,79 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
   if (w >= 8) {
     pa_fewer_registers<kPtOtherRegs>();
     if (w != 9) {
-      // ---------------- copies
-      const int cw = w == 8 ? 0 : w - 9;                      // 0 .. 2
-      const int lr = lane / CPR, lc = lane % CPR;             // this lane's row of a pass and piece
-      constexpr int RP = 32 / CPR;                            // rows of a pass
-      const int page_mask = (1 << a.page_shift) - 1;
-      const uint32_t lane_box = (uint32_t)(lc >> 3) * kPtBox;
-      uint32_t place[8 / RP];                                 // of this lane's piece of the rows lr + RP i of eight
-#pragma unroll
-      for (int i = 0; i < 8 / RP; ++i) place[i] = lane_box + (lr + i * RP) * 128 + (((lc & 7) ^ (lr + i * RP)) << 4);
-      const int box_blocks = min(kPtKeys, 1 << a.page_shift) / 8;   // eights of keys in a box of the maps
+      // ---------------- copies: warp 8 keys, values and, where whole queries fill a tile, the queries; else all three share the queries' rows
+      const int cw = w == 8 ? 0 : w - 9;
+      const int page_mask = (1 << a.page_shift) - 1, box_blocks = min(kPtKeys, 1 << a.page_shift) / 8;   // eights of keys in a box of the maps
       uint32_t kc = 0, qc = 0;
       int ks = 0, vs = 0;                                     // tiles asked for so far
-      bool ok = true;
+      bool ok = cw == 0 || !q_boxes;
       while (ok && next_item()) {
         const PtCounts n = pt_counts(a, run);
         if (n.most == 0) continue;
         const PagedSeq s = run.seq;
-        const int cap = min(s.len, a.max_blocks << a.page_shift);
+        const int cap = min(s.len, a.max_blocks << a.page_shift), k0 = run.k0, h = run.h;
         const int* table = a.table + run.b * a.table_stride;
-        const int64_t head = run.h * a.c_head + lc * 8;
-        // one tile of keys (or values): lane i < 16 knows the page of keys 8 i ..
-        auto load = [&](const CUtensorMap* map, const void* src, uint32_t dst, uint64_t* full, int tile, int entry) {
-          if ((tile + 1) * kPtKeys <= cap) {
-            // whole pages; one that there is not lies outside of the map and arrives as zeros
-            if (cw == 0) {
-              if (lane == 0) tc_mbar_expect_tx(full, BX * kPtBox);
-              __syncwarp();
-              const int page = __shfl_sync(0xffffffffu, entry, lane * box_blocks & 15);
-              if (lane * box_blocks < 16)
-#pragma unroll
-                for (int i = 0; i < BX; ++i)
-                  pt_load_4d(dst + i * kPtBox + lane * box_blocks * 1024, map, 64 * i, tile * kPtKeys & page_mask, run.h, page >= 0 ? page : a.num_pages, full);
-              if (lane > 0) pa_arrive(full);
-            } else {
-              pa_arrive(full);
-            }
-            return;
-          }
-          // the sequence's end: what lies behind it becomes zeros
-          const H* base = reinterpret_cast<const H*>(src) + head;
-          const int key0 = tile * kPtKeys + cw * 8 + lr;
-#pragma unroll 1
-          for (int b = cw; b < kPtKeys / 8; b += 3) {
-            const int page = __shfl_sync(0xffffffffu, entry, b), key = key0 + (b - cw) * 8;
-            const H* p = base + (page >= 0 ? page * a.c_page + (key & page_mask) * a.c_tok : 0);
-#pragma unroll
-            for (int i = 0; i < 8 / RP; ++i) {
-              const bool there = page >= 0 && key + i * RP < cap;
-              pt_cp16(dst + place[i] + b * 1024, there ? p + (int64_t)(i * RP) * a.c_tok : reinterpret_cast<const H*>(src), there);
-            }
-          }
-          pt_arrive_copies(full);
-        };
-        auto entry_of = [&](int tile) {
+        auto entry_of = [&](int tile) {   // lane i < 16: the page of keys 8 i ..
           const int key = tile * kPtKeys + (lane & 15) * 8;
           const int page = key < cap ? table[key >> a.page_shift] : -1;
           return page >= 0 && page < a.num_pages ? page : -1;
         };
+        // a tile of keys or values by boxes of a page; a page that there is not lies outside of the map and arrives as zeros
+        auto load = [&](const CUtensorMap* map, uint32_t dst, uint64_t* full, int tile, int entry) {
+          if (lane == 0) tc_mbar_expect_tx(full, BX * kPtBox);
+          __syncwarp();
+          const int page = __shfl_sync(0xffffffffu, entry, lane * box_blocks & 15);
+          if (lane * box_blocks < 16)
+#pragma unroll
+            for (int i = 0; i < BX; ++i)
+              pt_load_4d(dst + i * kPtBox + lane * box_blocks * 1024, map, 64 * i, tile * kPtKeys & page_mask, h, page >= 0 ? page : a.num_pages, full);
+        };
         auto load_k = [&](int j, int entry) {
           const uint32_t c = kc + j, st = c % NS;
           if (c >= NS && !tc_wait_or(s_u32(&k_empty[st]), (c / NS - 1) & 1, err, a.wait_limit)) return false;
-          load(&mapK, a.K, sK + st * BX * kPtBox, &k_full[st], run.k0 + j, entry);
-          ks = c + 1;
+          // read behind the tile's scores; a tile NS + 1 in front has been weighed when this one's copies begin
           const unsigned gone = __ballot_sync(0xffffffffu, entry < 0) & 0xffffu;
-          if (cw == 0 && lane == 0) {   // read behind the tile's scores; a tile NS + 1 in front has been weighed when this one's copies begin
-            gone_of[c & 7] = gone;
-            pa_arrive(&k_full[st]);
-          }
+          if (lane == 0) gone_of[c & 7] = gone;
+          load(&mapK, sK + st * BX * kPtBox, &k_full[st], k0 + j, entry);
+          ks = c + 1;
           return true;
         };
         // entries are looked up two tiles ahead
-        int entry = entry_of(run.k0), next = entry_of(run.k0 + 1), ahead = next;
-        ok = load_k(0, entry);
+        int entry = 0, next = 0;
+        if (cw == 0) {
+          entry = entry_of(k0);
+          next = entry_of(k0 + 1);
+          ok = load_k(0, entry);
+        }
         if (ok && qc > 0) ok = tc_wait_or(s_u32(q_empty), (qc - 1) & 1, err, a.wait_limit);
         if (!ok) break;
         ++qc;
         const int p0 = run.t * kPtTile, pairs = s.n * a.G;
         if (q_boxes) {
-          // whole queries to a tile: boxes of G heads (rows behind the sequence's are another's, and are not stored)
-          if (cw == 0) {
-            const int tiles = n.n[1] > 0 ? 2 : 1;
-            if (lane == 0) tc_mbar_expect_tx(q_full, tiles * BX * kPtBox);
-            __syncwarp();
-            if (lane < tiles * BX) pt_load_3d(sQ + lane * kPtBox, &mapQ, lane % BX * 64, run.h * a.G, s.row0 + a.by_G(p0 + lane / BX * kPtRows), q_full);
-            if (lane > 0) pa_arrive(q_full);
-          } else {
-            pa_arrive(q_full);
-          }
+          // boxes of G heads (rows behind the sequence's are another's, and are not stored)
+          const int tiles = n.n[1] > 0 ? 2 : 1;
+          if (lane == 0) tc_mbar_expect_tx(q_full, tiles * BX * kPtBox);
+          __syncwarp();
+          if (lane < tiles * BX) pt_load_3d(sQ + lane * kPtBox, &mapQ, lane % BX * 64, h * a.G, s.row0 + a.by_G(p0 + lane / BX * kPtRows), q_full);
         } else {
-        for (int r0 = cw * RP; r0 < (n.n[1] > 0 ? kPtTile : kPtRows); r0 += 3 * RP) {
-          const int r = r0 + lr, p = p0 + r;
-          const bool there = p < pairs;
-          const H* src = reinterpret_cast<const H*>(a.q);
-          if (there) src += (int64_t)(s.row0 + a.by_G(p)) * a.q_row + (int64_t)(run.h * a.G + (p - a.by_G(p) * a.G)) * a.q_head + lc * 8;
-          if (r < kPtTile) pt_cp16(sQ + (r >> 7) * BX * kPtBox + lane_box + (r & 127) * 128 + (((lc & 7) ^ (r & 7)) << 4), src, there);
-        }
-        pt_arrive_copies(q_full);
-        }
-        // tiles on their way to L2: shared memory holds two or four, less than what memory takes to answer
-        auto warm = [&](int tile, int entry) {
-          const int page = __shfl_sync(0xffffffffu, entry, lane * box_blocks & 15);
-          if (lane * box_blocks < 16 && page >= 0)
-#pragma unroll
-            for (int i = 0; i < BX; ++i) {
-              pt_prefetch_4d(&mapK, 64 * i, tile * kPtKeys & page_mask, run.h, page);
-              pt_prefetch_4d(&mapV, 64 * i, tile * kPtKeys & page_mask, run.h, page);
-            }
-        };
-        int far = entry_of(run.k0 + kPtAhead);
-        if (cw == 1)
-          for (int i = 1; i < min(kPtAhead, n.most); ++i) warm(run.k0 + i, entry_of(run.k0 + i));
-        for (int j = 0; j < n.most; ++j) {
-          if (cw == 1 && j + kPtAhead < n.most) {
-            warm(run.k0 + j + kPtAhead, far);
-            far = entry_of(run.k0 + j + kPtAhead + 1);
+          const int lr = lane / CPR, lc = lane % CPR;   // this lane's row of a pass and piece
+          constexpr int RP = 32 / CPR;                  // rows of a pass
+          for (int r0 = cw * RP; r0 < (n.n[1] > 0 ? kPtTile : kPtRows); r0 += 3 * RP) {
+            const int r = r0 + lr, p = p0 + r, query = a.by_G(p);
+            const bool there = p < pairs;
+            const H* src = reinterpret_cast<const H*>(a.q);
+            if (there) src += (int64_t)(s.row0 + query) * a.q_row + (int64_t)(h * a.G + p - query * a.G) * a.q_head + lc * 8;
+            if (r < kPtTile) pt_cp16(sQ + (r >> 7) * BX * kPtBox + (lc >> 3) * kPtBox + (r & 127) * 128 + (((lc & 7) ^ (r & 7)) << 4), src, there);
           }
-          ahead = entry_of(run.k0 + j + 2);
+          pt_arrive_copies(q_full);
+        }
+        if (cw != 0) continue;
+        for (int j = 0; j < n.most; ++j) {
+          const int ahead = entry_of(k0 + j + 2);
           if (j + 1 < n.most && !(ok = load_k(j + 1, next))) break;
           const uint32_t c = kc + j, st = c % NS;
           if (c >= NS && !(ok = tc_wait_or(s_u32(&v_empty[st]), (c / NS - 1) & 1, err, a.wait_limit))) break;
-          load(&mapV, a.V, sV + st * BX * kPtBox, &v_full[st], run.k0 + j, entry);
+          load(&mapV, sV + st * BX * kPtBox, &v_full[st], k0 + j, entry);
           vs = c + 1;
           entry = next;
           next = ahead;
@@ -273,6 +222,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
       if (cw == 0) {
         tc_land(s_u32(k_full), NS, ks);
         tc_land(s_u32(v_full), NS, vs);
+        if (q_boxes && qc > 0) tc_wait_short(s_u32(q_full), (qc - 1) & 1);
       }
     } else {
       // ---------------- products, issued by whole warps: 32 of them to a unit leave no time for a single lane's descriptors (2.35 -> ... us a unit).
@@ -300,7 +250,8 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
       while (ok && next_item()) {
         const PtCounts n = pt_counts(a, run);
         if (n.most == 0) continue;
-        ok = landed(q_full, qc) && landed(&k_full[kc % NS], kc / NS);
+        const int cap = min(run.seq.len, a.max_blocks << a.page_shift);
+        ok = landed(q_full, qc) && wait(&k_full[kc % NS], kc / NS);
         ++qc;
         if (!ok) break;
 #pragma unroll
@@ -311,8 +262,17 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
         for (int j = 0; j < n.most && ok; ++j) {
           const bool more = j + 1 < n.most;
           const uint32_t c = kc + j, st = c % NS, next = (c + 1) % NS;
-          ok = landed(&v_full[st], c / NS);
-          if (ok && more) ok = landed(&k_full[next], (c + 1) / NS);
+          ok = wait(&v_full[st], c / NS);
+          const int left = cap - (run.k0 + j) * kPtKeys;
+          if (ok && left < kPtKeys) {
+            // values behind the sequence's end: a weight of 0 times what lies there would be NaN where that is
+            for (int r = max(left, 0) * 8 + lane; r < kPtKeys * 8; r += 32)
+#pragma unroll
+              for (int i = 0; i < BX; ++i) *reinterpret_cast<uint4*>(smem + (2 + NS + st) * BX * kPtBox + i * kPtBox + r * 16) = make_uint4(0u, 0u, 0u, 0u);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+          if (ok && more) ok = wait(&k_full[next], (c + 1) / NS);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (!ok || j >= n.n[t]) continue;

@@ -788,11 +788,15 @@ static int64_t paged_ws_bytes(int dtype, int64_t pairs, int hd) {
 
 template <typename T, int NH>
 static int launch_paged_fma_n(int device, DeviceState* st, const PagedArgs& a, const PagedChoice& c, cudaStream_t s) {
-  if (c.RT == 4) {
+  static bool done[kMaxDevices] = {};
+  if (!done[device]) {
     TSB_CUDA(cudaFuncSetAttribute(paged_fma_kernel<T, NH, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, fma_smem<T>(NH, 1)));
+    TSB_CUDA(cudaFuncSetAttribute(paged_fma_kernel<T, NH, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, fma_smem<T>(NH, 4)));
+    done[device] = true;
+  }
+  if (c.RT == 4) {
     paged_fma_kernel<T, NH, 1><<<c.ctas, kFmaThreads, fma_smem<T>(NH, 1), s>>>(a);
   } else {
-    TSB_CUDA(cudaFuncSetAttribute(paged_fma_kernel<T, NH, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, fma_smem<T>(NH, 4)));
     paged_fma_kernel<T, NH, 4><<<c.ctas, kFmaThreads, fma_smem<T>(NH, 4), s>>>(a);
   }
   count_launch(device);
@@ -800,7 +804,11 @@ static int launch_paged_fma_n(int device, DeviceState* st, const PagedArgs& a, c
 }
 template <int D>
 static int launch_paged_tile(int device, const PagedArgs& a, const PagedChoice& c, cudaStream_t s) {
-  TSB_CUDA(cudaFuncSetAttribute(paged_f32_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem<D>()));
+  static bool done[kMaxDevices] = {};
+  if (!done[device]) {
+    TSB_CUDA(cudaFuncSetAttribute(paged_f32_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem<D>()));
+    done[device] = true;
+  }
   paged_f32_kernel<D><<<c.ctas, kTileThreads, tile_smem<D>(), s>>>(a);
   count_launch(device);
   return check_launch("paged_f32");
@@ -846,7 +854,11 @@ int TSB200_PagedPlan(int device, const int32_t* cached, const int32_t* fresh, in
   a.held = held; a.free_pages = free_pages; a.free_count = free_count; a.lens = lens; a.starts = starts; a.slots = slots; a.positions = positions;
   // a cluster for many rows
   const int smem = 6 * B * (int)sizeof(int), ctas = rows > 2048 ? 8 : 1;
-  if (smem > 40 * 1024) TSB_CUDA(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 6 * kPlanMaxB * (int)sizeof(int)));
+  static bool done[kMaxDevices] = {};
+  if (!done[device]) {
+    TSB_CUDA(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 6 * kPlanMaxB * (int)sizeof(int)));
+    done[device] = true;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kPlanThreads);

@@ -59,7 +59,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b) {
   PagedSeq s;
   s.row0 = r0;
   s.n = r0 >= 0 && r1 > r0 && r1 <= a.rows ? r1 - r0 : 0;   // rows that are not there are nobody's
-  s.len = max(a.lens[b], 0);
+  s.len = min(max(a.lens[b], 0), 0x7fff0000);   // positions and what is added to them stay below 2^31
   return s;
 }
 struct PagedTile {

@@ -532,3 +532,109 @@ def test_wrong_tensors_are_refused(cuda):
         Ops.PagedPlan(ints([1]), ints([1]), ints([[1]]), ints([0]), ints([0]), ints([1, 2]), 16, 4)
     with pytest.raises(N.TSB200Error):
         Ops.QKNormRopePaged(None, q, K[:2, 0, :2], K[:2, 0, :2], None, None, 1e-6, ints([0]), ints([0, 1]), K, V)
+
+
+@pytest.mark.parametrize("t,H,Hkv,n,lens", [(F16, 128, 1, 1, [700, 3]), (BF16, 256, 1, 1, [300]), (F16, 20, 1, 9, [260, 9]), (F16, 24, 2, 30, [500, 30]), (BF16, 64, 2, 4, [1000, 129, 128, 127]),
+                                            (F16, 7, 7, 65, [65, 400])])
+def test_large_and_odd_groups(cuda, t, H, Hkv, n, lens):
+    for hd, window in ((64, 0), (128, 50)):
+        a = problem(t, H, Hkv, hd, 8, lens, [n] * len(lens), seed=H)
+        assert check(Ops.PagedAttention(None, *a[:4], a[4], a[5], n, window=window), *a, hd ** -0.5, window).all()
+
+
+@pytest.mark.parametrize("t,n", [(F32, 1), (F32, 40), (F16, 1), (F16, 100)])
+def test_lengths_beyond_the_table(cuda, t, n):
+    # positions behind the table's last page: every key of the table is seen
+    q, K, V, table, starts, lens = problem(t, 4, 2, 64, 16, [320, 320], [n, n], extra=0, seed=8)
+    lens.copy_(ints([320 + 7, 2 ** 31 - 1]))
+    got = Ops.PagedAttention(None, q, K, V, table, starts, lens, n)
+    assert check(got, q, K, V, table, starts, ints([320 + n + 7, 320 + n + 7]), 0.125)[n:].all() if n == 1 else not got.isnan().any()
+    every = ints([320 + n, 320 + n])
+    want = Ops.PagedAttention(None, q, K, V, table, starts, every, n)
+    assert torch.equal(got[n:], want[n:])
+
+
+@pytest.mark.parametrize("t,n", [(F32, 1), (F32, 40), (F16, 1), (F16, 5), (BF16, 100)])
+def test_many_calls_at_once(cuda, t, n):
+    problems = [problem(t, 8, 2, 64, 16, [900 + 37 * i, n], [n, n], seed=20 + i) for i in range(6)]
+    want = [Ops.PagedAttention(None, *a[:4], a[4], a[5], n) for a in problems]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in problems]
+    got = []
+    for _ in range(3):
+        for s, a in zip(streams, problems):
+            with torch.cuda.stream(s):
+                got.append(Ops.PagedAttention(None, *a[:4], a[4], a[5], n))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i % 6]) for i, g in enumerate(got))
+
+
+def test_captured_plan_append_attention_verify(cuda):
+    """A step captured once and replayed with other lengths, its buffers a little larger than its rows."""
+    H, Hkv, hd, page, B, K, V = 8, 2, 64, 16, 3, 2, 40
+    pool = Pool(B, 20, page, 64, seed=4)
+    Kc, Vc = cache(64, Hkv, page, hd, F16)
+    cached, fresh = ints([0, 0, 0]), ints([1, 1, 1])
+    q, k, v = (torch.randn(12, h, hd, device="cuda").to(F16) for h in (H, Hkv, Hkv))
+    out, p = torch.zeros_like(q), torch.softmax(torch.randn(12, V, device="cuda"), -1)
+    draft, u = ints([[1, 2], [3, 4], [5, 6]]), torch.rand(B, K + 1, device="cuda")
+
+    def step():
+        lens, starts, slots, positions = Ops.PagedPlan(cached, fresh, pool.d_table, pool.d_held, pool.d_free, pool.d_count, page, 12)
+        qn = Ops.QKNormRopePaged(torch.zeros_like(q), q, k, v, None, None, 0.0, positions, slots, Kc, Vc)
+        Ops.PagedAttention(out, qn, Kc, Vc, pool.d_table, starts, lens, 8)
+        return (lens, starts, slots, positions, qn) + tuple(Ops.VerifyDraft(p, None, draft, u, starts))
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            got = step()
+        for new in ([5, 1, 3], [1, 0, 8], [3, 3, 3], [0, 0, 0]):
+            before = cached.tolist()
+            fresh.copy_(ints(new))
+            out.fill_(7.0)
+            g.replay()
+            s.synchronize()
+            want = R.plan(before, new, pool.table, pool.held, pool.free, page, 12)
+            assert [x.tolist() for x in got[:4]] == list(want)
+            total = sum(new)
+            owned = check(out, got[4], Kc, Vc, pool.d_table, got[1], got[0], hd ** -0.5)
+            assert owned[:total].all() and (out[total:] == 7.0).all()
+            counts = got[6].tolist()
+            assert all((c == 0) == (n == 0) and c <= max(n, 1) for c, n in zip(counts, new))
+            cached.copy_(got[0])
+
+
+# (a poll waits for some microseconds by itself, so that short calls get what they wait for)
+@pytest.mark.parametrize("H,hd,n,T", [(32, 128, 1, 20000), (32, 64, 12, 40000), (32, 128, 300, 20000), (24, 128, 300, 20000), (32, 64, 300, 40000)])
+def test_a_wait_that_runs_out(cuda, H, hd, n, T):
+    """One poll per wait (an environment variable, hence a process of its own): every warp gives up in its own place, copies and products in flight end before a
+    CTA leaves, the synchronisation says so, and the calls behind it are sound."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from seq2seqsharp_b200 import _native as N
+from seq2seqsharp_b200.ops import Ops
+H, hd, n, T = %d, %d, %d, %d
+pages = 2 * (T // 16 + 1)
+K, V = (torch.randn(pages, 8, 16, hd, device="cuda", dtype=torch.float16) for _ in range(2))
+q = torch.randn(2 * n, H, hd, device="cuda", dtype=torch.float16)
+i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+table = torch.arange(pages, dtype=torch.int32, device="cuda").view(2, -1)
+for _ in range(4):
+    out = Ops.PagedAttention(None, q, K, V, table, i([0, n, 2 * n]), i([T, T - 40]), n)
+torch.cuda.synchronize()
+try:
+    N.call("TSB200_Synchronize", 0, None)
+    print("silent")
+except N.TSB200Error as e:
+    print(e)
+N.call("TSB200_Synchronize", 0, None)
+print("usable", float(torch.ones(4, device="cuda").sum()))
+""" % (H, hd, n, T)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, env=dict(os.environ, TSB200_WAIT_LIMIT="1"),
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stderr
+    assert "gave up waiting" in r.stdout and "usable 4.0" in r.stdout, r.stdout
