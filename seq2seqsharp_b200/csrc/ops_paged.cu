@@ -140,7 +140,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs a, in
 //   y = x / sqrt(mean(x^2) + eps) * w;   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin),   angle = position * base^(-2 i / rot)
 // for every query and key head of a row; queries go to `out`, keys and values to the row's place in the cache.  Norm and rotation in fp32, rounded once;
 // angles in 64 bits (fp32 loses the angle of position 10^5 from the third digit on) as half turns, which are brought to [-1, 1] before they are rounded.
-// L = 2^k lanes hold a head, eight elements each (elements of a 16-bit head: 16 bytes per lane).  The cos / sin of a row are made once per CTA.
+// L = 2^k lanes hold a head, 8 C elements each; the cos / sin of a row are made once per CTA.  What bounds it: issue slots and bytes about equally.  Of 16384 rows
+// of 32 + 16 heads of 64 in bf16 (201 MB, 30.8 us at the rate of a copy): C = 1, six CTAs per SM 54.5 us; C = 2, four 44.4 (five 49.1, three 47.6); C = 4, two 63.
+// Rows first and heads second, with a head's addresses and weights kept in registers, is slower (61: a warp's lines lie in two places).
 struct RopePagedArgs {
   void* out;
   const void *q, *k, *v, *q_norm, *k_norm;
@@ -207,9 +209,9 @@ struct Eight {
   }
 };
 
-// STYLE as in RopePagedArgs; LT: lanes of a head, 0: as many as its size needs
-template <typename T, bool WIDE, int STYLE, int LT>
-__global__ void __launch_bounds__(kRopeThreads, WIDE && sizeof(T) == 2 ? 6 : 4) qk_norm_rope_paged_kernel(const __grid_constant__ RopePagedArgs a) {
+// STYLE as in RopePagedArgs; LT: lanes of a head, 0: as many as its size needs; C: pieces of eight elements per lane, L apart
+template <typename T, bool WIDE, int STYLE, int LT, int C>
+__global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_paged_kernel(const __grid_constant__ RopePagedArgs a) {
   constexpr bool WHOLE = STYLE != 2;
   __shared__ __align__(16) float wq[kRopeMaxHd], wk[kRopeMaxHd];
   __shared__ __align__(16) float2 turn[kRopeTurns];
@@ -226,16 +228,50 @@ __global__ void __launch_bounds__(kRopeThreads, WIDE && sizeof(T) == 2 ? 6 : 4) 
   }
   int L = LT ? LT : 1;
   if (LT == 0)
-    while (L * 8 < a.hd) L <<= 1;
+    while (L * C * 8 < a.hd) L <<= 1;
   const int li = tid & (L - 1), per = kRopeThreads / L, heads = a.H + 2 * a.Hkv;
-  const bool on = li * 8 < a.hd, turned = STYLE && li * 8 < a.rot, norms = a.q_norm || a.k_norm;
+  const bool norms = a.q_norm || a.k_norm;
   const float inv_hd = 1.0f / (float)a.hd;
-  // a lane has four elements and the four that they turn with (pairs (i, i + rot / 2)), or eight neighbours
-  const int e0 = STYLE == 2 && turned ? li * 4 : li * 8, e1 = STYLE == 2 && turned ? half + li * 4 : e0 + 4;
+  // C times, a lane has four elements and the four that they turn with (pairs (i, i + rot / 2)), or eight neighbours
+  bool on[C], turned[C];
+  int e0[C], e1[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int i = c * L + li;
+    on[c] = i * 8 < a.hd;
+    turned[c] = STYLE && i * 8 < a.rot;
+    e0[c] = STYLE == 2 && turned[c] ? i * 4 : i * 8;
+    e1[c] = STYLE == 2 && turned[c] ? half + i * 4 : e0[c] + 4;
+  }
   const int places = a.num_pages << a.page_shift;
-  const int row_first = (int)blockIdx.x * a.rows_here, row_end = min(a.rows, row_first + a.rows_here);
+  const int row_first = (int)blockIdx.x * a.rows_here, row_end = row_first + min(a.rows_here, a.rows - row_first);
   for (int row0 = row_first; row0 < row_end; row0 += rows_pass) {
     const int n = min(rows_pass, row_end - row0);
+    // (row, head) pairs go round the groups of L lanes; the next one is on its way while one is turned
+    const int stride = per * (int)gridDim.y, passes = (n * heads + stride - 1) / stride;
+    int head = (int)blockIdx.y * per + tid / L, r = 0;
+    Eight<T, WIDE> ahead[C];
+    int slot = -1;
+    auto fetch = [&](bool known) {
+      while (head >= heads) {
+        head -= heads;
+        ++r;
+      }
+      slot = r >= n ? -1 : known ? place[r] : 0;
+      if (slot < 0) return;
+      const int64_t row = row0 + r;
+      const T* p = head < a.H ? reinterpret_cast<const T*>(a.q) + row * a.q_row + (int64_t)head * a.q_head
+                              : (head < a.H + a.Hkv ? reinterpret_cast<const T*>(a.k) + row * a.k_row + (int64_t)(head - a.H) * a.k_head
+                                                    : reinterpret_cast<const T*>(a.v) + row * a.v_row + (int64_t)(head - a.H - a.Hkv) * a.v_head);
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (on[c]) ahead[c].template load<WHOLE>(p + e0[c], p + e1[c]);
+    };
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < Eight<T, WIDE>::N; ++i) ahead[c].r[i] = 0u;
+    fetch(false);   // of the first pass before the angles are made, whether it has a place or not
     __syncthreads();   // the pass before is done with both
     if (STYLE && ar < turn_rows)
       for (int r = ar; r < n; r += turn_rows) {
@@ -250,72 +286,62 @@ __global__ void __launch_bounds__(kRopeThreads, WIDE && sizeof(T) == 2 ? 6 : 4) 
       place[r] = slot >= 0 && slot < places ? slot : -1;
     }
     __syncthreads();
-    // (row, head) pairs go round the groups of L lanes; the next one is on its way while one is turned
-    const int stride = per * (int)gridDim.y, passes = (n * heads + stride - 1) / stride;
-    int head = (int)blockIdx.y * per + tid / L, r = 0;
-    Eight<T, WIDE> ahead;
-    int slot = -1;
-    auto fetch = [&]() {
-      while (head >= heads) {
-        head -= heads;
-        ++r;
-      }
-      slot = r < n && on ? place[r] : -1;
-      if (slot < 0) return;
-      const int64_t row = row0 + r;
-      const T* p = head < a.H ? reinterpret_cast<const T*>(a.q) + row * a.q_row + (int64_t)head * a.q_head
-                              : (head < a.H + a.Hkv ? reinterpret_cast<const T*>(a.k) + row * a.k_row + (int64_t)(head - a.H) * a.k_head
-                                                    : reinterpret_cast<const T*>(a.v) + row * a.v_row + (int64_t)(head - a.H - a.Hkv) * a.v_head);
-      ahead.template load<WHOLE>(p + e0, p + e1);
-    };
-#pragma unroll
-    for (int i = 0; i < Eight<T, WIDE>::N; ++i) ahead.r[i] = 0u;
-    fetch();
+    slot = r < n ? place[r] : -1;
 #pragma unroll 1
     for (int pass = 0; pass < passes; ++pass) {
-      float x[8];
-      ahead.get(x);
+      float x[C][8];
+#pragma unroll
+      for (int c = 0; c < C; ++c) ahead[c].get(x[c]);
       const int head_now = head, r_now = r, slot_now = slot;
       const bool is_q = head_now < a.H, is_v = head_now >= a.H + a.Hkv;
       head += stride;
-      fetch();
+      fetch(true);
       if (norms) {
         float ss = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+        for (int e = 0; e < 8 * C; ++e) ss += x[e / 8][e & 7] * x[e / 8][e & 7];
         if constexpr (LT > 0) {
 #pragma unroll
           for (int o = LT / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         } else {
           for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         }
-        if (on && !is_v && (is_q ? a.q_norm : a.k_norm)) {
+        if (!is_v && (is_q ? a.q_norm : a.k_norm)) {
           const float f = rsqrtf(ss * inv_hd + a.eps);   // off by two units in the last place, which the rounding to 16 bits and the sum of squares exceed
           const float* w = is_q ? wq : wk;
-          const float4 w0 = *reinterpret_cast<const float4*>(w + e0), w1 = *reinterpret_cast<const float4*>(w + e1);
-          x[0] *= f * w0.x; x[1] *= f * w0.y; x[2] *= f * w0.z; x[3] *= f * w0.w;
-          x[4] *= f * w1.x; x[5] *= f * w1.y; x[6] *= f * w1.z; x[7] *= f * w1.w;
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+            if (C == 1 || on[c]) {
+              const float4 w0 = *reinterpret_cast<const float4*>(w + e0[c]), w1 = *reinterpret_cast<const float4*>(w + e1[c]);
+              x[c][0] *= f * w0.x; x[c][1] *= f * w0.y; x[c][2] *= f * w0.z; x[c][3] *= f * w0.w;
+              x[c][4] *= f * w1.x; x[c][5] *= f * w1.y; x[c][6] *= f * w1.z; x[c][7] *= f * w1.w;
+            }
         }
       }
       if (slot_now >= 0) {
-        if (STYLE && turned && !is_v) {
-          const float4* t = reinterpret_cast<const float4*>(turn + r_now * slots + li * 4);
-          const float4 t0 = t[0], t1 = t[1];
-          const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y, t0.w, t1.y, t1.w};
+        if (STYLE && !is_v)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float &u = x[STYLE == 2 ? i : 2 * i], &v = x[STYLE == 2 ? 4 + i : 2 * i + 1];
-            const float y0 = u * c[i] - v * s[i], y1 = v * c[i] + u * s[i];
-            u = y0;
-            v = y1;
-          }
-        }
+          for (int c = 0; c < C; ++c)
+            if (turned[c]) {
+              const float4* t = reinterpret_cast<const float4*>(turn + r_now * slots + (c * L + li) * 4);
+              const float4 t0 = t[0], t1 = t[1];
+              const float co[4] = {t0.x, t0.z, t1.x, t1.z}, si[4] = {t0.y, t0.w, t1.y, t1.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float &u = x[c][STYLE == 2 ? i : 2 * i], &v = x[c][STYLE == 2 ? 4 + i : 2 * i + 1];
+                const float y0 = u * co[i] - v * si[i], y1 = v * co[i] + u * si[i];
+                u = y0;
+                v = y1;
+              }
+            }
         T* dst;
         if (is_q) dst = reinterpret_cast<T*>(a.out) + (int64_t)(row0 + r_now) * a.o_row + (int64_t)head_now * a.o_head;
         else
           dst = reinterpret_cast<T*>(is_v ? a.V : a.K) + (int64_t)(slot_now >> a.page_shift) * a.c_page + (int64_t)(slot_now & ((1 << a.page_shift) - 1)) * a.c_tok +
                 (int64_t)(head_now - (is_v ? a.H + a.Hkv : a.H)) * a.c_head;
-        Eight<T, WIDE>::template store<WHOLE>(dst + e0, dst + e1, x);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          if (on[c]) Eight<T, WIDE>::template store<WHOLE>(dst + e0[c], dst + e1[c], x[c]);
       }
     }
   }
@@ -323,9 +349,10 @@ __global__ void __launch_bounds__(kRopeThreads, WIDE && sizeof(T) == 2 ? 6 : 4) 
 
 template <typename T, bool WIDE, int STYLE>
 static void launch_rope_paged_l(const RopePagedArgs& a, dim3 grid, cudaStream_t s) {
-  if (WIDE && a.hd > 32 && a.hd <= 64) qk_norm_rope_paged_kernel<T, WIDE, STYLE, WIDE ? 8 : 0><<<grid, kRopeThreads, 0, s>>>(a);
-  else if (WIDE && a.hd > 64 && a.hd <= 128) qk_norm_rope_paged_kernel<T, WIDE, STYLE, WIDE ? 16 : 0><<<grid, kRopeThreads, 0, s>>>(a);
-  else qk_norm_rope_paged_kernel<T, WIDE, STYLE, 0><<<grid, kRopeThreads, 0, s>>>(a);
+  constexpr int C = WIDE && sizeof(T) == 2 ? 2 : 1;   // fp32: two pieces are no faster (7.8 us for 2036 rows of 8 + 16 heads of 64)
+  if (WIDE && a.hd > 32 && a.hd <= 64) qk_norm_rope_paged_kernel<T, WIDE, STYLE, WIDE ? 8 / C : 0, C><<<grid, kRopeThreads, 0, s>>>(a);
+  else if (WIDE && a.hd > 64 && a.hd <= 128) qk_norm_rope_paged_kernel<T, WIDE, STYLE, WIDE ? 16 / C : 0, C><<<grid, kRopeThreads, 0, s>>>(a);
+  else qk_norm_rope_paged_kernel<T, WIDE, STYLE, 0, 1><<<grid, kRopeThreads, 0, s>>>(a);
 }
 template <typename T, bool WIDE>
 static void launch_rope_paged(const RopePagedArgs& a, dim3 grid, cudaStream_t s) {
@@ -905,9 +932,10 @@ int TSB200_QKNormRopePaged(int device, int dtype, void* q_out, int64_t o_row, in
   const int V = 16 / (int)dtype_size(dtype);
   const bool wide = ((o_row | o_head | q_row | q_head | k_row | k_head | v_row | v_head | c_page | c_head | c_tok) % V) == 0 &&
                     (((uintptr_t)q_out | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cacheK | (uintptr_t)cacheV) % 16) == 0;
-  // Few rows: a CTA each, or several, so that every head has its lanes at once; many: six CTAs of an SM share them, at least a pass of angles each
-  const int L = hd <= 8 ? 1 : hd <= 16 ? 2 : hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32, heads = H + 2 * Hkv, parts = (heads * L + kRopeThreads - 1) / kRopeThreads;
-  const int ctas = 6 * st->sm_count;
+  // Few rows: a CTA each, or several, so that every head has its lanes at once; many: four CTAs of an SM share them, at least a pass of angles each
+  const int L = hd <= 8 ? 1 : hd <= 16 ? 2 : hd <= 32 ? 4 : hd <= 64 ? 8 : hd <= 128 ? 16 : 32, heads = H + 2 * Hkv;
+  const int pieces = wide && dtype != TSB200_F32 && hd > 32 && hd <= 128 ? 2 : 1, parts = (heads * L / pieces + kRopeThreads - 1) / kRopeThreads;
+  const int ctas = 4 * st->sm_count;
   dim3 grid;
   if (rows <= ctas / 2) {
     a.rows_here = 1;
