@@ -6,9 +6,10 @@
 // Products, differences and sums are 64-bit: u q and p - q are then exact, and a sum's rounding is far below the distance of two fp32 weights, so that
 // the order in which a vocabulary is added up does not decide which token is drawn.
 //
-// A cluster per sequence.  Its warps share the vocabulary in equal runs and push what theirs weigh to every CTA; after one cluster barrier the one warp whose run the
-// draw falls into looks for the token in it.  Rows that no draw needs are not read.  What bounds it: four dependent reads of memory and the launch for few sequences
-// (one of 32000 words: 44 us with one CTA and a run of the vocabulary per thread -> ...), bytes for many.
+// A cluster per sequence.  Its warps share the vocabulary in equal runs and push what theirs weigh to every CTA; after one cluster barrier all know the run that
+// the draw falls into, and that warp's CTA shares it out once more.  Rows that no draw needs are not read.  What bounds it: four dependent reads of memory, the
+// launch and the barriers for few sequences (one of 32000 words: 5.5 us; 44 with one CTA), and the widening of two numbers a word for many (64 of 50257 words, 25.7 MB:
+// 11.7 us; 17.8 with one warp looking for the token and widening before the comparison).
 #include "kernels.cuh"
 
 namespace tsb {
@@ -41,6 +42,8 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {   // inclusive
 }
 
 __global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __grid_constant__ VerifyArgs a, int ctas) {
+  __shared__ double parts[kVerifyWarps];
+  __shared__ int over, weighs;   // first thread whose words pass the draw, last one whose words weigh anything
   __shared__ double sums[2][kVerifyMaxCtas * kVerifyWarps];   // of every warp's run: of max(p - q, 0), and of p
   const int b = (int)blockIdx.x / ctas, rank = (int)blockIdx.x % ctas, tid = threadIdx.x, lane = tid & 31, w = rank * kVerifyWarps + (tid >> 5);
   const int row0 = a.starts ? a.starts[b] : b * (a.K + 1);
@@ -81,22 +84,31 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __gr
   const float* p = a.p + (int64_t)(row0 + taken) * a.p_row;
   const float* q = refused && a.q ? a.q + ((int64_t)b * a.K + taken) * a.q_row : nullptr;
   const int certain = refused && !a.q ? x[taken] : -1;
-  auto weigh = [&](int t, double& rest, double& all) {
-    const float pt = p[t], qt = q ? q[t] : 0.0f;
-    all = pt > 0.0f ? (double)pt : 0.0;
-    const double r = (double)pt - (q ? (double)qt : (t == certain ? 1.0 : 0.0));
-    rest = r > 0.0 ? r : 0.0;
+  constexpr int N = 8;   // steps of 32 words on their way at a time
+  float pt[N], qt[N];
+  auto fetch = [&](int t0, int end) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) pt[k] = t0 + 32 * k + lane < end ? p[t0 + 32 * k + lane] : 0.0f;
+    if (q) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) qt[k] = t0 + 32 * k + lane < end ? q[t0 + 32 * k + lane] : 0.0f;
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) qt[k] = t0 + 32 * k + lane == certain ? 1.0f : 0.0f;
+    }
   };
   // this warp's run of the vocabulary, 32 words at a time
   const int warps = ctas * kVerifyWarps, per = ((a.V + warps - 1) / warps + 31) & ~31, v0 = min((int64_t)a.V, (int64_t)w * per), v1 = min((int64_t)a.V, (int64_t)v0 + per);
   {
     double rest = 0.0, all = 0.0;
-#pragma unroll 8
-    for (int t = v0 + lane; t < v1; t += 32) {
-      double r, s;
-      weigh(t, r, s);
-      rest += r;
-      all += s;
+    for (int t0 = v0; t0 < v1; t0 += 32 * N) {
+      fetch(t0, v1);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float x = fmaxf(pt[k], 0.0f);   // of NaN: 0
+        all += (double)x;
+        rest += x > qt[k] ? (double)x - (double)qt[k] : 0.0;
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -157,28 +169,38 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draft_kernel(const __gr
     hit = last;
     start = r;   // its last word
   }
-  if (hit != w) return;
-  int token = -1, some = -1;
-  constexpr int N = 8;   // steps of 32 words on their way at a time
-  for (int t0 = v0; t0 < v1 && token < 0; t0 += 32 * N) {
-    double mine[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int t = t0 + 32 * k + lane;
-      double wr = 0.0, wa = 0.0;
-      if (t < v1) weigh(t, wr, wa);
-      mine[k] = rest ? wr : wa;
-    }
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const double to = start + warp_scan(mine[k], lane);
-      const unsigned over = __ballot_sync(0xffffffffu, any && mine[k] > 0.0 && to > r), weighs = __ballot_sync(0xffffffffu, mine[k] > 0.0);
-      if (token < 0 && weighs) some = t0 + 32 * k + 31 - __clz(weighs);
-      if (token < 0 && over) token = t0 + 32 * k + __ffs(over) - 1;
-      start = __shfl_sync(0xffffffffu, to, 31);
-    }
+  if (hit / kVerifyWarps != rank) return;
+  // its CTA shares the run out once more: so many neighbouring words to a thread
+  const int h0 = (int)min((int64_t)a.V, (int64_t)hit * per), h1 = (int)min((int64_t)a.V, (int64_t)h0 + per), each = per > kVerifyThreads ? (per + kVerifyThreads - 1) / kVerifyThreads : 1;
+  const int t0 = (int)min((int64_t)h1, (int64_t)h0 + (int64_t)tid * each), t1 = min(h1, t0 + each);
+  auto weight = [&](int t) {
+    const float pw = fmaxf(p[t], 0.0f), qw = q ? q[t] : t == certain ? 1.0f : 0.0f;
+    return !rest ? (double)pw : pw > qw ? (double)pw - (double)qw : 0.0;
+  };
+  double mine = 0.0;
+#pragma unroll 4
+  for (int t = t0; t < t1; ++t) mine += weight(t);
+  const double to = warp_scan(mine, lane);
+  if (lane == 31) parts[tid >> 5] = to;
+  if (tid == 0) over = kVerifyThreads, weighs = -1;
+  __syncthreads();
+  for (int i = 0; i < tid >> 5; ++i) start += parts[i];
+  start += to - mine;
+  if (mine > 0.0) {
+    if (any && start + mine > r) atomicMin(&over, tid);
+    atomicMax(&weighs, tid);
   }
-  if (lane == 0) out[taken] = token >= 0 ? token : some;
+  __syncthreads();
+  const bool drawn = over < kVerifyThreads;
+  if (tid != (drawn ? over : weighs)) return;
+  int token = -1, some = -1;
+  for (int t = t0; t < t1 && token < 0; ++t) {
+    const double v = weight(t);
+    start += v;
+    if (v > 0.0) some = t;
+    if (drawn && v > 0.0 && start > r) token = t;
+  }
+  out[taken] = token >= 0 ? token : some;
 }
 
 }  // namespace tsb
