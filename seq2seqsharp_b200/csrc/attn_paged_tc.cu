@@ -1,15 +1,19 @@
 // Attention of chunks over a paged cache on the 5th-generation tensor cores (16-bit types, head sizes 64 and 128): paged.cuh says what is computed.
 //
 // One CTA per SM takes its run of units.  An item is 256 (query, head) pairs of a KV head as two tiles of 128 rows; a unit is 128 of its keys.  Roles: warps 0-3 and
-// 4-7 do the softmax of one tile each (a thread owns a row), warp 9 issues the products, warps 8, 10 and 11 bring rows in.  TMEM: S0 | S1 | O0 | O1; P goes over S as 16-bit
+// 4-7 do the softmax of one tile each (a thread owns a row), warp 9 issues the products, warp 8 brings rows in (10 and 11 help with queries).  TMEM: S0 | S1 | O0 | O1; P goes over S as 16-bit
 // operand; the products of one tile run behind the exponentials of the other (PV0(j) QK0(j+1) PV1(j) QK1(j+1)), and those of the next item's first keys
 // behind the output of this one's last.
 //
 // Keys and values come by TMA tensor copies, a box per page (128-byte swizzle, any strides that are multiples of 16 bytes); an entry that names no page is a coordinate
 // outside of the map, which arrives as zeros, and the values behind a sequence's end are overwritten with zeros before their product.  Queries come by TMA where
 // whole ones fill a tile (1, 2, 4 .. heads to a KV head), else by cp.async into the same swizzle: generic-proxy writes, which the issuing warp orders before
-// its products with a proxy fence.  (cp.async for keys and values too: 2.4 instead of 1.8 ms for two chunks of 2048 over 32768; its latency and issue do
-// not fit the time of a unit.)
+// its products with a proxy fence.
+//
+// What bounds it: the chain of a unit (scores, maximum, exponentials, sums, weights back to TMEM), which two tiles hide from the tensor core only in part.  Two chunks
+// of 2048 over 32768, 32 / 8 heads of 128: 1.55 ms, 1110 TFLOP/s of the 1644 that a library product reaches; prompts of 16384 of heads of 128 1.88 ms, of 64 1.57.  What
+// was measured on the way (ms, same chunks): cp.async for keys and values 2.39; one lane for the products and outputs rescaled at every new maximum 1.81; boxes
+// prefetched to L2 1.74; scores of 64 keys at a time 1.78.
 #include "attn_tmem.cuh"
 #include "paged.cuh"
 
@@ -225,7 +229,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
         if (q_boxes && qc > 0) tc_wait_short(s_u32(q_full), (qc - 1) & 1);
       }
     } else {
-      // ---------------- products, issued by whole warps: 32 of them to a unit leave no time for a single lane's descriptors (2.35 -> ... us a unit).
+      // ---------------- products, issued by an elected lane of a converged warp: 32 to a unit leave no time for the descriptors of a diverged one.
       // Instruction descriptors: fp32 accumulator, A K-major, 128 rows; K: N = 128 K-major; V: N = HD MN-major
       const uint32_t fmt = (1u << 4) | (Pair16<H>::kUmmaFormat << 7) | (Pair16<H>::kUmmaFormat << 10) | ((uint32_t)(kPtRows >> 4) << 24);
       const uint32_t id_qk = fmt | ((uint32_t)(kPtKeys >> 3) << 17), id_pv = fmt | (1u << 16) | ((uint32_t)(HD >> 3) << 17);

@@ -110,14 +110,6 @@ __device__ __forceinline__ float2 pa_add2(float2 x, float2 y) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
   return r;
 }
-// the larger values of two registers of 16-bit pairs
-template <typename H>
-__device__ __forceinline__ uint32_t pa_max_pair(uint32_t x, uint32_t y) {
-  uint32_t r;
-  if constexpr (Pair16<H>::kBf16) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
-  else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
-  return r;
-}
 // sum += the two 16-bit values of a register, in fp32
 template <typename H>
 __device__ __forceinline__ void pa_add_pair(float& s, uint32_t v) {

@@ -11,7 +11,7 @@ namespace tsb {
 // want = ceil((cached + fresh) / page);  need = max(0, want - held), taken from the top of the stack of free pages in the order of the sequences;
 // held - want pages of a sequence that wants fewer go back, so that taking and giving back leaves the stack as it was;
 // starts = exclusive sum of the granted rows;  slot(row) = table[pos / page] * page + pos % page.
-// What bounds it: latency (two block scans, a few hundred KB at most).  Sums of rows and pages over sequences are 64-bit: their bounds are the caller's.
+// What bounds it: latency (three block scans, a few hundred KB at most; 8 sequences 5.4 us, 1024 sequences with 33000 rows 13).  Sums of rows and pages over sequences are 64-bit: their bounds are the caller's.
 struct PlanArgs {
   const int *cached, *fresh;
   int B, page_shift, max_blocks, num_pages, rows;
@@ -244,6 +244,10 @@ __global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_paged_kernel(con
     e1[c] = STYLE == 2 && turned[c] ? half + i * 4 : e0[c] + 4;
   }
   const int places = a.num_pages << a.page_shift;
+  auto place_of = [&](int row) {   // in the cache, or -1
+    const int slot = a.slots[row];
+    return slot >= 0 && slot < places ? slot : -1;
+  };
   const int row_first = (int)blockIdx.x * a.rows_here, row_end = row_first + min(a.rows_here, a.rows - row_first);
   for (int row0 = row_first; row0 < row_end; row0 += rows_pass) {
     const int n = min(rows_pass, row_end - row0);
@@ -257,7 +261,7 @@ __global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_paged_kernel(con
         head -= heads;
         ++r;
       }
-      slot = r >= n ? -1 : known ? place[r] : 0;
+      slot = r >= n ? -1 : known ? place[r] : place_of(row0 + r);
       if (slot < 0) return;
       const int64_t row = row0 + r;
       const T* p = head < a.H ? reinterpret_cast<const T*>(a.q) + row * a.q_row + (int64_t)head * a.q_head
@@ -271,7 +275,7 @@ __global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_paged_kernel(con
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int i = 0; i < Eight<T, WIDE>::N; ++i) ahead[c].r[i] = 0u;
-    fetch(false);   // of the first pass before the angles are made, whether it has a place or not
+    fetch(false);   // of the first pass before the angles are made
     __syncthreads();   // the pass before is done with both
     if (STYLE && ar < turn_rows)
       for (int r = ar; r < n; r += turn_rows) {
@@ -281,12 +285,8 @@ __global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_paged_kernel(con
         sincospif((float)x, &s, &c);
         turn[r * slots + ai] = make_float2(c, s);
       }
-    for (int r = tid; r < n; r += kRopeThreads) {
-      const int slot = a.slots[row0 + r];
-      place[r] = slot >= 0 && slot < places ? slot : -1;
-    }
+    for (int r = tid; r < n; r += kRopeThreads) place[r] = place_of(row0 + r);
     __syncthreads();
-    slot = r < n ? place[r] : -1;
 #pragma unroll 1
     for (int pass = 0; pass < passes; ++pass) {
       float x[C][8];
@@ -364,7 +364,8 @@ static void launch_rope_paged(const RopePagedArgs& a, dim3 grid, cudaStream_t s)
 // ------------------------------------------------------------------------------------------------------------------------ attention, every type
 // Four warps of RW rows; a tile of 32 keys and values is brought to shared memory by cp.async while the one before is used (places
 // that hold no visible key are filled with zeros, whatever the cache has there).  Scores: a lane per key; values: a lane per hd / 32 elements.
-// fp32 throughout: the products run on the FMA pipe, which is what bounds chunks; single tokens are bound by bytes.
+// fp32 throughout: the products run on the FMA pipe, which is what bounds chunks; single tokens are bound by bytes.  It serves what the kernels for tensor cores
+// do not: fp32 tokens, other head sizes, strides that no tensor map takes (8 fp32 tokens over 8000 keys, 8 / 8 heads of 64: 17 us).
 constexpr int kFmaThreads = 128, kFmaKeys = 32;
 __device__ __forceinline__ void paged_cp16(void* dst, const void* src, bool there) {   // zeros where there is nothing
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -768,7 +769,9 @@ int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int 
   return check_launch("paged_combine");
 }
 
-// The kernel that serves a call, its rows of a tile and its CTAs
+// The kernel that serves a call, its rows of a tile and its CTAs, by the most (query, head) pairs of a KV head that a sequence may have.  us, 8 sequences:
+//   16-bit, 4000 tokens, 32 / 8 heads of 128:  32 pairs mma.sync 35, tcgen05 38;  64: 38, 43;  96: 51, 41;  128: 60, 45
+//   fp32, 1000 tokens, 8 / 8 heads of 64:      16 pairs a lane per key 30, tiles 38;  32: 40, 38;  64: 57, 40
 struct PagedChoice {
   enum { FMA, TILE, MMA, TC } kind;
   int RT, KT, ctas;
@@ -994,7 +997,8 @@ int TSB200_PagedAttention(int device, int dtype, void* out, int64_t o_row, int64
   a.starts = starts; a.lens = lens; a.B = B; a.rows = rows; a.H = H; a.Hkv = Hkv; a.G = H / Hkv; a.hd = hd;
   a.by_G.set((uint32_t)a.G);
   a.c = scale * 1.44269504088896340736f;
-  a.window = window; cudaStream_t s = pick_stream(st, stream);
+  a.window = window;
+  cudaStream_t s = pick_stream(st, stream);
   // the kernels on tensor cores look for the largest score before it is scaled
   const PagedChoice c = paged_choose(st->sm_count, dtype, pairs, hd, scale > 0 && paged_tc_strides(a));
   TSB_CHECK(st->sm_count <= kSmCountMost, "paged_attention: %d SMs", st->sm_count);

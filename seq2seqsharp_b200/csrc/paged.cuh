@@ -267,7 +267,7 @@ struct PagedRun {
     tiles = (seq.n * a.G + RT - 1) / RT;
     if (off == l.units) step(a);
   }
-  __device__ __forceinline__ void step(const PagedArgs& a, int RT = 0) {
+  __device__ __forceinline__ void step(const PagedArgs& a) {
     off = 0;
     if (++h < a.Hkv) return;
     h = 0;
