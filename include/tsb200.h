@@ -259,7 +259,7 @@ TSB200_API int TSB200_PagedPlan(int device, const int32_t* cached, const int32_t
  * their places in the cache.  q, q_out [rows, H, hd], k, v [rows, Hkv, hd] with strides in elements (the last one is 1); q_out may be q.
  * rope_style 0: none, 1: pairs (2i, 2i + 1) of the first rope_dims elements, 2: pairs (i, i + rope_dims / 2) (rope_dims a multiple of 16); angle
  * position * rope_base^(-2i / rope_dims), in 64 bits.  A row whose slot is not one of the cache (-1) is left out: nothing of it is read or written.
- * The slots of a call differ.  Place o of page p, head h of cacheK and cacheV: element p * c_page + h * c_head + o * c_tok.  hd: a multiple of 8 up to 256. */
+ * The slots of a call differ.  Strides are below 2^31.  Place o of page p, head h of cacheK and cacheV: element p * c_page + h * c_head + o * c_tok.  hd: a multiple of 8 up to 256. */
 TSB200_API int TSB200_QKNormRopePaged(int device, int dtype, void* q_out, int64_t o_row, int64_t o_head, const void* q, int64_t q_row, int64_t q_head,
                                       const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* q_norm,
                                       const void* k_norm, float eps, const int32_t* positions, const int32_t* slots, int rows, int H, int Hkv, int hd,
@@ -267,7 +267,9 @@ TSB200_API int TSB200_QKNormRopePaged(int device, int dtype, void* q_out, int64_
                                       int64_t c_tok, int num_pages, int page, void* stream);
 /* Attention of the new rows over the pages: row i of the n of sequence b is at position lens[b] - n + i and sees the keys up to it (window > 0: the last
  * `window` of them), out = softmax(scale q k^T) v, query head h reading KV head h / (H / Hkv).  Entries of the table that name no page
- * hide their keys; a row that sees none becomes zeros; rows of no sequence are left as they were.  What the pages hold behind lens[b] is never used.
+ * hide their keys; a row that sees none becomes zeros; rows of no sequence are left as they were.  What the pages hold behind lens[b] is never used.  A key or value
+ * that is not finite may reach other rows of the call's own chunk of its sequence than those that see it (a weight of 0 times NaN).  scale <= 0 and strides of 0 are
+ * served by the general kernel.
  * max_new: the most new rows of a sequence, as far as the caller knows (it chooses the kernel; more rows are served as well, with a workspace for max_new).
  * Pointers on a boundary of 16 bytes, strides (elements) multiples of 16 bytes.  workspace >= TSB200_PagedAttentionWorkspaceBytes; calls that may overlap need one each. */
 TSB200_API int64_t TSB200_PagedAttentionWorkspaceBytes(int dtype, int H, int Hkv, int hd, int max_new);
