@@ -54,6 +54,10 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
   __shared__ PagedPlanShared plan;
   __shared__ int s_err;
   const int tid = threadIdx.x, lane = tid & 31, w = warp_index();
+  if (tid == kPmWarps * 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mapK) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mapV) : "memory");
+  }
   pdl_trigger();
   long long all;
   int runs;

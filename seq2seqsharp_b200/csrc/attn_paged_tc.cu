@@ -86,6 +86,11 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
   __shared__ int s_err;
 
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  if (tid == 8 * 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mapK) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mapQ) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mapV) : "memory");
+  }
   long long all;
   int runs;
   if (!paged_locate<kPtThreads, kPtTile, kPtKeys>(a, blockIdx.x, gridDim.x, plan, all, runs)) return;

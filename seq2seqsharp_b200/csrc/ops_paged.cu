@@ -755,7 +755,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_combine_kernel(const __gri
 
 template <typename T>
 static cudaError_t launch_join(const PagedArgs& a, int RT, int ctas, cudaStream_t s) {
-  const int W = RT <= 32 ? 8 : RT <= 64 ? 2 : 1, parts = (RT * a.hd / 4 * W + kJoinThreads - 1) / kJoinThreads;
+  const int W = RT <= 32 ? 8 : RT <= 64 ? 2 : 1, rows = a.most < RT ? a.most : RT, parts = (rows * a.hd / 4 * W + kJoinThreads - 1) / kJoinThreads;
   const dim3 grid(ctas - 1, parts < 16 ? parts : 16);   // most runs end between items: few CTAs each, which go round
   return launch_k(W == 8 ? paged_combine_kernel<T, 8> : W == 2 ? paged_combine_kernel<T, 2> : paged_combine_kernel<T, 1>, grid, dim3(kJoinThreads), 0, s, a, RT);
 }
@@ -973,7 +973,7 @@ int TSB200_PagedAttention(int device, int dtype, void* out, int64_t o_row, int64
   PagedArgs a{};
   TSB_CHECK(dtype == TSB200_F32 || dtype == TSB200_F16 || dtype == TSB200_BF16, "paged_attention: unsupported dtype %d", dtype);
   TSB_CHECK(B >= 0 && rows >= 0 && max_new >= 1, "paged_attention: %d sequences, %d rows, at most %d new", B, rows, max_new);
-  TSB_CHECK(H >= 1 && Hkv >= 1 && H % Hkv == 0, "paged_attention: %d query heads over %d key / value heads", H, Hkv);
+  TSB_CHECK(H >= 1 && H <= 65536 && Hkv >= 1 && H % Hkv == 0, "paged_attention: %d query heads over %d key / value heads", H, Hkv);
   TSB_CHECK(hd >= 8 && hd % 8 == 0 && hd <= 256, "paged_attention: head size %d, a multiple of 8 up to 256 is wanted", hd);
   TSB_CHECK(page_size_ok(page, &a.page_shift), "paged_attention: pages of %d tokens, a power of two from 8 to 256 is wanted", page);
   TSB_CHECK(max_blocks >= 1 && table_stride >= max_blocks && (int64_t)max_blocks * page <= 0x7fffff00, "paged_attention: %d pages per sequence (stride %lld)", max_blocks,
@@ -998,6 +998,7 @@ int TSB200_PagedAttention(int device, int dtype, void* out, int64_t o_row, int64
   a.by_G.set((uint32_t)a.G);
   a.c = scale * 1.44269504088896340736f;
   a.window = window;
+  a.most = (int)(pairs < 0x7fffffff ? pairs : 0x7fffffff);
   cudaStream_t s = pick_stream(st, stream);
   // the kernels on tensor cores look for the largest score before it is scaled
   const PagedChoice c = paged_choose(st->sm_count, dtype, pairs, hd, scale > 0 && paged_tc_strides(a));
