@@ -517,8 +517,18 @@ __global__ void __launch_bounds__(kFmaThreads) paged_fma_kernel(const __grid_con
 }
 
 // fp32 chunks: 64 rows and 64 keys at a time, a thread has 4 x 4 scores and 4 x D / 16 outputs (four elements of a row from shared memory feed 16 products).  What
-// bounds it: the FMA pipe and shared memory, about even.  (With 16 rows and a lane per key, shared memory alone: 2 x 512 rows over 3000, 32 / 8 heads of 128, 1890 us.)
+// bounds it: the FMA pipe and shared memory, about even.  2 x 512 rows over 3000, 32 / 8 heads of 128: 991 us (47 TFLOP/s with what the mask leaves out); 1090 with one product to an
+// instruction, 1890 with 16 rows and a lane per key (shared memory alone).
 constexpr int kTileThreads = 256, kTileRows = 64, kTileKeys = 64;
+// d += x y of two pairs: one instruction
+__device__ __forceinline__ void paged_fma2(float2& d, float2 x, float2 y) {
+  uint64_t a, b, c;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(x.x), "f"(x.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(y.x), "f"(y.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(c) : "f"(d.x), "f"(d.y));
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(c));
+}
 template <int D>
 constexpr int tile_smem() { return (kTileRows * (D + 4) + 2 * kTileKeys * (D + 4) + 2 * kTileKeys * D + kTileRows * (kTileKeys + 4)) * 4; }
 
@@ -564,7 +574,8 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) paged_f32_kerne
       if (p < pairs && e < pieces) x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + (int64_t)(s.row0 + query) * a.q_row + (run.h * a.G + p - query * a.G) * a.q_head + e * 4);
       *reinterpret_cast<float4*>(qs + r * (D + 4) + e * 4) = make_float4(x.x * a.c, x.y * a.c, x.z * a.c, x.w * a.c);
     }
-    float m[4], l[4], acc[4][C][4];
+    float m[4], l[4];
+    float2 acc[4][C][2];
     int lo[4], hi[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -576,18 +587,19 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) paged_f32_kerne
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][c][e] = 0.0f;
+        for (int e = 0; e < 2; ++e) acc[i][c][e] = make_float2(0.0f, 0.0f);
     }
     for (int kt = run.k0; kt < run.k1; ++kt) {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncthreads();   // this tile has landed, the one before has been used
       if (kt + 1 < run.k1) fetch(kt + 1);
       const float *k = ks + (kt & 1) * KT * (D + 4), *v = vs + (kt & 1) * KT * D;
-      float x[4][4];   // rows 4 ty + i, keys tx + 16 j
+      float2 x2[4][4];   // rows 4 ty + i, keys tx + 16 j: sums of the even and of the odd elements
+      float x[4][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
+        for (int j = 0; j < 4; ++j) x2[i][j] = make_float2(0.0f, 0.0f);
 #pragma unroll 4
       for (int e = 0; e < D; e += 4) {
         float4 q4[4], k4[4];
@@ -598,8 +610,15 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) paged_f32_kerne
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[i][j] += q4[i].x * k4[j].x + q4[i].y * k4[j].y + q4[i].z * k4[j].z + q4[i].w * k4[j].w;
+          for (int j = 0; j < 4; ++j) {
+            paged_fma2(x2[i][j], make_float2(q4[i].x, q4[i].y), make_float2(k4[j].x, k4[j].y));
+            paged_fma2(x2[i][j], make_float2(q4[i].z, q4[i].w), make_float2(k4[j].z, k4[j].w));
+          }
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i][j] = x2[i][j].x + x2[i][j].y;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float top = -INFINITY;
@@ -624,7 +643,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) paged_f32_kerne
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][c][e] *= f;
+          for (int e = 0; e < 2; ++e) acc[i][c][e].x *= f, acc[i][c][e].y *= f;
       }
       __syncwarp();   // a row's weights are made and used by the same half of a warp
 #pragma unroll 2
@@ -640,10 +659,8 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) paged_f32_kerne
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float p = u == 0 ? p4[i].x : u == 1 ? p4[i].y : u == 2 ? p4[i].z : p4[i].w;
-              acc[i][c][0] += p * v4.x;
-              acc[i][c][1] += p * v4.y;
-              acc[i][c][2] += p * v4.z;
-              acc[i][c][3] += p * v4.w;
+              paged_fma2(acc[i][c][0], make_float2(p, p), make_float2(v4.x, v4.y));
+              paged_fma2(acc[i][c][1], make_float2(p, p), make_float2(v4.z, v4.w));
             }
           }
       }
@@ -666,7 +683,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) paged_f32_kerne
       for (int c = 0; c < C; ++c) {
         const int e = c * 64 + tx * 4;
         if (e >= a.hd) continue;
-        *reinterpret_cast<float4*>((whole ? out : rec + 2 * RT + row * a.hd) + e) = make_float4(acc[i][c][0] * inv, acc[i][c][1] * inv, acc[i][c][2] * inv, acc[i][c][3] * inv);
+        *reinterpret_cast<float4*>((whole ? out : rec + 2 * RT + row * a.hd) + e) = make_float4(acc[i][c][0].x * inv, acc[i][c][0].y * inv, acc[i][c][1].x * inv, acc[i][c][1].y * inv);
       }
     }
   }
