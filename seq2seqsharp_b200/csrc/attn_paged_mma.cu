@@ -4,8 +4,8 @@
 // TMA tensor copies, a box per page (128-byte swizzle; an entry that names no page is a coordinate outside of the map and arrives as zeros), three or six
 // tiles ahead of their use.  Four warps multiply (mma.sync: the rows of a tensor-core tile of tcgen05 would be 7/8 empty): WR of them share the
 // rows, the others the keys of a tile, whose states (maximum, sum, output) meet in shared memory at an item's end.  No warp waits for another within an item.
-// What bounds it: bytes; 192 KB of an SM are on their way.  64 single tokens of 65536 keys in all, 32 / 8 heads of 128: 119 us, 5.7 TB/s; few short sequences are bound by
-// the chain lengths - page entries - copies - records (8 tokens over 32000 keys 19 us, one of 16384 11).
+// What bounds it: bytes; 192 KB of an SM are on their way.  64 single tokens over 165600 keys in all, 32 / 8 heads of 128: 119 us, 5.7 TB/s; few short sequences are bound by
+// the chain lengths - page entries - copies - records (8 tokens over 9600 keys 18 us, one over 530 10).
 #include <cfloat>
 
 #include "paged.cuh"

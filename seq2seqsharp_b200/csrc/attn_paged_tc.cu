@@ -11,7 +11,7 @@
 // its products with a proxy fence.
 //
 // What bounds it: the chain of a unit (scores, maximum, exponentials, sums, weights back to TMEM), which two tiles hide from the tensor core only in part.  Two chunks
-// of 2048 over 32768, 32 / 8 heads of 128: 1.55 ms, 1110 TFLOP/s of the 1644 that a library product reaches; prompts of 16384 of heads of 128 1.88 ms, of 64 1.57.  What
+// of up to 2048 over up to 32768, 32 / 8 heads of 128: 1.55 ms, 1110 TFLOP/s of the 1644 that a library product reaches; prompts of 16384 of heads of 128 1.88 ms, of 64 1.57.  What
 // was measured on the way (ms, same chunks): cp.async for keys and values 2.39; one lane for the products and outputs rescaled at every new maximum 1.81; boxes
 // prefetched to L2 1.74; scores of 64 keys at a time 1.78.
 #include "attn_tmem.cuh"

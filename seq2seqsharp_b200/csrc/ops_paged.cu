@@ -11,7 +11,7 @@ namespace tsb {
 // want = ceil((cached + fresh) / page);  need = max(0, want - held), taken from the top of the stack of free pages in the order of the sequences;
 // held - want pages of a sequence that wants fewer go back, so that taking and giving back leaves the stack as it was;
 // starts = exclusive sum of the granted rows;  slot(row) = table[pos / page] * page + pos % page.
-// What bounds it: latency (three block scans, a few hundred KB at most; 8 sequences 5.4 us, 1024 sequences with 33000 rows 13).  Sums of rows and pages over sequences are 64-bit: their bounds are the caller's.
+// What bounds it: latency (three block scans, a few hundred KB at most; 8 sequences 5.4 us, 1024 sequences with 92500 rows 13).  Sums of rows and pages over sequences are 64-bit: their bounds are the caller's.
 struct PlanArgs {
   const int *cached, *fresh;
   int B, page_shift, max_blocks, num_pages, rows;
@@ -365,7 +365,7 @@ static void launch_rope_paged(const RopePagedArgs& a, dim3 grid, cudaStream_t s)
 // Four warps of RW rows; a tile of 32 keys and values is brought to shared memory by cp.async while the one before is used (places
 // that hold no visible key are filled with zeros, whatever the cache has there).  Scores: a lane per key; values: a lane per hd / 32 elements.
 // fp32 throughout: the products run on the FMA pipe, which is what bounds chunks; single tokens are bound by bytes.  It serves what the kernels for tensor cores
-// do not: fp32 tokens, other head sizes, strides that no tensor map takes (8 fp32 tokens over 8000 keys, 8 / 8 heads of 64: 17 us).
+// do not: fp32 tokens, other head sizes, strides that no tensor map takes (8 fp32 tokens over 6000 keys, 8 / 8 heads of 64: 17 us).
 constexpr int kFmaThreads = 128, kFmaKeys = 32;
 __device__ __forceinline__ void paged_cp16(void* dst, const void* src, bool there) {   // zeros where there is nothing
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");

@@ -92,15 +92,17 @@ def _plain(op, dev, dtype, name, t, *shape):
 
 def _heads(op, dev, dtype, name, t, rows, heads, hd):
     """Address, row and head stride of a [rows, heads, hd] tensor.  The stride of a single entry means nothing and is 0."""
-    if t.dtype is not dtype or t.get_device() != dev or t.shape != (rows, heads, hd) or t.stride(2) != 1:
+    steps = t.stride()   # as a whole: a stride or size by number takes longer than all of them
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != (rows, heads, hd) or steps[2] != 1:
         raise N.TSB200Error("%s: %s is %s of %s with strides %s on %s, %s of %s with elements side by side on cuda:%d is wanted" % (
-            op, name, t.dtype, tuple(t.shape), t.stride(), t.device, dtype, (rows, heads, hd), dev))
-    return t.data_ptr(), t.stride(0) if rows > 1 else 0, t.stride(1) if heads > 1 else 0
+            op, name, t.dtype, tuple(t.shape), steps, t.device, dtype, (rows, heads, hd), dev))
+    return t.data_ptr(), steps[0] if rows > 1 else 0, steps[1] if heads > 1 else 0
 
 
 def _cache(op, dev, dtype, K, V):
     """Shape of a paged cache, its addresses and its page, head and token strides."""
-    _wrong(op, dev, dtype, cacheK=K, cacheV=V)
+    if K.dtype is not dtype or V.dtype is not dtype or K.get_device() != dev or V.get_device() != dev:
+        _wrong(op, dev, dtype, cacheK=K, cacheV=V)
     shape, steps = K.shape, K.stride()
     if len(shape) != 4 or V.shape != shape or steps[3] != 1 or (V.stride() != steps and any(n > 1 and x != y for n, x, y in zip(shape, steps, V.stride()))):
         raise N.TSB200Error("%s: keys %s with strides %s and values %s with strides %s, the same [pages, heads, page, head size] with elements side by side is wanted"
@@ -110,11 +112,12 @@ def _cache(op, dev, dtype, K, V):
 
 def _table(op, dev, t, B):
     """Address, row stride and width of a page table."""
-    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != 2 or t.size(0) != B or t.stride(1) != 1:
+    shape, steps = t.shape, t.stride()
+    if t.dtype is not _I32 or t.get_device() != dev or len(shape) != 2 or shape[0] != B or steps[1] != 1:
         raise N.TSB200Error("%s: table is %s of %s with strides %s on %s, int32 of [%d, pages of a sequence] with entries side by side on cuda:%d is wanted" % (
-            op, t.dtype, tuple(t.shape), t.stride(), t.device, B, dev))
-    width = t.size(1)
-    return t.data_ptr(), t.stride(0) if B > 1 else width, width
+            op, t.dtype, tuple(shape), steps, t.device, B, dev))
+    width = shape[1]
+    return t.data_ptr(), steps[0] if B > 1 else width, width
 
 
 class Ops:
@@ -362,12 +365,17 @@ class Ops:
             raise N.TSB200Error("VerifyDraft: targetProbs [rows, words] and draftTokens [sequences, drafts] are wanted")
         (rows, V), (B, K) = targetProbs.shape, draftTokens.shape
         _wrong(op, dev, _F32, targetProbs=targetProbs, draftProbs=draftProbs)
+        probs = []
         for name, t, n in (("targetProbs", targetProbs, rows), ("draftProbs", draftProbs, B * K)):
-            if t is not None and (t.shape != (n, V) or (V > 1 and t.stride(1) != 1)):
+            if t is None:
+                probs += None, 0
+                continue
+            steps = t.stride()
+            if t.shape != (n, V) or (V > 1 and steps[1] != 1):
                 raise N.TSB200Error("VerifyDraft: %s is %s, [%d, %d] with words side by side is wanted" % (name, tuple(t.shape), n, V))
-        args = (targetProbs.data_ptr(), targetProbs.stride(0), None if draftProbs is None else draftProbs.data_ptr(), 0 if draftProbs is None else draftProbs.stride(0),
-                _plain(op, dev, _I32, "draftTokens", draftTokens, B, K), None if starts is None else _plain(op, dev, _I32, "starts", starts, B + 1),
+            probs += t.data_ptr(), steps[0]
+        args = (*probs, _plain(op, dev, _I32, "draftTokens", draftTokens, B, K), None if starts is None else _plain(op, dev, _I32, "starts", starts, B + 1),
                 _plain(op, dev, _F32, "u", u, B, K + 1), B, K, V, rows)
-        out = torch.empty(B * (K + 2), dtype=_I32, device=u.device)
-        N.check(N.lib().TSB200_VerifyDraft(dev, out.data_ptr(), out.data_ptr() + 4 * B * (K + 1), *args, _queue(dev)), "TSB200_VerifyDraft")
-        return out[:B * (K + 1)].view(B, K + 1), out[B * (K + 1):]
+        tokens, counts = torch.empty((B, K + 1), dtype=_I32, device=u.device), torch.empty(B, dtype=_I32, device=u.device)
+        N.check(N.lib().TSB200_VerifyDraft(dev, tokens.data_ptr(), counts.data_ptr(), *args, _queue(dev)), "TSB200_VerifyDraft")
+        return tokens, counts
