@@ -1,9 +1,9 @@
 // Attention of chunks over a paged cache on the 5th-generation tensor cores (16-bit types, head sizes 64 and 128): paged.cuh says what is computed.
 //
 // One CTA per SM takes its run of units.  An item is 256 (query, head) pairs of a KV head as two tiles of 128 rows; a unit is 128 of its keys.  Roles: warps 0-3 and
-// 4-7 do the softmax of one tile each (a thread owns a row), warp 9 issues the products, warp 8 brings rows in (10 and 11 help with queries).  TMEM: S0 | S1 | O0 | O1; P goes over S as 16-bit
-// operand; the products of one tile run behind the exponentials of the other (PV0(j) QK0(j+1) PV1(j) QK1(j+1)), and those of the next item's first keys
-// behind the output of this one's last.
+// 4-7 do the softmax of one tile each (a thread owns a row), warp 9 issues the products, warp 8 brings rows in (10 and 11 help with queries).  TMEM: S0 | S1 |
+// O0 | O1; P goes over S as 16-bit operand; the products of one tile run behind the exponentials of the other (PV0(j) QK0(j+1) PV1(j) QK1(j+1)), and those of the
+// next item's first keys behind the output of this one's last.
 //
 // Keys and values come by TMA tensor copies, a box per page (128-byte swizzle, any strides that are multiples of 16 bytes); an entry that names no page is a coordinate
 // outside of the map, which arrives as zeros, and the values behind a sequence's end are overwritten with zeros before their product.  Queries come by TMA where
@@ -11,9 +11,9 @@
 // its products with a proxy fence.
 //
 // What bounds it: the chain of a unit (scores, maximum, exponentials, sums, weights back to TMEM), which two tiles hide from the tensor core only in part.  Two chunks
-// of up to 2048 over up to 32768, 32 / 8 heads of 128: 1.55 ms, 1110 TFLOP/s of the 1644 that a library product reaches; prompts of 16384 of heads of 128 1.88 ms, of 64 1.57.  What
-// was measured on the way (ms, same chunks): cp.async for keys and values 2.39; one lane for the products and outputs rescaled at every new maximum 1.81; boxes
-// prefetched to L2 1.74; scores of 64 keys at a time 1.78.
+// of up to 2048 over up to 32768, 32 / 8 heads of 128: 1.55 ms, 1110 TFLOP/s of the 1644 that a library product reaches; prompts of 16384 of heads of 128
+// 1.88 ms, of 64 1.57.  What was measured on the way (ms, same chunks): cp.async for keys and values 2.39; one lane for the products and outputs rescaled at every
+// new maximum 1.81; boxes prefetched to L2 1.74; scores of 64 keys at a time 1.78.
 #include "attn_tmem.cuh"
 #include "paged.cuh"
 
