@@ -539,9 +539,10 @@ static int pt_launch(int device, DeviceState* st, const PagedArgs& a, cudaStream
 int launch_paged_tc(int device, DeviceState* st, int dtype, PagedArgs a, cudaStream_t s) {
   a.wait_limit = tc_wait_limit();
   a.error = tc_error_word(device);
+  // us with ends moved by up to 1 | 4 units: 2 x 30 rows over 4096 24 | 28, 256 over 8192 53 | 57, a prompt of 1024 of heads of 64 29.5 | 28
   a.min_units = 4;
-  a.snap = 4;
-  a.start = 3;
+  a.snap = 1;
+  a.start = 2;
   st->waits = true;
   if (dtype == TSB200_F16) {
     if (a.hd == 64) TSB_TRY((pt_launch<__half, 1, 4>(device, st, a, s)));
