@@ -1,6 +1,6 @@
 // Attention of few rows per sequence over a paged cache (16-bit types, head sizes 64 and 128): single tokens, drafts, short chunks.  paged.cuh says what is computed.
 //
-// Two CTAs per SM take their runs of units; an item is 16, 32 or 64 (query, head) pairs of a KV head, a unit 64 of its keys.  A warp copies: keys and values come by
+// Two CTAs per SM take their runs of units; an item is 16 or 32 (query, head) pairs of a KV head, a unit 64 of its keys.  A warp copies: keys and values come by
 // TMA tensor copies, a box per page (128-byte swizzle; an entry that names no page is a coordinate outside of the map and arrives as zeros), three or six
 // tiles ahead of their use.  Four warps multiply (mma.sync: the rows of a tensor-core tile of tcgen05 would be 7/8 empty): WR of them share the
 // rows, the others the keys of a tile, whose states (maximum, sum, output) meet in shared memory at an item's end.  No warp waits for another within an item.
@@ -43,6 +43,7 @@ template <typename H, int BX, int WR>
 __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                                                                         const __grid_constant__ PagedArgs a) {
   constexpr int HD = BX * 64, NS = pm_stages(BX), RT = 16 * WR, KG = kPmWarps / WR, KS = HD / 16, NB = HD / 8;
+  static_assert(KG > 1, "the warps of other keys meet in shared memory");
   constexpr int SK = KG == 4 ? 16 : 32, STEPS = kPmKeys / KG / SK, SN = SK / 8;   // keys a warp weighs at a time
   extern __shared__ __align__(1024) unsigned char pm_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)pm_raw + 1023) & ~(uintptr_t)1023);
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
       lB += __shfl_xor_sync(0xffffffffu, lB, 1);
       lA += __shfl_xor_sync(0xffffffffu, lA, 2);
       lB += __shfl_xor_sync(0xffffffffu, lB, 2);
-      if constexpr (KG > 1) {
+      {
         // the warps of other keys: factors of every warp's rows first, then rows 0-7 and 8-15 through the same place
         if (t4 == 0) {
           float2* m2 = reinterpret_cast<float2*>(ml) + w * 16 + g8;
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
           }
         }
       }
-      if constexpr (KG > 1) named_sync<1, kPmWarps * 32>();   // the next item writes to the same places
+      named_sync<1, kPmWarps * 32>();   // the next item writes to the same places
     }
   }
   __syncthreads();
@@ -369,8 +370,7 @@ int launch_paged_mma(int device, DeviceState* st, int dtype, PagedArgs a, int RT
 #define TSB_PM(H, BX)                                                        \
   do {                                                                       \
     if (RT == 16) TSB_TRY((pm_launch<H, BX, 1>(device, st, a, s)));          \
-    else if (RT == 32) TSB_TRY((pm_launch<H, BX, 2>(device, st, a, s)));     \
-    else TSB_TRY((pm_launch<H, BX, 4>(device, st, a, s)));                   \
+    else TSB_TRY((pm_launch<H, BX, 2>(device, st, a, s)));                   \
   } while (0)
   if (dtype == TSB200_F16) {
     if (a.hd == 64) TSB_PM(__half, 1);

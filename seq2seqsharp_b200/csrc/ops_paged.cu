@@ -787,7 +787,7 @@ int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int 
 }
 
 // The kernel that serves a call, its rows of a tile and its CTAs, by the most (query, head) pairs of a KV head that a sequence may have.  us, 8 sequences:
-//   16-bit, 4000 tokens, 32 / 8 heads of 128:  32 pairs mma.sync 35, tcgen05 38;  64: 38, 43;  96: 51, 41;  128: 60, 45
+//   16-bit, 4000 tokens, 32 / 8 heads of 128:  32 pairs mma.sync 33.6, tcgen05 32.9 (one sequence: 18.4, 20.0);  64: 37.9, 36.0 (23.6, 21.1)
 //   fp32, 1000 tokens, 8 / 8 heads of 64:      16 pairs a lane per key 30, tiles 38;  32: 40, 38;  64: 57, 40
 struct PagedChoice {
   enum { FMA, TILE, MMA, TC } kind;
@@ -796,9 +796,9 @@ struct PagedChoice {
 static PagedChoice paged_choose(int sm_count, int dtype, int64_t pairs, int hd, bool positive) {
   PagedChoice c;
   if (is_16bit(dtype) && (hd == 64 || hd == 128) && positive) {
-    if (pairs <= 64) {
+    if (pairs <= 32) {
       c.kind = PagedChoice::MMA;
-      c.RT = pairs <= 16 ? 16 : pairs <= 32 ? 32 : 64;
+      c.RT = pairs <= 16 ? 16 : 32;
       c.KT = 64;
       c.ctas = 2 * sm_count;
       return c;
