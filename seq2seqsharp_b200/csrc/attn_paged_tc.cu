@@ -10,6 +10,10 @@
 // whole ones fill a tile (1, 2, 4 .. heads to a KV head), else by cp.async into the same swizzle: generic-proxy writes, which the issuing warp orders before
 // its products with a proxy fence.
 //
+// Weights are rounded to the cache's 16-bit type, because A and B of a product have one type; each is off by half a step at most, as the output is.  The sums add them as
+// rounded (1.3 to 2 % of the time: 1561 -> 1581 us for the chunks below): with sums of the unrounded ones, two at a time, weights that all round down left a
+// mean of equal values 2^-8 (fp16: 2^-11) below them.
+//
 // What bounds it: the chain of a unit (scores, maximum, exponentials, sums, weights back to TMEM), which two tiles hide from the tensor core only in part.  Two chunks
 // of up to 2048 over up to 32768, 32 / 8 heads of 128: 1.55 ms, 1110 TFLOP/s of the 1644 that a library product reaches; prompts of 16384 of heads of 128
 // 1.88 ms, of 64 1.57.  What was measured on the way (ms, same chunks): cp.async for keys and values 2.39; one lane for the products and outputs rescaled at every
@@ -48,8 +52,8 @@ __device__ __forceinline__ void pt_load_3d(uint32_t dst, const CUtensorMap* map,
       : "memory");
 }
 
-// A row's output is rescaled when its maximum is this much (in powers of two) above the one in use: weights are then up to 2^8, which neither type loses
-// anything by, and one of a warp's 32 rows has a new maximum in nearly every tile of the first hundred
+// A row's output is rescaled when its maximum is this much (in powers of two) above the one in use (a published method for attention on matrix units): one of a
+// warp's 32 rows has a new maximum in nearly every tile of the first hundred.  Weights are then up to 2^8, in range of both types; the largest is rounded like the others, no longer 1
 constexpr float kPtLag = 8.0f;
 
 // key tiles of the run that the two row tiles of an item need
@@ -390,7 +394,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
           }
         }
         const float mc = m == -INFINITY ? 0.0f : -m * c;   // no key seen yet: every weight is exp2(-inf)
-        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t y[32];
@@ -401,14 +405,14 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
             v.x = pa_ex2(v.x);
             v.y = pa_ex2(v.y);
             y[i] = Pair16<H>::put(v.x, v.y);
-            sum[i & 1] = pa_add2(sum[i & 1], v);
+            pa_add_pair<H>(sum[i & 3], y[i]);   // as rounded for the product: what rounding does to the numerator it does to the denominator
           }
           pa_st32(tS + h * 32, y);
           pa_st_wait();
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           pa_arrive(&p_full[2 * t + h]);
         }
-        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
       if (!ok) break;
       if (n > 0) {

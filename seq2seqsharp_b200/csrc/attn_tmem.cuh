@@ -100,16 +100,6 @@ __device__ __forceinline__ float2 pa_fma2(float a0, float a1, float b, float c) 
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
   return r;
 }
-// the sums of two pairs: one instruction
-__device__ __forceinline__ float2 pa_add2(float2 x, float2 y) {
-  uint64_t a, b, d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(x.x), "f"(x.y));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(y.x), "f"(y.y));
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
-  return r;
-}
 // sum += the two 16-bit values of a register, in fp32
 template <typename H>
 __device__ __forceinline__ void pa_add_pair(float& s, uint32_t v) {
