@@ -696,7 +696,7 @@ constexpr int kJoinThreads = 256;
 template <typename T, int W>
 __global__ void __launch_bounds__(kJoinThreads) paged_combine_kernel(const __grid_constant__ PagedArgs a, int RT) {
   constexpr int Q = kJoinThreads / W;   // quads of a CTA
-  __shared__ float shared_acc[W > 1 ? W : 1][W > 1 ? Q : 1][4];
+  __shared__ float4 shared_acc[W > 1 ? W : 1][W > 1 ? Q : 1];
   __shared__ float2 shared_ml[W > 1 ? W : 1][W > 1 ? Q : 1];
   const int c = (int)blockIdx.x + 1, share = W > 1 ? (int)threadIdx.x / Q : 0, at = (int)threadIdx.x % Q;
   pdl_wait();
@@ -740,7 +740,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_combine_kernel(const __gri
     if constexpr (W > 1) {
       __syncthreads();   // the elements before have been read
       if (share > 0) {
-        *reinterpret_cast<float4*>(shared_acc[share][at]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        shared_acc[share][at] = make_float4(acc[0], acc[1], acc[2], acc[3]);
         shared_ml[share][at] = make_float2(m, sum);
       }
       __syncthreads();
@@ -754,9 +754,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_combine_kernel(const __gri
       for (int q = 0; q < 4; ++q) acc[q] *= f0;
       for (int k = 1; k < most; ++k) {
         const float f = exp2f(shared_ml[k][at].x - from);
+        const float4 x = shared_acc[k][at];
         sum += shared_ml[k][at].y * f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) acc[q] += shared_acc[k][at][q] * f;
+        acc[0] += x.x * f;
+        acc[1] += x.y * f;
+        acc[2] += x.z * f;
+        acc[3] += x.w * f;
       }
     }
     if (!live) continue;
