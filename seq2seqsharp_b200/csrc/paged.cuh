@@ -194,6 +194,8 @@ __device__ __forceinline__ bool paged_locate(const PagedArgs& a, int c, int ctas
   const int tid = threadIdx.x, w = tid >> 5;
   // few sequences: every warp adds them up for itself, the first two look for an end each
   const bool few = a.B <= 32;
+  // the last run ends where no warp finds a unit; in front of the scans' barriers, behind which the other runs' ends are found by whichever warp has them
+  if (!few && tid == 0) sh.loc[1] = PagedLoc{a.B, 0, 0, 0, 0, 0};
   long long mine = paged_seq_units(a, few ? tid & 31 : tid, RT, KT), before = 0;
   if (few) {
     long long to = mine;
@@ -230,8 +232,6 @@ __device__ __forceinline__ bool paged_locate(const PagedArgs& a, int c, int ctas
       }
       if ((tid & 31) == 0) sh.loc[w] = l;
     }
-  } else if (tid == 0) {
-    sh.loc[1] = PagedLoc{a.B, 0, 0, 0, 0, all};
   }
   long long base = 0;
   for (int b0 = few ? a.B : 0; b0 < a.B && base <= x[1]; b0 += NT) {
