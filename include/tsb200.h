@@ -12,7 +12,8 @@
  *   - every entry point selects its device itself (the reference calls a backend from one thread per device:
  *     Seq2SeqSharp/Tools/BaseSeq2SeqFramework.cs:912) and is safe to call concurrently for different devices;
  *   - `stream` is a cudaStream_t passed as void*; NULL selects the library's own non-blocking stream of the
- *     device.  Nothing runs on the legacy NULL stream, unless it is named (cudaStreamLegacy, the handle 1);
+ *     device.  Nothing runs on the legacy NULL stream, unless it is named (cudaStreamLegacy, the handle 1).
+ *     Stand-alone calls on these two streams of a device run in the order in which they are made;
  *   - there is no CPU fallback: with no usable sm_100 device every compute entry point fails.
  */
 #ifndef TSB200_H_

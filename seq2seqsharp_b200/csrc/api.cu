@@ -43,7 +43,11 @@ int use_device(int device, DeviceState** st) {
       TSB_CUDA(cudaSetDevice(device));
       d.usable = (p.major == 10);
       d.sm_count = p.multiProcessorCount;
-      if (d.usable) TSB_CUDA(cudaStreamCreateWithFlags(&d.stream, cudaStreamNonBlocking));
+      if (d.usable) {
+        TSB_CUDA(cudaStreamCreateWithFlags(&d.stream, cudaStreamNonBlocking));
+        TSB_CUDA(cudaEventCreateWithFlags(&d.own_end, cudaEventDisableTiming));
+        TSB_CUDA(cudaEventCreateWithFlags(&d.legacy_end, cudaEventDisableTiming));
+      }
       d.ready = true;
     }
   }
@@ -51,6 +55,25 @@ int use_device(int device, DeviceState** st) {
   TSB_CUDA(cudaSetDevice(device));
   if (st) *st = &d;
   return 1;
+}
+
+static void order_behind(cudaStream_t s, cudaEvent_t end, cudaStream_t other) {
+  if (cudaEventRecord(end, other) == cudaSuccess && cudaStreamWaitEvent(s, end, 0) == cudaSuccess) return;
+  cudaGetLastError();
+  cudaStreamSynchronize(other);
+}
+// The marks are never taken back: a call of another thread may have set one and not yet launched.  Programs that use one of the streams pay nothing.
+cudaStream_t pick_stream(DeviceState* st, void* stream) {
+  if (stream == nullptr) {
+    st->own = true;
+    if (st->legacy) order_behind(st->stream, st->legacy_end, cudaStreamLegacy);
+    return st->stream;
+  }
+  if (stream == (void*)cudaStreamLegacy) {
+    st->legacy = true;
+    if (st->own) order_behind(cudaStreamLegacy, st->own_end, st->stream);
+  }
+  return (cudaStream_t)stream;
 }
 
 void count_launch(int device, long long n) {

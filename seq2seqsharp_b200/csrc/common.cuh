@@ -52,6 +52,8 @@ struct DeviceState {
   cudaStream_t stream = nullptr;  // library-owned non-blocking stream
   long long launches = 0;
   std::atomic<bool> waits{false};  // a stand-alone call has launched a kernel whose bounded waits raise the device's error words
+  std::atomic<bool> own{false}, legacy{false};  // a stand-alone call has gone to `stream`, to cudaStreamLegacy
+  cudaEvent_t own_end = nullptr, legacy_end = nullptr;
 };
 // Makes `device` current, lazily creates its state.  Fails when the device is absent or not sm_100.
 int use_device(int device, DeviceState** st);
@@ -69,7 +71,9 @@ struct KeepDevice {
     if (was >= 0 && cudaGetDevice(&now) == cudaSuccess && now != was) cudaSetDevice(was);
   }
 };
-inline cudaStream_t pick_stream(DeviceState* st, void* stream) { return stream ? (cudaStream_t)stream : st->stream; }
+// The stream of a stand-alone call: the one it names, or (null) the library's own.  That one is non-blocking, so that cudaStreamLegacy is not in order with it
+// by itself: a call on either waits, on the device, for the calls in front of it on the other.
+cudaStream_t pick_stream(DeviceState* st, void* stream);
 void count_launch(int device, long long n = 1);
 int check_launch(const char* what);
 

@@ -65,7 +65,8 @@ _I32, _F32 = torch.int32, torch.float32
 # The calls on the paged cache take five microseconds and less on the device, so their checks look at each tensor once, and say what is wrong only when something is.
 def _queue(device):
     """The stream that torch's work on `device` goes to.  Its default stream has the handle 0, which selects the library's own; named as
-    cudaStreamLegacy (1) the call takes its place among torch's work there without a wait of the host."""
+    cudaStreamLegacy (1) the call takes its place among torch's work there without a wait of the host.  The library keeps it in order with the calls on its
+    own stream, where `_stream` puts the other ops."""
     return torch._C._cuda_getCurrentRawStream(device) or 1
 
 
