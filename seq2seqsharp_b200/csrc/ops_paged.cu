@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PlanArgs a, in
 // ------------------------------------------------------------------------------------------------------------------------ norm, rotation, append
 //   y = x / sqrt(mean(x^2) + eps) * w;   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin),   angle = position * base^(-2 i / rot)
 // for every query and key head of a row; queries go to `out`, keys and values to the row's place in the cache.  Norm and rotation in fp32, rounded once;
-// angles in 64 bits (fp32 loses the angle of position 10^5 from the third digit on) as half turns, which are brought to [-1, 1] before they are rounded.
+// angles in 64 bits (fp32 loses the angle of position 10^5 from the third digit on) as half turns, which are brought to [-1, 1] before they are rounded to fp32 for the sine
+// and cosine: off by up to pi 2^-25, which 16-bit results do not show (the rotation's own fp32 sums are off by as much), and which is turned back for fp32.
 // L = 2^k lanes hold a head, 8 C elements each; the cos / sin of a row are made once per CTA.  What bounds it: issue slots and bytes about equally.  Of 16384 rows
 // of 32 + 16 heads of 64 in bf16 (201 MB, 30.8 us at the rate of a copy): C = 1, six CTAs per SM 54.5 us; C = 2, four 44.4 (five 49.1, three 47.6); C = 4, two 63.
 // Rows first and heads second, with a head's addresses and weights kept in registers, is slower (61: a warp's lines lie in two places).
@@ -281,8 +282,14 @@ __global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_paged_kernel(con
       for (int r = ar; r < n; r += turn_rows) {
         double x = (double)a.positions[row0 + r] * rate;
         x -= 2.0 * rint(0.5 * x);
+        const float near = (float)x;
         float s, c;
-        sincospif((float)x, &s, &c);
+        sincospif(near, &s, &c);
+        if constexpr (sizeof(T) == 4) {   // turned on by what the rounding took from the angle, below pi 2^-25
+          const float d = (float)((x - (double)near) * 3.14159265358979323846), t = s;
+          s = fmaf(c, d, s);
+          c = fmaf(-t, d, c);
+        }
         turn[r * slots + ai] = make_float2(c, s);
       }
     for (int r = tid; r < n; r += kRopeThreads) place[r] = place_of(row0 + r);
@@ -307,7 +314,7 @@ __global__ void __launch_bounds__(kRopeThreads, 4) qk_norm_rope_paged_kernel(con
           for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         }
         if (!is_v && (is_q ? a.q_norm : a.k_norm)) {
-          const float f = rsqrtf(ss * inv_hd + a.eps);   // off by two units in the last place, which the rounding to 16 bits and the sum of squares exceed
+          const float f = rsqrtf(ss * inv_hd + a.eps);   // off by 2^-22.9 of itself at most: the fp32 roundings of a root and a quotient would be 2^-23
           const float* w = is_q ? wq : wk;
 #pragma unroll
           for (int c = 0; c < C; ++c)

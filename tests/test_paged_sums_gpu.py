@@ -1,4 +1,4 @@
-"""The paged cache's numbers where a systematic error would hide behind random ones: weights that all round the same way."""
+"""The paged cache's numbers where a systematic error would hide behind random ones: weights that all round the same way, angles near whole half turns."""
 import math
 
 import pytest
@@ -38,3 +38,23 @@ def test_the_mean_of_equal_values_is_the_value(cuda, t, n, hd, T, up):
     out = Ops.PagedAttention(None, q, K, V, table, ints([0, n]), ints([T]), n, scale=1.0)
     off = (out.double() - 1).abs().max().item()
     assert off <= (2 * (T + 16) * 2.0 ** -24 if t is F32 else 0.0), off
+
+
+# ---------------------------------------------------------------------------------------------------------------------------- angles
+@pytest.mark.parametrize("style,rot", [(1, 64), (2, 64), (1, 18), (2, 16)])
+def test_angles_of_fp32_rows(cuda, style, rot):
+    """(1, 0) turned by an angle is its cosine and sine, each off by two units in the last place at most, also next to whole half turns where one of
+    them is nearly 0 (an angle rounded to fp32 before its sine is taken is off by up to pi 2^-25, whatever the sine's size).  2^-36: the 64-bit angle
+    itself, 4095 times a rate off by a few 2^-53."""
+    rows, hd = 4096, 64
+    q = torch.zeros(rows, 2, hd, device="cuda")
+    i = torch.arange(rot // 2, device="cuda")
+    lo, hi = (2 * i, 2 * i + 1) if style == 1 else (i, i + rot // 2)
+    q[..., lo] = 1.0
+    kv = torch.zeros(rows, 1, hd, device="cuda")
+    K, V = (torch.zeros(rows // 16, 1, 16, hd, device="cuda") for _ in range(2))
+    pos = torch.arange(rows, dtype=torch.int32, device="cuda")
+    got = Ops.QKNormRopePaged(None, q, kv, kv, None, None, 0.0, pos, pos, K, V, ropeStyle=style, ropeDims=rot, base=10000.0)
+    angle = pos.double()[:, None, None] * torch.exp(-2.0 * i.double() / rot * math.log(10000.0))
+    for want, x in ((angle.cos(), got[..., lo]), (angle.sin(), got[..., hi])):
+        assert ((x.double() - want).abs() <= 2 * 2.0 ** -23 * want.abs() + 2.0 ** -36).all()
