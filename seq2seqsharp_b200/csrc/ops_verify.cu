@@ -3,8 +3,8 @@
 // Row i of a sequence holds the target's probabilities p_i after i drafted tokens; draft i was drawn from q_i (null: it was certain).  Draft i is accepted
 // while u_i q_i(x_i) < p_i(x_i), which holds with probability min(1, p / q).  At the first refusal the token is drawn from max(p_i - q_i, 0), behind
 // the last accepted draft from p_i: the smallest t with w_0 + .. + w_t > u (w_0 + .. + w_{V-1}).  So the tokens are distributed as the target's own.
-// Products, differences and sums are 64-bit: u q and p - q are then exact, and a sum's rounding is far below the distance of two fp32 weights, so that
-// the order in which a vocabulary is added up does not decide which token is drawn.
+// Products, differences and sums are 64-bit: u q is then exact, p - q off by 2^-53 of itself at most (exact unless the two are further apart than 2^29), and a sum of V
+// weights by V 2^-53 of itself.  The order in which a vocabulary is added up can decide which token is drawn only where u times the whole is that near to the border of two.
 //
 // A cluster per sequence.  Its warps share the vocabulary in equal runs and push what theirs weigh to every CTA; after one cluster barrier all know the run that
 // the draw falls into, and that warp's CTA shares it out once more.  Rows that no draw needs are not read.  What bounds it: four dependent reads of memory, the
