@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
                                                                         const __grid_constant__ PagedArgs a) {
   constexpr int HD = BX * 64, NS = pm_stages(BX), RT = 16 * WR, KG = kPmWarps / WR, KS = HD / 16, NB = HD / 8;
   static_assert(KG > 1, "the warps of other keys meet in shared memory");
-  constexpr int SK = KG == 4 ? 16 : 32, STEPS = kPmKeys / KG / SK, SN = SK / 8;   // keys a warp weighs at a time
+  constexpr int SK = kPmKeys / KG, SN = SK / 8;   // keys of a tile that a warp weighs
   extern __shared__ __align__(1024) unsigned char pm_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)pm_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t ring = s_u32(smem);
@@ -161,87 +161,84 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
           for (int r = max(left, 0) + (lane >> 3); r < kPmKeys; r += 4)
 #pragma unroll
             for (int i = 0; i < BX; ++i)
-              if (r / (kPmKeys / KG) == kg) *reinterpret_cast<uint4*>(smem + (st * 2 + 1) * BX * kPmBox + i * kPmBox + r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+              if (r / SK == kg) *reinterpret_cast<uint4*>(smem + (st * 2 + 1) * BX * kPmBox + i * kPmBox + r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
           __syncwarp();
         }
-#pragma unroll 1
-        for (int sl = 0; sl < STEPS; ++sl) {
-          const int t0 = kg * (kPmKeys / KG) + sl * SK, key0 = kt * kPmKeys + t0;
-          float sc[SN][4];
+        const int t0 = kg * SK, key0 = kt * kPmKeys + t0;
+        float sc[SN][4];
 #pragma unroll
-          for (int n = 0; n < SN; ++n)
+        for (int n = 0; n < SN; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[n][e] = 0.0f;
+          for (int e = 0; e < 4; ++e) sc[n][e] = 0.0f;
 #pragma unroll
-          for (int k = 0; k < KS / 2; ++k)
-#pragma unroll
-            for (int n = 0; n < SN; ++n) {
-              uint32_t b[4];
-              const int ch = k * 4 + (lane >> 3), r = t0 + n * 8 + (lane & 7);
-              pm_ldmatrix(kb + (ch >> 3) * kPmBox + r * 128 + (((ch & 7) ^ (r & 7)) << 4), b);
-              mma_16816<H>(sc[n], qa[2 * k][0], qa[2 * k][1], qa[2 * k][2], qa[2 * k][3], b[0], b[1]);
-              mma_16816<H>(sc[n], qa[2 * k + 1][0], qa[2 * k + 1][1], qa[2 * k + 1][2], qa[2 * k + 1][3], b[2], b[3]);
-            }
-          if (gone != 0 || key0 + SK > see_to || key0 < see_from) {
-#pragma unroll
-            for (int n = 0; n < SN; ++n) {
-              const bool none = gone >> ((t0 >> 3) + n) & 1;
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int j = key0 + n * 8 + 2 * t4 + e;
-                if (!(j < hiA && j >= loA && !none)) sc[n][e] = -INFINITY;
-                if (!(j < hiB && j >= loB && !none)) sc[n][2 + e] = -INFINITY;
-              }
-            }
-          }
-          float xA = fmaxf(sc[0][0], sc[0][1]), xB = fmaxf(sc[0][2], sc[0][3]);
-#pragma unroll
-          for (int n = 1; n < SN; ++n) {
-            xA = fmaxf(xA, fmaxf(sc[n][0], sc[n][1]));
-            xB = fmaxf(xB, fmaxf(sc[n][2], sc[n][3]));
-          }
-          xA = fmaxf(xA, __shfl_xor_sync(0xffffffffu, xA, 1));
-          xB = fmaxf(xB, __shfl_xor_sync(0xffffffffu, xB, 1));
-          xA = fmaxf(xA, __shfl_xor_sync(0xffffffffu, xA, 2));
-          xB = fmaxf(xB, __shfl_xor_sync(0xffffffffu, xB, 2));
-          if (__any_sync(0xffffffffu, xA > mA || xB > mB)) {
-            // maxima of scores as they are, and from there exp2(c (score - maximum)); no key seen yet: every weight is exp2(-inf)
-            const float uA = fmaxf(mA, xA), uB = fmaxf(mB, xB);
-            const float fA = uA == -INFINITY ? 1.0f : pm_ex2((mA - uA) * a.c), fB = uB == -INFINITY ? 1.0f : pm_ex2((mB - uB) * a.c);
-            mA = uA;
-            mB = uB;
-            lA *= fA;
-            lB *= fB;
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-              o[n][0] *= fA;
-              o[n][1] *= fA;
-              o[n][2] *= fB;
-              o[n][3] *= fB;
-            }
-          }
-          const float nA = mA == -INFINITY ? 0.0f : -mA * a.c, nB = mB == -INFINITY ? 0.0f : -mB * a.c;
-          uint32_t p[SN][2];
+        for (int k = 0; k < KS / 2; ++k)
 #pragma unroll
           for (int n = 0; n < SN; ++n) {
-            p[n][0] = Pair16<H>::put(pm_ex2(fmaf(sc[n][0], a.c, nA)), pm_ex2(fmaf(sc[n][1], a.c, nA)));
-            p[n][1] = Pair16<H>::put(pm_ex2(fmaf(sc[n][2], a.c, nB)), pm_ex2(fmaf(sc[n][3], a.c, nB)));
-            // the weights as they are rounded for the product: what rounding does to the numerator it does to the denominator
-            const float2 a2 = Pair16<H>::get(p[n][0]), b2 = Pair16<H>::get(p[n][1]);
-            lA += a2.x + a2.y;
-            lB += b2.x + b2.y;
+            uint32_t b[4];
+            const int ch = k * 4 + (lane >> 3), r = t0 + n * 8 + (lane & 7);
+            pm_ldmatrix(kb + (ch >> 3) * kPmBox + r * 128 + (((ch & 7) ^ (r & 7)) << 4), b);
+            mma_16816<H>(sc[n], qa[2 * k][0], qa[2 * k][1], qa[2 * k][2], qa[2 * k][3], b[0], b[1]);
+            mma_16816<H>(sc[n], qa[2 * k + 1][0], qa[2 * k + 1][1], qa[2 * k + 1][2], qa[2 * k + 1][3], b[2], b[3]);
           }
+        if (gone != 0 || key0 + SK > see_to || key0 < see_from) {
 #pragma unroll
-          for (int i = 0; i < SN / 2; ++i) {
-            const int vr = t0 + i * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+          for (int n = 0; n < SN; ++n) {
+            const bool none = gone >> ((t0 >> 3) + n) & 1;
 #pragma unroll
-            for (int n = 0; n < NB / 2; ++n) {
-              uint32_t b[4];
-              const int ch = n * 2 + (lane >> 4);
-              pm_ldmatrix_trans(vb + (ch >> 3) * kPmBox + vr * 128 + (((ch & 7) ^ (vr & 7)) << 4), b);
-              mma_16816<H>(o[2 * n], p[2 * i][0], p[2 * i][1], p[2 * i + 1][0], p[2 * i + 1][1], b[0], b[1]);
-              mma_16816<H>(o[2 * n + 1], p[2 * i][0], p[2 * i][1], p[2 * i + 1][0], p[2 * i + 1][1], b[2], b[3]);
+            for (int e = 0; e < 2; ++e) {
+              const int j = key0 + n * 8 + 2 * t4 + e;
+              if (!(j < hiA && j >= loA && !none)) sc[n][e] = -INFINITY;
+              if (!(j < hiB && j >= loB && !none)) sc[n][2 + e] = -INFINITY;
             }
+          }
+        }
+        float xA = fmaxf(sc[0][0], sc[0][1]), xB = fmaxf(sc[0][2], sc[0][3]);
+#pragma unroll
+        for (int n = 1; n < SN; ++n) {
+          xA = fmaxf(xA, fmaxf(sc[n][0], sc[n][1]));
+          xB = fmaxf(xB, fmaxf(sc[n][2], sc[n][3]));
+        }
+        xA = fmaxf(xA, __shfl_xor_sync(0xffffffffu, xA, 1));
+        xB = fmaxf(xB, __shfl_xor_sync(0xffffffffu, xB, 1));
+        xA = fmaxf(xA, __shfl_xor_sync(0xffffffffu, xA, 2));
+        xB = fmaxf(xB, __shfl_xor_sync(0xffffffffu, xB, 2));
+        if (__any_sync(0xffffffffu, xA > mA || xB > mB)) {
+          // maxima of scores as they are, and from there exp2(c (score - maximum)); no key seen yet: every weight is exp2(-inf)
+          const float uA = fmaxf(mA, xA), uB = fmaxf(mB, xB);
+          const float fA = uA == -INFINITY ? 1.0f : pm_ex2((mA - uA) * a.c), fB = uB == -INFINITY ? 1.0f : pm_ex2((mB - uB) * a.c);
+          mA = uA;
+          mB = uB;
+          lA *= fA;
+          lB *= fB;
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            o[n][0] *= fA;
+            o[n][1] *= fA;
+            o[n][2] *= fB;
+            o[n][3] *= fB;
+          }
+        }
+        const float nA = mA == -INFINITY ? 0.0f : -mA * a.c, nB = mB == -INFINITY ? 0.0f : -mB * a.c;
+        uint32_t p[SN][2];
+#pragma unroll
+        for (int n = 0; n < SN; ++n) {
+          p[n][0] = Pair16<H>::put(pm_ex2(fmaf(sc[n][0], a.c, nA)), pm_ex2(fmaf(sc[n][1], a.c, nA)));
+          p[n][1] = Pair16<H>::put(pm_ex2(fmaf(sc[n][2], a.c, nB)), pm_ex2(fmaf(sc[n][3], a.c, nB)));
+          // the weights as they are rounded for the product: what rounding does to the numerator it does to the denominator
+          const float2 a2 = Pair16<H>::get(p[n][0]), b2 = Pair16<H>::get(p[n][1]);
+          lA += a2.x + a2.y;
+          lB += b2.x + b2.y;
+        }
+#pragma unroll
+        for (int i = 0; i < SN / 2; ++i) {
+          const int vr = t0 + i * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+          for (int n = 0; n < NB / 2; ++n) {
+            uint32_t b[4];
+            const int ch = n * 2 + (lane >> 4);
+            pm_ldmatrix_trans(vb + (ch >> 3) * kPmBox + vr * 128 + (((ch & 7) ^ (vr & 7)) << 4), b);
+            mma_16816<H>(o[2 * n], p[2 * i][0], p[2 * i][1], p[2 * i + 1][0], p[2 * i + 1][1], b[0], b[1]);
+            mma_16816<H>(o[2 * n + 1], p[2 * i][0], p[2 * i][1], p[2 * i + 1][0], p[2 * i + 1][1], b[2], b[3]);
           }
         }
         if (ragged) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the zeros above, before the next copy to this place

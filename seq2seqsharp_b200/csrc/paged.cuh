@@ -87,7 +87,7 @@ struct PagedJoin {
 };
 static_assert(sizeof(PagedJoin) == 2 * sizeof(int4), "a join is written as two pieces");
 struct PagedPlanShared {
-  long long warp[32], base[2];
+  long long warp[32];
   PagedLoc loc[2];
 };
 
@@ -270,7 +270,8 @@ __device__ __forceinline__ bool paged_locate(const PagedArgs& a, int c, int ctas
   }
   return true;
 }
-// Items of a run, one after the other.  done() when there is none left; [k0, k1) the key tiles of the item that are this run's.
+// Items of a run, one after the other: begin(), then next() for each, which is false when there is none left, and step() behind it.  [k0, k1): the key tiles of the
+// item that are this run's.
 struct PagedRun {
   int b, t, h, tiles;
   int k0, k1;            // key tiles
