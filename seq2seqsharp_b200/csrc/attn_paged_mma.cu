@@ -20,12 +20,6 @@ constexpr int pm_merge_floats(int BX) { return 3 * 8 * BX * 64 + kPmWarps * 16 *
 constexpr int pm_smem(int BX) { return 2 * pm_stages(BX) * BX * kPmBox + pm_merge_floats(BX) * 4 + 1024; }
 static_assert(kPmCtas * (pm_smem(2) + 1024 + 1024) <= 228 * 1024 && kPmCtas * (pm_smem(1) + 1024 + 1024) <= 228 * 1024, "two CTAs on an SM");
 
-__device__ __forceinline__ void pm_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map), "r"(bar), "r"(c0),
-      "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
 __device__ __forceinline__ void pm_ldmatrix(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -107,8 +101,8 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
           const int z = page >= 0 ? page : a.num_pages, y = kt * kPmKeys & page_mask;
 #pragma unroll
           for (int i = 0; i < BX; ++i) {
-            pm_load_4d(at + i * kPmBox + lane * blocks * 1024, &mapK, 64 * i, y, run.h, z, bar);
-            pm_load_4d(at + (BX + i) * kPmBox + lane * blocks * 1024, &mapV, 64 * i, y, run.h, z, bar);
+            tma_load_4d(at + i * kPmBox + lane * blocks * 1024, &mapK, 64 * i, y, run.h, z, bar);
+            tma_load_4d(at + (BX + i) * kPmBox + lane * blocks * 1024, &mapV, 64 * i, y, run.h, z, bar);
           }
         }
       }

@@ -31,25 +31,9 @@ static_assert(256 * kPtSoftmaxRegs + 128 * kPtOtherRegs <= kPtThreads * 168, "th
 constexpr int kPtStage = 32 * 64;   // bytes of a softmax warp to turn rows of outputs into lines
 constexpr int pt_smem(int BX, int NS) { return (2 + 2 * NS) * BX * kPtBox + 8 * kPtStage + 1024; }
 
-__device__ __forceinline__ void pt_cp16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 // one arrival of this thread when its copies so far have landed
 __device__ __forceinline__ void pt_arrive_copies(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(s_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void pt_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map),
-      "r"(s_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
-__device__ __forceinline__ void pt_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map),
-      "r"(s_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
 }
 
 // A row's output is rescaled when its maximum is this much (in powers of two) above the one in use (a published method for attention on matrix units): one of a
@@ -176,7 +160,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
           if (lane * box_blocks < 16)
 #pragma unroll
             for (int i = 0; i < BX; ++i)
-              pt_load_4d(dst + i * kPtBox + lane * box_blocks * 1024, map, 64 * i, tile * kPtKeys & page_mask, h, page >= 0 ? page : a.num_pages, full);
+              tma_load_4d(dst + i * kPtBox + lane * box_blocks * 1024, map, 64 * i, tile * kPtKeys & page_mask, h, page >= 0 ? page : a.num_pages, s_u32(full));
         };
         auto load_k = [&](int j, int entry) {
           const uint32_t c = kc + j, st = c % NS;
@@ -204,7 +188,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
           const int tiles = n.n[1] > 0 ? 2 : 1;
           if (lane == 0) tc_mbar_expect_tx(q_full, tiles * BX * kPtBox);
           __syncwarp();
-          if (lane < tiles * BX) pt_load_3d(sQ + lane * kPtBox, &mapQ, lane % BX * 64, h * a.G, s.row0 + a.by_G(p0 + lane / BX * kPtRows), q_full);
+          if (lane < tiles * BX) tma_load_3d(sQ + lane * kPtBox, &mapQ, lane % BX * 64, h * a.G, s.row0 + a.by_G(p0 + lane / BX * kPtRows), s_u32(q_full));
         } else {
           const int lr = lane / CPR, lc = lane % CPR;   // this lane's row of a pass and piece
           constexpr int RP = 32 / CPR;                  // rows of a pass
@@ -213,7 +197,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
             const bool there = p < pairs;
             const H* src = reinterpret_cast<const H*>(a.q);
             if (there) src += (int64_t)(s.row0 + query) * a.q_row + (int64_t)(h * a.G + p - query * a.G) * a.q_head + lc * 8;
-            if (r < kPtTile) pt_cp16(sQ + (r >> 7) * BX * kPtBox + (lc >> 3) * kPtBox + (r & 127) * 128 + (((lc & 7) ^ (r & 7)) << 4), src, there);
+            if (r < kPtTile) paged_cp16(sQ + (r >> 7) * BX * kPtBox + (lc >> 3) * kPtBox + (r & 127) * 128 + (((lc & 7) ^ (r & 7)) << 4), src, there);
           }
           pt_arrive_copies(q_full);
         }

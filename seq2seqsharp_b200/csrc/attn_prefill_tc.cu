@@ -43,18 +43,6 @@ struct PaArgs {
   int* error;
 };
 
-__device__ __forceinline__ void pa_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map),
-      "r"(s_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
-__device__ __forceinline__ void pa_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst), "l"(map),
-      "r"(s_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
 template <int QB, int VB>
 constexpr int pa_smem(int nks, int nvs) { return (2 * QB + nks * QB + nvs * VB) * kPaBox + 1024 + 256; }
 
@@ -127,7 +115,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) attn_prefill_tc_kernel(const __
       for (int t = 0; t < 2; ++t) {
         if (n_of[t] == 0) continue;
         tc_mbar_expect_tx(&q_full[t], QB * kPaBox);
-        for (int i = 0; i < QB; ++i) pa_load_4d(sQ + (t * QB + i) * kPaBox, &mapQ, 64 * i, kvh * a.G, (a.starts ? row0 : 0) + q0 + t * a.QT, a.starts ? 0 : b, &q_full[t]);
+        for (int i = 0; i < QB; ++i) tma_load_4d(sQ + (t * QB + i) * kPaBox, &mapQ, 64 * i, kvh * a.G, (a.starts ? row0 : 0) + q0 + t * a.QT, a.starts ? 0 : b, s_u32(&q_full[t]));
       }
       const int z = b * a.z_seq + kvh * a.z_head;
       int ks = 0, vs = 0;   // tiles asked for so far
@@ -137,8 +125,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) attn_prefill_tc_kernel(const __
         tc_mbar_expect_tx(&k_full[st], QB * kPaBox);
 #pragma unroll
         for (int i = 0; i < QB; ++i) {
-          if (i < a.k_boxes) pa_load_3d(sK + (st * QB + i) * kPaBox, &mapK, kvh * a.kx + 64 * i, j * kPaKeys, z, &k_full[st]);
-          else pa_load_3d(sK + (st * QB + i) * kPaBox, &mapR, a.rx + 64 * (i - a.k_boxes), j * kPaKeys, b, &k_full[st]);
+          if (i < a.k_boxes) tma_load_3d(sK + (st * QB + i) * kPaBox, &mapK, kvh * a.kx + 64 * i, j * kPaKeys, z, s_u32(&k_full[st]));
+          else tma_load_3d(sK + (st * QB + i) * kPaBox, &mapR, a.rx + 64 * (i - a.k_boxes), j * kPaKeys, b, s_u32(&k_full[st]));
         }
         ks = j + 1;
         return true;
@@ -150,7 +138,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) attn_prefill_tc_kernel(const __
         if (j >= NVS && !pa_wait(&v_empty[st], (unsigned)((j / NVS - 1) & 1), err, a.wait_limit)) break;
         tc_mbar_expect_tx(&v_full[st], VB * kPaBox);
 #pragma unroll
-        for (int i = 0; i < VB; ++i) pa_load_3d(sV + (st * VB + i) * kPaBox, &mapV, a.vx0 + kvh * a.vx + 64 * i, j * kPaKeys, z, &v_full[st]);
+        for (int i = 0; i < VB; ++i) tma_load_3d(sV + (st * VB + i) * kPaBox, &mapV, a.vx0 + kvh * a.vx + 64 * i, j * kPaKeys, z, s_u32(&v_full[st]));
         vs = j + 1;
       }
       // copies in flight land before the CTA ends (tc_land): they need nobody's help, and a wait may run out after this thread has asked for its last

@@ -374,9 +374,6 @@ static void launch_rope_paged(const RopePagedArgs& a, dim3 grid, cudaStream_t s)
 // fp32 throughout: the products run on the FMA pipe, which is what bounds chunks; single tokens are bound by bytes.  It serves what the kernels for tensor cores
 // do not: fp32 tokens, other head sizes, strides that no tensor map takes (8 fp32 tokens over 6000 keys, 8 / 8 heads of 64: 17 us).
 constexpr int kFmaThreads = 128, kFmaKeys = 32;
-__device__ __forceinline__ void paged_cp16(void* dst, const void* src, bool there) {   // zeros where there is nothing
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 template <typename T>
 constexpr int fma_row_bytes(int NH) { return NH * 32 * (int)sizeof(T) + 16; }   // odd in units of 16 bytes: lanes of neighbouring keys meet no bank twice
 template <typename T>

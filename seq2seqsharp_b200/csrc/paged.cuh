@@ -49,6 +49,12 @@ struct PagedArgs {
   int* error;
 };
 
+// 16 bytes to shared memory, zeros where there is nothing
+__device__ __forceinline__ void paged_cp16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void paged_cp16(void* dst, const void* src, bool there) { paged_cp16((uint32_t)__cvta_generic_to_shared(dst), src, there); }
+
 // a record: (maximum, sum) of RT rows, then their accumulators
 __host__ __device__ inline int64_t paged_record_floats(int RT, int hd) { return (int64_t)RT * (hd + 2); }
 
