@@ -268,9 +268,9 @@ TSB200_API int TSB200_QKNormRopePaged(int device, int dtype, void* q_out, int64_
                                       int64_t c_tok, int num_pages, int page, void* stream);
 /* Attention of the new rows over the pages: row i of the n of sequence b is at position lens[b] - n + i and sees the keys up to it (window > 0: the last
  * `window` of them), out = softmax(scale q k^T) v, query head h reading KV head h / (H / Hkv).  Entries of the table that name no page
- * hide their keys; a row that sees none becomes zeros; rows of no sequence are left as they were.  What the pages hold behind lens[b] is never used.  A key or value
- * that is not finite may reach other rows of the call's own chunk of its sequence than those that see it (a weight of 0 times NaN).  scale <= 0 and strides of 0 are
- * served by the general kernel.
+ * hide their keys; a row that sees none becomes zeros; rows of no sequence are left as they were.  What the pages hold behind lens[b], or in front of the windows
+ * of all rows of a sequence, is never used.  A key or value that is not finite and that one row of a sequence sees may reach the call's other rows of that sequence (a weight
+ * of 0 times NaN).  scale <= 0 and strides of 0 are served by the general kernel.
  * max_new: the most new rows of a sequence, as far as the caller knows (it chooses the kernel; more rows are served as well, with a workspace for max_new).
  * Pointers on a boundary of 16 bytes, strides (elements) multiples of 16 bytes.  workspace >= TSB200_PagedAttentionWorkspaceBytes; calls that may overlap need one each. */
 TSB200_API int64_t TSB200_PagedAttentionWorkspaceBytes(int dtype, int H, int Hkv, int hd, int max_new);

@@ -148,16 +148,15 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
         if (!ok) continue;
         const unsigned gone = gone_of[st];
         const uint32_t kb = ring + st * 2 * BX * kPmBox, vb = kb + BX * kPmBox;
-        const int left = cap - kt * kPmKeys;   // keys of the tile that exist
-        const bool ragged = left < kPmKeys;
-        if (ragged) {
-          // values behind the sequence's end: a weight of 0 times what lies there would be NaN where that is
-          for (int r = max(left, 0) + (lane >> 3); r < kPmKeys; r += 4)
+        // values that no row sees, in front of every window or behind the sequence's end: a weight of 0 times what lies there would be NaN where that is, or an infinity
+        const auto clear = [&](int from, int to) {   // of this warp's keys
+          for (int r = max(from, kg * SK) + (lane >> 3); r < min(to, (kg + 1) * SK); r += 4)
 #pragma unroll
-            for (int i = 0; i < BX; ++i)
-              if (r / SK == kg) *reinterpret_cast<uint4*>(smem + (st * 2 + 1) * BX * kPmBox + i * kPmBox + r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < BX; ++i) *reinterpret_cast<uint4*>(smem + (st * 2 + 1) * BX * kPmBox + i * kPmBox + r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the next copy to this place
           __syncwarp();
-        }
+        };
+        if (cap - kt * kPmKeys < kPmKeys) clear(cap - kt * kPmKeys, kPmKeys);
         const int t0 = kg * SK, key0 = kt * kPmKeys + t0;
         float sc[SN][4];
 #pragma unroll
@@ -175,6 +174,7 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
             mma_16816<H>(sc[n], qa[2 * k + 1][0], qa[2 * k + 1][1], qa[2 * k + 1][2], qa[2 * k + 1][3], b[2], b[3]);
           }
         if (gone != 0 || key0 + SK > see_to || key0 < see_from) {
+          if (key0 < see_from) clear(0, paged_front(a, s, run.t * RT) - kt * kPmKeys);
 #pragma unroll
           for (int n = 0; n < SN; ++n) {
             const bool none = gone >> ((t0 >> 3) + n) & 1;
@@ -235,7 +235,6 @@ __global__ void __launch_bounds__(kPmThreads, kPmCtas) paged_mma_kernel(const __
             mma_16816<H>(o[2 * n + 1], p[2 * i][0], p[2 * i][1], p[2 * i + 1][0], p[2 * i + 1][1], b[2], b[3]);
           }
         }
-        if (ragged) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the zeros above, before the next copy to this place
         __syncwarp();
         if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s_u32(&empty[st])) : "memory");
       }

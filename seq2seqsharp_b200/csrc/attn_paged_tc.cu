@@ -6,7 +6,7 @@
 // next item's first keys behind the output of this one's last.
 //
 // Keys and values come by TMA tensor copies, a box per page (128-byte swizzle, any strides that are multiples of 16 bytes); an entry that names no page is a coordinate
-// outside of the map, which arrives as zeros, and the values behind a sequence's end are overwritten with zeros before their product.  Queries come by TMA where
+// outside of the map, which arrives as zeros, and the values behind a sequence's end and in front of every window are overwritten with zeros before their product.  Queries come by TMA where
 // whole ones fill a tile (1, 2, 4 .. heads to a KV head), else by cp.async into the same swizzle: generic-proxy writes, which the issuing warp orders before
 // its products with a proxy fence.
 //
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
       while (ok && next_item()) {
         const PtCounts n = pt_counts(a, run);
         if (n.most == 0) continue;
-        const int cap = min(run.seq.len, a.max_blocks << a.page_shift);
+        const int cap = min(run.seq.len, a.max_blocks << a.page_shift), front = paged_front(a, run.seq, run.t * kPtTile);
         ok = landed(q_full, qc) && wait(&k_full[kc % NS], kc / NS);
         ++qc;
         if (!ok) break;
@@ -260,12 +260,13 @@ __global__ void __launch_bounds__(kPtThreads, 1) paged_tc_kernel(const __grid_co
           const bool more = j + 1 < n.most;
           const uint32_t c = kc + j, st = c % NS, next = (c + 1) % NS;
           ok = wait(&v_full[st], c / NS);
-          const int left = cap - (run.k0 + j) * kPtKeys;
-          if (ok && left < kPtKeys) {
-            // values behind the sequence's end: a weight of 0 times what lies there would be NaN where that is
-            for (int r = max(left, 0) * 8 + lane; r < kPtKeys * 8; r += 32)
+          const int hidden = front - (run.k0 + j) * kPtKeys, left = cap - (run.k0 + j) * kPtKeys;   // keys of the tile in front of every window, and up to the sequence's end
+          if (ok && (left < kPtKeys || hidden > 0)) {
+            // values that no row sees: a weight of 0 times what lies there would be NaN where that is, or an infinity
+            for (int r = hidden > 0 ? lane : max(left, 0) * 8 + lane; r < kPtKeys * 8; r += 32)
 #pragma unroll
-              for (int i = 0; i < BX; ++i) *reinterpret_cast<uint4*>(smem + (2 + NS + st) * BX * kPtBox + i * kPtBox + r * 16) = make_uint4(0u, 0u, 0u, 0u);
+              for (int i = 0; i < BX; ++i)
+                if (r < hidden * 8 || r >= left * 8) *reinterpret_cast<uint4*>(smem + (2 + NS + st) * BX * kPtBox + i * kPtBox + r * 16) = make_uint4(0u, 0u, 0u, 0u);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
           }

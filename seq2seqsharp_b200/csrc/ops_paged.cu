@@ -370,7 +370,7 @@ static void launch_rope_paged(const RopePagedArgs& a, dim3 grid, cudaStream_t s)
 
 // ------------------------------------------------------------------------------------------------------------------------ attention, every type
 // Four warps of RW rows; a tile of 32 keys and values is brought to shared memory by cp.async while the one before is used (places
-// that hold no visible key are filled with zeros, whatever the cache has there).  Scores: a lane per key; values: a lane per hd / 32 elements.
+// that hold no visible key, behind the sequence's end, in front of every window or in no page, are filled with zeros, whatever the cache has there).  Scores: a lane per key; values: a lane per hd / 32 elements.
 // fp32 throughout: the products run on the FMA pipe, which is what bounds chunks; single tokens are bound by bytes.  It serves what the kernels for tensor cores
 // do not: fp32 tokens, other head sizes, strides that no tensor map takes (8 fp32 tokens over 6000 keys, 8 / 8 heads of 64: 17 us).
 constexpr int kFmaThreads = 128, kFmaKeys = 32;
@@ -396,13 +396,13 @@ __global__ void __launch_bounds__(kFmaThreads) paged_fma_kernel(const __grid_con
   for (; run.next(a, plan, RT, KT); run.step(a)) {
     const PagedSeq& s = run.seq;
     const int p0 = run.t * RT, pairs = s.n * a.G;
-    const int cap = min(s.len, a.max_blocks << a.page_shift);
+    const int cap = min(s.len, a.max_blocks << a.page_shift), front = paged_front(a, s, p0);
     const int* table = a.table + run.b * a.table_stride;
     auto fetch = [&](int kt) {
       unsigned char* ks = fma_sm + (kt & 1) * 2 * KT * RB;
       for (int i = tid; i < KT * (D / EV); i += kFmaThreads) {
         const int k = i / (D / EV), e = i % (D / EV), j = kt * KT + k;
-        bool there = j < cap && e < pieces;
+        bool there = j < cap && j >= front && e < pieces;
         const int page = there ? table[j >> a.page_shift] : 0;
         there = there && page >= 0 && page < a.num_pages;
         const int64_t at = there ? page * a.c_page + run.h * a.c_head + (j & mask) * a.c_tok + e * EV : 0;
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) paged_f32_kerne
   run.begin(a, plan, RT);
   for (; run.next(a, plan, RT, KT); run.step(a)) {
     const PagedSeq& s = run.seq;
-    const int p0 = run.t * RT, pairs = s.n * a.G, cap = min(s.len, a.max_blocks << a.page_shift);
+    const int p0 = run.t * RT, pairs = s.n * a.G, cap = min(s.len, a.max_blocks << a.page_shift), front = paged_front(a, s, p0);
     const int* table = a.table + run.b * a.table_stride;
     auto fetch = [&](int kt) {
       float *k = ks + (kt & 1) * KT * (D + 4), *v = vs + (kt & 1) * KT * D;
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kTileThreads, D == 64 ? 2 : 1) paged_f32_kerne
         const int j = kt * KT + r, page = j < cap ? table[j >> a.page_shift] : -1;
         const bool there = page >= 0 && page < a.num_pages;
         if (e == 0 && (r & 7) == 0) there_s[kt & 1][r >> 3] = there;
-        const bool get = there && e < pieces;
+        const bool get = there && j >= front && e < pieces;
         const int64_t at = get ? page * a.c_page + run.h * a.c_head + (j & mask) * a.c_tok + e * 4 : 0;
         paged_cp16(k + r * (D + 4) + e * 4, reinterpret_cast<const float*>(a.K) + at, get);
         paged_cp16(v + r * D + e * 4, reinterpret_cast<const float*>(a.V) + at, get);

@@ -69,16 +69,20 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int b) {
   s.len = min(max(a.lens[b], 0), 0x7fff0000);   // positions and what is added to them stay below 2^31
   return s;
 }
+// the first key that a tile of pairs sees, the first of which is p0
+__device__ __forceinline__ int paged_front(const PagedArgs& a, const PagedSeq& s, int p0) {
+  const int first = s.len - s.n + a.by_G(p0);
+  return a.window > 0 && a.window <= first ? first - a.window + 1 : 0;
+}
 struct PagedTile {
   int k0, units;   // first key tile, how many
 };
 __device__ __forceinline__ PagedTile paged_tile(const PagedArgs& a, const PagedSeq& s, int t, int RT, int KT) {
   const int p1 = min(s.n * a.G, (t + 1) * RT) - 1;
-  const int first = s.len - s.n + a.by_G(t * RT), last = s.len - s.n + a.by_G(p1);   // positions of the tile
+  const int last = s.len - s.n + a.by_G(p1);   // its position
   const int hi = min(last + 1, a.max_blocks << a.page_shift);
-  const int lo = a.window > 0 && a.window <= first ? first - a.window + 1 : 0;
   PagedTile r;
-  r.k0 = lo / KT;
+  r.k0 = paged_front(a, s, t * RT) / KT;
   r.units = max(1, (hi + KT - 1) / KT - r.k0);   // a tile without keys is still written
   return r;
 }
