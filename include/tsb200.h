@@ -67,8 +67,8 @@ TSB200_API int TSB200_MemcpyD2H(int device, void* dst, const void* src, int64_t 
 TSB200_API int TSB200_MemcpyD2D(int device, void* dst, const void* src, int64_t bytes, void* stream);
 /* cross-device copy; replaces cuMemcpyPeer in TensorSharp.CUDA/KernelOps/CopyOps.cs:47-97 */
 TSB200_API int TSB200_MemcpyPeer(int dst_device, void* dst, int src_device, const void* src, int64_t bytes);
-/* Waits for the stream.  Fails with "a kernel gave up waiting" when a bounded wait inside a stand-alone linear or prompt attention
- * ran out since the last such report (so does TSB200_MemcpyD2H); those calls themselves return before their kernels have run. */
+/* Waits for the stream.  Fails with "a kernel gave up waiting" when a bounded wait inside a stand-alone linear, prompt attention or attention
+ * over pages ran out since the last such report (so does TSB200_MemcpyD2H); those calls themselves return before their kernels have run. */
 TSB200_API int TSB200_Synchronize(int device, void* stream);
 /* IAllocator.GetAllocatedMemoryRatio (TensorSharp/IAllocator.cs:19) */
 TSB200_API int TSB200_MemoryInfo(int device, int64_t* free_bytes, int64_t* total_bytes);
@@ -271,6 +271,7 @@ TSB200_API int TSB200_QKNormRopePaged(int device, int dtype, void* q_out, int64_
  * hide their keys; a row that sees none becomes zeros; rows of no sequence are left as they were.  What the pages hold behind lens[b], or in front of the windows
  * of all rows of a sequence, is never used.  A key or value that is not finite and that one row of a sequence sees may reach the call's other rows of that sequence (a weight
  * of 0 times NaN).  scale <= 0 and strides of 0 are served by the general kernel.
+ * The call returns before its kernels have run: a wait that runs out in one of them is reported by TSB200_Synchronize and TSB200_MemcpyD2H, and its rows are incomplete.
  * max_new: the most new rows of a sequence, as far as the caller knows (it chooses the kernel; more rows are served as well, with a workspace for max_new).
  * Pointers on a boundary of 16 bytes, strides (elements) multiples of 16 bytes.  workspace >= TSB200_PagedAttentionWorkspaceBytes; calls that may overlap need one each. */
 TSB200_API int64_t TSB200_PagedAttentionWorkspaceBytes(int dtype, int H, int Hkv, int hd, int max_new);

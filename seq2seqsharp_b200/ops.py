@@ -339,7 +339,7 @@ class Ops:
     def PagedAttention(result, q, cacheK, cacheV, table, starts, lens, maxNew, scale=None, window=0):
         """Attention of packed new rows q [rows, H, hd] over cacheK, cacheV [pages, Hkv, page, hd]: rows starts[b] .. starts[b + 1] are the last tokens of the lens[b]
         of sequence b, whose pages are table[b]; each sees the keys up to its own (window > 0: the last `window` of them).  maxNew: the most rows of a
-        sequence.  scale None: 1 / sqrt(hd).  Rows of no sequence keep what `result` held."""
+        sequence.  scale None: 1 / sqrt(hd).  Rows of no sequence keep what `result` held.  A bounded wait of the kernels that runs out is reported by TSB200_Synchronize."""
         op, dev, dt = "PagedAttention", _device("PagedAttention", q), q.dtype
         code = _MODEL_DT.get(dt)
         if code is None or q.dim() != 3:
