@@ -4,7 +4,9 @@
 // TMA tensor copies, a box per page (128-byte swizzle; an entry that names no page is a coordinate outside of the map and arrives as zeros), three or six
 // tiles ahead of their use.  Four warps multiply (mma.sync: the rows of a tensor-core tile of tcgen05 would be 7/8 empty): WR of them share the
 // rows, the others the keys of a tile, whose states (maximum, sum, output) meet in shared memory at an item's end.  No warp waits for another within an item.
-// What bounds it: bytes; 192 KB of an SM are on their way.  64 single tokens over 165600 keys in all, 32 / 8 heads of 128: 119 us, 5.7 TB/s; few short sequences are bound by
+// Weights are rounded to the cache's 16-bit type, because A and B of a product have one type, and the sums add them as rounded; all else is fp32 up to the output.
+// What bounds it: bytes; 192 KB of an SM are on their way.  64 single tokens over 165600 keys in all, 32 / 8 heads of 128: 119 us, 5.7 TB/s; with heads of 64 a unit has half
+// the bytes and the same chain (16 x 5 rows over up to 16384: 4.9 TB/s); few short sequences are bound by
 // the chain lengths - page entries - copies - records (8 tokens over 9600 keys 18 us, one over 530 10).
 #include <cfloat>
 

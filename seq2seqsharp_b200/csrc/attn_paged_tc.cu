@@ -15,8 +15,8 @@
 // mean of equal values 2^-8 (fp16: 2^-11) below them.
 //
 // What bounds it: the chain of a unit (scores, maximum, exponentials, sums, weights back to TMEM), which two tiles hide from the tensor core only in part.  Two chunks
-// of up to 2048 over up to 32768, 32 / 8 heads of 128: 1.55 ms, 1110 TFLOP/s of the 1644 that a library product reaches; prompts of 16384 of heads of 128
-// 1.88 ms, of 64 1.57.  What was measured on the way (ms, same chunks): cp.async for keys and values 2.39; one lane for the products and outputs rescaled at every
+// of up to 2048 over up to 32768, 32 / 8 heads of 128: 1.56 ms, 1105 TFLOP/s of the 1644 that a library product reaches; prompts of 16384 of heads of 128
+// 1.90 ms, of 64 1.58.  What was measured on the way (ms, same chunks): cp.async for keys and values 2.39; one lane for the products and outputs rescaled at every
 // new maximum 1.81; boxes prefetched to L2 1.74; scores of 64 keys at a time 1.78.
 #include "attn_tmem.cuh"
 #include "paged.cuh"
@@ -528,7 +528,7 @@ static int pt_launch(int device, DeviceState* st, const PagedArgs& a, cudaStream
 int launch_paged_tc(int device, DeviceState* st, int dtype, PagedArgs a, cudaStream_t s) {
   a.wait_limit = tc_wait_limit();
   a.error = tc_error_word(device);
-  // us with ends moved by up to 1 | 4 units: 2 x 30 rows over 4096 24 | 28, 256 over 8192 53 | 57, a prompt of 1024 of heads of 64 29.5 | 28
+  // us with ends moved by up to 1 | 4 units: 2 x 30 rows over 4096 24 | 28, 256 over 8192 53 | 57, a prompt of 1024 of heads of 64 29 | 28
   a.min_units = 4;
   a.snap = 1;
   a.start = 2;

@@ -11,7 +11,7 @@ namespace tsb {
 // want = ceil((cached + fresh) / page);  need = max(0, want - held), taken from the top of the stack of free pages in the order of the sequences;
 // held - want pages of a sequence that wants fewer go back, so that taking and giving back leaves the stack as it was;
 // starts = exclusive sum of the granted rows;  slot(row) = table[pos / page] * page + pos % page.
-// What bounds it: latency (three block scans, a few hundred KB at most; 8 sequences 5.4 us, 1024 sequences with 92500 rows 13).  Sums of rows and pages over sequences are 64-bit: their bounds are the caller's.
+// What bounds it: latency (three block scans, a few hundred KB at most; 8 sequences 5.4 us, 1024 sequences with 92500 rows 13, where the search of each row's sequence takes half).  Sums of rows and pages over sequences are 64-bit: their bounds are the caller's.
 struct PlanArgs {
   const int *cached, *fresh;
   int B, page_shift, max_blocks, num_pages, rows;
@@ -372,7 +372,7 @@ static void launch_rope_paged(const RopePagedArgs& a, dim3 grid, cudaStream_t s)
 // Four warps of RW rows; a tile of 32 keys and values is brought to shared memory by cp.async while the one before is used (places
 // that hold no visible key, behind the sequence's end, in front of every window or in no page, are filled with zeros, whatever the cache has there).  Scores: a lane per key; values: a lane per hd / 32 elements.
 // fp32 throughout: the products run on the FMA pipe, which is what bounds chunks; single tokens are bound by bytes.  It serves what the kernels for tensor cores
-// do not: fp32 tokens, other head sizes, strides that no tensor map takes (8 fp32 tokens over 6000 keys, 8 / 8 heads of 64: 17 us).
+// do not: fp32 tokens, other head sizes, strides that no tensor map takes (8 fp32 tokens over 6000 keys, 8 / 8 heads of 64: 17.6 us; 8 fp16 tokens over up to 4096, heads of 96: 47.5).
 constexpr int kFmaThreads = 128, kFmaKeys = 32;
 template <typename T>
 constexpr int fma_row_bytes(int NH) { return NH * 32 * (int)sizeof(T) + 16; }   // odd in units of 16 bytes: lanes of neighbouring keys meet no bank twice
@@ -793,9 +793,18 @@ int launch_paged_combine(int device, int dtype, const PagedArgs& a, int RT, int 
   return check_launch("paged_combine");
 }
 
-// The kernel that serves a call, its rows of a tile and its CTAs, by the most (query, head) pairs of a KV head that a sequence may have.  us, 8 sequences:
-//   16-bit, 4000 tokens, 32 / 8 heads of 128:  32 pairs mma.sync 33.6, tcgen05 32.9 (one sequence: 18.4, 20.0);  64: 37.9, 36.0 (23.6, 21.1)
-//   fp32, 1000 tokens, 8 / 8 heads of 64:      16 pairs a lane per key 30, tiles 38;  32: 40, 38;  64: 57, 40
+// The kernel that serves a call, its rows of a tile and its CTAs, by the most (query, head) pairs of a KV head that a sequence may have.  us at both sides of the rules, 8 KV heads:
+//   16-bit, mma.sync | tcgen05      1 sequence of 500   1 of 16000      8 of 4000      32 of 4000
+//     heads of 128, 32 pairs           14.7 | 19.5     30.0 | 31.7    35.5 | 34.5    79.5 | 79.9
+//                   64 (two tiles)     16.4 | 20.1     35.5 | 32.4    47.8 | 37.9     127 | 93
+//     heads of  64, 32 pairs           12.3 | 17.1     21.8 | 27.3    24.2 | 29.3    50.5 | 68.6
+//                   64 (two tiles)     13.0 | 17.1     25.3 | 27.6    31.7 | 31.7    79.9 | 79.2
+//   fp32, a lane per key | tiles     1 of 300            1 of 4000       8 of 1000      32 of 4000
+//     heads of  64, 16 pairs           25.6 | 13.7     28.3 | 32.4    30.0 | 31.1     217 | 366
+//                   32                 25.9 | 14.0     34.5 | 33.8    37.9 | 31.7     422 | 374
+//     heads of 128, 16 pairs           34.5 | 17.1     42.0 | 46.4    43.7 | 53.6     324 | 718
+//                   32                 35.1 | 18.4     51.9 | 47.1    58.0 | 55.0     627 | 721
+// One number each, between the sides that most sizes have: short single sequences of 33 pairs and more lose up to 5 us in 16 bits, of 16 and fewer in fp32 up to 18.
 struct PagedChoice {
   enum { FMA, TILE, MMA, TC } kind;
   int RT, KT, ctas;
