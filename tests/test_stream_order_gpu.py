@@ -82,3 +82,27 @@ def test_calls_of_the_library_without_a_stream(cuda):
         e.record()
         N.call("TSB200_Synchronize", 0, None)
         assert e.query()
+
+
+def test_a_call_without_a_stream_while_another_stream_is_captured(cuda):
+    # both streams are in use; the order between them is no part of a capture that goes on beside
+    n, T = 64, 512
+    x, K, V, table, starts, lens = problem(n, T)
+    q = x.to(F16).view(n, 16, 64)
+    want = Ops.PagedAttention(None, q, K, V, table, starts, lens, n)
+    a, b, out = torch.randn(1000, device="cuda"), torch.zeros(1000, device="cuda"), torch.zeros_like(q)
+    N.call("TSB200_MemcpyD2D", 0, b.data_ptr(), a.data_ptr(), 4000, None)
+    torch.cuda.synchronize()
+    b.zero_()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            Ops.PagedAttention(out, q, K, V, table, starts, lens, n)
+            N.call("TSB200_MemcpyD2D", 0, b.data_ptr(), a.data_ptr(), 4000, None)
+        N.call("TSB200_Synchronize", 0, None)
+        assert torch.equal(a, b)                              # it ran at once
+        g.replay()
+        s.synchronize()
+    assert torch.equal(out, want)
