@@ -67,8 +67,8 @@ TSB200_API int TSB200_MemcpyD2H(int device, void* dst, const void* src, int64_t 
 TSB200_API int TSB200_MemcpyD2D(int device, void* dst, const void* src, int64_t bytes, void* stream);
 /* cross-device copy; replaces cuMemcpyPeer in TensorSharp.CUDA/KernelOps/CopyOps.cs:47-97 */
 TSB200_API int TSB200_MemcpyPeer(int dst_device, void* dst, int src_device, const void* src, int64_t bytes);
-/* Waits for the stream.  Fails with "a kernel gave up waiting" when a bounded wait inside a stand-alone linear, prompt attention or attention
- * over pages ran out since the last such report (so does TSB200_MemcpyD2H); those calls themselves return before their kernels have run. */
+/* Waits for the stream.  Fails with "a kernel gave up waiting" when a bounded wait inside a stand-alone linear (8-bit ones too), prompt attention or
+ * attention over pages ran out since the last such report (so does TSB200_MemcpyD2H); those calls themselves return before their kernels have run. */
 TSB200_API int TSB200_Synchronize(int device, void* stream);
 /* IAllocator.GetAllocatedMemoryRatio (TensorSharp/IAllocator.cs:19) */
 TSB200_API int TSB200_MemoryInfo(int device, int64_t* free_bytes, int64_t* total_bytes);
@@ -287,6 +287,31 @@ TSB200_API int TSB200_PagedAttention(int device, int dtype, void* out, int64_t o
  * Out: tokens [B, K + 1] (accepted drafts, the drawn token, -1 behind), counts [B] = accepted + 1, 0 for a sequence without rows. */
 TSB200_API int TSB200_VerifyDraft(int device, int32_t* tokens, int32_t* counts, const float* p, int64_t p_row, const float* q, int64_t q_row,
                                   const int32_t* draft, const int32_t* starts, const float* u, int B, int K, int V, int rows, void* stream);
+
+/* ------------------------------------------------------------------------------------------------ linears in 8-bit integers, and log probabilities
+ * A row of bytes q with one scale stands for q * scale: rows of activations (a scale per token), rows of weights (a scale per output channel).  Rows of bytes lie
+ * q_row apart, which should be a multiple of 16, as the pointer: others are served by a slow kernel.  dtype TSB200_F32, TSB200_F16 or TSB200_BF16.  `rows` may be 0.
+ * These calls leave the caller's current device as it was.  (The reference has 8-bit weights in model files only, Models/Model_4_ProtoBufSerializer.cs:233-323.)
+ *
+ * RMSNormInt8: h = x + residual, rounded to dtype and written (residual and h both null: h = x, nothing is written; h may be x or residual itself);
+ * y = h / sqrt(mean(h^2) + eps) * gamma; scale = max|y| / 127 (0 for a row of zeros), q = y / scale rounded to nearest, half to even.  The bytes do not
+ * depend on how many rows there are.  A row that leaves fp32 (infinities, NaN, squares beyond 3e38) has the scale NaN and bytes of 0. */
+TSB200_API int TSB200_RMSNormInt8(int device, int dtype, void* q, int64_t q_row, float* scale, void* h, int64_t h_row, const void* x, int64_t x_row,
+                                  const void* residual, int64_t residual_row, const void* gamma, float eps, int64_t rows, int d, void* stream);
+/* RowsInt8: v = act(src) [* gate], gate may be null; scale and q of v as above.  act: TSB200_ACT_NONE .. TSB200_ACT_SIGMOID (GLU_NOACT is NONE, SWIGLU is SILU).  With
+ * NONE and no gate it turns rows as they are into bytes: what an attention gives, or a weight matrix [N, K] (a scale per output channel). */
+TSB200_API int TSB200_RowsInt8(int device, int dtype, void* q, int64_t q_row, float* scale, const void* src, int64_t src_row, const void* gate, int64_t gate_row,
+                               int act, int64_t rows, int d, void* stream);
+/* LinearInt8: y[m, n] = (sum over k of q[m, k] w[n, k]) * (q_scale[m] * w_scale[n]) + bias[n], the sum exact in 32-bit integers, y and bias (may be null) of dtype.
+ * w [N, K] has a row per output channel.  K < 2^17. */
+TSB200_API int TSB200_LinearInt8(int device, int dtype, void* y, int64_t y_row, const void* q, int64_t q_row, const float* q_scale, const void* w, int64_t w_row,
+                                 const float* w_scale, const void* bias, int64_t rows, int K, int N, void* stream);
+/* TokenLogProbs: of every row of logits [rows, V]: the log probability of tokens[row], the entropy in nats, the token's rank (0: the most likely; the lower id first among
+ * equal logits), and the `top` (0 .. 32, at most V) most likely tokens in that order with their log probabilities ([rows, top]).  -infinity is a word that
+ * cannot come.  A negative token (a row without one) gives 0 and the rank -1, one beyond the vocabulary NaN and -1.  A row with a NaN or +infinity, or
+ * with nothing but -infinity, gives NaN (its alternatives are ordered all the same, NaN last). */
+TSB200_API int TSB200_TokenLogProbs(int device, int dtype, float* logprobs, float* entropy, int32_t* ranks, int32_t* top_tokens, float* top_logprobs, int top,
+                                    const void* logits, int64_t logits_row, const int32_t* tokens, int64_t rows, int V, void* stream);
 
 /* ------------------------------------------------------------------------------------------------ GPT engine
  * The whole token loop of GPT.RunForwardOnSingleDevice / Decoder.GPTDecode / GPTDecoder.Decode

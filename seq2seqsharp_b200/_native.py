@@ -18,7 +18,7 @@ F32, F16, F64, I32, U8, BF16 = 0, 1, 2, 3, 4, 5
 MIXER_LATENT, MIXER_GROUPED, MIXER_MEMORY = 0, 1, 2
 BLOCK_GATED, BLOCK_SANDWICH = 0, 1
 ATTN_QK_NORM, ATTN_QKV_BIAS, ATTN_SINK, ATTN_HEAD_GATE = 1, 2, 4, 8
-ACT_NONE, ACT_RELU, ACT_SILU, ACT_LEAKYRELU, ACT_GLU_NOACT, ACT_SWIGLU, ACT_GELU = -1, 0, 1, 2, 3, 4, 5
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_LEAKYRELU, ACT_GLU_NOACT, ACT_SWIGLU, ACT_GELU, ACT_SIGMOID = -1, 0, 1, 2, 3, 4, 5, 6
 
 
 class TSB200Error(RuntimeError):
@@ -142,6 +142,10 @@ def lib():
         "TSB200_PagedAttentionWorkspaceBytes": (i64, [i32] * 5),
         "TSB200_PagedAttention": (i32, [i32, i32] + [vp, i64, i64] * 2 + [vp, vp, i64, i64, i64, i32, i32, vp, i64, i32, vp, vp] + [i32] * 6 + [f32, i32, vp, i64, vp]),
         "TSB200_VerifyDraft": (i32, [i32, vp, vp, vp, i64, vp, i64, vp, vp, vp, i32, i32, i32, i32, vp]),
+        "TSB200_RMSNormInt8": (i32, [i32, i32, vp, i64, vp, vp, i64, vp, i64, vp, i64, vp, f32, i64, i32, vp]),
+        "TSB200_RowsInt8": (i32, [i32, i32, vp, i64, vp, vp, i64, vp, i64, i32, i64, i32, vp]),
+        "TSB200_LinearInt8": (i32, [i32, i32, vp, i64, vp, i64, vp, vp, i64, vp, vp, i64, i32, i32, vp]),
+        "TSB200_TokenLogProbs": (i32, [i32, i32, vp, vp, vp, vp, vp, i32, vp, i64, vp, i64, i32, vp]),
         "TSB200_GptCreate": (i32, [C.POINTER(GptConfig), C.POINTER(vp)]),
         "TSB200_GptCreateLayered": (i32, [C.POINTER(LayeredConfigC), C.POINTER(LayerDescC), C.POINTER(vp)]),
         "TSB200_GptDestroy": (i32, [vp]),

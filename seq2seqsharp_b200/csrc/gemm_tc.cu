@@ -421,20 +421,6 @@ constexpr int kPThreads = 320, kPWarps = 8;
 constexpr int kPStageBytes = kPWarps * kStageFloats * 4;
 constexpr int kP_BN = 256;
 
-struct TcTile {
-  int m_tile, n_tile;
-};
-// bands of `rows` row tiles; inside a band column-major (all rows of a column tile are neighbours in time): the CTAs that run at the same
-// time share A and B tiles in L2
-__device__ __forceinline__ TcTile tc_tile_of(int t, int m_tiles, int n_tiles, int rows) {
-  const int band = t / (rows * n_tiles);
-  const int here = min(rows, m_tiles - band * rows);
-  const int r = t - band * rows * n_tiles;
-  TcTile o;
-  o.n_tile = r / here;
-  o.m_tile = band * rows + r % here;
-  return o;
-}
 // Rows sorted by the matrix they meet, in blocks of up to 128 (RowGroups): row tile m covers rows [row0, row0 + rows) and multiplies them
 // with the packed matrix `matrix`; the number of blocks is read from the device.  One CTA per SM walks tiles of 128 rows x 256 columns
 // (blocks of different matrices share no columns, so a CTA pair has nothing to share either).
@@ -584,26 +570,6 @@ struct PairTile {
   static constexpr int kSmem = kStages * kStage + 1024 + 256 + kPStageBytes;
   static constexpr int kCols = BN / 2;                      // columns of an epilogue warp
 };
-
-__device__ __forceinline__ uint32_t tc_leader_addr(uint32_t addr) {   // the same place in the shared memory of CTA 0 of the pair
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
-  return r;
-}
-__device__ __forceinline__ void tc_pair_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
-      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(dst), "l"(map),
-      "r"(bar), "r"(c0), "r"(c1)
-      : "memory");
-}
-__device__ __forceinline__ void tc_pair_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
-      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst), "l"(map),
-      "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
-}
 
 template <typename H, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)

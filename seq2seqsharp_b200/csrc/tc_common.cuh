@@ -80,7 +80,7 @@ __device__ __forceinline__ bool elect_one() {
 }
 __device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr, uint32_t lbo_bytes) { return ((smem_addr >> 4) & 0x3FFF) | ((lbo_bytes >> 4) << 16); }
 __device__ __forceinline__ uint32_t desc_hi(uint32_t sbo_bytes) { return (sbo_bytes >> 4) | (1u << 14) | (2u << 29); }
-#define TSB_ELECTED_MMA(NAME, GROUP)                                                                                                        \
+#define TSB_ELECTED_MMA(NAME, GROUP, KIND)                                                                                                      \
   __device__ __forceinline__ void NAME(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,       \
                                        uint32_t accumulate) {                                                                               \
     asm volatile(                                                                                                                           \
@@ -88,12 +88,14 @@ __device__ __forceinline__ uint32_t desc_hi(uint32_t sbo_bytes) { return (sbo_by
         "elect.sync _|q, 0xffffffff;\n\t"                                                                                                  \
         "setp.ne.b32 p, %6, 0;\n\t"                                                                                                        \
         "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"                                                                              \
-        "@q tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(tmem_d),                                           \
+        "@q tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], da, db, %5, p;\n\t}" ::"r"(tmem_d),                                           \
         "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)                                                             \
         : "memory");                                                                                                                        \
   }
-TSB_ELECTED_MMA(umma_el, "1")
-TSB_ELECTED_MMA(umma_pair_el, "2")
+TSB_ELECTED_MMA(umma_el, "1", "f16")
+TSB_ELECTED_MMA(umma_pair_el, "2", "f16")
+TSB_ELECTED_MMA(umma_i8_el, "1", "i8")
+TSB_ELECTED_MMA(umma_i8_pair_el, "2", "i8")
 #undef TSB_ELECTED_MMA
 __device__ __forceinline__ void umma_commit_el(uint32_t bar) {
   asm volatile(
@@ -177,6 +179,40 @@ __device__ __forceinline__ bool tc_wait_short(uint32_t bar, unsigned parity) {  
 __device__ __forceinline__ void tc_land(uint32_t full, int stages, int asked) {
 #pragma unroll 1
   for (int j = max(0, asked - stages); j < asked; ++j) tc_wait_short(full + (j % stages) * 8, (unsigned)((j / stages) & 1));
+}
+// ---- CTA pairs (cta_group::2) and their tiles ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t tc_leader_addr(uint32_t addr) {   // the same place in the shared memory of CTA 0 of the pair
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void tc_pair_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(dst), "l"(map),
+      "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tc_pair_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst), "l"(map),
+      "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+struct TcTile {
+  int m_tile, n_tile;
+};
+// bands of `rows` row tiles; inside a band column-major (all rows of a column tile are neighbours in time): the CTAs that run at the same
+// time share A and B tiles in L2
+__device__ __forceinline__ TcTile tc_tile_of(int t, int m_tiles, int n_tiles, int rows) {
+  const int band = t / (rows * n_tiles);
+  const int here = min(rows, m_tiles - band * rows);
+  const int r = t - band * rows * n_tiles;
+  TcTile o;
+  o.n_tile = r / here;
+  o.m_tile = band * rows + r % here;
+  return o;
 }
 // what a warp's index is to the compiler: the same in all lanes
 __device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }

@@ -121,6 +121,30 @@ def _table(op, dev, t, B):
     return t.data_ptr(), steps[0] if B > 1 else width, width
 
 
+def _matrix(op, dev, dtype, name, t, rows, cols):
+    """Address and row stride of a [rows, cols] tensor.  The stride of a single row means nothing and is the row's length."""
+    steps = t.stride()
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != (rows, cols) or (cols > 1 and steps[1] != 1):
+        raise N.TSB200Error("%s: %s is %s of %s with strides %s on %s, %s of %s with elements side by side on cuda:%d is wanted" % (
+            op, name, t.dtype, tuple(t.shape), steps, t.device, dtype, (rows, cols), dev))
+    return t.data_ptr(), steps[0] if rows > 1 else cols
+
+
+def _written(op, name, at, rows, cols):
+    if at[1] < cols and rows > 1:
+        raise N.TSB200Error("%s: rows of %s lie %d apart and overlap" % (op, name, at[1]))
+    return at
+
+
+def _bytes_of(op, dev, result, like, rows, cols):
+    """Write target of rows of bytes: `result`, or new ones that start on 16 bytes each."""
+    if result is None:
+        result = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=like.device)
+        if result.shape[1] != cols:
+            result = result[:, :cols]
+    return result, _written(op, "result", _matrix(op, dev, torch.int8, "result", result, rows, cols), rows, cols)
+
+
 class Ops:
     """Static facade with the reference's op names."""
 
@@ -380,3 +404,86 @@ class Ops:
         tokens, counts = torch.empty((B, K + 1), dtype=_I32, device=u.device), torch.empty(B, dtype=_I32, device=u.device)
         N.check(N.lib().TSB200_VerifyDraft(dev, tokens.data_ptr(), counts.data_ptr(), *args, _queue(dev)), "TSB200_VerifyDraft")
         return tokens, counts
+
+    # ---- linears in 8-bit integers, log probabilities (include/tsb200.h: TSB200_RMSNormInt8 and what follows it)
+    @staticmethod
+    def RMSNormInt8(result, src, residual, gamma, eps=1e-6, sum=None):
+        """RMSNorm of src + residual (residual None: of src) in bytes: src [rows, d], gamma [d].  Returns the bytes (int8 [rows, d], `result` or new rows that start on 16
+        bytes each), their scales [rows], and the sum rounded to src's type (`sum`: where to write it, src and residual themselves are allowed; src where there is no
+        residual)."""
+        op, dev, dt = "RMSNormInt8", _device("RMSNormInt8", src), src.dtype
+        code = _MODEL_DT.get(dt)
+        if code is None or src.dim() != 2:
+            raise N.TSB200Error("RMSNormInt8: unsupported src, %s of %s" % (dt, tuple(src.shape)))
+        rows, d = src.shape
+        x, res, at = _matrix(op, dev, dt, "src", src, rows, d), (None, 0), (None, 0)
+        if residual is not None:
+            res = _matrix(op, dev, dt, "residual", residual, rows, d)
+            if sum is None:
+                sum = torch.empty((rows, d), dtype=dt, device=src.device)
+            at = _written(op, "sum", _matrix(op, dev, dt, "sum", sum, rows, d), rows, d)
+        elif sum is not None:
+            raise N.TSB200Error("RMSNormInt8: sum without a residual")
+        else:
+            sum = src
+        g = _plain(op, dev, dt, "gamma", gamma, d)
+        result, q = _bytes_of(op, dev, result, src, rows, d)
+        scale = torch.empty(rows, dtype=_F32, device=src.device)
+        N.check(N.lib().TSB200_RMSNormInt8(dev, code, *q, scale.data_ptr(), *at, *x, *res, g, eps, rows, d, _queue(dev)), "TSB200_RMSNormInt8")
+        return result, scale, sum
+
+    @staticmethod
+    def RowsInt8(result, src, gate=None, act=N.ACT_NONE):
+        """act(src) [* gate] in bytes: src, gate [rows, d] (views of one tensor, for instance), act one of N.ACT_*.  Returns the bytes (as RMSNormInt8) and their scales [rows].
+        Without act and gate: rows as they are, as weights [N, K] with a scale per output channel."""
+        op, dev, dt = "RowsInt8", _device("RowsInt8", src), src.dtype
+        code = _MODEL_DT.get(dt)
+        if code is None or src.dim() != 2:
+            raise N.TSB200Error("RowsInt8: unsupported src, %s of %s" % (dt, tuple(src.shape)))
+        rows, d = src.shape
+        x, g = _matrix(op, dev, dt, "src", src, rows, d), (None, 0) if gate is None else _matrix(op, dev, dt, "gate", gate, rows, d)
+        result, q = _bytes_of(op, dev, result, src, rows, d)
+        scale = torch.empty(rows, dtype=_F32, device=src.device)
+        N.check(N.lib().TSB200_RowsInt8(dev, code, *q, scale.data_ptr(), *x, *g, act, rows, d, _queue(dev)), "TSB200_RowsInt8")
+        return result, scale
+
+    @staticmethod
+    def LinearInt8(result, src, srcScale, weight, weightScale, bias=None, dtype=torch.float16):
+        """src [rows, K] and weight [N, K] in bytes with scales [rows] and [N]: the exact integer product times both scales, plus bias [N], in `result` [rows, N] (None: a new
+        tensor of `dtype`; bias is of that type).  Rows of bytes that do not start on 16 bytes are served by a slow kernel.  A bounded wait that runs out is reported by
+        TSB200_Synchronize."""
+        op, dev = "LinearInt8", _device("LinearInt8", src)
+        if src.dim() != 2 or weight.dim() != 2:
+            raise N.TSB200Error("LinearInt8: src [rows, K] and weight [N, K] are wanted")
+        (rows, K), n = src.shape, weight.shape[0]
+        q, w = _matrix(op, dev, torch.int8, "src", src, rows, K), _matrix(op, dev, torch.int8, "weight", weight, n, K)
+        sq, sw = _plain(op, dev, _F32, "srcScale", srcScale, rows), _plain(op, dev, _F32, "weightScale", weightScale, n)
+        if result is None:
+            result = torch.empty((rows, n), dtype=dtype, device=src.device)
+        dt = result.dtype
+        code = _MODEL_DT.get(dt)
+        if code is None:
+            raise N.TSB200Error("LinearInt8: unsupported result, %s" % dt)
+        y = _written(op, "result", _matrix(op, dev, dt, "result", result, rows, n), rows, n)
+        b = None if bias is None else _plain(op, dev, dt, "bias", bias, n)
+        N.check(N.lib().TSB200_LinearInt8(dev, code, *y, *q, sq, *w, sw, b, rows, K, n, _queue(dev)), "TSB200_LinearInt8")
+        return result
+
+    @staticmethod
+    def TokenLogProbs(logits, tokens, top=0):
+        """Of every row of logits [rows, V]: the log probability of its token (tokens [rows] int32; negative: none, 0), the row's entropy, the token's rank, and the `top` (up
+        to 32) most likely tokens [rows, top] with their log probabilities [rows, top]; the lower id first among equal logits."""
+        op, dev, dt = "TokenLogProbs", _device("TokenLogProbs", logits), logits.dtype
+        code = _MODEL_DT.get(dt)
+        if code is None or logits.dim() != 2:
+            raise N.TSB200Error("TokenLogProbs: unsupported logits, %s of %s" % (dt, tuple(logits.shape)))
+        rows, V = logits.shape
+        x, t = _matrix(op, dev, dt, "logits", logits, rows, V), _plain(op, dev, _I32, "tokens", tokens, rows)
+        if not 0 <= top <= 32:
+            raise N.TSB200Error("TokenLogProbs: %d alternatives, 0 to 32 are wanted" % top)
+        floats, ints = torch.empty(rows * (2 + top), dtype=_F32, device=logits.device), torch.empty(rows * (1 + top), dtype=_I32, device=logits.device)
+        f, i = floats.data_ptr(), ints.data_ptr()
+        N.check(N.lib().TSB200_TokenLogProbs(dev, code, f, f + 4 * rows, i, i + 4 * rows, f + 8 * rows, top, *x, t, rows, V, _queue(dev)), "TSB200_TokenLogProbs")
+        lp, entropy, best = floats.split_with_sizes((rows, rows, rows * top))
+        rank, ids = ints.split_with_sizes((rows, rows * top))
+        return lp, entropy, rank, ids.view(rows, top), best.view(rows, top)
