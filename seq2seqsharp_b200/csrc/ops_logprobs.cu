@@ -9,13 +9,13 @@
 // kLpRoom (many equal logits, nearly all of them -infinity), the bound is raised to the top-th largest (logit, index) by eight histograms of eight bits.
 //
 // Few rows: a cluster of up to eight CTAs shares a row, and the first one joins what all have pushed to it.  Many rows: a CTA per row.
-#include <math_constants.h>
+#include <cmath>
+#include <type_traits>
 
 #include "kernels.cuh"
 
 namespace tsb {
 
-constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
 constexpr int kLpTop = 32;       // most alternatives
 constexpr int kLpRoom = 1024;    // words that a CTA orders
 constexpr int kLpCluster = 8;
@@ -39,9 +39,9 @@ __device__ __forceinline__ float lp_max_nan(float a, float b) {   // a NaN stays
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float lp_exp2(float v) {   // off by 2 ulp; 0 for -infinity
+__device__ __forceinline__ float lp_exp2(float v) {   // off by 2 ulp; 0 below 2^-126
   float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 // whole numbers that order as the numbers do, a zero having one sign; NaN comes last
@@ -49,47 +49,110 @@ __device__ __forceinline__ uint32_t lp_order(float v) {
   const uint32_t b = __float_as_uint(v + 0.0f);
   return v != v ? 0u : (b & 0x80000000u ? ~b : b | 0x80000000u);
 }
-__device__ __forceinline__ float lp_value(uint32_t o) { return o == 0u ? CUDART_NAN_F : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+__device__ __forceinline__ float lp_value(uint32_t o) { return o == 0u ? NAN : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ uint64_t lp_key(float v, int j) { return ((uint64_t)lp_order(v) << 32) | (uint32_t)~j; }
 
-template <typename T> struct LpVec {
-  static constexpr int N = 16 / (int)sizeof(T);
-  uint4 raw;
-  __device__ __forceinline__ float get(int e) const;
-};
-template <> __device__ __forceinline__ float LpVec<float>::get(int e) const { return __uint_as_float(e == 0 ? raw.x : e == 1 ? raw.y : e == 2 ? raw.z : raw.w); }
-template <> __device__ __forceinline__ float LpVec<__half>::get(int e) const {
-  const uint32_t p = (e >> 1) == 0 ? raw.x : (e >> 1) == 1 ? raw.y : (e >> 1) == 2 ? raw.z : raw.w;
-  const float2 f = Pair16<__half>::get(p);
-  return e & 1 ? f.y : f.x;
+__device__ __forceinline__ uint64_t lp_two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
-template <> __device__ __forceinline__ float LpVec<__nv_bfloat16>::get(int e) const {
-  const uint32_t p = (e >> 1) == 0 ? raw.x : (e >> 1) == 1 ? raw.y : (e >> 1) == 2 ? raw.z : raw.w;
-  return __uint_as_float(e & 1 ? p & 0xffff0000u : p << 16);
+__device__ __forceinline__ float2 lp_apart(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t lp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t lp_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
-// A row as pieces of 16 bytes on their boundaries: the first one begins `off` elements in front of the row
+// 16 bytes of logits.  What needs no wider type (largest, smallest, count of those at least some value) is done for two 16-bit ones at a time.
+template <typename T> struct LpVec {
+  static constexpr int N = 8;
+  typedef typename std::conditional<Pair16<T>::kBf16, __nv_bfloat162, __half2>::type Two;
+  uint4 raw;
+  __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? raw.x : i == 1 ? raw.y : i == 2 ? raw.z : raw.w; }
+  __device__ __forceinline__ Two two(int i) const { const uint32_t r = word(i); return *reinterpret_cast<const Two*>(&r); }
+  __device__ __forceinline__ float2 pair(int i) const { return Pair16<T>::get(word(i)); }   // elements 2 i, 2 i + 1
+  __device__ __forceinline__ float get(int e) const { const float2 f = pair(e >> 1); return e & 1 ? f.y : f.x; }
+};
+template <> struct LpVec<float> {
+  static constexpr int N = 4;
+  uint4 raw;
+  __device__ __forceinline__ float get(int e) const { return __uint_as_float(e == 0 ? raw.x : e == 1 ? raw.y : e == 2 ? raw.z : raw.w); }
+  __device__ __forceinline__ float2 pair(int i) const { return make_float2(get(2 * i), get(2 * i + 1)); }
+};
+// largest of some vectors; a NaN is passed over
+template <typename T> struct LpLargest {
+  typename LpVec<T>::Two hi;
+  __device__ __forceinline__ LpLargest() {
+    const uint32_t h = Pair16<T>::put(-INFINITY, -INFINITY);
+    hi = *reinterpret_cast<const typename LpVec<T>::Two*>(&h);
+  }
+  __device__ __forceinline__ void add(const LpVec<T>& x) { hi = __hmax2(hi, __hmax2(__hmax2(x.two(0), x.two(1)), __hmax2(x.two(2), x.two(3)))); }
+  __device__ __forceinline__ float get() const { const float2 f = Pair16<T>::get(*reinterpret_cast<const uint32_t*>(&hi)); return fmaxf(f.x, f.y); }
+};
+template <> struct LpLargest<float> {
+  float hi;
+  __device__ __forceinline__ LpLargest() : hi(-INFINITY) {}
+  __device__ __forceinline__ void add(const LpVec<float>& x) { hi = fmaxf(fmaxf(hi, fmaxf(x.get(0), x.get(1))), fmaxf(x.get(2), x.get(3))); }
+  __device__ __forceinline__ float get() const { return hi; }
+};
+// how many logits are at least `v`: counted in the type's own numbers (at most 16 in each half, which they hold), added up by total()
+template <typename T> struct LpCount {
+  typename LpVec<T>::Two n;
+  __device__ __forceinline__ LpCount() {
+    const uint32_t zero = 0u;
+    n = *reinterpret_cast<const typename LpVec<T>::Two*>(&zero);
+  }
+  __device__ __forceinline__ void add(const LpVec<T>& x, uint32_t v) {
+    const typename LpVec<T>::Two a = *reinterpret_cast<const typename LpVec<T>::Two*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n = __hadd2(n, __hge2(x.two(i), a));
+  }
+  __device__ __forceinline__ int total() const { const float2 f = Pair16<T>::get(*reinterpret_cast<const uint32_t*>(&n)); return (int)(f.x + f.y); }
+};
+template <> struct LpCount<float> {
+  int n = 0;
+  __device__ __forceinline__ void add(const LpVec<float>& x, uint32_t v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) n += x.get(e) >= __uint_as_float(v);
+  }
+  __device__ __forceinline__ int total() const { return n; }
+};
+// a number of the type for LpCount::add (twice in 32 bits for 16-bit types), and the next larger one (of infinity and NaN: a NaN, which nothing reaches)
+__device__ __forceinline__ uint32_t lp_bits(float v) { return __float_as_uint(v); }
+__device__ __forceinline__ uint32_t lp_bits(__half v) { return (uint32_t)__half_as_ushort(v) * 0x10001u; }
+__device__ __forceinline__ uint32_t lp_bits(__nv_bfloat16 v) { return (uint32_t)__bfloat16_as_ushort(v) * 0x10001u; }
+template <typename T>
+__device__ __forceinline__ uint32_t lp_bits_above(T v) {
+  const float f = to_f<T>(v);
+  const uint32_t one = sizeof(T) == 4 ? 1u : 0x10001u, b = lp_bits(v);
+  return f != f ? b : f == 0.0f ? one : f > 0.0f ? b + one : b - one;
+}
+
+// A row as pieces of 16 bytes on their boundaries, `head` elements in front of the first and `tail` behind the last
 template <typename T>
 struct LpRow {
   static constexpr int N = LpVec<T>::N;
   const T* x;
-  int off, V;
-  __device__ __forceinline__ LpRow(const T* p, int v) : x(p), off((int)(((uintptr_t)p & 15) / sizeof(T))), V(v) {}
-  __device__ __forceinline__ int pieces() const { return (int)(((int64_t)V + off + N - 1) / N); }
-  __device__ __forceinline__ int first(int v) const { return v * N - off; }   // index of a piece's first element
-  __device__ __forceinline__ bool whole(int v) const { return first(v) >= 0 && (int64_t)first(v) + N <= V; }
+  int head, pieces, tail;
+  __device__ __forceinline__ LpRow(const T* p, int V) : x(p) {
+    head = min(V, (int)((-(uintptr_t)p & 15) / sizeof(T)));
+    pieces = (V - head) / N;
+    tail = V - head - pieces * N;
+  }
+  __device__ __forceinline__ int first(int v) const { return head + v * N; }   // index of a piece's first element
   __device__ __forceinline__ LpVec<T> load(int v) const {
     LpVec<T> r;
-    const int j0 = first(v);
-    if (whole(v)) {
-      r.raw = *reinterpret_cast<const uint4*>(x + j0);
-    } else {
-      // what is not there is -infinity
-      struct __align__(16) { T e[N]; } t;
-#pragma unroll
-      for (int e = 0; e < N; ++e) t.e[e] = j0 + e >= 0 && j0 + e < V ? x[j0 + e] : from_f<T>(-CUDART_INF_F);
-      r.raw = *reinterpret_cast<const uint4*>(&t);
-    }
+    r.raw = *reinterpret_cast<const uint4*>(x + first(v));
     return r;
   }
 };
@@ -105,7 +168,7 @@ __device__ __forceinline__ float lp_gap(float m, float to) {
 struct LpSums {
   float m, s, t;   // maximum; sums, over the logits, of 2^exponent and of the exponent times it
   __device__ __forceinline__ void raise(float to) {   // to > m
-    if (m > -CUDART_INF_F) {
+    if (m > -INFINITY) {
       const float d = lp_gap(m, to), f = lp_exp2(d);
       t = f * fmaf(d, s, t);
       s *= f;
@@ -114,39 +177,47 @@ struct LpSums {
   }
 };
 // the same joined, in 64 bits
-struct LpJoined {
+struct __align__(16) LpJoined {
   double s, t;
   float m;
   int rank;
 };
 __device__ __forceinline__ void lp_rebase(double& s, double& t, float m, float to) {   // both are maxima, m <= to
-  if (m == to || !(m > -CUDART_INF_F)) return;   // (a share of -infinity has sums of 0, or NaN)
+  if (m == to || !(m > -INFINITY)) return;   // (a share of -infinity has sums of 0, or NaN)
   const float d = lp_gap(m, to);
   const double f = (double)lp_exp2(d);
   t = f * (t + (double)d * s);
   s *= f;
 }
-__device__ __forceinline__ void lp_join(LpJoined& c, LpJoined o) {
-  const float m = fmaxf(c.m, o.m);
-  lp_rebase(c.s, c.t, c.m, m);
-  lp_rebase(o.s, o.t, o.m, m);
-  c = LpJoined{c.s + o.s, c.t + o.t, m, c.rank + o.rank};
-}
-
-__device__ __forceinline__ double lp_shfl_sum(double v) {
+template <int LANES>
+__device__ __forceinline__ double lp_sum(double v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// `n` of them (at most LANES) by a whole warp; every lane has the result
+template <int LANES>
+__device__ __forceinline__ LpJoined lp_join(const LpJoined* from, int n) {
+  const int lane = (int)threadIdx.x & 31;
+  LpJoined c{0.0, 0.0, -INFINITY, 0};
+  if ((lane & (LANES - 1)) < n) c = from[lane & (LANES - 1)];
+  const float m = lp_value(__reduce_max_sync(0xffffffffu, lp_order(c.m)));
+  lp_rebase(c.s, c.t, c.m, m);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) c.rank += __shfl_xor_sync(0xffffffffu, c.rank, o);
+  return LpJoined{lp_sum<LANES>(c.s), lp_sum<LANES>(c.t), m, c.rank};
+}
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads) log_probs_kernel(LogProbArgs a) {
+template <typename T, int kLpThreads>
+__global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kernel(LogProbArgs a) {
+  constexpr int kLpWarps = kLpThreads / 32;
   __shared__ LpJoined s_join[kLpWarps];
   __shared__ LpJoined s_part[kLpCluster];            // (first CTA) of every CTA of the row
   __shared__ uint32_t s_bound[kLpWarps];
   __shared__ uint64_t s_words[kLpRoom];
   __shared__ uint64_t s_best[kLpCluster * kLpTop];   // (first CTA) of every CTA of the row, 0: none
   __shared__ uint32_t s_hist[256];
+  __shared__ uint8_t s_lane[kLpWarps][32];
   __shared__ uint64_t s_prefix;
   __shared__ int s_count, s_need;
 
@@ -159,70 +230,93 @@ __global__ void __launch_bounds__(kLpThreads) log_probs_kernel(LogProbArgs a) {
   }
   const LpRow<T> row(reinterpret_cast<const T*>(a.x) + r * a.x_row, a.V);
   constexpr int N = LpVec<T>::N;
-  const int all = row.pieces(), v0 = (int)((int64_t)all * part / parts), v1 = (int)((int64_t)all * (part + 1) / parts);
+  const int v0 = (int)((int64_t)row.pieces * part / parts), v1 = (int)((int64_t)row.pieces * (part + 1) / parts);
   const int token = a.tokens[r];
 
-  LpSums mine{-CUDART_INF_F, 0.0f, 0.0f};
-  int rank = 0;
-  LpVec<T> x[kLpUnroll];
+  struct Group { LpVec<T> of[kLpUnroll]; };
+  Group next;   // on its way while one is added up
   auto fetch = [&](int v) {
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u)
-      if (v + u * kLpThreads < v1) x[u] = row.load(v + u * kLpThreads);
+      if (v + u * kLpThreads < v1) next.of[u] = row.load(v + u * kLpThreads);
   };
   fetch(v0 + tid);
-  // what the token's rank is counted against: x >= before in front of it, x >= behind behind it (a NaN: never)
+  // one element more for some threads: of the row's ends
+  int end_j = -1;
+  if (part == 0 && tid < row.head + row.tail) end_j = tid < row.head ? tid : row.pieces * N + tid;
+  const float end_x = end_j >= 0 ? to_f<T>(row.x[end_j]) : -INFINITY;
+  // what the token's rank is counted against: in pieces in front of its own x >= xt, in those behind it x >= the next larger number (a NaN: never)
   const bool given = token >= 0 && token < a.V;
-  const float xt = given ? to_f<T>(row.x[token]) + 0.0f : CUDART_NAN_F;
-  const float behind = xt < CUDART_INF_F ? nextafterf(xt, CUDART_INF_F) : CUDART_NAN_F;
+  const T given_x = given ? row.x[token] : from_f<T>(NAN);
+  const float xt = to_f<T>(given_x);
+  const uint32_t from = lp_bits(given_x), above = lp_bits_above<T>(given_x), never = lp_bits(from_f<T>(NAN));
+  const int own = token < row.head ? -1 : (token - row.head) / N;   // the token's piece
+  auto outranks = [&](float y, int j) { return y > xt || (y == xt && j < token); };
+  int rank = end_j >= 0 && outranks(end_x, end_j);
+  if (tid < N && given && own >= v0 && own < v1) rank += outranks(to_f<T>(row.x[row.first(own) + tid]), row.first(own) + tid);
 
-  for (int v = v0 + tid; v < v1; v += kLpUnroll * kLpThreads) {
-    if (v != v0 + tid) fetch(v);
-    float top = -CUDART_INF_F;
+  LpSums mine{-INFINITY, 0.0f, 0.0f};
+  auto add = [&](float y, float m, float ref) {   // -infinity, and products that leave fp32, too
+    const float d = lp_max_nan(lp_far(m) ? (y - m) * kLog2e : fmaf(y, kLog2e, -ref), -1000.0f), p = lp_exp2(d);
+    mine.s += p;
+    mine.t = fmaf(d, p, mine.t);
+  };
+  if (end_j >= 0) {
+    mine.m = end_x > -INFINITY ? end_x : -INFINITY;   // (not a NaN)
+    const float m = mine.m > -INFINITY ? mine.m : 0.0f;
+    add(end_x, m, __fmul_rn(m, kLog2e));
+  }
+  // the pieces v, v + kLpThreads, .. of a group: all of them, or those in front of v1
+  auto group = [&](const LpVec<T>* x, int v, auto all) {
+    constexpr bool kAll = decltype(all)::value;
+    LpLargest<T> largest;
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u)
-      if (v + u * kLpThreads < v1) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) top = fmaxf(top, x[u].get(e));
-      }
+      if (kAll || v + u * kLpThreads < v1) largest.add(x[u]);
+    const float top = largest.get();
     if (top > mine.m) mine.raise(top);
-    float gs = 0.0f, gt = 0.0f;
-    auto add = [&](auto exponent) {
-#pragma unroll
-      for (int u = 0; u < kLpUnroll; ++u) {
-        if (v + u * kLpThreads >= v1) break;
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float d = lp_max_nan(exponent(x[u].get(e)), -1000.0f), p = lp_exp2(d);
-          gs += p;
-          gt = fmaf(d, p, gt);
-        }
-      }
-    };
-    const float m = mine.m > -CUDART_INF_F ? mine.m : 0.0f, ref = __fmul_rn(m, kLog2e);   // nothing but -infinity (and NaN) yet: sums of 0 (of NaN)
-    if (!lp_far(m)) add([&](float y) { return fmaf(y, kLog2e, -ref); });
-    else add([&](float y) { return (y - m) * kLog2e; });
-    mine.s += gs;
-    mine.t += gt;
+    const float m = mine.m > -INFINITY ? mine.m : 0.0f, ref = __fmul_rn(m, kLog2e);   // nothing but -infinity (and NaN) yet: sums of 0 (of NaN)
+    // two at a time
+    const uint64_t scale = lp_two(kLog2e, kLog2e), minus = lp_two(-ref, -ref);
+    uint64_t gs = 0u, gt = 0u;
+    LpCount<T> count;
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u) {
       const int at = v + u * kLpThreads;
-      if (at >= v1) break;
-      const int j0 = row.first(at);
-      if (row.whole(at) && (j0 > token || j0 + N <= token)) {
-        const float against = j0 > token ? behind : xt;
+      if (!kAll && at >= v1) break;
 #pragma unroll
-        for (int e = 0; e < N; ++e) rank += x[u].get(e) >= against;
-      } else {
+      for (int i = 0; i < N / 2; ++i) {
+        const float2 y = x[u].pair(i);
+        const uint64_t d = lp_fma2(lp_two(y.x, y.y), scale, minus);
+        const float2 e = lp_apart(d);
+        const uint64_t p = lp_two(lp_exp2(e.x), lp_exp2(e.y));
+        gs = lp_add2(gs, p);
+        gt = lp_fma2(d, p, gt);
+      }
+      count.add(x[u], at < own ? from : at > own ? above : never);
+    }
+    rank += count.total();
+    const float2 s = lp_apart(gs), t = lp_apart(gt);
+    if (t.x + t.y == t.x + t.y && !lp_far(m)) {
+      mine.s += s.x + s.y;
+      mine.t += t.x + t.y;
+    } else {
+      // an exponent of -infinity is among them (0 times it is none), or a NaN
+#pragma unroll 1
+      for (int u = 0; u < kLpUnroll && v + u * kLpThreads < v1; ++u) {
+        const LpVec<T> y = row.load(v + u * kLpThreads);
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const int j = j0 + e;
-          const float y = x[u].get(e);
-          rank += j >= 0 && j < a.V && (y > xt || (y == xt && j < token));
-        }
+        for (int e = 0; e < N; ++e) add(y.get(e), m, ref);
       }
     }
+  };
+  int v = v0 + tid;
+  for (; v + (kLpUnroll - 1) * kLpThreads < v1; v += kLpUnroll * kLpThreads) {
+    const Group now = next;
+    fetch(v + kLpUnroll * kLpThreads);
+    group(now.of, v, std::true_type());
   }
+  if (v < v1) group(next.of, v, std::false_type());
 
   // ---------------- the CTA's sums, against its maximum
   const uint32_t mine_o = lp_order(mine.m), warp_o = __reduce_max_sync(0xffffffffu, mine_o);
@@ -230,8 +324,8 @@ __global__ void __launch_bounds__(kLpThreads) log_probs_kernel(LogProbArgs a) {
     const float m = lp_value(warp_o);
     double s = mine.s, t = mine.t;
     lp_rebase(s, t, mine.m, m);
-    s = lp_shfl_sum(s);
-    t = lp_shfl_sum(t);
+    s = lp_sum<32>(s);
+    t = lp_sum<32>(t);
     rank = __reduce_add_sync(0xffffffffu, rank);
     if (lane == 0) s_join[w] = LpJoined{s, t, m, rank};
   }
@@ -258,26 +352,36 @@ __global__ void __launch_bounds__(kLpThreads) log_probs_kernel(LogProbArgs a) {
 #pragma unroll
       for (int i = 0; i < kLpWarps; ++i) larger += s_bound[i] > o || (s_bound[i] == o && i < (lane & (kLpWarps - 1)));
       bound = __shfl_sync(0xffffffffu, o, __ffs(__ballot_sync(0xffffffffu, larger == warps - 1)) - 1);
-      if (bound <= lp_order(-CUDART_INF_F)) bound = 0u;   // threads without a number have this maximum too: every word counts
+      if (bound <= lp_order(-INFINITY)) bound = 0u;   // threads without a number have this maximum too: every word counts
     }
-    // every element of the thread's share
-    auto look = [&](bool any, auto f) {
-      if (!any) return;
-      for (int v = v0 + tid; v < v1; v += kLpUnroll * kLpThreads) {
+    // every element that is not below least_x, in the shares of the warp's lanes with `any`: f(key).  The warp reads them together.
+    auto look = [&](bool any, float least_x, auto f) {
+      const uint32_t lanes = __ballot_sync(0xffffffffu, any);
+      if (any) s_lane[w][__popc(lanes & ((1u << lane) - 1u))] = (uint8_t)lane;
+      __syncwarp();
+      const int first = v0 + w * 32, each = v1 > first ? (v1 - first + kLpThreads - 1) / kLpThreads : 0, items = __popc(lanes) * each;   // (pieces of the first lane, the most)
+      for (int i = lane; i < items; i += 32 * kLpUnroll) {
         LpVec<T> y[kLpUnroll];
-#pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u)
-          if (v + u * kLpThreads < v1) y[u] = row.load(v + u * kLpThreads);
+        int at[kLpUnroll];
 #pragma unroll
         for (int u = 0; u < kLpUnroll; ++u) {
-          const int v_at = v + u * kLpThreads;
-          if (v_at >= v1) break;
-          const int j0 = row.first(v_at);
+          const int k = i + 32 * u, of = k / each;
+          at[u] = k < items ? first + (int)s_lane[w][of] + (k - of * each) * kLpThreads : v1;
+          if (at[u] < v1) y[u] = row.load(at[u]);
+        }
 #pragma unroll
-          for (int e = 0; e < N; ++e)
-            if (j0 + e >= 0 && j0 + e < a.V) f(lp_key(y[u].get(e), j0 + e));
+        for (int u = 0; u < kLpUnroll; ++u) {
+          if (at[u] >= v1) continue;
+          const int j0 = row.first(at[u]);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float z = y[u].get(e);
+            if (!(z < least_x)) f(lp_key(z, j0 + e));
+          }
         }
       }
+      if (end_j >= 0) f(lp_key(end_x, end_j));
+      __syncwarp();
     };
     uint64_t least = (uint64_t)bound << 32;
     auto take = [&](uint64_t k) {
@@ -285,7 +389,7 @@ __global__ void __launch_bounds__(kLpThreads) log_probs_kernel(LogProbArgs a) {
       const int at = atomicAdd(&s_count, 1);
       if (at < kLpRoom) s_words[at] = k;
     };
-    look(mine_o >= bound, take);
+    look(mine_o >= bound, bound ? lp_value(bound) : -INFINITY, take);
     __syncthreads();
     if (s_count > kLpRoom) {
       // the top-th largest key, eight bits at a time
@@ -297,7 +401,7 @@ __global__ void __launch_bounds__(kLpThreads) log_probs_kernel(LogProbArgs a) {
         for (int i = tid; i < 256; i += kLpThreads) s_hist[i] = 0u;
         __syncthreads();
         const uint64_t prefix = s_prefix;
-        look(true, [&](uint64_t k) {
+        look(true, -INFINITY, [&](uint64_t k) {
           if (shift == 56 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(k >> shift) & 255], 1u);
         });
         __syncthreads();
@@ -311,7 +415,7 @@ __global__ void __launch_bounds__(kLpThreads) log_probs_kernel(LogProbArgs a) {
         __syncthreads();
       }
       least = s_prefix;
-      look(true, take);
+      look(true, -INFINITY, take);
       __syncthreads();
     }
     if (parts > 1) cluster_wait();
@@ -335,38 +439,36 @@ __global__ void __launch_bounds__(kLpThreads) log_probs_kernel(LogProbArgs a) {
   } else if (parts > 1) {
     cluster_wait();
   }
-  if (tid == 0) {
-    LpJoined c = s_join[0];
-    for (int i = 1; i < kLpWarps; ++i) lp_join(c, s_join[i]);
+  if (w == kLpWarps - 1) {   // (the first warps order words)
+    const LpJoined c = lp_join<kLpWarps>(s_join, kLpWarps);
     uint32_t to = (uint32_t)__cvta_generic_to_shared(&s_part[part]);
     if (parts > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(to));
-    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(c.s) : "memory");
-    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to + 8), "d"(c.t) : "memory");
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 16), "f"(c.m) : "memory");
-    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(to + 20), "r"(c.rank) : "memory");
+    if (lane == 0) {
+      asm volatile("st.shared::cluster.v2.f64 [%0], {%1, %2};" ::"r"(to), "d"(c.s), "d"(c.t) : "memory");
+      asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(to + 16), "r"(__float_as_uint(c.m)), "r"(c.rank) : "memory");
+    }
   }
   if (parts > 1) cluster_sync();
   else __syncthreads();
   if (part != 0) return;
 
   // ---------------- the row
-  if (w == 0 || tid < parts * top) {
-    LpJoined c = s_part[0];
-    for (int i = 1; i < parts; ++i) lp_join(c, s_part[i]);
-    const bool none = !(c.m > -CUDART_INF_F);   // nothing but -infinity and NaN
+  if (w * 32 < max(1, parts * top)) {   // whole warps
+    LpJoined c = lp_join<kLpCluster>(s_part, parts);
+    const bool none = !(c.m > -INFINITY);   // nothing but -infinity and NaN
     if (!none && !lp_far(c.m)) {
       // The maximum's own exponent is what rounding left of it, and its power of two is off by 2 ulp of 1: as much as all other words have where it is nearly certain
       const float own = fmaf(c.m, kLog2e, -__fmul_rn(c.m, kLog2e));
       c.s += exp2((double)own) - (double)lp_exp2(own);
     }
-    const double ln2 = 0.693147180559945309417, log_s = none ? CUDART_NAN : log(c.s), ref = (double)__fmul_rn(c.m, kLog2e);
+    const double ln2 = 0.693147180559945309417, log_s = none ? (double)NAN : log(c.s), ref = (double)__fmul_rn(c.m, kLog2e);
     // rounding may leave a little over 0 of a certain token
     auto value = [&](float v) {
       const double l = (lp_far(c.m) ? (double)v - (double)c.m : ((double)v * (double)kLog2e - ref) * ln2) - log_s;
       return (float)(l > 0.0 ? 0.0 : l);
     };
     if (tid == 0) {
-      a.lp[r] = given ? value(xt) : token < 0 ? 0.0f : CUDART_NAN_F;
+      a.lp[r] = given ? value(xt) : token < 0 ? 0.0f : NAN;
       a.rank[r] = given ? c.rank : -1;
       const double h = log_s - c.t / c.s * ln2;
       a.entropy[r] = (float)(h < 0.0 ? 0.0 : h);
@@ -387,13 +489,14 @@ __global__ void __launch_bounds__(kLpThreads) log_probs_kernel(LogProbArgs a) {
 
 template <typename T>
 static int log_probs_launch(LogProbArgs a, int64_t rows, int sms, cudaStream_t s) {
-  // CTAs of a row: as many as keep all rows resident at once (two per SM), each with a round of its threads' loads at least
+  // CTAs of a row: as many as keep all rows resident at once (four per SM), each with a piece a thread at least
   const int pieces = (a.V + LpVec<T>::N - 1) / LpVec<T>::N;
   a.parts = 1;
-  while (a.parts < kLpCluster && rows * a.parts * 2 <= 2 * sms && pieces / (a.parts * 2) >= kLpThreads) a.parts *= 2;
+  while (a.parts < kLpCluster && rows * a.parts * 2 <= 4 * sms && pieces / (a.parts * 2) >= 256) a.parts *= 2;
+  const bool wide = rows * a.parts <= sms && pieces / a.parts >= 512;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * a.parts));
-  cfg.blockDim = dim3(kLpThreads);
+  cfg.blockDim = dim3(wide ? 512 : 256);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -402,7 +505,7 @@ static int log_probs_launch(LogProbArgs a, int64_t rows, int sms, cudaStream_t s
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  TSB_CUDA(cudaLaunchKernelEx(&cfg, log_probs_kernel<T>, a));
+  TSB_CUDA(cudaLaunchKernelEx(&cfg, wide ? log_probs_kernel<T, 512> : log_probs_kernel<T, 256>, a));
   return 1;
 }
 

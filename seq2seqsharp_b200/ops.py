@@ -136,12 +136,17 @@ def _written(op, name, at, rows, cols):
     return at
 
 
+def _new(like, rows, cols, dtype, pitch=None):
+    """A new [rows, cols] tensor, its rows `pitch` apart (strides given: torch.empty takes half as long again)."""
+    return torch.empty_strided((rows, cols), (pitch or cols, 1), dtype=dtype, device=like.device)
+
+
 def _bytes_of(op, dev, result, like, rows, cols):
     """Write target of rows of bytes: `result`, or new ones that start on 16 bytes each."""
     if result is None:
-        result = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=like.device)
-        if result.shape[1] != cols:
-            result = result[:, :cols]
+        pitch = (cols + 15) & -16
+        result = _new(like, rows, cols, torch.int8, pitch)
+        return result, (result.data_ptr(), pitch)
     return result, _written(op, "result", _matrix(op, dev, torch.int8, "result", result, rows, cols), rows, cols)
 
 
@@ -420,7 +425,7 @@ class Ops:
         if residual is not None:
             res = _matrix(op, dev, dt, "residual", residual, rows, d)
             if sum is None:
-                sum = torch.empty((rows, d), dtype=dt, device=src.device)
+                sum = _new(src, rows, d, dt)
             at = _written(op, "sum", _matrix(op, dev, dt, "sum", sum, rows, d), rows, d)
         elif sum is not None:
             raise N.TSB200Error("RMSNormInt8: sum without a residual")
@@ -459,7 +464,7 @@ class Ops:
         q, w = _matrix(op, dev, torch.int8, "src", src, rows, K), _matrix(op, dev, torch.int8, "weight", weight, n, K)
         sq, sw = _plain(op, dev, _F32, "srcScale", srcScale, rows), _plain(op, dev, _F32, "weightScale", weightScale, n)
         if result is None:
-            result = torch.empty((rows, n), dtype=dtype, device=src.device)
+            result = _new(src, rows, n, dtype)
         dt = result.dtype
         code = _MODEL_DT.get(dt)
         if code is None:
@@ -481,9 +486,9 @@ class Ops:
         x, t = _matrix(op, dev, dt, "logits", logits, rows, V), _plain(op, dev, _I32, "tokens", tokens, rows)
         if not 0 <= top <= 32:
             raise N.TSB200Error("TokenLogProbs: %d alternatives, 0 to 32 are wanted" % top)
-        floats, ints = torch.empty(rows * (2 + top), dtype=_F32, device=logits.device), torch.empty(rows * (1 + top), dtype=_I32, device=logits.device)
-        f, i = floats.data_ptr(), ints.data_ptr()
-        N.check(N.lib().TSB200_TokenLogProbs(dev, code, f, f + 4 * rows, i, i + 4 * rows, f + 8 * rows, top, *x, t, rows, V, _queue(dev)), "TSB200_TokenLogProbs")
-        lp, entropy, best = floats.split_with_sizes((rows, rows, rows * top))
-        rank, ids = ints.split_with_sizes((rows, rows * top))
-        return lp, entropy, rank, ids.view(rows, top), best.view(rows, top)
+        out = torch.empty(rows * (3 + 2 * top), dtype=_F32, device=logits.device)
+        at = out.data_ptr()
+        N.check(N.lib().TSB200_TokenLogProbs(dev, code, at, at + 4 * rows, at + 8 * rows, at + 12 * rows, at + (12 + 4 * top) * rows, top, *x, t, rows, V, _queue(dev)),
+                "TSB200_TokenLogProbs")
+        lp, entropy, rank, ids, best = out.split_with_sizes((rows, rows, rows, rows * top, rows * top))
+        return lp, entropy, rank.view(_I32), ids.view(_I32).view(rows, top), best.view(rows, top)
