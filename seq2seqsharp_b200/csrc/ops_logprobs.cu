@@ -208,6 +208,30 @@ __device__ __forceinline__ LpJoined lp_join(const LpJoined* from, int n) {
   return LpJoined{lp_sum<LANES>(c.s), lp_sum<LANES>(c.t), m, c.rank};
 }
 
+// what the joined sums of a row make of a logit
+struct LpWhole {
+  double log_s, entropy;
+  float m;
+  int rank;
+  __device__ __forceinline__ LpWhole() {}
+  __device__ __forceinline__ explicit LpWhole(LpJoined c) : m(c.m), rank(c.rank) {
+    const bool none = !(m > -INFINITY);   // nothing but -infinity and NaN
+    if (!none && !lp_far(m) && c.s < 1.5) {
+      // The maximum's own exponent is what rounding left of it, and its power of two is off by 2 ulp of 1: as much as all other words have where it is nearly certain
+      const float own = fmaf(m, kLog2e, -__fmul_rn(m, kLog2e));
+      c.s += exp2((double)own) - (double)lp_exp2(own);
+    }
+    log_s = none ? (double)NAN : log(c.s);
+    entropy = log_s - c.t / c.s * kLn2;
+  }
+  static constexpr double kLn2 = 0.693147180559945309417;
+  // rounding may leave a little over 0 of a certain token
+  __device__ __forceinline__ float value(float v) const {
+    const double l = (lp_far(m) ? (double)v - (double)m : ((double)v * (double)kLog2e - (double)__fmul_rn(m, kLog2e)) * kLn2) - log_s;
+    return (float)(l > 0.0 ? 0.0 : l);
+  }
+};
+
 template <typename T, int kLpThreads>
 __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kernel(LogProbArgs a) {
   constexpr int kLpWarps = kLpThreads / 32;
@@ -220,6 +244,7 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
   __shared__ uint8_t s_lane[kLpWarps][32];
   __shared__ uint64_t s_prefix;
   __shared__ int s_count, s_need;
+  __shared__ LpWhole s_whole;
 
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int parts = a.parts, part = (int)(blockIdx.x % parts);
@@ -254,6 +279,12 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
   auto outranks = [&](float y, int j) { return y > xt || (y == xt && j < token); };
   int rank = end_j >= 0 && outranks(end_x, end_j);
   if (tid < N && given && own >= v0 && own < v1) rank += outranks(to_f<T>(row.x[row.first(own) + tid]), row.first(own) + tid);
+
+  auto tell = [&](const LpWhole& whole) {
+    a.lp[r] = given ? whole.value(xt) : token < 0 ? 0.0f : NAN;
+    a.rank[r] = given ? whole.rank : -1;
+    a.entropy[r] = (float)(whole.entropy < 0.0 ? 0.0 : whole.entropy);
+  };
 
   LpSums mine{-INFINITY, 0.0f, 0.0f};
   auto add = [&](float y, float m, float ref) {   // -infinity, and products that leave fp32, too
@@ -372,6 +403,9 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
 #pragma unroll
         for (int u = 0; u < kLpUnroll; ++u) {
           if (at[u] >= v1) continue;
+          LpLargest<T> largest;
+          largest.add(y[u]);
+          if (largest.get() < least_x) continue;
           const int j0 = row.first(at[u]);
 #pragma unroll
           for (int e = 0; e < N; ++e) {
@@ -419,13 +453,17 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
       __syncthreads();
     }
     if (parts > 1) cluster_wait();
-    // in order: a key's place is the number of larger ones.  To the first CTA of the row.
+    // in order: a key's place is the number of larger ones, which four lanes count.  To the first CTA of the row.
     const int n = min(s_count, kLpRoom);
-    for (int i = tid; i < n; i += kLpThreads) {
-      const uint64_t k = s_words[i];
+    for (int i0 = w * 8; i0 < n; i0 += kLpWarps * 8) {
+      const int i = i0 + (lane >> 2);
+      const uint64_t k = i < n ? s_words[i] : 0u;
       int at = 0;
-      for (int j = 0; j < n; ++j) at += s_words[j] > k;
-      if (at < top) {
+#pragma unroll 4
+      for (int j = lane & 3; j < n; j += 4) at += s_words[j] > k;
+      at += __shfl_xor_sync(0xffffffffu, at, 1);
+      at += __shfl_xor_sync(0xffffffffu, at, 2);
+      if (i < n && at < top && (lane & 3) == 0) {
         uint32_t to = (uint32_t)__cvta_generic_to_shared(&s_best[part * kLpTop + at]);
         if (parts > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(to));
         asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(k) : "memory");
@@ -439,40 +477,40 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
   } else if (parts > 1) {
     cluster_wait();
   }
-  if (w == kLpWarps - 1) {   // (the first warps order words)
+  if (w == kLpWarps - 1) {   // (while the first warps order words)
     const LpJoined c = lp_join<kLpWarps>(s_join, kLpWarps);
-    uint32_t to = (uint32_t)__cvta_generic_to_shared(&s_part[part]);
-    if (parts > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(to));
-    if (lane == 0) {
+    if (parts == 1) {
+      const LpWhole whole(c);
+      if (lane == 0) {
+        s_whole = whole;
+        tell(whole);
+      }
+    } else if (lane == 0) {
+      uint32_t to = (uint32_t)__cvta_generic_to_shared(&s_part[part]);
+      asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(to));
       asm volatile("st.shared::cluster.v2.f64 [%0], {%1, %2};" ::"r"(to), "d"(c.s), "d"(c.t) : "memory");
       asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(to + 16), "r"(__float_as_uint(c.m)), "r"(c.rank) : "memory");
     }
   }
-  if (parts > 1) cluster_sync();
-  else __syncthreads();
+  if (parts == 1) {
+    if (top == 0) return;
+    __syncthreads();
+    if (tid < top) {   // in order already
+      const uint64_t k = s_best[tid];
+      if (k != 0u) {
+        a.best[r * top + tid] = (int)~(uint32_t)k;
+        a.best_lp[r * top + tid] = s_whole.value(lp_value((uint32_t)(k >> 32)));
+      }
+    }
+    return;
+  }
+  cluster_sync();
   if (part != 0) return;
 
-  // ---------------- the row
+  // ---------------- the row of several CTAs
   if (w * 32 < max(1, parts * top)) {   // whole warps
-    LpJoined c = lp_join<kLpCluster>(s_part, parts);
-    const bool none = !(c.m > -INFINITY);   // nothing but -infinity and NaN
-    if (!none && !lp_far(c.m)) {
-      // The maximum's own exponent is what rounding left of it, and its power of two is off by 2 ulp of 1: as much as all other words have where it is nearly certain
-      const float own = fmaf(c.m, kLog2e, -__fmul_rn(c.m, kLog2e));
-      c.s += exp2((double)own) - (double)lp_exp2(own);
-    }
-    const double ln2 = 0.693147180559945309417, log_s = none ? (double)NAN : log(c.s), ref = (double)__fmul_rn(c.m, kLog2e);
-    // rounding may leave a little over 0 of a certain token
-    auto value = [&](float v) {
-      const double l = (lp_far(c.m) ? (double)v - (double)c.m : ((double)v * (double)kLog2e - ref) * ln2) - log_s;
-      return (float)(l > 0.0 ? 0.0 : l);
-    };
-    if (tid == 0) {
-      a.lp[r] = given ? value(xt) : token < 0 ? 0.0f : NAN;
-      a.rank[r] = given ? c.rank : -1;
-      const double h = log_s - c.t / c.s * ln2;
-      a.entropy[r] = (float)(h < 0.0 ? 0.0 : h);
-    }
+    const LpWhole whole(lp_join<kLpCluster>(s_part, parts));
+    if (tid == 0) tell(whole);
     if (tid < parts * top) {
       const int p = tid / top;
       const uint64_t k = s_best[p * kLpTop + tid - p * top];
@@ -481,7 +519,7 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
         for (int j = 0; j < top; ++j) at += s_best[q * kLpTop + j] > k;
       if (k != 0u && at < top) {
         a.best[r * top + at] = (int)~(uint32_t)k;
-        a.best_lp[r * top + at] = value(lp_value((uint32_t)(k >> 32)));
+        a.best_lp[r * top + at] = whole.value(lp_value((uint32_t)(k >> 32)));
       }
     }
   }
@@ -493,10 +531,14 @@ static int log_probs_launch(LogProbArgs a, int64_t rows, int sms, cudaStream_t s
   const int pieces = (a.V + LpVec<T>::N - 1) / LpVec<T>::N;
   a.parts = 1;
   while (a.parts < kLpCluster && rows * a.parts * 2 <= 4 * sms && pieces / (a.parts * 2) >= 256) a.parts *= 2;
+  // Threads of a CTA: 512 where CTAs are fewer than SMs (8 rows of 131072 fp32, 20 alternatives: 11.1 us against 15.2 with 256); 128 for short rows, and where
+  // there are several waves of eight CTAs per SM and few alternatives, so that a row's end, where most threads wait, holds up fewer of them (us, 128 | 256: 4096 rows of 2000 bf16,
+  // 5 alternatives 23 | 36, of 32000 fp16, 1: 62 | 70, of 50257 bf16, 1: 87 | 94, 20: 147 | 133; 1200 rows of 50257, 5: 44 | 38).
   const bool wide = rows * a.parts <= sms && pieces / a.parts >= 512;
+  const bool narrow = a.parts == 1 && (pieces < 1024 || (a.top <= 8 && pieces <= 8192 && rows >= 24 * (int64_t)sms));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * a.parts));
-  cfg.blockDim = dim3(wide ? 512 : 256);
+  cfg.blockDim = dim3(wide ? 512 : narrow ? 128 : 256);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -505,7 +547,7 @@ static int log_probs_launch(LogProbArgs a, int64_t rows, int sms, cudaStream_t s
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  TSB_CUDA(cudaLaunchKernelEx(&cfg, wide ? log_probs_kernel<T, 512> : log_probs_kernel<T, 256>, a));
+  TSB_CUDA(cudaLaunchKernelEx(&cfg, wide ? log_probs_kernel<T, 512> : narrow ? log_probs_kernel<T, 128> : log_probs_kernel<T, 256>, a));
   return 1;
 }
 
