@@ -5,7 +5,7 @@
 //
 // Both operands are rows of K bytes side by side, as checkpoints and ops_int8.cu hold them: K-major operands of tcgen05.mma kind::i8 (32 k to an instruction), that TMA
 // lays down in boxes of 128 bytes x rows with the 128-byte swizzle.  K and rows beyond the tensors are zero-filled.  Three kernels:
-//  * up to 128 rows: the weights are the 128-row operand, the rows its N dimension; K ranges on the CTAs of a cluster (i8_cluster_kernel);
+//  * up to 64 rows: the weights are the 128-row operand, the rows its N dimension; K ranges on the CTAs of a cluster (i8_cluster_kernel);
 //  * more rows: pairs of CTAs on tiles of 256 rows x 256 or 128 channels (i8_pair_kernel);
 //  * rows that do not start on 16 bytes, which TMA cannot read: tiles of 64 x 64 on the integer pipe (i8_plain_kernel).
 // Every mbarrier wait is bounded; on timeout an error word is raised, copies and products in flight end, TMEM is freed and the kernel returns.
@@ -70,10 +70,60 @@ __device__ __forceinline__ void i8_store4(const I8Args& a, int row, int c, const
     if (c + e < a.N) y[e] = from_f<T>(i8_value(v[e], sq, sw[e], bias[e]));
 }
 
+// Scales and bias of what a lane finishes of 32 channels from c on: channels 4 u .. of the eight groups of four, or (rows that start anywhere) channel `lane`.
+// As loaded: nothing waits for them before they are used.
+template <typename T>
+struct I8Channels {
+  float4 sw;
+  I8Four<T> bias;
+  __device__ __forceinline__ void load(const I8Args& a, int c, int u, int lane) {
+    const T* b = reinterpret_cast<const T*>(a.bias);
+    sw = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias.e[e] = from_f<T>(0.0f);
+    if (a.four) {
+      if (c + 4 * u >= a.N) return;
+      sw = *reinterpret_cast<const float4*>(a.sw + c + 4 * u);
+      if (b) bias = *reinterpret_cast<const I8Four<T>*>(b + c + 4 * u);
+    } else if (c + lane < a.N) {
+      sw.x = a.sw[c + lane];
+      if (b) bias.e[0] = b[c + lane];
+    }
+  }
+  __device__ __forceinline__ void get(float* s, float* b) const {
+    s[0] = sw.x; s[1] = sw.y; s[2] = sw.z; s[3] = sw.w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = to_f<T>(bias.e[e]);
+  }
+};
+
+// 32 accumulators of a lane: asked for, and there (the registers mean nothing in between)
+#define TSB_V32(v)                                                                                                                                                        \
+  "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]),          \
+      "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]),         \
+      "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+__device__ __forceinline__ void i8_tmem_ask(uint32_t taddr, uint32_t* r) {
+  __syncwarp();
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void i8_tmem_have(uint32_t* r) {
+  __syncwarp();
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : TSB_V32(r)::"memory");
+}
+
 // instruction descriptor: signed bytes, 32-bit sums, both operands K-major
 constexpr uint32_t i8_idesc(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 
-// ---- up to 128 rows ------------------------------------------------------------------------------------------------------
+// ---- up to 64 rows ------------------------------------------------------------------------------------------------------
 // A CTA owns 128 channels over a range of K; the 1 .. 8 CTAs of a cluster share the channels and push their sums, four rows at a time, into the shared
 // memory of the CTA that finishes them (1 / ks of the channels each); the stores report to its mbarrier.
 // warp 0: copies; warp 1: TMEM and products; warps 2-5: accumulators out of TMEM; all warps: sums and outputs.
@@ -105,8 +155,9 @@ __global__ void __launch_bounds__(kI8Threads) i8_cluster_kernel(const __grid_con
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int S = a.stages, ks = a.ks, M = a.M;
-  int* red = reinterpret_cast<int*>(smem + S * kStage);   // [source rank][row quad][channel of a group][group][4 rows]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S * kStage + NR * 512);
+  // sums: [source rank][row quad][channel of a group][group][4 rows]; of one CTA alone over the ring, which the products have read by then
+  int* red = reinterpret_cast<int*>(smem + (ks > 1 ? S * kStage : 0));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S * kStage + (ks > 1 ? NR * 512 : 0));
   const uint32_t full = s_u32(bars), empty = full + 16 * 8, acc = empty + 16 * 8, sums = acc + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 34);
   __shared__ int s_err, s_asked;   // s_asked: steps whose copies are under way or done (warp 0)
@@ -117,23 +168,38 @@ __global__ void __launch_bounds__(kI8Threads) i8_cluster_kernel(const __grid_con
   const int steps = (a.K + 127) >> 7, k0 = (int)((int64_t)steps * rank / ks), n_it = (int)((int64_t)steps * (rank + 1) / ks) - k0;   // blocks of 128 k
   const int quads = (M + 3) >> 2;
 
-  if (tid == 0) {
-    for (int i = 0; i < S; ++i) {
-      tc_mbar_init(bars + i, 1);
-      tc_mbar_init(bars + 16 + i, 1);
+  const uint32_t ring = s_u32(smem);
+  auto copy = [&](int i, int s) {
+    const uint32_t dst = ring + s * kStage, bar = full + s * 8;
+    tc_mbar_expect_el(bar, kStage);
+    tma_load_2d_el(dst, &mapW, (k0 + i) * 128, col0, bar);
+    tma_load_2d_el(dst + kI8W, &mapQ, (k0 + i) * 128, 0, bar);
+  };
+  const int n_pre = min(S, n_it);
+  if (w == 0) {
+    if (lane == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&mapW) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&mapQ) : "memory");
+      for (int i = 0; i < S; ++i) {
+        tc_mbar_init(bars + i, 1);
+        tc_mbar_init(bars + 16 + i, 1);
+      }
+      tc_mbar_init(bars + 32, 1);
+      tc_mbar_init(bars + 33, 1);
+      s_err = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (ks > 1) tc_mbar_expect_tx(bars + 33, quads * 2048);   // 128 / ks channels from each of ks CTAs
     }
-    tc_mbar_init(bars + 32, 1);
-    tc_mbar_init(bars + 33, 1);
-    s_err = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (ks > 1) tc_mbar_expect_tx(bars + 33, quads * 2048);   // 128 / ks channels from each of ks CTAs
+    __syncwarp();
+    for (int i = 0; i < n_pre; ++i) copy(i, i);   // on their way while the others get TMEM
   }
   if (w == 1) {
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_u32(tmem_slot)), "r"(kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (tid < M) s_sq[tid] = a.sq[tid];   // (M <= 128 < threads)
+  if (w >= 2 && tid - 64 < M) s_sq[tid - 64] = a.sq[tid - 64];   // (M <= 64)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -143,7 +209,6 @@ __global__ void __launch_bounds__(kI8Threads) i8_cluster_kernel(const __grid_con
   }
   const uint32_t tmem = *tmem_slot;
   volatile int* err = &s_err;
-  const uint32_t ring = s_u32(smem);
 
   // this CTA finishes 128 / ks of the channels, in groups of four, of every row: a thread's channels are the same in all of its rows
   const int gsh = 5 - (31 - __clz(ks)), G = 1 << gsh;          // groups here
@@ -151,16 +216,12 @@ __global__ void __launch_bounds__(kI8Threads) i8_cluster_kernel(const __grid_con
   const int c = col0 + ((rank << gsh) + g) * 4, row0 = (tid >> (gsh + 2)) * 4 + (tid & 3), step = (kI8Threads >> (gsh + 2)) * 4;
 
   if (w == 0) {
-    // ---------------- copies
-    int s = 0;
-    unsigned phase = 1;   // parity of the ring's previous round
-    int i = 0;
+    // ---------------- copies behind the first round
+    int s = 0, i = n_pre;
+    unsigned phase = 0;
     for (; i < n_it; ++i) {
-      if (i >= S && !tc_wait_or(empty + s * 8, phase, err, a.wait_limit)) break;
-      const uint32_t dst = ring + s * kStage, bar = full + s * 8;
-      tc_mbar_expect_el(bar, kStage);
-      tma_load_2d_el(dst, &mapW, (k0 + i) * 128, col0, bar);
-      tma_load_2d_el(dst + kI8W, &mapQ, (k0 + i) * 128, 0, bar);
+      if (!tc_wait_or(empty + s * 8, phase, err, a.wait_limit)) break;
+      copy(i, s);
       if (++s == S) s = 0, phase ^= 1;
     }
     if (lane == 0) s_asked = i;
@@ -377,45 +438,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8PThreads, 1)
       const int row0 = (tl.m_tile * 2 + rank) * 128 + q * 32, n0 = tl.n_tile * BN + half * P::kCols;
       const int n_live = min(32, a.M - row0);
       const float sq = lane < n_live ? a.sq[row0 + lane] : 0.0f;
+      I8Channels<T> now, then;   // of a chunk of 32 channels, and of the next one
+      if (n_live > 0) now.load(a, n0, u, lane);
       if (!tc_wait_or(acc_full + buf * 8, (unsigned)((n_done >> 1) & 1), err, a.wait_limit)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * P::kCols);
+      const int cols = n_live > 0 ? min(P::kCols, a.N - n0) : 0;
+      uint32_t v[32];
+      if (cols > 0) {
+        i8_tmem_ask(acc, v);
+        i8_tmem_have(v);
+      }
 #pragma unroll 1
-      for (int c = 0; c < P::kCols && n_live > 0 && n0 + c < a.N; c += 32) {
-        float sw[4], bias[4];
-        const int col = n0 + c + (a.four ? u * 4 : lane);
-        if (a.four) {
-          i8_channels<T>(a, col, sw, bias);
-        } else {
-          sw[0] = col < a.N ? a.sw[col] : 0.0f;
-          bias[0] = a.bias && col < a.N ? to_f<T>(reinterpret_cast<const T*>(a.bias)[col]) : 0.0f;
-        }
-        uint32_t v[32];
-        tmem_ld32(acc + c, v);
+      for (int c = 0; c < cols; c += 32) {
         int4* mine = stage + lane * 8;
 #pragma unroll
         for (int j = 0; j < 8; ++j) mine[j ^ (lane & 7)] = make_int4((int)v[4 * j], (int)v[4 * j + 1], (int)v[4 * j + 2], (int)v[4 * j + 3]);
         __syncwarp();
+        const bool more = c + 32 < cols;
+        if (more) {   // on their way while these leave
+          then.load(a, n0 + c + 32, u, lane);
+          i8_tmem_ask(acc + c + 32, v);
+        }
         if (a.four) {
+          float sw[4], bias[4];
+          now.get(sw, bias);
 #pragma unroll
           for (int it = 0; it < 8; ++it) {
             const int rr = it * 4 + r;
             const float s = __shfl_sync(0xffffffffu, sq, rr);
             const int4 x = stage[rr * 8 + (u ^ (rr & 7))];
             const int e[4] = {x.x, x.y, x.z, x.w};
-            if (rr < n_live) i8_store4<T>(a, row0 + rr, col, e, s, sw, bias);
+            if (rr < n_live) i8_store4<T>(a, row0 + rr, n0 + c + u * 4, e, s, sw, bias);
           }
         } else {
           // a lane per channel: rows of y start anywhere
+          const int col = n0 + c + lane;
+          const float sw = now.sw.x, bias = to_f<T>(now.bias.e[0]);
           T* y = reinterpret_cast<T*>(a.y) + (int64_t)row0 * a.y_row + col;
-#pragma unroll 4
+#pragma unroll 8
           for (int rr = 0; rr < n_live; ++rr, y += a.y_row) {
             const float s = __shfl_sync(0xffffffffu, sq, rr);
             const int x = reinterpret_cast<const int*>(stage)[(rr * 8 + ((lane >> 2) ^ (rr & 7))) * 4 + (lane & 3)];
-            if (col < a.N) *y = from_f<T>(i8_value(x, s, sw[0], bias[0]));
+            if (col < a.N) *y = from_f<T>(i8_value(x, s, sw, bias));
           }
         }
         __syncwarp();   // the warp's shared memory is free again
+        if (more) i8_tmem_have(v);
+        now = then;
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -511,13 +581,14 @@ static int i8_cluster(DeviceState* st, int device, EncodeTiledFn enc, I8Args a, 
   const int groups = (a.N + 127) / 128, steps = (a.K + 127) / 128;
   a.ks = 1;
   while (a.ks < 8 && (int64_t)groups * a.ks * 2 <= 2 * st->sm_count && steps / (a.ks * 2) >= 2) a.ks *= 2;
-  // two CTAs per SM up to 64 rows
-  a.stages = ((NR <= 64 ? 112 : 225) * 1024 - 1024 - 512 - NR * 512) / kStage;
+  // rings for two CTAs per SM (one with the whole of it: a cluster of eight no longer fits a GPC twice, and 16 of them make two waves)
+  const int sums = a.ks > 1 ? NR * 512 : 0;
+  a.stages = (112 * 1024 - 1024 - 512 - sums) / kStage;
   if (a.stages > 16) a.stages = 16;
-  const int smem = a.stages * kStage + NR * 512 + 512 + 1024;
+  const int smem = a.stages * kStage + sums + 512 + 1024;
   static bool done[kMaxDevices] = {};
   if (!done[device]) {
-    TSB_CUDA(cudaFuncSetAttribute(i8_cluster_kernel<T, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (NR <= 64 ? 112 : 225) * 1024));
+    TSB_CUDA(cudaFuncSetAttribute(i8_cluster_kernel<T, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024));
     done[device] = true;
   }
   CUtensorMap mapW, mapQ;
@@ -573,7 +644,6 @@ static int i8_linear(DeviceState* st, int device, I8Args a, cudaStream_t s) {
   if (a.M <= 16) return i8_cluster<T, 16>(st, device, enc, a, s);
   if (a.M <= 32) return i8_cluster<T, 32>(st, device, enc, a, s);
   if (a.M <= 64) return i8_cluster<T, 64>(st, device, enc, a, s);
-  if (a.M <= 128) return i8_cluster<T, 128>(st, device, enc, a, s);
   // whole waves of pairs times steps of 128 k, and the last tile's outputs
   const int pairs = st->sm_count / 2, m_tiles = (a.M + 255) / 256, k_total = (a.K + 127) / 128;
   const int64_t t256 = (int64_t)m_tiles * ((a.N + 255) / 256), t128 = (int64_t)m_tiles * ((a.N + 127) / 128);
