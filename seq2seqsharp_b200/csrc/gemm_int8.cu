@@ -24,7 +24,8 @@ struct I8Args {
   int64_t y_row;
   int M, N, K;
   int ks, stages;       // i8_cluster_kernel
-  int four;             // whether four neighbouring channels lie on a boundary of theirs in y, sw and bias
+  int four;             // whether four neighbouring channels lie on a boundary of theirs in y, sw and bias (i8_cluster_kernel)
+  int units;            // whether rows of y start on 16 bytes (i8_pair_kernel)
   unsigned wait_limit;
   int* error;
 };
@@ -52,50 +53,22 @@ __device__ __forceinline__ void i8_channels(const I8Args& a, int c, float* sw, f
   }
 }
 template <typename T>
+__device__ __forceinline__ void i8_put4(T* y, float y0, float y1, float y2, float y3) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(y) = make_float4(y0, y1, y2, y3);
+  else *reinterpret_cast<uint2*>(y) = make_uint2(Pair16<T>::put(y0, y1), Pair16<T>::put(y2, y3));
+}
+template <typename T>
 __device__ __forceinline__ void i8_store4(const I8Args& a, int row, int c, const int* v, float sq, const float* sw, const float* bias) {
   T* y = reinterpret_cast<T*>(a.y) + (int64_t)row * a.y_row + c;
   if (a.four) {
     if (c >= a.N) return;
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(y) = make_float4(i8_value(v[0], sq, sw[0], bias[0]), i8_value(v[1], sq, sw[1], bias[1]), i8_value(v[2], sq, sw[2], bias[2]),
-                                                  i8_value(v[3], sq, sw[3], bias[3]));
-    } else {
-      *reinterpret_cast<uint2*>(y) = make_uint2(Pair16<T>::put(i8_value(v[0], sq, sw[0], bias[0]), i8_value(v[1], sq, sw[1], bias[1])),
-                                                Pair16<T>::put(i8_value(v[2], sq, sw[2], bias[2]), i8_value(v[3], sq, sw[3], bias[3])));
-    }
+    i8_put4<T>(y, i8_value(v[0], sq, sw[0], bias[0]), i8_value(v[1], sq, sw[1], bias[1]), i8_value(v[2], sq, sw[2], bias[2]), i8_value(v[3], sq, sw[3], bias[3]));
     return;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (c + e < a.N) y[e] = from_f<T>(i8_value(v[e], sq, sw[e], bias[e]));
 }
-
-// Scales and bias of what a lane finishes of 32 channels from c on: channels 4 u .. of the eight groups of four, or (rows that start anywhere) channel `lane`.
-// As loaded: nothing waits for them before they are used.
-template <typename T>
-struct I8Channels {
-  float4 sw;
-  I8Four<T> bias;
-  __device__ __forceinline__ void load(const I8Args& a, int c, int u, int lane) {
-    const T* b = reinterpret_cast<const T*>(a.bias);
-    sw = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) bias.e[e] = from_f<T>(0.0f);
-    if (a.four) {
-      if (c + 4 * u >= a.N) return;
-      sw = *reinterpret_cast<const float4*>(a.sw + c + 4 * u);
-      if (b) bias = *reinterpret_cast<const I8Four<T>*>(b + c + 4 * u);
-    } else if (c + lane < a.N) {
-      sw.x = a.sw[c + lane];
-      if (b) bias.e[0] = b[c + lane];
-    }
-  }
-  __device__ __forceinline__ void get(float* s, float* b) const {
-    s[0] = sw.x; s[1] = sw.y; s[2] = sw.z; s[3] = sw.w;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) b[e] = to_f<T>(bias.e[e]);
-  }
-};
 
 // 32 accumulators of a lane: asked for, and there (the registers mean nothing in between)
 #define TSB_V32(v)                                                                                                                                                        \
@@ -331,25 +304,30 @@ __global__ void __launch_bounds__(kI8Threads) i8_cluster_kernel(const __grid_con
 // Warp 0: copies; warp 1: TMEM and products; warps 2..9: outputs (two per quarter of the TMEM lanes, each half of a tile's channels).
 constexpr int kI8PThreads = 320, kI8PWarps = 8;
 constexpr int kI8A = 128 * 128;
-template <int BN>
+template <typename T, int BN>
 struct I8Pair {
   static constexpr int kB = BN / 2 * 128;               // weight bytes of a stage and CTA
-  static constexpr int kStages = BN == 256 ? 6 : 8;
+  static constexpr int kStages = BN == 256 ? (sizeof(T) == 4 ? 4 : 5) : (sizeof(T) == 4 ? 6 : 7);
   static constexpr int kStage = kI8A + kB;
-  static constexpr int kOut = kI8PWarps * 4096;         // 32 x 32 sums of a warp on their way from rows of TMEM to rows of y
-  static constexpr int kSmem = kStages * kStage + 1024 + 256 + kOut;
+  static constexpr int kBox = 32 * 32 * (int)sizeof(T); // outputs of a warp on their way from rows of TMEM to y: two of these in turn,
+  static constexpr int kOut = 2 * kBox + 1024;          // and scales and biases of the warp's channels
+  static constexpr int kSmem = kStages * kStage + 1024 + 256 + kI8PWarps * kOut;
   static constexpr int kCols = BN / 2;                  // channels of an output warp
 };
+__device__ __forceinline__ void i8_store_box(const CUtensorMap* map, uint32_t from, int c0, int c1) {   // by one lane
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(from), "r"(c0), "r"(c1) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
 
 template <typename T, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8PThreads, 1)
-    i8_pair_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapW, I8Args a, int m_tiles, int n_tiles) {
-  typedef I8Pair<BN> P;
+    i8_pair_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapY, I8Args a, int m_tiles, int n_tiles) {
+  typedef I8Pair<T, BN> P;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sA = s_u32(smem), sB = sA + P::kStages * kI8A;
   unsigned char* outs = smem + P::kStages * P::kStage;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(outs + P::kOut);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(outs + kI8PWarps * P::kOut);
   // full: the leader's counts the copies of both CTAs; acc_empty: the leader's, both CTAs' output warps arrive
   const uint32_t full = s_u32(bars), empty = full + P::kStages * 8, acc_full = empty + P::kStages * 8, acc_empty = acc_full + 16, drain = acc_empty + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * P::kStages + 5);
@@ -429,68 +407,106 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8PThreads, 1)
   } else if (w >= 2) {
     // ---------------- outputs: TMEM lanes 32 (w % 4) .. = rows of this CTA's half, channels kCols ((w - 2) / 4) ..
     const int q = w & 3, half = (w - 2) >> 2;
-    int4* stage = reinterpret_cast<int4*>(outs + (w - 2) * 4096);   // 32 rows of eight 16-byte units, XOR-ed with the row
-    const int r = lane >> 3, u = lane & 7;
-    int n_done = 0;
-    for (int t = pair; t < n_total; t += n_pairs, ++n_done) {
+    unsigned char* mine = outs + (w - 2) * P::kOut;
+    float* s_w = reinterpret_cast<float*>(mine + 2 * P::kBox);   // scales of the tile's channels, biases behind them
+    constexpr int kPer = P::kCols / 32;
+    constexpr int kUnits = 2 * (int)sizeof(T);   // 16-byte units of a line of 32 outputs; which of them a lane begins with is the swizzle of the tensor map
+    const int swz = sizeof(T) == 4 ? lane & 7 : (lane >> 1) & 3;
+    // of the next tile: what it has of scales and biases is on its way while one leaves
+    int row0 = 0, n0 = 0, n_live = 0;
+    float sq = 0.0f, nw[kPer], nb[kPer];
+    auto ahead = [&](int t) {
       const TcTile tl = tc_tile_of(t, m_tiles, n_tiles, 8);
-      const int buf = n_done & 1;
-      const int row0 = (tl.m_tile * 2 + rank) * 128 + q * 32, n0 = tl.n_tile * BN + half * P::kCols;
-      const int n_live = min(32, a.M - row0);
-      const float sq = lane < n_live ? a.sq[row0 + lane] : 0.0f;
-      I8Channels<T> now, then;   // of a chunk of 32 channels, and of the next one
-      if (n_live > 0) now.load(a, n0, u, lane);
+      row0 = (tl.m_tile * 2 + rank) * 128 + q * 32;
+      n0 = tl.n_tile * BN + half * P::kCols;
+      n_live = min(32, a.M - row0);
+      sq = lane < n_live ? a.sq[row0 + lane] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int col = n0 + k * 32 + lane;
+        const bool there = n_live > 0 && col < a.N;
+        nw[k] = there ? a.sw[col] : 0.0f;
+        nb[k] = there && a.bias ? to_f<T>(reinterpret_cast<const T*>(a.bias)[col]) : 0.0f;
+      }
+    };
+    if (pair < n_total) ahead(pair);
+    int n_done = 0, n_boxes = 0;
+    for (int t = pair; t < n_total; t += n_pairs, ++n_done) {
+      const int buf = n_done & 1, row = row0, col0 = n0, live = n_live;
+      const float scale = sq;
       if (!tc_wait_or(acc_full + buf * 8, (unsigned)((n_done >> 1) & 1), err, a.wait_limit)) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * P::kCols);
-      const int cols = n_live > 0 ? min(P::kCols, a.N - n0) : 0;
+      const int cols = live > 0 ? min(P::kCols, a.N - col0) : 0;
       uint32_t v[32];
-      if (cols > 0) {
-        i8_tmem_ask(acc, v);
-        i8_tmem_have(v);
+      if (cols > 0) i8_tmem_ask(acc, v);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        s_w[k * 32 + lane] = nw[k];
+        s_w[P::kCols + k * 32 + lane] = nb[k];
       }
-#pragma unroll 1
-      for (int c = 0; c < cols; c += 32) {
-        int4* mine = stage + lane * 8;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mine[j ^ (lane & 7)] = make_int4((int)v[4 * j], (int)v[4 * j + 1], (int)v[4 * j + 2], (int)v[4 * j + 3]);
+      if (t + n_pairs < n_total) ahead(t + n_pairs);
+      // the accumulator is free once this warp's last 32 sums of it are in registers (nothing that it wrote has to be seen by anyone)
+      auto done = [&]() {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(tc_leader_addr(acc_empty + buf * 8)) : "memory");
+      };
+      if (cols <= 0) {
+        done();
+        continue;
+      }
+      i8_tmem_have(v);
+      // a lane's row: 32 channels finished, in the type of y, and laid down as the tensor map wants them
+#pragma unroll 1
+      for (int c = 0; c < cols; c += 32, ++n_boxes) {
         const bool more = c + 32 < cols;
-        if (more) {   // on their way while these leave
-          then.load(a, n0 + c + 32, u, lane);
-          i8_tmem_ask(acc + c + 32, v);
-        }
-        if (a.four) {
-          float sw[4], bias[4];
-          now.get(sw, bias);
+        if (!more) done();
+        unsigned char* box = mine + (n_boxes & 1) * P::kBox;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");   // the box before the last one has left
+        __syncwarp();
+        unsigned char* line = box + lane * (32 * (int)sizeof(T));
 #pragma unroll
-          for (int it = 0; it < 8; ++it) {
-            const int rr = it * 4 + r;
-            const float s = __shfl_sync(0xffffffffu, sq, rr);
-            const int4 x = stage[rr * 8 + (u ^ (rr & 7))];
-            const int e[4] = {x.x, x.y, x.z, x.w};
-            if (rr < n_live) i8_store4<T>(a, row0 + rr, n0 + c + u * 4, e, s, sw, bias);
+        for (int j = 0; j < kUnits; ++j) {
+          constexpr int kE = 16 / (int)sizeof(T);
+          float y[kE];
+#pragma unroll
+          for (int e = 0; e < kE; e += 4) {
+            const float4 sw = *reinterpret_cast<const float4*>(s_w + c + j * kE + e), b = *reinterpret_cast<const float4*>(s_w + P::kCols + c + j * kE + e);
+            const uint32_t* x = v + j * kE + e;
+            y[e] = i8_value((int)x[0], scale, sw.x, b.x);
+            y[e + 1] = i8_value((int)x[1], scale, sw.y, b.y);
+            y[e + 2] = i8_value((int)x[2], scale, sw.z, b.z);
+            y[e + 3] = i8_value((int)x[3], scale, sw.w, b.w);
           }
+          uint4 o;
+          if constexpr (sizeof(T) == 4) o = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+          else o = make_uint4(Pair16<T>::put(y[0], y[1]), Pair16<T>::put(y[2], y[3]), Pair16<T>::put(y[4], y[5]), Pair16<T>::put(y[6], y[7]));
+          *reinterpret_cast<uint4*>(line + ((j ^ swz) << 4)) = o;
+        }
+        if (more) i8_tmem_ask(acc + c + 32, v);   // on their way while these leave
+        if (a.units) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) i8_store_box(&mapY, s_u32(box), col0 + c, row);   // rows and channels that are not there are left out
         } else {
           // a lane per channel: rows of y start anywhere
-          const int col = n0 + c + lane;
-          const float sw = now.sw.x, bias = to_f<T>(now.bias.e[0]);
-          T* y = reinterpret_cast<T*>(a.y) + (int64_t)row0 * a.y_row + col;
+          __syncwarp();
+          const int col = col0 + c + lane, rows = col < a.N ? live : 0;
+          T* at = reinterpret_cast<T*>(a.y) + (int64_t)row * a.y_row + col;
 #pragma unroll 8
-          for (int rr = 0; rr < n_live; ++rr, y += a.y_row) {
-            const float s = __shfl_sync(0xffffffffu, sq, rr);
-            const int x = reinterpret_cast<const int*>(stage)[(rr * 8 + ((lane >> 2) ^ (rr & 7))) * 4 + (lane & 3)];
-            if (col < a.N) *y = from_f<T>(i8_value(x, s, sw, bias));
+          for (int rr = 0; rr < 32; ++rr, at += a.y_row) {
+            constexpr int kE = 16 / (int)sizeof(T);
+            const int unit = (lane / kE) ^ (sizeof(T) == 4 ? rr & 7 : (rr >> 1) & 3);
+            if (rr < rows) *at = reinterpret_cast<const T*>(box + rr * (32 * (int)sizeof(T)) + (unit << 4))[lane % kE];
           }
         }
-        __syncwarp();   // the warp's shared memory is free again
         if (more) i8_tmem_have(v);
-        now = then;
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(tc_leader_addr(acc_empty + buf * 8)) : "memory");
+      __syncwarp();   // scales and biases have been read
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // shared memory is not given back before it has been read
+    __syncwarp();
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -574,6 +590,19 @@ static int i8_map(CUtensorMap* map, EncodeTiledFn enc, const int8_t* at, int64_t
   TSB_CHECK(r == CUDA_SUCCESS, "linear_int8: cuTensorMapEncodeTiled failed with %d", (int)r);
   return 1;
 }
+// outputs, in boxes of 32 x 32
+template <typename T>
+static int i8_map_out(CUtensorMap* map, EncodeTiledFn enc, const I8Args& a) {
+  const cuuint64_t dims[2] = {(cuuint64_t)a.N, (cuuint64_t)a.M};
+  const cuuint64_t strides[1] = {(cuuint64_t)a.y_row * sizeof(T)};
+  const cuuint32_t box[2] = {32, 32};
+  const cuuint32_t el[2] = {1, 1};
+  const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;   // moved as they are
+  const CUresult r = enc(map, type, 2, a.y, dims, strides, box, el, CU_TENSOR_MAP_INTERLEAVE_NONE, sizeof(T) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TSB_CHECK(r == CUDA_SUCCESS, "linear_int8: cuTensorMapEncodeTiled failed with %d for the outputs", (int)r);
+  return 1;
+}
 
 template <typename T, int NR>
 static int i8_cluster(DeviceState* st, int device, EncodeTiledFn enc, I8Args a, cudaStream_t s) {
@@ -614,21 +643,23 @@ template <typename T, int BN>
 static int i8_pair(DeviceState* st, int device, EncodeTiledFn enc, const I8Args& a, cudaStream_t s) {
   static bool done[kMaxDevices] = {};
   if (!done[device]) {
-    TSB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, I8Pair<BN>::kSmem));
+    TSB_CUDA(cudaFuncSetAttribute(i8_pair_kernel<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, I8Pair<T, BN>::kSmem));
     done[device] = true;
   }
-  CUtensorMap mapW, mapQ;
+  CUtensorMap mapW, mapQ, mapY{};
+  if (a.units) TSB_TRY(i8_map_out<T>(&mapY, enc, a));
   TSB_TRY(i8_map(&mapW, enc, a.w, a.w_row, a.N, a.K, BN / 2));
   TSB_TRY(i8_map(&mapQ, enc, a.q, a.q_row, a.M, a.K, 128));
   const int pairs = st->sm_count / 2, m_tiles = (a.M + 255) / 256, n_tiles = (a.N + BN - 1) / BN;
   const int64_t tiles = (int64_t)m_tiles * n_tiles;
-  i8_pair_kernel<T, BN><<<2 * (int)(tiles < pairs ? tiles : pairs), kI8PThreads, I8Pair<BN>::kSmem, s>>>(mapQ, mapW, a, m_tiles, n_tiles);
+  i8_pair_kernel<T, BN><<<2 * (int)(tiles < pairs ? tiles : pairs), kI8PThreads, I8Pair<T, BN>::kSmem, s>>>(mapQ, mapW, mapY, a, m_tiles, n_tiles);
   return 1;
 }
 
 template <typename T>
 static int i8_linear(DeviceState* st, int device, I8Args a, cudaStream_t s) {
   a.four = a.N % 4 == 0 && (uintptr_t)a.y % (4 * sizeof(T)) == 0 && (a.M == 1 || a.y_row % 4 == 0) && (uintptr_t)a.sw % 16 == 0 && (uintptr_t)a.bias % (4 * sizeof(T)) == 0;
+  a.units = (uintptr_t)a.y % 16 == 0 && a.y_row * sizeof(T) % 16 == 0;
   const bool boxes = ((uintptr_t)a.q | (uintptr_t)a.w) % 16 == 0 && (a.M == 1 || (a.q_row % 16 == 0 && a.q_row >= a.K)) &&
                      (a.N == 1 || (a.w_row % 16 == 0 && a.w_row >= a.K));
   EncodeTiledFn enc = boxes ? get_encode() : nullptr;
