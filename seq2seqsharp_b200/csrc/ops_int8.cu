@@ -12,7 +12,7 @@
 // elements or of one otherwise.
 #include <type_traits>
 
-#include "kernels.cuh"
+#include "stream_common.cuh"
 
 namespace tsb {
 
@@ -32,8 +32,14 @@ struct Int8Rows {
 
 template <typename T, int N> struct __align__(N * sizeof(T)) Int8Piece { T e[N]; };
 
-// silu, sigmoid: exp and the quotient by the approximate instructions, off by a few 2^-22 of what they return; a step of q is 2^-7 of the row's largest value
-__device__ __forceinline__ float int8_sigmoid(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+// silu, sigmoid: the power of two (off by 2 ulp, its exponent by one of itself) and the reciprocal (1 ulp) by the approximate instructions: a few 2^-22 of what they return, where
+// a step of q is 2^-7 of the row's largest value
+__device__ __forceinline__ float int8_sigmoid(float v) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.44269504088896341f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
 template <int ACT>
 __device__ __forceinline__ float int8_act(float v) {
   if constexpr (ACT == TSB200_ACT_SILU) return v * int8_sigmoid(v);
@@ -48,23 +54,37 @@ __device__ __forceinline__ uint32_t int8_pack(const float* v, float inv) {
   return __byte_perm(lo, hi, 0x5410);
 }
 
-// sum of squares and maximum (as the bits of a number without its sign: a NaN is larger than all) over the threads of a row: a warp, or the CTA
-template <bool WARP>
-__device__ __forceinline__ void int8_reduce(float& sum, uint32_t& top) {
-  sum = warp_sum(sum);
-  top = __reduce_max_sync(0xffffffffu, top);
+// larger of what is there and two values, without their signs; a NaN stays one
+__device__ __forceinline__ float int8_top(float top, float a, float b) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(top), "f"(a), "f"(b));
+  return r;
+}
+template <int N>
+__device__ __forceinline__ float int8_top(float top, const float* v) {
+#pragma unroll
+  for (int e = 0; e + 1 < N; e += 2) top = int8_top(top, v[e], v[e + 1]);
+  return N % 2 ? int8_top(top, v[N - 1], v[N - 1]) : top;
+}
+// sum of squares (of a norm) and maximum (as bits: those of a NaN are larger than all) over the threads of a row: a warp, or the CTA
+// (turn: 0 and 1 in alternation where a CTA has several rows, so that one barrier a row is enough)
+template <bool WARP, bool NORM>
+__device__ __forceinline__ uint32_t int8_reduce(float& sum, float largest, int turn = 0) {
+  uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest) & 0x7fffffffu);
+  if constexpr (NORM) sum = warp_sum(sum);
   if constexpr (!WARP) {
-    __shared__ float s_sum[32];
-    __shared__ uint32_t s_top[32];
+    __shared__ float s_sum[2][32];
+    __shared__ uint32_t s_top[2][32];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
     if (lane == 0) {
-      s_sum[w] = sum;
-      s_top[w] = top;
+      if (NORM) s_sum[turn][w] = sum;
+      s_top[turn][w] = top;
     }
     __syncthreads();
-    sum = warp_sum(lane < warps ? s_sum[lane] : 0.0f);
-    top = __reduce_max_sync(0xffffffffu, lane < warps ? s_top[lane] : 0u);
+    if constexpr (NORM) sum = warp_sum(lane < warps ? s_sum[turn][lane] : 0.0f);
+    top = __reduce_max_sync(0xffffffffu, lane < warps ? s_top[turn][lane] : 0u);
   }
+  return top;
 }
 
 // What a row's statistics make of it: the factor of v, and the scale (written by one thread).  `up`: a power of two that v is multiplied by first, so that 127 / max|v|
@@ -102,7 +122,7 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(Int8Rows p) {
   }
   float v[NC][VEC];
   float sum = 0.0f;
-  uint32_t top = 0u;
+  float largest = 0.0f;
   if constexpr (NORM) {
     T* h = reinterpret_cast<T*>(p.h) + r * p.h_row;
     const T* gamma = reinterpret_cast<const T*>(p.gamma);
@@ -146,11 +166,8 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(Int8Rows p) {
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c)
-    if (i0 + c * step < p.d) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) top = max(top, __float_as_uint(v[c][e]) & 0x7fffffffu);
-    }
-  int8_reduce<WARP>(sum, top);
+    if (i0 + c * step < p.d) largest = int8_top<VEC>(largest, v[c]);
+  const uint32_t top = int8_reduce<WARP, NORM>(sum, largest);
   float up;
   const float inv = int8_finish<NORM>(p, r, sum, top, threadIdx.x == 0, up);
   int8_t* q = p.q + r * p.q_row;
@@ -178,7 +195,7 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(Int8Rows p) {
   T* h = reinterpret_cast<T*>(p.h) + r * p.h_row;
   const bool two = p.b != nullptr;
   float sum = 0.0f;
-  uint32_t top = 0u;
+  float largest = 0.0f;
   auto value = [&](int i) {
     float v = ep_act(to_f<T>(a[i]), p.act);
     return two ? v * to_f<T>(b[i]) : v;
@@ -197,9 +214,9 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(Int8Rows p) {
     } else {
       v = value(i);
     }
-    top = max(top, __float_as_uint(v) & 0x7fffffffu);
+    largest = int8_top(largest, v, v);
   }
-  int8_reduce<false>(sum, top);
+  const uint32_t top = int8_reduce<false, NORM>(sum, largest);
   float up;
   const float inv = int8_finish<NORM>(p, r, sum, top, threadIdx.x == 0, up);
   for (int i = threadIdx.x; i < p.d; i += 1024) {
@@ -210,21 +227,162 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(Int8Rows p) {
   }
 }
 
+// Many rows that start on 16 bytes: CTAs walk over rows, whose inputs a ring of bulk copies brings into shared memory several rows ahead.  All threads have read a row when its
+// sums are joined, so that the barrier which does that also gives the row's place to the next copy.
+struct Int8Ring {
+  int stages, bytes;      // of a row and input
+  unsigned wait_limit;
+  int* error;
+};
+template <typename T, int NC, bool NORM>
+__global__ void __launch_bounds__(512, NC == 1 ? 3 : 2) int8_ring_kernel(Int8Rows p, Int8Ring ring) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  typedef Int8Piece<T, VEC> Piece;
+  extern __shared__ __align__(128) unsigned char rows_smem[];
+  __shared__ __align__(8) uint64_t bars[8];
+  __shared__ int s_late[2];   // a thread has given up waiting for a row; in alternation, so that no thread's next row is taken for this one
+  const bool two = p.b != nullptr;
+  const int per = ring.bytes * (two ? 2 : 1), step = (int)blockDim.x * VEC, i0 = (int)threadIdx.x * VEC;
+  auto copy = [&](int64_t r, int s) {   // by one thread
+    mbar_expect_tx(bars + s, (unsigned)per);
+    bulk_g2s(rows_smem + s * per, reinterpret_cast<const T*>(p.a) + r * p.a_row, (unsigned)ring.bytes, bars + s);
+    if (two) bulk_g2s(rows_smem + s * per + ring.bytes, reinterpret_cast<const T*>(p.b) + r * p.b_row, (unsigned)ring.bytes, bars + s);
+  };
+  int asked = 0;   // copies (of thread 0)
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ring.stages; ++s) mbar_init(bars + s, 1);
+    s_late[0] = s_late[1] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    for (; asked < ring.stages && blockIdx.x + (int64_t)asked * gridDim.x < p.rows; ++asked) copy(blockIdx.x + (int64_t)asked * gridDim.x, asked);
+  }
+  Piece g[NORM ? NC : 1];
+  if constexpr (NORM) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (i0 + c * step < p.d) g[c] = *reinterpret_cast<const Piece*>(reinterpret_cast<const T*>(p.gamma) + i0 + c * step);
+  }
+  __syncthreads();
+  int s = 0, turn = 0;
+  unsigned phase = 0;
+  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1) {
+    if (!mbar_wait(bars + s, phase, ring.wait_limit)) s_late[turn] = 1;   // what is read then means nothing
+    const T* a = reinterpret_cast<const T*>(rows_smem + s * per) + i0;
+    const T* b = reinterpret_cast<const T*>(rows_smem + s * per + ring.bytes) + i0;
+    float v[NC][VEC];
+    float sum = 0.0f;
+    float largest = 0.0f;
+    if constexpr (NORM) {
+      T* h = reinterpret_cast<T*>(p.h) + r * p.h_row + i0;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if (i0 + c * step >= p.d) continue;
+        Piece x = *reinterpret_cast<const Piece*>(a + c * step);
+        if (two) {
+          const Piece y = *reinterpret_cast<const Piece*>(b + c * step);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) x.e[e] = from_f<T>(to_f<T>(x.e[e]) + to_f<T>(y.e[e]));
+          *reinterpret_cast<Piece*>(h + c * step) = x;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float f = to_f<T>(x.e[e]);
+          sum = fmaf(f, f, sum);
+          v[c][e] = f * to_f<T>(g[c].e[e]);
+        }
+      }
+    } else {
+      auto apply = [&](auto act) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          if (i0 + c * step >= p.d) continue;
+          const Piece x = *reinterpret_cast<const Piece*>(a + c * step);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[c][e] = int8_act<decltype(act)::value>(to_f<T>(x.e[e]));
+          if (two) {
+            const Piece y = *reinterpret_cast<const Piece*>(b + c * step);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[c][e] *= to_f<T>(y.e[e]);
+          }
+        }
+      };
+      switch (p.act) {
+        case TSB200_ACT_RELU: apply(std::integral_constant<int, TSB200_ACT_RELU>()); break;
+        case TSB200_ACT_SILU: apply(std::integral_constant<int, TSB200_ACT_SILU>()); break;
+        case TSB200_ACT_LEAKYRELU: apply(std::integral_constant<int, TSB200_ACT_LEAKYRELU>()); break;
+        case TSB200_ACT_GELU: apply(std::integral_constant<int, TSB200_ACT_GELU>()); break;
+        case TSB200_ACT_SIGMOID: apply(std::integral_constant<int, TSB200_ACT_SIGMOID>()); break;
+        default: apply(std::integral_constant<int, TSB200_ACT_NONE>()); break;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (i0 + c * step < p.d) largest = int8_top<VEC>(largest, v[c]);
+    const uint32_t top = int8_reduce<false, NORM>(sum, largest, turn);
+    if (*(volatile int*)&s_late[turn]) {
+      // all leave; copies in flight land before the CTA gives its shared memory back (a place whose copy is not there takes no other)
+      if (threadIdx.x == 0) {
+        *ring.error = 1;
+        for (int k = max(0, asked - ring.stages); k < asked; ++k) mbar_wait(bars + k % ring.stages, (unsigned)((k / ring.stages) & 1));
+      }
+      return;
+    }
+    if (threadIdx.x == 0 && r + (int64_t)ring.stages * gridDim.x < p.rows) {
+      copy(r + (int64_t)ring.stages * gridDim.x, s);
+      ++asked;
+    }
+    if (++s == ring.stages) s = 0, phase ^= 1;
+    float up;
+    const float inv = int8_finish<NORM>(p, r, sum, top, threadIdx.x == 0, up);
+    const bool plain = up == 1.0f && inv > 0.0f;
+    int8_t* q = p.q + r * p.q_row + i0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (i0 + c * step >= p.d) continue;
+      if (!plain) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[c][e] = inv > 0.0f ? v[c][e] * up : 0.0f;
+      }
+      if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q + c * step) = make_uint2(int8_pack(v[c], inv), int8_pack(v[c] + 4, inv));
+      else *reinterpret_cast<uint32_t*>(q + c * step) = int8_pack(v[c], inv);
+    }
+  }
+}
+
 template <typename T, int VEC, int NC, bool NORM>
 static int int8_launch(const Int8Rows& p, cudaStream_t s) {
   const int threads = ((p.d + VEC * NC - 1) / (VEC * NC) + 31) / 32 * 32;
-  if (threads == 32) {
-    // a warp per row, eight rows to a CTA
-    const int64_t grid = (p.rows + 7) / 8;
-    int8_rows_kernel<T, VEC, NC, NORM, true><<<(unsigned)grid, dim3(32, 8), 0, s>>>(p);
-  } else {
-    int8_rows_kernel<T, VEC, NC, NORM, false><<<(unsigned)p.rows, threads, 0, s>>>(p);
+  if constexpr (VEC * NC == 8) {
+    if (threads == 32) {   // a warp per row, eight rows to a CTA
+      int8_rows_kernel<T, VEC, NC, NORM, true><<<(unsigned)((p.rows + 7) / 8), dim3(32, 8), 0, s>>>(p);
+      return 1;
+    }
   }
+  int8_rows_kernel<T, VEC, NC, NORM, false><<<(unsigned)p.rows, threads, 0, s>>>(p);
+  return 1;
+}
+
+// ctas: per SM; two rows of each are on their way or being worked on
+template <typename T, int NC, bool NORM>
+static int int8_ring(int device, DeviceState* st, const Int8Rows& p, int threads, int ctas, cudaStream_t s) {
+  static bool done[kMaxDevices] = {};
+  if (!done[device]) {
+    TSB_CUDA(cudaFuncSetAttribute(int8_ring_kernel<T, NC, NORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024));   // (2 rows of 2 x 16384 16-bit elements)
+    done[device] = true;
+  }
+  Int8Ring ring;
+  ring.stages = 2;
+  ring.bytes = p.d * (int)sizeof(T);
+  ring.wait_limit = tc_wait_limit();
+  ring.error = tc_error_word(device);
+  st->waits = true;
+  const int64_t grid = (int64_t)ctas * st->sm_count;
+  int8_ring_kernel<T, NC, NORM><<<(unsigned)(grid < p.rows ? grid : p.rows), threads, 2 * ring.bytes * (p.b ? 2 : 1), s>>>(p, ring);
   return 1;
 }
 
 template <typename T, bool NORM>
-static int int8_rows_t(DeviceState* st, const Int8Rows& p, cudaStream_t s) {
+static int int8_rows_t(int device, DeviceState* st, const Int8Rows& p, cudaStream_t s) {
   constexpr int kWide = 16 / (int)sizeof(T);
   if (p.d > 32768) {
     int8_long_rows_kernel<T, NORM><<<(unsigned)p.rows, 1024, 0, s>>>(p);
@@ -237,6 +395,23 @@ static int int8_rows_t(DeviceState* st, const Int8Rows& p, cudaStream_t s) {
   };
   // elements a thread: 8 where there are few rows (the loads of a row at once), 16 or 32 where a CTA has no more threads
   const int e = p.d <= 8 * 1024 ? 8 : (p.d <= 16 * 1024 ? 16 : 32);
+  if constexpr (sizeof(T) == 2) {
+    // The ring, where it was the faster one (us, ring | a CTA per row): long rows on two CTAs of 512 threads per SM (8192 of 8192, gated silu 51 | 68, 4096 of 11008 37 | 70, norm of
+    // 8192 of 8192 82 | 88); shorter ones with a thread for eight elements (norm of 16384 of 4096 81 | 85), or for 32 where there is one input only
+    // (norm of 16384 of 4096 51 | 64, plain rows of 8192 of 4096 18 | 25).  Not: fp32 (8192 of 4096 74 | 66), two inputs of up to 2048 (16384 of 2048 44 | 44), few rows.
+    const bool many = p.rows > 4 * (int64_t)st->sm_count && fits(kWide) && p.d <= 16384;
+    if (many && p.d > 4096) {
+      return p.d <= 8192 ? int8_ring<T, 2, NORM>(device, st, p, 512, 2, s) : int8_ring<T, 4, NORM>(device, st, p, 512, p.d <= 12288 ? 2 : 1, s);
+    }
+    if (many && !p.b && p.d >= 1024) {
+      const int threads = ((p.d + 31) / 32 + 31) / 32 * 32;
+      return int8_ring<T, 4, NORM>(device, st, p, threads, 8, s);
+    }
+    if (many && p.d > 2048) {
+      const int threads = ((p.d + 7) / 8 + 31) / 32 * 32;
+      return int8_ring<T, 1, NORM>(device, st, p, threads, 1536 / threads, s);
+    }
+  }
   if (fits(kWide)) return e == 8 ? int8_launch<T, kWide, 8 / kWide, NORM>(p, s) : (e == 16 ? int8_launch<T, kWide, 16 / kWide, NORM>(p, s) : int8_launch<T, kWide, 32 / kWide, NORM>(p, s));
   if constexpr (sizeof(T) == 2) {
     if (fits(2)) return e == 8 ? int8_launch<T, 2, 4, NORM>(p, s) : (e == 16 ? int8_launch<T, 2, 8, NORM>(p, s) : int8_launch<T, 2, 16, NORM>(p, s));
@@ -251,9 +426,9 @@ static int int8_rows(int device, int dtype, Int8Rows& p, void* stream) {
   DeviceState* st;
   TSB_TRY(use_device(device, &st));
   cudaStream_t s = pick_stream(st, stream);
-  if (dtype == TSB200_F32) TSB_TRY((int8_rows_t<float, NORM>(st, p, s)));
-  else if (dtype == TSB200_F16) TSB_TRY((int8_rows_t<__half, NORM>(st, p, s)));
-  else TSB_TRY((int8_rows_t<__nv_bfloat16, NORM>(st, p, s)));
+  if (dtype == TSB200_F32) TSB_TRY((int8_rows_t<float, NORM>(device, st, p, s)));
+  else if (dtype == TSB200_F16) TSB_TRY((int8_rows_t<__half, NORM>(device, st, p, s)));
+  else TSB_TRY((int8_rows_t<__nv_bfloat16, NORM>(device, st, p, s)));
   count_launch(device);
   return check_launch(op);
 }

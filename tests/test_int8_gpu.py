@@ -59,6 +59,31 @@ def test_norm(cuda, t, rows, d, residual):
     check_bytes(q, scale, v, root, 0.0, 28 + d / 2048)
 
 
+@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("d", [1024, 2040, 2048, 3016, 4096, 4104, 8192, 8200, 12288, 12296, 16384])
+@pytest.mark.parametrize("two", [True, False])
+def test_many_rows(cuda, t, d, two):
+    """Enough rows for CTAs that walk over several; the sum in place, one row of zeros and one that is not finite among them."""
+    g, rows = gen(d), 1203
+    x, r = randn(g, rows, d, t=t), randn(g, rows, d, t=t, scale=3.0) if two else None
+    x[700] = 0
+    x[1202, d - 1] = float("nan")
+    if two:
+        r[700] = 0
+    gamma = (1 + 0.3 * torch.randn(d, generator=g, device="cuda")).to(t)
+    fine = torch.arange(rows, device="cuda") != 1202
+    want, v, root = norm_exact(x, r, gamma, 1e-5)
+    a = x.clone()
+    q, scale, h = Ops.RMSNormInt8(None, a, r, gamma, 1e-5, sum=a if two else None)
+    assert torch.equal(h[fine], want[fine]) and h is a and scale[700] == 0 and scale[1202].isnan() and (q[[700, 1202]] == 0).all()
+    check_bytes(q[fine], scale[fine], v[fine], root[fine], 0.0, 28 + d / 2048)
+    q, scale = Ops.RowsInt8(None, x, r, N.ACT_LEAKYRELU)
+    v = ACTS[N.ACT_LEAKYRELU](x.double()) * (r.double() if two else 1)
+    check_bytes(q[fine], scale[fine], v[fine], 1.0, 127 * U, 5)
+    assert scale[700] == 0 and scale[1202].isnan() and (q[[700, 1202]] == 0).all()
+    N.call("TSB200_Synchronize", 0, 1)   # no wait has run out
+
+
 @pytest.mark.parametrize("t", [F32, F16, BF16])
 def test_norm_strides_and_places(cuda, t):
     """Rows cut out of wider ones, at odd places; the sum written over either operand; bytes in rows of the caller's."""
@@ -277,6 +302,32 @@ except N.TSB200Error as e:
 N.call("TSB200_Synchronize", 0, 1)
 print("usable", torch.equal(w.flip(1).flip(1), w), float(torch.ones(4, device="cuda").sum()))
 """ % (M, K, n)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                       env=dict(os.environ, TSB200_WAIT_LIMIT="1"))
+    assert r.returncode == 0, r.stderr
+    assert "gave up waiting" in r.stdout and "usable True 4.0" in r.stdout, r.stdout
+
+
+def test_rows_end_in_order_when_a_wait_runs_out(cuda):
+    """The same for rows that come through a ring of copies."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from seq2seqsharp_b200 import _native as N
+from seq2seqsharp_b200.ops import Ops
+x, r = (torch.randn(6000, 16384, device="cuda", dtype=torch.float16) for _ in range(2))
+for i in range(4):
+    Ops.RMSNormInt8(None, x, r, torch.ones(16384, device="cuda", dtype=torch.float16))
+try:
+    N.call("TSB200_Synchronize", 0, 1)
+    print("silent or gave up waiting")   # a poll may take as long as a copy does
+except N.TSB200Error as e:
+    print(e)
+N.call("TSB200_Synchronize", 0, 1)
+print("usable", torch.equal(x.flip(1).flip(1), x), float(torch.ones(4, device="cuda").sum()))
+"""
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                        env=dict(os.environ, TSB200_WAIT_LIMIT="1"))
     assert r.returncode == 0, r.stderr
