@@ -608,8 +608,10 @@ template <typename T, int NR>
 static int i8_cluster(DeviceState* st, int device, EncodeTiledFn enc, I8Args a, cudaStream_t s) {
   constexpr int kStage = kI8W + NR * 128;
   const int groups = (a.N + 127) / 128, steps = (a.K + 127) / 128;
+  // K ranges: as long as every CTA has an SM of its own and four blocks of 128 k; with ten blocks also two CTAs to an SM.  us with 1, 2, 4, 8 ranges: one row of 4096 -> 4096
+  // 6.6, 5.8, 5.3, 6.1; of 2048 -> 2048 5.0, 5.0, 4.2, 4.7; of 768 -> 768 3.9, 4.2; 64 rows of 4096 -> 4096 8.4, 8.5, 7.4, 8.9; of 11008 -> 4096 27, 19, 14.0, 13.5
   a.ks = 1;
-  while (a.ks < 8 && (int64_t)groups * a.ks * 2 <= 2 * st->sm_count && steps / (a.ks * 2) >= 2) a.ks *= 2;
+  while (a.ks < 8 && (((int64_t)groups * a.ks * 2 <= st->sm_count && steps / (a.ks * 2) >= 4) || ((int64_t)groups * a.ks * 2 <= 2 * st->sm_count && steps / (a.ks * 2) >= 10))) a.ks *= 2;
   // rings for two CTAs per SM (one with the whole of it: a cluster of eight no longer fits a GPC twice, and 16 of them make two waves)
   const int sums = a.ks > 1 ? NR * 512 : 0;
   a.stages = (112 * 1024 - 1024 - 512 - sums) / kStage;

@@ -97,7 +97,7 @@ __device__ __forceinline__ float int8_finish(const Int8Rows& p, int64_t r, float
   if (first) {
     float s = mx;
     if constexpr (NORM) s *= 1.0f / sqrtf(sum / (float)p.d + p.eps);
-    p.scale[r] = fine ? s / 127.0f : NAN;
+    p.scale[r] = fine ? (mx > 0.0f ? s / 127.0f : 0.0f) : NAN;   // (eps may be 0)
   }
   return fine && mx > 0.0f ? 127.0f / (mx * up) : 0.0f;
 }

@@ -426,7 +426,9 @@ class Ops:
             res = _matrix(op, dev, dt, "residual", residual, rows, d)
             if sum is None:
                 sum = _new(src, rows, d, dt)
-            at = _written(op, "sum", _matrix(op, dev, dt, "sum", sum, rows, d), rows, d)
+                at = sum.data_ptr(), d
+            else:
+                at = _written(op, "sum", _matrix(op, dev, dt, "sum", sum, rows, d), rows, d)
         elif sum is not None:
             raise N.TSB200Error("RMSNormInt8: sum without a residual")
         else:
@@ -463,14 +465,16 @@ class Ops:
         (rows, K), n = src.shape, weight.shape[0]
         q, w = _matrix(op, dev, torch.int8, "src", src, rows, K), _matrix(op, dev, torch.int8, "weight", weight, n, K)
         sq, sw = _plain(op, dev, _F32, "srcScale", srcScale, rows), _plain(op, dev, _F32, "weightScale", weightScale, n)
-        if result is None:
-            result = _new(src, rows, n, dtype)
-        dt = result.dtype
+        dt = dtype if result is None else result.dtype
         code = _MODEL_DT.get(dt)
         if code is None:
             raise N.TSB200Error("LinearInt8: unsupported result, %s" % dt)
-        y = _written(op, "result", _matrix(op, dev, dt, "result", result, rows, n), rows, n)
         b = None if bias is None else _plain(op, dev, dt, "bias", bias, n)
+        if result is None:
+            result = _new(src, rows, n, dt)
+            y = result.data_ptr(), n
+        else:
+            y = _written(op, "result", _matrix(op, dev, dt, "result", result, rows, n), rows, n)
         N.check(N.lib().TSB200_LinearInt8(dev, code, *y, *q, sq, *w, sw, b, rows, K, n, _queue(dev)), "TSB200_LinearInt8")
         return result
 

@@ -412,3 +412,60 @@ def test_captured_block_with_other_inputs(cuda, rows):
         if k:
             for dst, src in zip((x, stream, tokens), keep):
                 dst.copy_(src)
+
+
+def test_first_calls_of_a_process_may_be_captured(cuda):
+    """What the library asks the driver for once (entry points, attributes of kernels) can be asked for while a stream is captured."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch
+from seq2seqsharp_b200 import _native as N
+from seq2seqsharp_b200.ops import Ops
+g, out = torch.cuda.CUDAGraph(), {}
+x = torch.randn(700, 4096, device="cuda", dtype=torch.float16)
+gain, w, sw = torch.ones(4096, device="cuda", dtype=torch.float16), torch.randint(-9, 9, (512, 4096), device="cuda", dtype=torch.int8), torch.ones(512, device="cuda")
+tokens = torch.zeros(700, device="cuda", dtype=torch.int32)
+def run(rows):
+    q, s, h = Ops.RMSNormInt8(None, x[:rows], x[:rows], gain)
+    y = Ops.LinearInt8(None, q, s, w, sw, dtype=torch.float32)
+    return (q, s, h, y, *Ops.TokenLogProbs(y, tokens[:rows], 3))
+torch.cuda.synchronize()
+with torch.cuda.graph(g):
+    for rows in (1, 20, 50, 700):
+        out[rows] = run(rows)
+g.replay()
+torch.cuda.synchronize()
+print(all(torch.equal(a, b) for rows in out for a, b in zip(out[rows], run(rows))))
+N.call("TSB200_Synchronize", 0, 1)
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and r.stdout.strip() == "True", r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_two_linears_at_once(cuda, M):
+    """Two streams, no order between them: the calls share nothing."""
+    g = gen(M)
+    sets = [(bytes_of(g, M, 2048), scales(g, M), bytes_of(g, 4096, 2048), scales(g, 4096)) for _ in range(2)]
+    want = [Ops.LinearInt8(None, *s, dtype=F32) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(Ops.LinearInt8(None, *sets[k], dtype=F32))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(v, want[k]) for v in got[k])
+    N.call("TSB200_Synchronize", 0, 1)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+def test_norm_without_eps(cuda, t):
+    x = torch.zeros(3, 40, device="cuda", dtype=t)
+    x[1] = 2
+    q, scale, _ = Ops.RMSNormInt8(None, x, None, torch.ones(40, device="cuda", dtype=t), 0.0)
+    assert scale.tolist() == [0.0, float(np.float32(1) / np.float32(127)), 0.0] and (q[1] == 127).all() and (q[[0, 2]] == 0).all()
