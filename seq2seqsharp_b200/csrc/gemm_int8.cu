@@ -100,6 +100,8 @@ constexpr uint32_t i8_idesc(int m, int n) { return (2u << 4) | (1u << 7) | (1u <
 // A CTA owns 128 channels over a range of K; the 1 .. 8 CTAs of a cluster share the channels and push their sums, four rows at a time, into the shared
 // memory of the CTA that finishes them (1 / ks of the channels each); the stores report to its mbarrier.
 // warp 0: copies; warp 1: TMEM and products; warps 2-5: accumulators out of TMEM; all warps: sums and outputs.
+// What bounds it: the bytes of the weights (one row of 4096 -> 22016 16.7 us, 5.4 TB/s) and, in the small ones, start, first copies, exchange and end of the launch (one row of 4096 -> 4096
+// 5.3 us, of 768 -> 768 3.9; 64 rows of 11008 -> 4096 13.6).  The first round of copies is under way before TMEM is allotted and the warps have met (17.5 -> 16.8 us for the first of these).
 constexpr int kI8Threads = 256;
 constexpr int kI8W = 128 * 128;   // weight bytes of a stage
 
@@ -302,6 +304,10 @@ __global__ void __launch_bounds__(kI8Threads) i8_cluster_kernel(const __grid_con
 // memory, the leader issues the products of both, each CTA's TMEM receives its own 128 rows.  Persistent; the accumulator is double buffered, so that a tile's
 // outputs leave while the products of the next are running and the copies run ahead across tiles.
 // Warp 0: copies; warp 1: TMEM and products; warps 2..9: outputs (two per quarter of the TMEM lanes, each half of a tile's channels).
+// What bounds it: the tensor pipe and from a few waves on the power limit (8192 x 4096 -> 22016 443 to 470 us, up to 3330 TOP/s; 4096 x 4096 -> 32000 3150); with few k the outputs (8192 x 512 -> 4096
+// 26 us, where the products take 9).  An output warp finishes a row of sums in its lane, in straight code: with edges and biases decided per chunk it fetched more instructions than it
+// executed (51 us for the last of these), and sums that cross shared memory as integers, to be finished by columns, took 34.  Scales and biases of a tile's channels lie in the warp's shared
+// memory, read for the next tile while this one leaves; boxes of 32 x 32 outputs go out by TMA, two in turn.
 constexpr int kI8PThreads = 320, kI8PWarps = 8;
 constexpr int kI8A = 128 * 128;
 template <typename T, int BN>

@@ -80,17 +80,17 @@ __device__ __forceinline__ bool elect_one() {
 }
 __device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr, uint32_t lbo_bytes) { return ((smem_addr >> 4) & 0x3FFF) | ((lbo_bytes >> 4) << 16); }
 __device__ __forceinline__ uint32_t desc_hi(uint32_t sbo_bytes) { return (sbo_bytes >> 4) | (1u << 14) | (2u << 29); }
-#define TSB_ELECTED_MMA(NAME, GROUP, KIND)                                                                                                      \
-  __device__ __forceinline__ void NAME(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,       \
-                                       uint32_t accumulate) {                                                                               \
-    asm volatile(                                                                                                                           \
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"                                                                                    \
-        "elect.sync _|q, 0xffffffff;\n\t"                                                                                                  \
-        "setp.ne.b32 p, %6, 0;\n\t"                                                                                                        \
-        "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"                                                                              \
-        "@q tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], da, db, %5, p;\n\t}" ::"r"(tmem_d),                                           \
-        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)                                                             \
-        : "memory");                                                                                                                        \
+#define TSB_ELECTED_MMA(NAME, GROUP, KIND)                                                                                          \
+  __device__ __forceinline__ void NAME(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, \
+                                       uint32_t accumulate) {                                                                       \
+    asm volatile(                                                                                                                   \
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"                                                                            \
+        "elect.sync _|q, 0xffffffff;\n\t"                                                                                           \
+        "setp.ne.b32 p, %6, 0;\n\t"                                                                                                 \
+        "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"                                                                        \
+        "@q tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], da, db, %5, p;\n\t}" ::"r"(tmem_d),                               \
+        "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)                                                     \
+        : "memory");                                                                                                                \
   }
 TSB_ELECTED_MMA(umma_el, "1", "f16")
 TSB_ELECTED_MMA(umma_pair_el, "2", "f16")
