@@ -232,7 +232,8 @@ struct LpWhole {
   }
 };
 
-template <typename T, int kLpThreads>
+// kTrack: several alternatives; which piece a thread's maximum lies in is kept
+template <typename T, int kLpThreads, bool kTrack>
 __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kernel(LogProbArgs a) {
   constexpr int kLpWarps = kLpThreads / 32;
   __shared__ LpJoined s_join[kLpWarps];
@@ -287,6 +288,8 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
   };
 
   LpSums mine{-INFINITY, 0.0f, 0.0f};
+  int highest = -1;            // the piece of the maximum (-1: an end's, or none)
+  float second = -INFINITY;    // the largest of what is not in it
   auto add = [&](float y, float m, float ref) {   // -infinity, and products that leave fp32, too
     const float d = lp_max_nan(lp_far(m) ? (y - m) * kLog2e : fmaf(y, kLog2e, -ref), -1000.0f), p = lp_exp2(d);
     mine.s += p;
@@ -305,7 +308,28 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
     for (int u = 0; u < kLpUnroll; ++u)
       if (kAll || v + u * kLpThreads < v1) largest.add(x[u]);
     const float top = largest.get();
-    if (top > mine.m) mine.raise(top);
+    if (top > mine.m) {
+      if constexpr (kTrack) {   // rarely
+        bool found = false;
+        second = mine.m;
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u) {
+          if (!kAll && v + u * kLpThreads >= v1) break;
+          LpLargest<T> one;
+          one.add(x[u]);
+          const float y = one.get();
+          if (!found && y == top) {
+            found = true;
+            highest = v + u * kLpThreads;
+          } else {
+            second = fmaxf(second, y);
+          }
+        }
+      }
+      mine.raise(top);
+    } else if constexpr (kTrack) {
+      second = fmaxf(second, top);
+    }
     const float m = mine.m > -INFINITY ? mine.m : 0.0f, ref = __fmul_rn(m, kLog2e);   // nothing but -infinity (and NaN) yet: sums of 0 (of NaN)
     // two at a time
     const uint64_t scale = lp_two(kLog2e, kLog2e), minus = lp_two(-ref, -ref);
@@ -385,34 +409,45 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
       bound = __shfl_sync(0xffffffffu, o, __ffs(__ballot_sync(0xffffffffu, larger == warps - 1)) - 1);
       if (bound <= lp_order(-INFINITY)) bound = 0u;   // threads without a number have this maximum too: every word counts
     }
-    // every element that is not below least_x, in the shares of the warp's lanes with `any`: f(key).  The warp reads them together.
+    // f(key) of every element of piece `at` that is not below least_x.  Little code, one element at a time: there are few such pieces.
+    auto each_of = [&](int at, float least_x, auto f) {
+      const int j0 = row.first(at);
+#pragma unroll 1
+      for (int j = j0; j < j0 + N; ++j) {
+        const float z = to_f<T>(row.x[j]);
+        if (!(z < least_x)) f(lp_key(z, j));
+      }
+    };
+    // The same of the whole shares of the warp's lanes with `any`, which the warp reads together, and of the ends.
     auto look = [&](bool any, float least_x, auto f) {
       const uint32_t lanes = __ballot_sync(0xffffffffu, any);
       if (any) s_lane[w][__popc(lanes & ((1u << lane) - 1u))] = (uint8_t)lane;
       __syncwarp();
       const int first = v0 + w * 32, each = v1 > first ? (v1 - first + kLpThreads - 1) / kLpThreads : 0, items = __popc(lanes) * each;   // (pieces of the first lane, the most)
+      auto piece = [&](int k) {
+        const int of = k / each;
+        return first + (int)s_lane[w][of] + (k - of * each) * kLpThreads;
+      };
+#pragma unroll 1
       for (int i = lane; i < items; i += 32 * kLpUnroll) {
         LpVec<T> y[kLpUnroll];
-        int at[kLpUnroll];
+        uint32_t hits = 0u;
 #pragma unroll
         for (int u = 0; u < kLpUnroll; ++u) {
-          const int k = i + 32 * u, of = k / each;
-          at[u] = k < items ? first + (int)s_lane[w][of] + (k - of * each) * kLpThreads : v1;
-          if (at[u] < v1) y[u] = row.load(at[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u) {
-          if (at[u] >= v1) continue;
-          LpLargest<T> largest;
-          largest.add(y[u]);
-          if (largest.get() < least_x) continue;
-          const int j0 = row.first(at[u]);
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float z = y[u].get(e);
-            if (!(z < least_x)) f(lp_key(z, j0 + e));
+          const int k = i + 32 * u, at = k < items ? piece(k) : v1;
+          if (at < v1) {
+            y[u] = row.load(at);
+            hits |= 1u << u;
           }
         }
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u) {
+          LpLargest<T> largest;
+          largest.add(y[u]);
+          if (largest.get() < least_x) hits &= ~(1u << u);
+        }
+#pragma unroll 1
+        for (; hits; hits &= hits - 1u) each_of(piece(i + 32 * (__ffs(hits) - 1)), least_x, f);
       }
       if (end_j >= 0) f(lp_key(end_x, end_j));
       __syncwarp();
@@ -423,9 +458,38 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
       const int at = atomicAdd(&s_count, 1);
       if (at < kLpRoom) s_words[at] = k;
     };
-    look(mine_o >= bound, bound ? lp_value(bound) : -INFINITY, take);
-    __syncthreads();
-    if (s_count > kLpRoom) {
+    // Most threads above the bound have one piece that is: the others' shares alone are read again as a whole.  (Pieces lie kLpThreads apart, so that a share's are as many trips to
+    // memory where L2 has let go of the row: 4096 rows of 50257 bf16, 20 alternatives 134 us when all of them read theirs.)
+    const float bound_x = lp_value(bound);
+    if (bound != 0u) {
+      const bool whole_share = kTrack ? lp_order(second) >= bound : mine_o >= bound;
+      if (!whole_share && mine_o >= bound && highest >= 0) each_of(highest, bound_x, take);
+      look(whole_share, bound_x, take);
+      __syncthreads();
+    } else {
+      // nearly all words are -infinity, or the share is short: what is larger, then, by index, as many of those as are wanted
+      least = (uint64_t)(lp_order(-INFINITY) + 1u) << 32;
+      look(true, -3.402823466e38f, take);
+      __syncthreads();
+      auto take_none = [&](uint64_t k) {
+        if ((uint32_t)(k >> 32) == lp_order(-INFINITY)) s_words[atomicAdd(&s_count, 1)] = k;
+      };
+      int have = s_count;
+      if (have < top) {
+        constexpr int kSome = kLpRoom / 16;   // pieces: of at most half the room
+        for (int from_v = v0; from_v < v1 && have < top; from_v += kSome) {
+          __syncthreads();   // (all have read the count)
+          if (tid < kSome && from_v + tid < v1) each_of(from_v + tid, -INFINITY, take_none);
+          __syncthreads();
+          have = s_count;
+        }
+        __syncthreads();
+        if (end_j >= 0) take_none(lp_key(end_x, end_j));
+        __syncthreads();
+      }
+    }
+    // too many of them, or NaN among the words that are wanted
+    if (s_count > kLpRoom || s_count < min(top, (v1 - v0) * N + (part == 0 ? row.head + row.tail : 0))) {
       // the top-th largest key, eight bits at a time
       if (tid == 0) {
         s_prefix = 0u;
@@ -436,7 +500,15 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
         __syncthreads();
         const uint64_t prefix = s_prefix;
         look(true, -INFINITY, [&](uint64_t k) {
-          if (shift == 56 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(k >> shift) & 255], 1u);
+          if (shift == 56 || (k >> (shift + 8)) == (prefix >> (shift + 8))) {
+            // most often the lanes that are here have the same digit: one of them counts for all
+            const int d = (int)((k >> shift) & 255);
+            const uint32_t here = __activemask();
+            int same;
+            __match_all_sync(here, d, &same);
+            if (!same) atomicAdd(&s_hist[d], 1u);
+            else if (lane == __ffs(here) - 1) atomicAdd(&s_hist[d], (uint32_t)__popc(here));
+          }
         });
         __syncthreads();
         if (tid == 0) {
@@ -547,7 +619,9 @@ static int log_probs_launch(LogProbArgs a, int64_t rows, int sms, cudaStream_t s
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  TSB_CUDA(cudaLaunchKernelEx(&cfg, wide ? log_probs_kernel<T, 512> : narrow ? log_probs_kernel<T, 128> : log_probs_kernel<T, 256>, a));
+  auto k = a.top > 1 ? (wide ? log_probs_kernel<T, 512, true> : narrow ? log_probs_kernel<T, 128, true> : log_probs_kernel<T, 256, true>)
+                     : (wide ? log_probs_kernel<T, 512, false> : narrow ? log_probs_kernel<T, 128, false> : log_probs_kernel<T, 256, false>);
+  TSB_CUDA(cudaLaunchKernelEx(&cfg, k, a));
   return 1;
 }
 

@@ -93,6 +93,30 @@ def test_masked_words(cuda, t, rows, V, low):
         check(y, torch.full_like(tok, keep.start), 1)
 
 
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("rows,V", [(1, 50257), (40, 9000), (300, 1500)])
+def test_fewer_words_than_alternatives(cuda, t, rows, V):
+    """Alternatives that cannot come follow by index, those at the row's ends and behind its last piece too; a NaN comes after them."""
+    x, tok = rows_of(11, rows, V + 1, t)
+    for off in (0, 1):
+        z = x[:, off: off + V]
+        for keep in ([], [3, V // 2], list(range(0, 10)), [V - 1, V - 2], list(range(31)), list(range(0, V, V // 33))[:33]):
+            y = torch.full_like(z, -float("inf"))
+            y[:, keep] = z[:, keep]
+            if keep:
+                check(y, torch.full_like(tok, keep[0]), 32)
+            order = torch.sort(y.float(), dim=1, descending=True, stable=True).indices[:, :32].int()
+            wide = torch.empty(rows, V + 1, dtype=t, device="cuda")
+            wide[:, off: off + V] = y
+            got = Ops.TokenLogProbs(wide[:, off: off + V], tok, 32)
+            assert torch.equal(got[3], order)
+    y = torch.full((rows, V), float("nan"), dtype=t, device="cuda")
+    y[:, V - 3] = 1
+    y[:, 5] = -float("inf")
+    ids = Ops.TokenLogProbs(y, tok, 4)[3]
+    assert (ids == torch.tensor([V - 3, 5, 0, 1], dtype=torch.int32, device="cuda")).all()
+
+
 @pytest.mark.parametrize("t", [F32, F16, BF16])
 def test_rows_of_the_lowest_value_are_uniform(cuda, t):
     for rows, V in ((1, 32000), (200, 1000)):
