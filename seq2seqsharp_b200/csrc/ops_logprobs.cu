@@ -5,8 +5,11 @@
 // One pass over the logits.  A thread keeps a running maximum and both sums of its share in fp32, with powers of two (x log2 e is taken against the rounded m log2 e, any
 // reference being as good as the maximum itself); what threads have is joined in 64 bits, so that a probability near 1 keeps its digits (log S of a sum a little over 1).
 // The threads' maxima are also a bound for the alternatives: where r = ceil(top / warps) lanes of ceil(top / r) warps have a logit of at least B, `top` words have, and only threads
-// whose maximum is at least B look through their share again, in L2.  What they find (some 50 words for random logits) is ordered by counting.  Should that be over
-// kLpRoom (many equal logits, nearly all of them -infinity), the bound is raised to the top-th largest (logit, index) by eight histograms of eight bits.
+// whose maximum is at least B have one, nearly always in the piece of their maximum alone, which is read again.  What they find (some 40 words for random logits) is ordered by counting.
+// Should that be over kLpRoom (many equal logits), the bound is raised to the top-th largest (logit, index) by eight histograms of eight bits.
+//
+// What bounds it: issue slots, about ten instructions a 16-bit logit (28.7 before two at a time, counts in the type's own numbers and rows' ends apart: 4096 rows of 50257 bf16 327 us, now 86, floor 63),
+// and bytes; for few rows two dependent reads, the words' second look and a cluster barrier (one row of 32000 fp32, 5 alternatives 6.6 us).
 //
 // Few rows: a cluster of up to eight CTAs shares a row, and the first one joins what all have pushed to it.  Many rows: a CTA per row.
 #include <cmath>
@@ -603,11 +606,11 @@ static int log_probs_launch(LogProbArgs a, int64_t rows, int sms, cudaStream_t s
   const int pieces = (a.V + LpVec<T>::N - 1) / LpVec<T>::N;
   a.parts = 1;
   while (a.parts < kLpCluster && rows * a.parts * 2 <= 4 * sms && pieces / (a.parts * 2) >= 256) a.parts *= 2;
-  // Threads of a CTA: 512 where CTAs are fewer than SMs (8 rows of 131072 fp32, 20 alternatives: 11.1 us against 15.2 with 256); 128 for short rows, and where
-  // there are several waves of eight CTAs per SM and few alternatives, so that a row's end, where most threads wait, holds up fewer of them (us, 128 | 256: 4096 rows of 2000 bf16,
-  // 5 alternatives 23 | 36, of 32000 fp16, 1: 62 | 70, of 50257 bf16, 1: 87 | 94, 20: 147 | 133; 1200 rows of 50257, 5: 44 | 38).
+  // Threads of a CTA: 512 where CTAs are fewer than SMs (8 rows of 131072 fp32, 20 alternatives: 11.1 us against 15.2 with 256); 128 for rows that are short, or not too long and many, so that
+  // a row's end, where most threads wait, holds up fewer of them (us, 128 | 256: 4096 rows of 2000 fp16, 1 alternative 23 | 38, of 8000 bf16 33 | 49, of 50257 85 | 96, with 20: 110 | 120;
+  // 700 rows of 32000 fp32 22 | 27; 760 of 131072 bf16 52 | 48).
   const bool wide = rows * a.parts <= sms && pieces / a.parts >= 512;
-  const bool narrow = a.parts == 1 && (pieces < 1024 || (a.top <= 8 && pieces <= 8192 && rows >= 24 * (int64_t)sms));
+  const bool narrow = a.parts == 1 && (pieces < 1024 || (pieces <= 8192 && rows >= 4 * (int64_t)sms));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * a.parts));
   cfg.blockDim = dim3(wide ? 512 : narrow ? 128 : 256);
