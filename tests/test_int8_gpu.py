@@ -309,7 +309,7 @@ print("usable", torch.equal(w.flip(1).flip(1), w), float(torch.ones(4, device="c
 
 
 def test_rows_end_in_order_when_a_wait_runs_out(cuda):
-    """The same for rows that come through a ring of copies."""
+    """The same for rows that come through a ring of copies.  A copy is short enough for the one poll to see it at times: then nothing is reported, and the outputs are right."""
     import os
     import subprocess
     import sys
@@ -318,11 +318,11 @@ import torch
 from seq2seqsharp_b200 import _native as N
 from seq2seqsharp_b200.ops import Ops
 x, r = (torch.randn(6000, 16384, device="cuda", dtype=torch.float16) for _ in range(2))
-for i in range(4):
-    Ops.RMSNormInt8(None, x, r, torch.ones(16384, device="cuda", dtype=torch.float16))
+gain = torch.ones(16384, device="cuda", dtype=torch.float16)
+got = [Ops.RMSNormInt8(None, x, r, gain) for i in range(4)]
 try:
     N.call("TSB200_Synchronize", 0, 1)
-    print("silent or gave up waiting")   # a poll may take as long as a copy does
+    print("right", all(torch.equal(h, x + r) for _, _, h in got))
 except N.TSB200Error as e:
     print(e)
 N.call("TSB200_Synchronize", 0, 1)
@@ -331,7 +331,7 @@ print("usable", torch.equal(x.flip(1).flip(1), x), float(torch.ones(4, device="c
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                        env=dict(os.environ, TSB200_WAIT_LIMIT="1"))
     assert r.returncode == 0, r.stderr
-    assert "gave up waiting" in r.stdout and "usable True 4.0" in r.stdout, r.stdout
+    assert ("gave up waiting" in r.stdout or "right True" in r.stdout) and "usable True 4.0" in r.stdout, r.stdout
 
 
 # ---------------------------------------------------------------------------------------------------------------------------- together
