@@ -160,14 +160,14 @@ struct LpRow {
   }
 };
 
-// Exponents are taken as x log2 e - m log2 e with the second product rounded, one instruction a logit; from 2e38 on (a mask of the type's lowest value, over a whole
-// share) these products leave fp32 and the difference comes first.
-__device__ __forceinline__ bool lp_far(float m) { return !(fabsf(m) < 2e38f); }
-// exponent of 2 between two maxima, at most 0; 2^-1000 is 0, and so is its product with the exponent
-__device__ __forceinline__ float lp_gap(float m, float to) {
-  const float d = lp_far(m) || lp_far(to) ? __fmul_rn(m - to, kLog2e) : __fsub_rn(__fmul_rn(m, kLog2e), __fmul_rn(to, kLog2e));
-  return lp_max_nan(d, -1000.0f);
-}
+// Exponents are taken as x log2 e - m log2 e with the second product rounded, one instruction a logit.  What that product's rounding leaves is an exponent that all logits of
+// a share have more: below 2^20 at most a sixteenth, but whole powers where a step of m log2 e is no longer small (440 at -1e10, so that sums of words masked by that are infinite).  From
+// 2^20 on, and for infinities, the difference comes first.
+__device__ __forceinline__ bool lp_far(float m) { return !(fabsf(m) < 0x1p20f); }
+// what the rounding of m log2 e leaves, exact (a product and its rounding differ by a number of fp32)
+__device__ __forceinline__ float lp_left(float m) { return lp_far(m) ? 0.0f : fmaf(m, kLog2e, -__fmul_rn(m, kLog2e)); }
+// exponent of 2 between two maxima, at most 0, as their sums have them; 2^-1000 is 0, and so is its product with the exponent
+__device__ __forceinline__ float lp_gap(float m, float to) { return lp_max_nan(fmaf(m - to, kLog2e, lp_left(to) - lp_left(m)), -1000.0f); }
 struct LpSums {
   float m, s, t;   // maximum; sums, over the logits, of 2^exponent and of the exponent times it
   __device__ __forceinline__ void raise(float to) {   // to > m
@@ -219,9 +219,9 @@ struct LpWhole {
   __device__ __forceinline__ LpWhole() {}
   __device__ __forceinline__ explicit LpWhole(LpJoined c) : m(c.m), rank(c.rank) {
     const bool none = !(m > -INFINITY);   // nothing but -infinity and NaN
-    if (!none && !lp_far(m) && c.s < 1.5) {
+    if (!none && c.s < 1.5) {
       // The maximum's own exponent is what rounding left of it, and its power of two is off by 2 ulp of 1: as much as all other words have where it is nearly certain
-      const float own = fmaf(m, kLog2e, -__fmul_rn(m, kLog2e));
+      const float own = lp_left(m);
       c.s += exp2((double)own) - (double)lp_exp2(own);
     }
     log_s = none ? (double)NAN : log(c.s);
@@ -359,7 +359,8 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
       mine.s += s.x + s.y;
       mine.t += t.x + t.y;
     } else {
-      // an exponent of -infinity is among them (0 times it is none), or a NaN
+      // the difference first; or an exponent of -infinity is among them (0 times it is none), or a NaN.  (1024 rows of 50257 bf16, all but ten words at -1e10 or -infinity 47 us, at -1e4
+      // 28; the differences taken by a second copy of the loop above, 38, cost other calls registers: 2048 rows of 50257 fp32, 20 alternatives 87 -> 90.)
 #pragma unroll 1
       for (int u = 0; u < kLpUnroll && v + u * kLpThreads < v1; ++u) {
         const LpVec<T> y = row.load(v + u * kLpThreads);
