@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(512, NC == 1 ? 3 : 2) int8_ring_kernel(Int8Row
     if (*(volatile int*)&s_late[turn]) {
       // all leave; copies in flight land before the CTA gives its shared memory back (a place whose copy is not there takes no other)
       if (threadIdx.x == 0) {
-        *ring.error = 1;
+        if (ring.error) *ring.error = 1;
         for (int k = max(0, asked - ring.stages); k < asked; ++k) mbar_wait(bars + k % ring.stages, (unsigned)((k / ring.stages) & 1));
       }
       return;
