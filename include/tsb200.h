@@ -295,7 +295,8 @@ TSB200_API int TSB200_VerifyDraft(int device, int32_t* tokens, int32_t* counts, 
  *
  * RMSNormInt8: h = x + residual, rounded to dtype and written (residual and h both null: h = x, nothing is written; h may be x or residual itself);
  * y = h / sqrt(mean(h^2) + eps) * gamma; scale = max|y| / 127 (0 for a row of zeros), q = y / scale rounded to nearest, half to even.  The bytes do not
- * depend on how many rows there are.  A row that leaves fp32 (infinities, NaN, squares beyond 3e38) has the scale NaN and bytes of 0. */
+ * depend on how many rows there are.  A row that leaves fp32 upwards (infinities, NaN, squares beyond 3e38) has the scale NaN and bytes of 0; one that leaves it downwards (squares below 1e-38) has
+ * the scale and bytes of its values, with an eps of 0 too.  eps is at least 0. */
 TSB200_API int TSB200_RMSNormInt8(int device, int dtype, void* q, int64_t q_row, float* scale, void* h, int64_t h_row, const void* x, int64_t x_row,
                                   const void* residual, int64_t residual_row, const void* gamma, float eps, int64_t rows, int d, void* stream);
 /* RowsInt8: v = act(src) [* gate], gate may be null; scale and q of v as above.  act: TSB200_ACT_NONE .. TSB200_ACT_SIGMOID (GLU_NOACT is NONE, SWIGLU is SILU).  With

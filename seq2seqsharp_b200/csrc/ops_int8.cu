@@ -68,7 +68,7 @@ __device__ __forceinline__ float int8_top(float top, const float* v) {
 }
 // sum of squares (of a norm) and maximum (as bits: those of a NaN are larger than all) over the threads of a row: a warp, or the CTA
 // (turn: 0 and 1 in alternation where a CTA has several rows, so that one barrier a row is enough)
-template <bool WARP, bool NORM>
+template <bool WARP, int NORM>
 __device__ __forceinline__ uint32_t int8_reduce(float& sum, float largest, int turn = 0) {
   uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest) & 0x7fffffffu);
   if constexpr (NORM) sum = warp_sum(sum);
@@ -89,7 +89,7 @@ __device__ __forceinline__ uint32_t int8_reduce(float& sum, float largest, int t
 
 // What a row's statistics make of it: the factor of v, and the scale (written by one thread).  `up`: a power of two that v is multiplied by first, so that 127 / max|v|
 // stays below infinity where the row is nearly zero.
-template <bool NORM>
+template <int NORM>
 __device__ __forceinline__ float int8_finish(const Int8Rows& p, int64_t r, float sum, uint32_t top, bool first, float& up) {
   const float mx = __uint_as_float(top);
   const bool fine = top < 0x7f800000u && (!NORM || sum < INFINITY);   // (a NaN is not below)
@@ -102,7 +102,56 @@ __device__ __forceinline__ float int8_finish(const Int8Rows& p, int64_t r, float
   return fine && mx > 0.0f ? 127.0f / (mx * up) : 0.0f;
 }
 
-template <typename T, int VEC, int NC, bool NORM, bool WARP>
+// Norms with an eps below 2^-100 (NORM 2; 1: the others).  A result is of ordinary size then however small its row is, but squares vanish below 1e-23 and have few digits above, and
+// products with the gain below 1e-38.  Such rows are taken again, in 64 bits, by the threads that wrote them: the scale where the mean of the squares is below 2^-100, the bytes too where
+// max|v| is, so that bytes do not depend on the order of a sum.  With a larger eps squares that vanish are nothing beside it, and what a product's last step of 2^-149 makes of the result is
+// below 2^-99.  Kernels of their own: in the ones for every eps this cost 81 -> 87 us (16384 rows of 4096 bf16) and 32 -> 41 (16000 of 1001) in registers and issue slots.
+constexpr float kInt8Small = 0x1p-100f;
+template <typename T, bool WARP>
+__device__ __noinline__ void int8_small_row(const T* h, const T* gamma, int8_t* q, float* scale, int d, float eps, bool bytes) {
+  if constexpr (WARP) __syncwarp();
+  else __syncthreads();   // the row's sums and first bytes are written
+  const int i0 = threadIdx.x, step = WARP ? 32 : (int)blockDim.x;
+  double sum = 0.0, top = 0.0;
+  for (int i = i0; i < d; i += step) {
+    const double x = (double)to_f<T>(h[i]);
+    sum = fma(x, x, sum);
+    top = fmax(top, fabs(x * (double)to_f<T>(gamma[i])));   // (exact)
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if constexpr (!WARP) {
+    __shared__ double s_sum[32], s_top[32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (lane == 0) {
+      s_sum[w] = sum;
+      s_top[w] = top;
+    }
+    __syncthreads();
+    sum = top = 0.0;
+    for (int i = 0; i < warps; ++i) {
+      sum += s_sum[i];
+      top = fmax(top, s_top[i]);
+    }
+    __syncthreads();   // the CTA's next row may come here
+  }
+  if (threadIdx.x == 0) *scale = top > 0.0 ? (float)(top / (127.0 * sqrt(sum / d + (double)eps))) : 0.0f;
+  if (!bytes) return;
+  const double inv = top > 0.0 ? 127.0 / top : 0.0;
+  for (int i = i0; i < d; i += step) q[i] = (int8_t)__double2int_rn((double)to_f<T>(h[i]) * (double)to_f<T>(gamma[i]) * inv);
+}
+// 0: the row is fine, 1: its scale, 2: its bytes too (all threads of a row have the same sum and maximum)
+__device__ __forceinline__ int int8_small(const Int8Rows& p, float sum, uint32_t top) { return __uint_as_float(top) < kInt8Small ? 2 : sum < kInt8Small * (float)p.d ? 1 : 0; }
+template <typename T, bool WARP>
+__device__ __forceinline__ void int8_small_row(const Int8Rows& p, int64_t r, int what) {
+  int8_small_row<T, WARP>(reinterpret_cast<const T*>(p.b ? p.h : p.a) + r * (p.b ? p.h_row : p.a_row), reinterpret_cast<const T*>(p.gamma), p.q + r * p.q_row, p.scale + r, p.d, p.eps,
+                          what == 2);
+}
+
+template <typename T, int VEC, int NC, int NORM, bool WARP>
 __global__ void __launch_bounds__(1024) int8_rows_kernel(Int8Rows p) {
   const int64_t r = WARP ? (int64_t)blockIdx.x * blockDim.y + threadIdx.y : (int64_t)blockIdx.x;
   if (r >= p.rows) return;   // (whole warps)
@@ -184,10 +233,13 @@ __global__ void __launch_bounds__(1024) int8_rows_kernel(Int8Rows p) {
     else if constexpr (VEC == 2) *reinterpret_cast<uint16_t*>(q + i) = (uint16_t)__byte_perm(int8_low(v[c][0], inv), int8_low(v[c][1], inv), 0x0040);
     else q[i] = (int8_t)int8_low(v[c][0], inv);
   }
+  if constexpr (NORM == 2) {
+    if (const int what = int8_small(p, sum, top)) int8_small_row<T, WARP>(p, r, what);
+  }
 }
 
 // Rows of more than 32768 elements: read twice, the second time out of L2 (an element by the thread that wrote its sum)
-template <typename T, bool NORM>
+template <typename T, int NORM>
 __global__ void __launch_bounds__(1024) int8_long_rows_kernel(Int8Rows p) {
   const int64_t r = blockIdx.x;
   const T* a = reinterpret_cast<const T*>(p.a) + r * p.a_row;
@@ -225,6 +277,9 @@ __global__ void __launch_bounds__(1024) int8_long_rows_kernel(Int8Rows p) {
     else v = value(i);
     p.q[r * p.q_row + i] = inv == 0.0f ? (int8_t)0 : (int8_t)int8_low(v * up, inv);
   }
+  if constexpr (NORM == 2) {
+    if (const int what = int8_small(p, sum, top)) int8_small_row<T, false>(p, r, what);
+  }
 }
 
 // Many rows that start on 16 bytes: CTAs walk over rows, whose inputs a ring of bulk copies brings into shared memory several rows ahead.  All threads have read a row when its
@@ -234,7 +289,7 @@ struct Int8Ring {
   unsigned wait_limit;
   int* error;
 };
-template <typename T, int NC, bool NORM>
+template <typename T, int NC, int NORM>
 __global__ void __launch_bounds__(512, NC == 1 ? 3 : 2) int8_ring_kernel(Int8Rows p, Int8Ring ring) {
   constexpr int VEC = 16 / (int)sizeof(T);
   typedef Int8Piece<T, VEC> Piece;
@@ -265,6 +320,7 @@ __global__ void __launch_bounds__(512, NC == 1 ? 3 : 2) int8_ring_kernel(Int8Row
   __syncthreads();
   int s = 0, turn = 0;
   unsigned phase = 0;
+  bool small = false;   // rows of the CTA have to be taken again
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x, turn ^= 1) {
     if (!mbar_wait(bars + s, phase, ring.wait_limit)) s_late[turn] = 1;   // what is read then means nothing
     const T* a = reinterpret_cast<const T*>(rows_smem + s * per) + i0;
@@ -346,10 +402,23 @@ __global__ void __launch_bounds__(512, NC == 1 ? 3 : 2) int8_ring_kernel(Int8Row
       if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q + c * step) = make_uint2(int8_pack(v[c], inv), int8_pack(v[c] + 4, inv));
       else *reinterpret_cast<uint32_t*>(q + c * step) = int8_pack(v[c], inv);
     }
+    if constexpr (NORM == 2) {
+      if (const int what = int8_small(p, sum, top)) {
+        small = true;
+        if (threadIdx.x == 0) p.scale[r] = (float)-what;   // for the end: taken again here, the row cost the others registers
+      }
+    }
+  }
+  if (small) {
+    __syncthreads();
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+      const float mark = *(volatile float*)(p.scale + r);
+      if (mark < 0.0f) int8_small_row<T, false>(p, r, (int)-mark);
+    }
   }
 }
 
-template <typename T, int VEC, int NC, bool NORM>
+template <typename T, int VEC, int NC, int NORM>
 static int int8_launch(const Int8Rows& p, cudaStream_t s) {
   const int threads = ((p.d + VEC * NC - 1) / (VEC * NC) + 31) / 32 * 32;
   if constexpr (VEC * NC == 8) {
@@ -363,7 +432,7 @@ static int int8_launch(const Int8Rows& p, cudaStream_t s) {
 }
 
 // ctas: per SM; two rows of each are on their way or being worked on
-template <typename T, int NC, bool NORM>
+template <typename T, int NC, int NORM>
 static int int8_ring(int device, DeviceState* st, const Int8Rows& p, int threads, int ctas, cudaStream_t s) {
   static bool done[kMaxDevices] = {};
   if (!done[device]) {
@@ -381,7 +450,7 @@ static int int8_ring(int device, DeviceState* st, const Int8Rows& p, int threads
   return 1;
 }
 
-template <typename T, bool NORM>
+template <typename T, int NORM>
 static int int8_rows_t(int device, DeviceState* st, const Int8Rows& p, cudaStream_t s) {
   constexpr int kWide = 16 / (int)sizeof(T);
   if (p.d > 32768) {
@@ -419,7 +488,7 @@ static int int8_rows_t(int device, DeviceState* st, const Int8Rows& p, cudaStrea
   return e == 8 ? int8_launch<T, 1, 8, NORM>(p, s) : (e == 16 ? int8_launch<T, 1, 16, NORM>(p, s) : int8_launch<T, 1, 32, NORM>(p, s));
 }
 
-template <bool NORM>
+template <int NORM>
 static int int8_rows(int device, int dtype, Int8Rows& p, void* stream) {
   const char* op = NORM ? "rmsnorm_int8" : "rows_int8";
   KeepDevice keep;
@@ -465,7 +534,7 @@ int TSB200_RMSNormInt8(int device, int dtype, void* q, int64_t q_row, float* sca
   p.a = x; p.a_row = x_row;
   p.b = residual; p.b_row = residual ? residual_row : 0;
   p.gamma = gamma; p.eps = eps; p.rows = rows; p.d = d;
-  return int8_rows<true>(device, dtype, p, stream);
+  return eps < kInt8Small ? int8_rows<2>(device, dtype, p, stream) : int8_rows<1>(device, dtype, p, stream);
 }
 
 int TSB200_RowsInt8(int device, int dtype, void* q, int64_t q_row, float* scale, const void* src, int64_t src_row, const void* gate, int64_t gate_row, int act, int64_t rows, int d,
@@ -482,7 +551,7 @@ int TSB200_RowsInt8(int device, int dtype, void* q, int64_t q_row, float* scale,
   p.a = src; p.a_row = src_row;
   p.b = gate; p.b_row = gate ? gate_row : 0;
   p.act = act; p.rows = rows; p.d = d;
-  return int8_rows<false>(device, dtype, p, stream);
+  return int8_rows<0>(device, dtype, p, stream);
 }
 
 }  // extern "C"
