@@ -18,6 +18,7 @@
 //
 // Replaces cublasGemmEx (TensorSharp.CUDA/MatrixMul/CudaMatrixMulMM.cs:305-362, fp16 accumulate there) plus the bias
 // copy, activation and residual kernels around it.
+#include <climits>
 #include <cstdlib>
 
 #include "tc_common.cuh"
@@ -766,12 +767,12 @@ int tc_take_error() {
 }
 
 unsigned tc_wait_limit() {
-  static unsigned limit = 0;
-  if (!limit) {
+  static const unsigned limit = [] {
     const char* e = getenv("TSB200_WAIT_LIMIT");
-    const int n = e ? atoi(e) : 0;
-    limit = n > 0 ? (unsigned)n : kTcSpin;
-  }
+    char* end = nullptr;
+    const long n = e ? strtol(e, &end, 10) : -1;
+    return e && end != e && n >= 0 && n <= INT_MAX ? (unsigned)n : kTcSpin;
+  }();
   return limit;
 }
 
