@@ -290,7 +290,8 @@ TSB200_API int TSB200_VerifyDraft(int device, int32_t* tokens, int32_t* counts, 
 
 /* ------------------------------------------------------------------------------------------------ linears in 8-bit integers, and log probabilities
  * A row of bytes q with one scale stands for q * scale: rows of activations (a scale per token), rows of weights (a scale per output channel).  Rows of bytes lie
- * q_row apart, which should be a multiple of 16, as the pointer: others are served by a slow kernel.  dtype TSB200_F32, TSB200_F16 or TSB200_BF16.  `rows` may be 0.
+ * q_row apart, which should be a multiple of 16, as the pointer: other products are served by a kernel that takes 20 to 45 times as long.  dtype TSB200_F32, TSB200_F16 or
+ * TSB200_BF16.  `rows` may be 0.
  * These calls leave the caller's current device as it was.  (The reference has 8-bit weights in model files only, Models/Model_4_ProtoBufSerializer.cs:233-323.)
  *
  * RMSNormInt8: h = x + residual, rounded to dtype and written (residual and h both null: h = x, nothing is written; h may be x or residual itself);
@@ -309,7 +310,7 @@ TSB200_API int TSB200_LinearInt8(int device, int dtype, void* y, int64_t y_row, 
                                  const float* w_scale, const void* bias, int64_t rows, int K, int N, void* stream);
 /* TokenLogProbs: of every row of logits [rows, V]: the log probability of tokens[row], the entropy in nats, the token's rank (0: the most likely; the lower id first among
  * equal logits), and the `top` (0 .. 32, at most V) most likely tokens in that order with their log probabilities ([rows, top]).  -infinity is a word that
- * cannot come.  A negative token (a row without one) gives 0 and the rank -1, one beyond the vocabulary NaN and -1.  A row with a NaN or +infinity, or
+ * cannot come, and so in effect is one far below the others (a mask of -1e10, or of the type's lowest value).  A negative token (a row without one) gives 0 and the rank -1, one beyond the vocabulary NaN and -1.  A row with a NaN or +infinity, or
  * with nothing but -infinity, gives NaN (its alternatives are ordered all the same, NaN last). */
 TSB200_API int TSB200_TokenLogProbs(int device, int dtype, float* logprobs, float* entropy, int32_t* ranks, int32_t* top_tokens, float* top_logprobs, int top,
                                     const void* logits, int64_t logits_row, const int32_t* tokens, int64_t rows, int V, void* stream);

@@ -546,7 +546,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8PThreads, 1)
 
 // ---- rows that start anywhere --------------------------------------------------------------------------------------------
 // 64 x 64 outputs of a CTA, 64 k at a time through shared memory, four bytes to a dp4a.  Bound by the loads, a byte each; it is there for views that TMA cannot read
-// (256 x 4001 -> 4096: 320 us, of rows at multiples of 16 bytes 15).
+// (256 x 4001 -> 4096: 320 us, of rows at multiples of 16 bytes 15; one row 295 and 6.5).
 template <typename T>
 __global__ void __launch_bounds__(256) i8_plain_kernel(I8Args a, int n_tiles) {
   __shared__ int sq[64][17], sw[64][17];   // words of four k; an odd stride: no two rows of a column in one bank
@@ -683,7 +683,9 @@ static int i8_linear(DeviceState* st, int device, I8Args a, cudaStream_t s) {
   if (a.M <= 16) return i8_cluster<T, 16>(st, device, enc, a, s);
   if (a.M <= 32) return i8_cluster<T, 32>(st, device, enc, a, s);
   if (a.M <= 64) return i8_cluster<T, 64>(st, device, enc, a, s);
-  // whole waves of pairs times steps of 128 k, and the last tile's outputs
+  // us: whole waves of pairs times steps of 128 k (0.33 for a tile of 256 channels, 0.19 for one of 128) and the last tile's outputs; launch and start, some 4, are the same for both.  Measured (us,
+  // 256 | 128): 100 x 4096 -> 4096 14.9 | 9.9, 256 x 11008 -> 4096 31 | 21, 1024 x 4096 -> 22016 63 | 74, 2048 x 4096 -> 32000 166 | 216, 4096 x 4096 -> 4096 66 | 50.  Of 120 products of 65 to 8192
+  // rows the slower one is taken, by more than 5 %, for four: 512 x 4096 -> 32000 52 | 55, 4096 x 1000 -> 2047 17.9 | 19.2, 4096 x 2048 -> 8192 59 | 55, 8192 x 512 -> 4096 26 | 28.
   const int pairs = st->sm_count / 2, m_tiles = (a.M + 255) / 256, k_total = (a.K + 127) / 128;
   const int64_t t256 = (int64_t)m_tiles * ((a.N + 255) / 256), t128 = (int64_t)m_tiles * ((a.N + 127) / 128);
   TSB_CHECK(t128 < (1 << 30), "linear_int8: too many tiles");

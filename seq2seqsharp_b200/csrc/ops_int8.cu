@@ -8,8 +8,11 @@
 // v, sums and maxima are fp32; 127 v / max|v| has one rounding in v, one in 127 / max|v| and one in the product's sum with 1.5 2^23, whose low byte
 // is the rounded integer (half to even).  A row whose values or squares leave fp32 (infinities, NaN) gets the scale NaN and bytes of 0.
 //
-// A row is held in registers, 8 to 32 elements a thread: every tensor is read once.  Accesses of 16 bytes where all rows start on such a boundary, of two
-// elements or of one otherwise.
+// Every tensor is read once (rows beyond 32768 elements twice): a row lies in registers, 8 to 32 elements a thread.  With 32 (rows beyond 16384; the ring's norms without a residual) what does not
+// fit into 64 registers goes to the stack, 46 to 316 bytes a thread: 2000 rows of 20000, gated silu, 83 us where the bytes take 31.  Accesses of 16 bytes where all rows start on such a boundary,
+// of two elements or of one otherwise (16000 rows of 1001 bf16 with a residual 49 us, bytes 17).
+// What bounds it: bytes where nothing but products is taken of an element (8192 rows of 8192 bf16, gated relu, 51 us, bytes 51), with silu its two instructions on the XU pipe (59; 55 % of
+// that pipe, 65 % of the issue slots), with gelu erff (98); few rows the launch (8 of 11008 3.1 us).
 #include <type_traits>
 
 #include "stream_common.cuh"
@@ -465,9 +468,10 @@ static int int8_rows_t(int device, DeviceState* st, const Int8Rows& p, cudaStrea
   // elements a thread: 8 where there are few rows (the loads of a row at once), 16 or 32 where a CTA has no more threads
   const int e = p.d <= 8 * 1024 ? 8 : (p.d <= 16 * 1024 ? 16 : 32);
   if constexpr (sizeof(T) == 2) {
-    // The ring, where it was the faster one (us, ring | a CTA per row): long rows on two CTAs of 512 threads per SM (8192 of 8192, gated silu 51 | 68, 4096 of 11008 37 | 70, norm of
-    // 8192 of 8192 82 | 88); shorter ones with a thread for eight elements (norm of 16384 of 4096 81 | 85), or for 32 where there is one input only
-    // (norm of 16384 of 4096 51 | 64, plain rows of 8192 of 4096 18 | 25).  Not: fp32 (8192 of 4096 74 | 66), two inputs of up to 2048 (16384 of 2048 44 | 44), few rows.
+    // The ring, where it was the faster one (us, ring | a CTA per row): long rows on two CTAs of 512 threads per SM (8192 of 8192, gated silu 59 | 69, gated relu 51 | 69, gated gelu 98 | 115, 4096
+    // of 11008, gated silu 42 | 80, norm of 8192 of 8192 83 | 87); shorter ones with a thread for eight elements (norm of 16384 of 4096 82 | 84; but gated silu of 8192 of 4096 36 | 34), or for 32
+    // where there is one input only (norm of 16384 of 4096 52 | 64, plain rows of 8192 of 4096 18 | 28; but norm of 16384 of 2048 38 | 33).  Not: fp32 (8192 of 4096 74 | 66), two inputs of up
+    // to 2048 (16384 of 2048 44 | 44), few rows.
     const bool many = p.rows > 4 * (int64_t)st->sm_count && fits(kWide) && p.d <= 16384;
     if (many && p.d > 4096) {
       return p.d <= 8192 ? int8_ring<T, 2, NORM>(device, st, p, 512, 2, s) : int8_ring<T, 4, NORM>(device, st, p, 512, p.d <= 12288 ? 2 : 1, s);

@@ -415,7 +415,7 @@ class Ops:
     def RMSNormInt8(result, src, residual, gamma, eps=1e-6, sum=None):
         """RMSNorm of src + residual (residual None: of src) in bytes: src [rows, d], gamma [d].  Returns the bytes (int8 [rows, d], `result` or new rows that start on 16
         bytes each), their scales [rows], and the sum rounded to src's type (`sum`: where to write it, src and residual themselves are allowed; src where there is no
-        residual)."""
+        residual).  A bounded wait that runs out is reported by TSB200_Synchronize."""
         op, dev, dt = "RMSNormInt8", _device("RMSNormInt8", src), src.dtype
         code = _MODEL_DT.get(dt)
         if code is None or src.dim() != 2:
@@ -442,7 +442,7 @@ class Ops:
     @staticmethod
     def RowsInt8(result, src, gate=None, act=N.ACT_NONE):
         """act(src) [* gate] in bytes: src, gate [rows, d] (views of one tensor, for instance), act one of N.ACT_*.  Returns the bytes (as RMSNormInt8) and their scales [rows].
-        Without act and gate: rows as they are, as weights [N, K] with a scale per output channel."""
+        Without act and gate: rows as they are, as weights [N, K] with a scale per output channel.  A bounded wait that runs out is reported by TSB200_Synchronize."""
         op, dev, dt = "RowsInt8", _device("RowsInt8", src), src.dtype
         code = _MODEL_DT.get(dt)
         if code is None or src.dim() != 2:
@@ -457,8 +457,8 @@ class Ops:
     @staticmethod
     def LinearInt8(result, src, srcScale, weight, weightScale, bias=None, dtype=torch.float16):
         """src [rows, K] and weight [N, K] in bytes with scales [rows] and [N]: the exact integer product times both scales, plus bias [N], in `result` [rows, N] (None: a new
-        tensor of `dtype`; bias is of that type).  Rows of bytes that do not start on 16 bytes are served by a slow kernel.  A bounded wait that runs out is reported by
-        TSB200_Synchronize."""
+        tensor of `dtype`; bias is of that type).  Rows of bytes that do not start on 16 bytes (a contiguous weight whose K is no multiple of 16, for instance) are served by a
+        kernel that takes 20 to 45 times as long: copy them once into rows that do, as RowsInt8 returns them.  A bounded wait that runs out is reported by TSB200_Synchronize."""
         op, dev = "LinearInt8", _device("LinearInt8", src)
         if src.dim() != 2 or weight.dim() != 2:
             raise N.TSB200Error("LinearInt8: src [rows, K] and weight [N, K] are wanted")
