@@ -79,3 +79,28 @@ def test_bytes_do_not_depend_on_the_kernel(cuda):
         for i in (0, 3, 60, 150, 199, 200, 201, 202, 350, 699):
             assert torch.equal(Ops.RMSNormInt8(None, x[i: i + 1], None, gamma, eps)[0], q[i: i + 1])
         assert torch.equal(Ops.RMSNormInt8(None, x[190: 260], None, gamma, eps)[0], q[190: 260])
+
+
+@pytest.mark.parametrize("rows,d", [(5, 96), (9, 4096), (3, 40000), (700, 4096), (700, 8192)])
+@pytest.mark.parametrize("place", ["src", "residual"])
+def test_in_place_in_a_graph_and_between_other_rows(cuda, rows, d, place):
+    """The sum over an operand, rows of the caller's that lie apart, captured; small rows between ordinary ones."""
+    g = gen(rows + d)
+    size = torch.ones(rows, 1, device="cuda")
+    size[1::2] = 1e-24
+    x0, r0 = (randn(g, rows, d) * size).to(BF16), (randn(g, rows, d) * size).to(BF16)
+    gamma = (1 + 0.3 * torch.randn(d, generator=g, device="cuda")).to(BF16)
+    want = Ops.RMSNormInt8(None, x0, r0, gamma, 0.0)
+    x, r = x0.clone(), r0.clone()
+    wide = torch.full((rows, d + 32), 99, dtype=torch.int8, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q, scale, h = Ops.RMSNormInt8(wide[:, 16: 16 + d], x, r, gamma, 0.0, sum=x if place == "src" else r)
+    for _ in range(2):
+        x.copy_(x0)
+        r.copy_(r0)
+        graph.replay()
+        assert torch.equal(q, want[0]) and torch.equal(scale, want[1]) and torch.equal(h, want[2])
+        assert (wide[:, :16] == 99).all() and (wide[:, 16 + d:] == 99).all()
+    assert (scale > 1e-3).all() and (q.abs().amax(1) == 127).all()
